@@ -50,14 +50,17 @@ enum {
 };
 
 /* dtype codes 1-4 are the reference's (runtime_args.py:94-110, common.py:171-194);
- * 5 (float16) and 6 (bfloat16) are additive extensions for the gfx950 MFMA paths. */
+ * 5 (float16) and 6 (bfloat16) are additive extensions for the gfx950 MFMA paths, 7 (int8) and
+ * 8 (float8 e4m3fn) for the caches of the serving entries, the only ones that take them. */
 enum {
   KG_DTYPE_F32 = 1,
   KG_DTYPE_F64 = 2,
   KG_DTYPE_I32 = 3,
   KG_DTYPE_I64 = 4,
   KG_DTYPE_F16 = 5,
-  KG_DTYPE_BF16 = 6
+  KG_DTYPE_BF16 = 6,
+  KG_DTYPE_I8 = 7,
+  KG_DTYPE_E4M3 = 8
 };
 
 /* Byte-for-byte the reference's _ArgSlot / _CArgSlot (runtime_args.py:228-237;
@@ -121,6 +124,60 @@ int kg_gfx950_conv2d_entry(const KgArgSlot* ordered_args, unsigned long long arg
 int kg_gfx950_flash_attention_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
 
 /*
+ * Serving entries (no counterpart in the reference): a paged cache of keys and values written and read
+ * back, attention of drafted tokens over it, and a projection with low-rank adapters beside it. Same slot
+ * structure, return codes, launch modes and workspaces as the entries above. Memory must lie on the
+ * current device; all but the last axis of a tensor may have any non-negative strides, and the last is contiguous
+ * (page_table, lens, starts, slots, mask, index and scales: any). Values that lie in device memory (slots,
+ * page tables, lengths, masks, adapter indexes) are not checked by the host: each entry says below what it makes of
+ * values that are out of range. None of them reads or writes outside the tensors.
+ *
+ * Caches: k_cache, v_cache [pages, heads, page_size, D] (D 1..512, any page_size), f32, f16, bf16, or 8-bit
+ * (i8, e4m3) with k_scale, v_scale f32 [pages, heads, page_size] (absent otherwise). An 8-bit element stands
+ * for code x scale. Token i of a sequence lies on page page_table[b, i / page_size] at offset i % page_size.
+ */
+
+/*
+ * (k_cache, v_cache, k_scale | absent, v_scale | absent, k[T, heads, D], v[T, heads, D], slots[T] i64)
+ * Writes the rows of token t to slot slots[t] = page * page_size + offset. A slot outside
+ * 0 .. pages * page_size - 1 (-1, say) writes nothing. k, v: f32, f16 or bf16; a cache that is not in 8 bits has
+ * their type. 8 bits: scale = max|x| / 448 (e4m3) or / 127 (i8), as a 32-bit product with the divisor's rounded
+ * inverse; code = x / scale, nearest, ties to even. A row with an infinity or NaN reads back as NaN throughout. Two tokens
+ * of a call must not name the same slot: it would hold an unspecified mix of them.
+ */
+int kg_gfx950_kv_cache_store_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (k_out[B, heads, S, D], v_out[B, heads, S, D], k_cache, v_cache, k_scale | absent, v_scale | absent,
+ *  page_table[B, P] i32, lengths[B] i32)
+ * Rows 0 .. min(lengths[b], S, P * page_size) - 1 of each sequence, the layout flash attention takes. Other
+ * rows, and rows on pages outside 0 .. pages - 1, are left as they are. k_out, v_out: f32, f16 or bf16; of a cache
+ * that is not in 8 bits, its type.
+ */
+int kg_gfx950_kv_cache_load_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (out[T, Hq, D], q[T, Hq, D], k_cache, v_cache, k_scale | absent, v_scale | absent, page_table[B, P] i32,
+ *  context_lens[B] i32, starts[B + 1] i32, mask[T, W] i64 | absent, scale FLOAT)
+ * Request b has the tokens starts[b] .. starts[b + 1] - 1 (starts ascend; none is allowed), whose keys and values lie in the cache
+ * at positions context_lens[b] + j. Token j sees positions below context_lens[b] and those drafted tokens i whose
+ * bit i % 64 of mask[starts[b] + j, i / 64] is set (bits past the request's tokens say nothing); without a mask,
+ * i <= j: a decoding step (one token), a chain of drafts, a piece of a prompt. Query head h reads key head h / (Hq / heads).
+ * Rows that see nothing get zeros; rows of no request are left as they are. Positions past P * page_size and
+ * pages outside 0 .. pages - 1 are not seen. What is not seen has no influence, infinities and NaN included. q, out:
+ * f32, f16 or bf16; of a cache that is not in 8 bits, its type. P * page_size < 2^31. out must not overlap q.
+ */
+int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (out[M, N], x[M, K], weight[K, N], bias[N] | absent, a[L, K, R], b[L, R, N], index[M] i32, scale[L] f32 | absent)
+ * out[m] = x[m] weight + bias + scale[l] (x[m] a[l]) b[l], l = index[m]; an index outside 0 .. L - 1 is a row without an
+ * adapter; an absent scale is 1. dtypes as matmul's, a and b the operands'. R <= 512. Adapters of unequal
+ * rank are padded with zeros. out must not overlap an operand.
+ */
+int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
  * Launch control (no counterpart in the reference, whose execute() is synchronous and
  * rejects a stream: compiler.py:286-291). synchronous != 0 (default): every entry
  * synchronizes its stream before returning. synchronous == 0: entries only enqueue on
@@ -155,7 +212,7 @@ int kg_gfx950_finish_launch(const char* what);
 const char* kg_gfx950_last_error(void);
 
 /* ABI revision of this library (bumped on any change of a declaration here or of the slot
- * contract). 2: kg_gfx950_cost writes five kinds (KG_COST_MFMA_CYCLES added). 3: the
+ * contract; entries and dtype codes that are only added leave it). 2: kg_gfx950_cost writes five kinds (KG_COST_MFMA_CYCLES added). 3: the
  * measurement aid kg_gfx950_mfma_rate left the library (bench.py's probe library has it);
  * memory_stage slots on the attention (slot 8) and conv2d (slot 17) entries. */
 int kg_gfx950_abi_version(void);

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "kg_gfx950.h"
+#include "kg_gfx950/adapter.h"
 #include "kg_gfx950/common.h"
 #include "kg_gfx950/conv2d.h"
 #include "kg_gfx950/flash_attn.h"
@@ -31,6 +32,8 @@
 #include "kg_gfx950/flash_attn_mfma.h"
 #include "kg_gfx950/flash_attn_decode.h"
 #include "kg_gfx950/flash_attn_f32.h"
+#include "kg_gfx950/kv_cache.h"
+#include "kg_gfx950/tree_attn.h"
 #include "kg_gfx950/instances.h"  // the heavy kernel families are compiled in their own translation units
 
 namespace {
@@ -113,6 +116,8 @@ const char* dtype_name(int code) {
     case KG_DTYPE_I64: return "i64";
     case KG_DTYPE_F16: return "f16";
     case KG_DTYPE_BF16: return "bf16";
+    case KG_DTYPE_I8: return "i8";
+    case KG_DTYPE_E4M3: return "e4m3";
     default: return "unknown";
   }
 }
@@ -1234,6 +1239,349 @@ int flash_attention_impl(const KgArgSlot* args, unsigned long long n) {
   }
 }
 
+// ---------------------------------------------------------------------------------------
+// serving: the paged cache of keys and values, attention over it, adapters
+// ---------------------------------------------------------------------------------------
+
+// These entries check a call in two steps: what the slots say (kind, rank, dtype, shape, strides), for
+// all of them, and only then the memory behind them, which must lie on the current device.
+constexpr unsigned kFloatTypes = 1u << KG_DTYPE_F32 | 1u << KG_DTYPE_F16 | 1u << KG_DTYPE_BF16;
+constexpr unsigned kCacheTypes = kFloatTypes | 1u << KG_DTYPE_I8 | 1u << KG_DTYPE_E4M3;
+
+long long element_bytes(int dtype) {
+  switch (dtype) {
+    case KG_DTYPE_F64:
+    case KG_DTYPE_I64: return 8;
+    case KG_DTYPE_F32:
+    case KG_DTYPE_I32: return 4;
+    case KG_DTYPE_F16:
+    case KG_DTYPE_BF16: return 2;
+    default: return 1;
+  }
+}
+
+int read_view(const KgArgSlot* slots, int idx, int rank, unsigned types, bool allow_absent, const char* name, Mem* out) {
+  const KgArgSlot& s = slots[idx];
+  if (s.kind != KG_ARG_MEMORY) return fail(kInvalid, "slot %d (%s): expected memory slot, got kind %d", idx, name, s.kind);
+  if (allow_absent && s.data == nullptr && s.rank <= 1) return kOk;  // (an empty tensor of the right rank is present)
+  if ((int)s.rank != rank) return fail(kInvalid, "slot %d (%s): expected rank %d, got %llu", idx, name, rank, s.rank);
+  if (s.shape == nullptr || s.stride == nullptr) return fail(kInvalid, "slot %d (%s): missing shape/stride", idx, name);
+  if (s.dtype_code < 1 || s.dtype_code > 31 || !(types >> s.dtype_code & 1u))
+    return fail(kInvalid, "slot %d (%s): unsupported dtype_code %d (%s)", idx, name, s.dtype_code, dtype_name(s.dtype_code));
+  out->data = s.data;
+  out->rank = rank;
+  out->dtype = s.dtype_code;
+  out->present = true;
+  for (int i = 0; i < rank; ++i) {
+    if (s.shape[i] < 0) return fail(kInvalid, "slot %d (%s): negative extent", idx, name);
+    if (s.stride[i] < 0) return fail(kInvalid, "slot %d (%s): negative stride", idx, name);
+    if (s.shape[i] > 0x7fffffffLL) return fail(kUnsupported, "slot %d (%s): extent exceeds int32", idx, name);
+    if (s.shape[i] > 1 && s.stride[i] > (1LL << 45))
+      return fail(kInvalid, "slot %d (%s): stride %lld is beyond any allocation", idx, name, s.stride[i]);
+    out->shape[i] = s.shape[i];
+    out->stride[i] = s.stride[i];
+  }
+  return kOk;
+}
+
+int check_view(const Mem& m, const char* name) {
+  if (!m.present || m.numel() == 0) return kOk;
+  if (m.data == nullptr) return fail(kInvalid, "%s: memory slot has no data", name);
+  hipPointerAttribute_t attr;
+  if (hipPointerGetAttributes(&attr, m.data) != hipSuccess || attr.type != hipMemoryTypeDevice) {
+    (void)hipGetLastError();
+    return fail(kInvalid, "%s: data is not a device pointer", name);
+  }
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || attr.device != device)
+    return fail(kInvalid, "%s: memory of device %d, the current device is %d", name, attr.device, device);
+  hipDeviceptr_t base = nullptr;
+  size_t size = 0;
+  if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)m.data) != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(kInvalid, "%s: cannot query device allocation", name);
+  }
+  unsigned __int128 last = 0;
+  for (int i = 0; i < m.rank; ++i) last += (unsigned __int128)(m.shape[i] - 1) * m.stride[i];
+  const unsigned __int128 need = (size_t)((const char*)m.data - (const char*)base) + (last + 1) * element_bytes(m.dtype);
+  if (need > size) return fail(kInvalid, "%s: view runs past its allocation of %zu bytes", name, size);
+  return kOk;
+}
+
+bool row_contiguous(const Mem& m) { return m.shape[m.rank - 1] <= 1 || m.stride[m.rank - 1] == 1; }
+
+// The two caches and their scales, the same of every entry that takes them: [pages, heads, page_size, D] and
+// [pages, heads, page_size].
+struct KvSlots {
+  Mem cache[2], scale[2];
+  long long pages = 0, heads = 0, page_size = 0, d = 0;
+  int dtype = 0;
+  bool scaled() const { return dtype == KG_DTYPE_I8 || dtype == KG_DTYPE_E4M3; }
+};
+
+int read_kv(const KgArgSlot* args, int at, const char* op, KvSlots* kv) {
+  int rc;
+  if ((rc = read_view(args, at, 4, kCacheTypes, false, "k_cache", &kv->cache[0]))) return rc;
+  if ((rc = read_view(args, at + 1, 4, kCacheTypes, false, "v_cache", &kv->cache[1]))) return rc;
+  if ((rc = read_view(args, at + 2, 3, 1u << KG_DTYPE_F32, true, "k_scale", &kv->scale[0]))) return rc;
+  if ((rc = read_view(args, at + 3, 3, 1u << KG_DTYPE_F32, true, "v_scale", &kv->scale[1]))) return rc;
+  const Mem& k = kv->cache[0];
+  kv->dtype = k.dtype;
+  kv->pages = k.shape[0];
+  kv->heads = k.shape[1];
+  kv->page_size = k.shape[2];
+  kv->d = k.shape[3];
+  if (kv->cache[1].dtype != k.dtype)
+    return fail(kInvalid, "%s: k_cache/v_cache dtypes must match (%s, %s)", op, dtype_name(k.dtype), dtype_name(kv->cache[1].dtype));
+  for (int x = 0; x < 2; ++x) {
+    for (int i = 0; i < 4; ++i)
+      if (kv->cache[x].shape[i] != k.shape[i]) return fail(kInvalid, "%s: k_cache/v_cache shape mismatch at dim %d", op, i);
+    if (!row_contiguous(kv->cache[x])) return fail(kInvalid, "%s: the rows of a cache must be contiguous", op);
+    if (kv->scale[x].present != kv->scaled())
+      return fail(kInvalid, kv->scaled() ? "%s: an 8-bit cache (%s) needs k_scale and v_scale" : "%s: a cache of %s takes no scales",
+                  op, dtype_name(kv->dtype));
+    if (kv->scaled())
+      for (int i = 0; i < 3; ++i)
+        if (kv->scale[x].shape[i] != k.shape[i]) return fail(kInvalid, "%s: cache/scale shape mismatch at dim %d", op, i);
+  }
+  if (kv->page_size < 1) return fail(kInvalid, "%s: pages must hold at least one token", op);
+  if (kv->d < 1 || kv->d > 512) return fail(kUnsupported, "%s: head dim %lld not in 1..512", op, kv->d);
+  return kOk;
+}
+
+int check_kv(const KvSlots& kv) {
+  int rc;
+  if ((rc = check_view(kv.cache[0], "k_cache"))) return rc;
+  if ((rc = check_view(kv.cache[1], "v_cache"))) return rc;
+  if ((rc = check_view(kv.scale[0], "k_scale"))) return rc;
+  return check_view(kv.scale[1], "v_scale");
+}
+
+// (a [pages, heads, page_size] view's strides; zeros where there are no scales)
+KvSide kv_side(const KvSlots& kv, int x, const Mem& rows) {
+  const Mem &c = kv.cache[x], &s = kv.scale[x];
+  return KvSide{c.data, static_cast<float*>(s.data), rows.data, c.stride[0], c.stride[1], c.stride[2],
+                s.stride[0], s.stride[1], s.stride[2], rows.stride[0], rows.stride[1], rows.stride[2]};
+}
+
+// Calls f(type of the dense rows, type of the cache's elements): the same, or 8 bits.
+template <typename F>
+int with_kv_types(int dtype, int cache, F&& f) {
+  auto with = [&](auto rows) {
+    using T = decltype(rows);
+    return cache == KG_DTYPE_E4M3 ? f(rows, E4m3{}) : cache == KG_DTYPE_I8 ? f(rows, int8_t{}) : f(rows, T{});
+  };
+  return dtype == KG_DTYPE_F32 ? with(float{}) : dtype == KG_DTYPE_BF16 ? with((__bf16)0.f) : with((_Float16)0.f);
+}
+
+int kv_cache_store_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 7) return fail(kInvalid, "kv_cache_store expects 7 slots, got %llu", n);
+  KvSlots kv;
+  Mem rows[2], slots;
+  int rc;
+  if ((rc = read_kv(args, 0, "kv_cache_store", &kv))) return rc;
+  if ((rc = read_view(args, 4, 3, kFloatTypes, false, "k", &rows[0]))) return rc;
+  if ((rc = read_view(args, 5, 3, kFloatTypes, false, "v", &rows[1]))) return rc;
+  if ((rc = read_view(args, 6, 1, 1u << KG_DTYPE_I64, false, "slots", &slots))) return rc;
+  const long long tokens = rows[0].shape[0];
+  for (int x = 0; x < 2; ++x) {
+    if (rows[x].shape[0] != tokens || rows[x].shape[1] != kv.heads || rows[x].shape[2] != kv.d)
+      return fail(kInvalid, "kv_cache_store: k and v must be [tokens, %lld, %lld] as the cache's rows", kv.heads, kv.d);
+    if (rows[x].dtype != rows[0].dtype || (!kv.scaled() && rows[x].dtype != kv.dtype))
+      return fail(kInvalid, "kv_cache_store: k/v dtypes must match each other and a cache that is not in 8 bits");
+    if (!row_contiguous(rows[x])) return fail(kInvalid, "kv_cache_store: the rows of k and v must be contiguous");
+  }
+  if (slots.shape[0] != tokens) return fail(kInvalid, "kv_cache_store: %lld slots for %lld tokens", slots.shape[0], tokens);
+  if ((rc = check_kv(kv)) || (rc = check_view(rows[0], "k")) || (rc = check_view(rows[1], "v")) ||
+      (rc = check_view(slots, "slots")))
+    return rc;
+  if (tokens == 0 || kv.heads == 0 || kv.pages == 0) return finish_launch("kv_cache_store(empty)");
+  KvStoreArgs a;
+  for (int x = 0; x < 2; ++x) a.side[x] = kv_side(kv, x, rows[x]);
+  a.slots = static_cast<const long long*>(slots.data);
+  a.slot_stride = slots.stride[0];
+  a.tokens = (int)tokens;
+  a.heads = (int)kv.heads;
+  a.d = (int)kv.d;
+  a.page_size = (int)kv.page_size;
+  a.total_slots = kv.pages * kv.page_size;
+  const long long items = 2 * tokens * kv.heads;
+  if (cdiv(items, 4) > 0x7fffffffLL) return fail(kUnsupported, "kv_cache_store: %lld rows exceed the grid limit", items);
+  return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
+    hipLaunchKernelGGL((kv_store_any_kernel<decltype(t), decltype(c)>), dim3((unsigned)cdiv(items, 4)), dim3(256), 0, g_stream, a);
+    return finish_launch("kv_cache_store");
+  });
+}
+
+int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 8) return fail(kInvalid, "kv_cache_load expects 8 slots, got %llu", n);
+  KvSlots kv;
+  Mem rows[2], table, lens;
+  int rc;
+  if ((rc = read_view(args, 0, 4, kFloatTypes, false, "k_out", &rows[0]))) return rc;
+  if ((rc = read_view(args, 1, 4, kFloatTypes, false, "v_out", &rows[1]))) return rc;
+  if ((rc = read_kv(args, 2, "kv_cache_load", &kv))) return rc;
+  if ((rc = read_view(args, 6, 2, 1u << KG_DTYPE_I32, false, "page_table", &table))) return rc;
+  if ((rc = read_view(args, 7, 1, 1u << KG_DTYPE_I32, false, "lengths", &lens))) return rc;
+  const long long batch = rows[0].shape[0], reach = rows[0].shape[2];
+  for (int x = 0; x < 2; ++x) {
+    if (rows[x].shape[0] != batch || rows[x].shape[1] != kv.heads || rows[x].shape[2] != reach || rows[x].shape[3] != kv.d)
+      return fail(kInvalid, "kv_cache_load: k_out and v_out must be [batch, %lld, rows, %lld]", kv.heads, kv.d);
+    if (rows[x].dtype != rows[0].dtype || (!kv.scaled() && rows[x].dtype != kv.dtype))
+      return fail(kInvalid, "kv_cache_load: k_out/v_out dtypes must match each other and a cache that is not in 8 bits");
+    if (!row_contiguous(rows[x])) return fail(kInvalid, "kv_cache_load: the rows of k_out and v_out must be contiguous");
+  }
+  if (table.shape[0] != batch || lens.shape[0] != batch)
+    return fail(kInvalid, "kv_cache_load: page_table and lengths must have a row for each of %lld sequences", batch);
+  if ((rc = check_view(rows[0], "k_out")) || (rc = check_view(rows[1], "v_out")) || (rc = check_kv(kv)) ||
+      (rc = check_view(table, "page_table")) || (rc = check_view(lens, "lengths")))
+    return rc;
+  if (rows[0].numel() == 0 || table.shape[1] == 0) return finish_launch("kv_cache_load(empty)");
+  KvLoadArgs a;
+  for (int x = 0; x < 2; ++x) a.side[x] = kv_side(kv, x, rows[x]);
+  a.table = static_cast<const int*>(table.data);
+  a.lens = static_cast<const int*>(lens.data);
+  a.table_stride0 = table.stride[0];
+  a.table_stride1 = table.stride[1];
+  a.len_stride = lens.stride[0];
+  a.batch = (int)batch;
+  a.heads = (int)kv.heads;
+  a.d = (int)kv.d;
+  a.page_size = (int)kv.page_size;
+  a.per = (int)table.shape[1];
+  a.reach = (int)reach;
+  a.pages = kv.pages;
+  a.div = page_div((int)kv.page_size);
+  if (batch * kv.heads > 0x7fffffffLL || cdiv(2 * batch * kv.heads, 4) > 0x7fffffffLL / reach)
+    return fail(kUnsupported, "kv_cache_load: %lld x %lld rows exceed the grid limit", batch * kv.heads, reach);
+  return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
+    hipLaunchKernelGGL((kv_load_any_kernel<decltype(c), decltype(t)>), dim3((unsigned)cdiv(2 * batch * kv.heads * reach, 4)),
+                       dim3(256), 0, g_stream, a);
+    return finish_launch("kv_cache_load");
+  });
+}
+
+int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 11) return fail(kInvalid, "tree_attention expects 11 slots, got %llu", n);
+  KvSlots kv;
+  Mem out, q, table, lens, starts, mask;
+  double scale;
+  int rc;
+  if ((rc = read_view(args, 0, 3, kFloatTypes, false, "out", &out))) return rc;
+  if ((rc = read_view(args, 1, 3, kFloatTypes, false, "q", &q))) return rc;
+  if ((rc = read_kv(args, 2, "tree_attention", &kv))) return rc;
+  if ((rc = read_view(args, 6, 2, 1u << KG_DTYPE_I32, false, "page_table", &table))) return rc;
+  if ((rc = read_view(args, 7, 1, 1u << KG_DTYPE_I32, false, "context_lens", &lens))) return rc;
+  if ((rc = read_view(args, 8, 1, 1u << KG_DTYPE_I32, false, "starts", &starts))) return rc;
+  if ((rc = read_view(args, 9, 2, 1u << KG_DTYPE_I64, true, "mask", &mask))) return rc;
+  if ((rc = read_float(args, 10, "scale", &scale))) return rc;
+  if (!std::isfinite((float)scale)) return fail(kInvalid, "tree_attention: scale must be finite");
+  const long long tokens = q.shape[0], heads_q = q.shape[1], batch = lens.shape[0];
+  for (int i = 0; i < 3; ++i)
+    if (out.shape[i] != q.shape[i]) return fail(kInvalid, "tree_attention: q/out shape mismatch at dim %d", i);
+  if (q.shape[2] != kv.d) return fail(kInvalid, "tree_attention: head dim %lld of q, %lld of the cache", q.shape[2], kv.d);
+  if (kv.heads == 0 ? heads_q != 0 : heads_q % kv.heads != 0)
+    return fail(kInvalid, "tree_attention: %lld query heads are no multiple of %lld key heads", heads_q, kv.heads);
+  if (q.dtype != out.dtype || (!kv.scaled() && q.dtype != kv.dtype))
+    return fail(kInvalid, "tree_attention: q/out dtypes must match each other and a cache that is not in 8 bits");
+  if (!row_contiguous(q) || !row_contiguous(out)) return fail(kInvalid, "tree_attention: the rows of q and out must be contiguous");
+  if (table.shape[0] != batch) return fail(kInvalid, "tree_attention: page_table has %lld rows for %lld requests", table.shape[0], batch);
+  if (starts.shape[0] != batch + 1)
+    return fail(kInvalid, "tree_attention: starts must have %lld values, got %lld", batch + 1, starts.shape[0]);
+  if (mask.present && mask.shape[0] != tokens)
+    return fail(kInvalid, "tree_attention: mask has %lld rows for %lld tokens", mask.shape[0], tokens);
+  if (table.shape[1] * kv.page_size > 0x7fffffffLL)
+    return fail(kUnsupported, "tree_attention: a page table of %lld x %lld tokens exceeds int32", table.shape[1], kv.page_size);
+  if ((rc = check_view(out, "out")) || (rc = check_view(q, "q")) || (rc = check_kv(kv)) || (rc = check_view(table, "page_table")) ||
+      (rc = check_view(lens, "context_lens")) || (rc = check_view(starts, "starts")) || (rc = check_view(mask, "mask")))
+    return rc;
+  if (out.numel() == 0 || batch == 0) return finish_launch("tree_attention(empty)");
+  TreeArgs a;
+  a.q = q.data;
+  a.out = out.data;
+  a.k = kv.cache[0].data;
+  a.v = kv.cache[1].data;
+  a.k_scale = static_cast<const float*>(kv.scale[0].data);
+  a.v_scale = static_cast<const float*>(kv.scale[1].data);
+  a.table = static_cast<const int*>(table.data);
+  a.lens = static_cast<const int*>(lens.data);
+  a.starts = static_cast<const int*>(starts.data);
+  a.mask = static_cast<const long long*>(mask.data);
+  a.q_token = q.stride[0], a.q_head = q.stride[1];
+  a.o_token = out.stride[0], a.o_head = out.stride[1];
+  a.k_page = kv.cache[0].stride[0], a.k_head = kv.cache[0].stride[1], a.k_row = kv.cache[0].stride[2];
+  a.v_page = kv.cache[1].stride[0], a.v_head = kv.cache[1].stride[1], a.v_row = kv.cache[1].stride[2];
+  a.ks_page = kv.scale[0].stride[0], a.ks_head = kv.scale[0].stride[1], a.ks_row = kv.scale[0].stride[2];
+  a.vs_page = kv.scale[1].stride[0], a.vs_head = kv.scale[1].stride[1], a.vs_row = kv.scale[1].stride[2];
+  a.table_0 = table.stride[0], a.table_1 = table.stride[1];
+  a.len_stride = lens.stride[0], a.start_stride = starts.stride[0];
+  a.mask_0 = mask.stride[0], a.mask_1 = mask.stride[1];
+  a.tokens = (int)tokens, a.batch = (int)batch, a.heads_q = (int)heads_q, a.heads = (int)kv.heads;
+  a.group = (int)(heads_q / kv.heads), a.d = (int)kv.d, a.page_size = (int)kv.page_size, a.per = (int)table.shape[1];
+  a.words = mask.present ? (int)mask.shape[1] : -1;
+  a.pages = kv.pages;
+  a.div = page_div((int)kv.page_size);
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  if (tokens * heads_q > 0x7fffffffLL) return fail(kUnsupported, "tree_attention: %lld rows exceed the grid limit", tokens * heads_q);
+  return with_kv_types(q.dtype, kv.dtype, [&](auto t, auto c) {
+    hipLaunchKernelGGL((tree_attn_any_kernel<decltype(t), decltype(c)>), dim3((unsigned)(tokens * heads_q)), dim3(256), 0, g_stream, a);
+    return finish_launch("tree_attention");
+  });
+}
+
+int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 8) return fail(kInvalid, "adapter_matmul expects 8 slots, got %llu", n);
+  Mem out, x, w, bias, a, b, index, scale;
+  int rc;
+  if ((rc = read_view(args, 0, 2, kFloatTypes, false, "out", &out))) return rc;
+  if ((rc = read_view(args, 1, 2, kFloatTypes, false, "x", &x))) return rc;
+  if ((rc = read_view(args, 2, 2, kFloatTypes, false, "weight", &w))) return rc;
+  if ((rc = read_view(args, 3, 1, kFloatTypes, true, "bias", &bias))) return rc;
+  if ((rc = read_view(args, 4, 3, kFloatTypes, false, "a", &a))) return rc;
+  if ((rc = read_view(args, 5, 3, kFloatTypes, false, "b", &b))) return rc;
+  if ((rc = read_view(args, 6, 1, 1u << KG_DTYPE_I32, false, "index", &index))) return rc;
+  if ((rc = read_view(args, 7, 1, 1u << KG_DTYPE_F32, true, "scale", &scale))) return rc;
+  const long long M = x.shape[0], K = x.shape[1], N = w.shape[1], count = a.shape[0], rank = a.shape[2];
+  if (w.shape[0] != K) return fail(kInvalid, "adapter_matmul: x K=%lld != weight K=%lld", K, w.shape[0]);
+  if (out.shape[0] != M || out.shape[1] != N)
+    return fail(kInvalid, "adapter_matmul: out shape [%lld,%lld] != [%lld,%lld]", out.shape[0], out.shape[1], M, N);
+  if (bias.present && bias.shape[0] != N) return fail(kInvalid, "adapter_matmul: bias extent %lld != N=%lld", bias.shape[0], N);
+  if (a.shape[1] != K) return fail(kInvalid, "adapter_matmul: a must be [adapters, %lld, rank]", K);
+  if (b.shape[0] != count || b.shape[1] != rank || b.shape[2] != N)
+    return fail(kInvalid, "adapter_matmul: b must be [%lld, %lld, %lld]", count, rank, N);
+  if (index.shape[0] != M) return fail(kInvalid, "adapter_matmul: %lld indexes for %lld rows", index.shape[0], M);
+  if (scale.present && scale.shape[0] != count) return fail(kInvalid, "adapter_matmul: %lld scales for %lld adapters", scale.shape[0], count);
+  if (x.dtype != out.dtype || w.dtype != out.dtype || a.dtype != out.dtype || b.dtype != out.dtype)
+    return fail(kInvalid, "adapter_matmul: out/x/weight/a/b dtypes must match");
+  if (bias.present && bias.dtype != out.dtype && bias.dtype != KG_DTYPE_F32)
+    return fail(kInvalid, "adapter_matmul: bias dtype %s must be f32 or match out", dtype_name(bias.dtype));
+  const bool adapters = count > 0 && rank > 0;
+  if (adapters && rank > kAdapterMaxRank) return fail(kUnsupported, "adapter_matmul: rank %lld > %d", rank, kAdapterMaxRank);
+  for (const Mem* m : {&out, &x, &a, &b})
+    if (!row_contiguous(*m)) return fail(kInvalid, "adapter_matmul: the rows of out, x, a and b must be contiguous");
+  if ((rc = check_view(out, "out")) || (rc = check_view(x, "x")) || (rc = check_view(w, "weight")) || (rc = check_view(bias, "bias")) ||
+      (rc = check_view(a, "a")) || (rc = check_view(b, "b")) || (rc = check_view(index, "index")) || (rc = check_view(scale, "scale")))
+    return rc;
+  if (M == 0 || N == 0) return finish_launch("adapter_matmul(empty)");
+  AdapterArgs p;
+  p.x = x.data, p.w = w.data, p.bias = bias.data, p.a = a.data, p.b = b.data, p.out = out.data;
+  p.index = static_cast<const int*>(index.data);
+  p.scale = static_cast<const float*>(scale.data);
+  p.ldx = x.stride[0], p.ldw = w.stride[0], p.ldo = out.stride[0];
+  p.a_l = a.stride[0], p.a_k = a.stride[1], p.b_l = b.stride[0], p.b_r = b.stride[1];
+  p.index_stride = index.stride[0], p.scale_stride = scale.stride[0];
+  p.m = (int)M, p.n = (int)N, p.k = (int)K, p.rank = (int)rank, p.count = (int)count;
+  if ((rc = matmul_impl(args, 4)) || !adapters) return rc;
+  return with_kv_types(out.dtype, out.dtype, [&](auto t, auto) {
+    hipLaunchKernelGGL((adapter_add_kernel<decltype(t)>), dim3((unsigned)M), dim3(256), 0, g_stream, p);
+    return finish_launch("adapter_matmul");
+  });
+}
+
 }  // namespace
 
 extern "C" {
@@ -1248,6 +1596,22 @@ int kg_gfx950_conv2d_entry(const KgArgSlot* ordered_args, unsigned long long arg
 
 int kg_gfx950_flash_attention_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
   return flash_attention_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_kv_cache_store_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return kv_cache_store_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_kv_cache_load_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return kv_cache_load_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return tree_attention_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return adapter_matmul_impl(ordered_args, arg_count);
 }
 
 int kg_gfx950_fail(int code, const char* message) { return fail(code, "%s", message ? message : ""); }

@@ -35,11 +35,17 @@ DTYPE_CODES = {
     "float16": 5,
     "bfloat16": 6,
 }
+# of the serving entries' caches alone
+CACHE_DTYPE_CODES = {"int8": 7, "float8_e4m3fn": 8}
 
 ENTRY_POINTS = (
     "kg_gfx950_matmul_entry",
     "kg_gfx950_conv2d_entry",
     "kg_gfx950_flash_attention_entry",
+    "kg_gfx950_kv_cache_store_entry",
+    "kg_gfx950_kv_cache_load_entry",
+    "kg_gfx950_tree_attention_entry",
+    "kg_gfx950_adapter_matmul_entry",
 )
 CONTROL_SYMBOLS = (
     "kg_gfx950_set_launch_mode",
@@ -172,7 +178,7 @@ def dtype_code_of(value: Any) -> int:
     code = _DTYPE_CODE_OF.get(dtype)
     if code is None:
         name = str(dtype).replace("torch.", "")
-        code = DTYPE_CODES.get(name)
+        code = DTYPE_CODES.get(name) or CACHE_DTYPE_CODES.get(name)
         if code is None:
             raise NativeLibraryError(f"unsupported memory dtype {name!r}", -1)
         _DTYPE_CODE_OF[dtype] = code
@@ -321,3 +327,36 @@ def flash_attention(out, q, k, v, br: int = 64, bc: int = 64, scale: float = 1.0
     stage = () if memory_stage is None else (int(memory_stage),)
     call_entry("kg_gfx950_flash_attention_entry",
                (out, q, k, v, int(br), int(bc), float(scale), int(bool(causal)), *stage))
+
+
+def kv_cache_store(k_cache, v_cache, k_scale, v_scale, k, v, slots) -> None:
+    """Write rows k, v [T, heads, D] to the slots (int64 [T], page * page_size + offset; -1: none) of
+    caches [pages, heads, page_size, D]; 8-bit ones (int8, float8_e4m3fn) with scales [pages, heads,
+    page_size] (float32), others with None. No two tokens may name one slot."""
+
+    call_entry("kg_gfx950_kv_cache_store_entry", (k_cache, v_cache, k_scale, v_scale, k, v, slots))
+
+
+def kv_cache_load(k_out, v_out, k_cache, v_cache, k_scale, v_scale, page_table, lengths) -> None:
+    """Read the first lengths[b] (int32 [B]) rows of each sequence back into k_out, v_out [B, heads, S, D],
+    by its pages page_table[b] (int32 [B, P]). Rows past them are left as they are."""
+
+    call_entry("kg_gfx950_kv_cache_load_entry", (k_out, v_out, k_cache, v_cache, k_scale, v_scale, page_table, lengths))
+
+
+def tree_attention(out, q, k_cache, v_cache, k_scale, v_scale, page_table, context_lens, starts, mask=None,
+                   scale: float = 1.0) -> None:
+    """Attention of the tokens q [T, Hq, D] over the cache. Request b has tokens starts[b] to
+    starts[b + 1] - 1 (int32 [B + 1]), whose own keys and values lie behind its context_lens[b] cached ones.
+    Token j sees the context and the request's drafted tokens i with bit i % 64 of mask[starts[b] + j, i / 64]
+    (int64 [T, W]); without a mask i <= j: a decoding step, a chain of drafts, a piece of a prompt."""
+
+    call_entry("kg_gfx950_tree_attention_entry",
+               (out, q, k_cache, v_cache, k_scale, v_scale, page_table, context_lens, starts, mask, float(scale)))
+
+
+def adapter_matmul(out, x, weight, bias, a, b, index, scale=None) -> None:
+    """out = x @ weight + bias, plus scale[l] * (x[m] @ a[l]) @ b[l] in each row m whose l = index[m]
+    (int32 [M]) is an adapter (a [L, K, R], b [L, R, N]; scale: float32 [L], 1 where None)."""
+
+    call_entry("kg_gfx950_adapter_matmul_entry", (out, x, weight, bias, a, b, index, scale))

@@ -1,0 +1,202 @@
+"""Writing a cache of keys and values and reading it back, bit for bit against the documented formula on the CPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kernelcode_generate_amd import native
+from tests.serving_util import HALF, LARGEST, f64, page_table, quantised
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+MODELS = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def cache_type(name, model):
+    return {"same": model, "int8": torch.int8, "e4m3": E4M3}[name]
+
+
+def empty_cache(pages, heads, page, d, dtype, device, fill=3):
+    caches = [torch.full((pages, heads, page, d), fill, dtype=torch.int8).to(dtype).to(device) for _ in range(2)]
+    scales = [torch.full((pages, heads, page), 7.0, device=device) if dtype in LARGEST else None for _ in range(2)]
+    return caches, scales
+
+
+def expected_store(caches, scales, rows, slots, page):
+    """The caches after the documented store, on the CPU."""
+
+    caches, scales = [c.cpu().clone() for c in caches], [None if s is None else s.cpu().clone() for s in scales]
+    for x in range(2):
+        codes, size = quantised(rows[x], caches[x].dtype) if scales[x] is not None else (rows[x].cpu(), None)
+        for t, slot in enumerate(slots.tolist()):
+            if not 0 <= slot < caches[x].shape[0] * page:
+                continue
+            caches[x].view(torch.uint8 if caches[x].dtype == E4M3 else caches[x].dtype)[slot // page, :, slot % page] = (
+                codes[t].view(torch.uint8) if caches[x].dtype == E4M3 else codes[t])
+            if size is not None:
+                scales[x][slot // page, :, slot % page] = size[t]
+    return caches, scales
+
+
+def same_bits(a, b):
+    wide = {1: torch.int8, 2: torch.int16, 4: torch.int32}[a.element_size()]
+    return torch.equal(a.cpu().contiguous().view(wide), b.cpu().contiguous().view(wide))
+
+
+@pytest.mark.parametrize("kind", ["same", "int8", "e4m3"])
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("tokens,heads,d,page", [(1, 1, 128, 16), (37, 3, 128, 16), (130, 8, 64, 64), (19, 2, 80, 24),
+                                                 (33, 1, 256, 1), (5, 2, 37, 5), (3, 2, 512, 16), (6, 5, 8, 7)])
+def test_store(device, tokens, heads, d, page, model, kind):
+    gen = torch.Generator().manual_seed(tokens * d)
+    dtype = cache_type(kind, model)
+    pages = -(-2 * tokens // page) + 1
+    caches, scales = empty_cache(pages, heads, page, d, dtype, device)
+    fused = (torch.randn(tokens, 2 * heads, d, generator=gen) * torch.exp(torch.randn(tokens, 2 * heads, 1, generator=gen))).to(model)
+    rows = [fused.to(device)[:, :heads], fused.to(device)[:, heads:]]  # strided, as one projection's output
+    slots = torch.randperm(pages * page, generator=gen)[:tokens]
+    slots[tokens // 2] = -1
+    want_caches, want_scales = expected_store(caches, scales, [fused[:, :heads], fused[:, heads:]], slots, page)
+    native.kv_cache_store(*caches, *scales, *rows, slots.to(device))
+    for x in range(2):
+        assert same_bits(caches[x], want_caches[x])
+        if scales[x] is not None:
+            assert same_bits(scales[x], want_scales[x])
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_a_code_is_the_nearest_one(device, kind):
+    """Against 64 bits: a code's value is within half a step of x. The step of e4m3 is 2^-3 of the power of two
+    below the value (2^-9 under 2^-6), of int8 one; the quotient's and the scale's rounding add 2^-22 of the value."""
+
+    gen = torch.Generator().manual_seed(4)
+    dtype, tokens, d = cache_type(kind, None), 64, 128
+    caches, scales = empty_cache(4, 1, 16, d, dtype, device)
+    x = torch.randn(tokens, 1, d, generator=gen) * torch.exp(3 * torch.randn(tokens, 1, d, generator=gen))
+    native.kv_cache_store(*caches, *scales, x.to(device), x.to(device), torch.arange(tokens).to(device))
+    size = f64(scales[0]).reshape(tokens, 1)
+    true = f64(x).reshape(tokens, d) / size
+    code = f64(caches[0]).reshape(tokens, d)
+    import numpy as np
+
+    half = 0.5 if kind == "int8" else np.exp2(np.maximum(np.floor(np.log2(np.maximum(np.abs(true), 1e-30))), -6) - 4)
+    assert (np.abs(true - code) <= half + 2.0**-22 * np.abs(true)).all()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("d", [128, 37])
+def test_store_of_zeros_small_rows_and_non_finite_rows(device, kind, d):
+    dtype = cache_type(kind, None)
+    x = torch.randn(8, 1, d, generator=torch.Generator().manual_seed(1))
+    x[0] = 0.0
+    x[1] *= 1e-38  # scales below the least normal value
+    x[2] *= 1e-43
+    x[3] = 2.0**-149
+    x[4] *= 1e37
+    x[5, 0, 3] = float("inf")
+    x[6, 0, 5] = float("nan")
+    x[7, 0, 1] = -float("inf")
+    caches, scales = empty_cache(1, 1, 8, d, dtype, device)
+    want, want_scales = expected_store(caches, scales, [x, x], torch.arange(8), 8)
+    native.kv_cache_store(*caches, *scales, x.to(device), x.to(device), torch.arange(8).to(device))
+    out = [torch.zeros(1, 1, 8, d, device=device) for _ in range(2)]
+    native.kv_cache_load(*out, *caches, *scales, torch.zeros(1, 1, dtype=torch.int32, device=device),
+                         torch.tensor([8], dtype=torch.int32, device=device))
+    assert same_bits(caches[0][:, :, :5], want[0][:, :, :5]) and same_bits(scales[0][:, :, :5], want_scales[0][:, :, :5])
+    assert torch.isfinite(out[0][0, 0, :5]).all() and not out[0][0, 0, 0].any()
+    assert torch.isnan(out[0][0, 0, 5:]).all() and torch.isnan(out[1][0, 0, 5:]).all()
+
+
+@pytest.mark.parametrize("d", [128, 20])
+def test_slots_out_of_range_write_nothing(device, d):
+    caches, scales = empty_cache(3, 2, 16, d, E4M3, device)
+    before = [c.clone() for c in (*caches, *scales)]
+    slots = torch.tensor([-1, 48, -(2**62), 2**62, 2**32, 2**32 + 5, 2**31], dtype=torch.int64, device=device)
+    rows = torch.randn(7, 2, d, device=device)
+    native.kv_cache_store(*caches, *scales, rows, rows, slots)
+    for a, b in zip((*caches, *scales), before):
+        assert same_bits(a, b)
+
+
+def test_store_through_strides(device):
+    """Caches [pages, page_size, heads, D] seen as the entry's layout, every second slot of a list."""
+
+    gen = torch.Generator().manual_seed(2)
+    base = [torch.zeros(4, 16, 3, 128, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    caches = [b.transpose(1, 2) for b in base]
+    rows = torch.randn(9, 3, 128, generator=gen).to(torch.bfloat16).to(device)
+    slots = torch.randperm(64, generator=gen).to(device)[:18][::2]
+    native.kv_cache_store(*caches, None, None, rows, rows, slots)
+    want, _ = expected_store([c.contiguous() * 0 for c in caches], [None, None], [rows, rows], slots, 16)
+    assert same_bits(caches[0], want[0]) and same_bits(caches[1], want[1])
+
+
+@pytest.mark.parametrize("kind", ["same", "int8", "e4m3"])
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("lengths,heads,d,page,reach", [([1], 1, 128, 16, 1), ([40, 0, 7, 133], 3, 128, 16, 140), ([100], 2, 64, 64, 77),
+                                                        ([33, 50], 2, 80, 24, 50), ([5, 2], 1, 256, 1, 6), ([9, 30], 2, 37, 5, 30)])
+def test_load(device, lengths, heads, d, page, reach, model, kind):
+    gen = torch.Generator().manual_seed(sum(lengths) * d)
+    dtype = cache_type(kind, model)
+    pages = sum(-(-n // page) for n in lengths) + 2
+    x = torch.randn(pages, heads, page, d, generator=gen).to(model)
+    codes, scale = quantised(x, dtype) if kind != "same" else (x, None)
+    table = page_table(lengths, page, pages, gen)
+    outs = [torch.full((len(lengths), heads, reach, d), 5.0, dtype=model, device=device) for _ in range(2)]
+    dev = [t if t is None else t.to(device) for t in (codes, codes, scale, scale)]
+    native.kv_cache_load(*outs, *dev, table.to(device), torch.tensor(lengths, dtype=torch.int32, device=device))
+    values = codes if scale is None else codes.float() * scale[..., None]
+    want = torch.full((len(lengths), heads, reach, d), 5.0, dtype=model)
+    for b, n in enumerate(lengths):
+        for i in range(min(n, reach)):
+            want[b, :, i] = values[table[b, i // page], :, i % page].to(model)
+    assert same_bits(outs[0], want) and same_bits(outs[1], want)
+
+
+def test_load_leaves_what_has_no_page(device):
+    """Lengths past the table's reach or the output's rows, pages that do not exist, negative lengths; outputs
+    as a strided view."""
+
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(4, 2, 16, 64, generator=gen).to(torch.float16).to(device)
+    table = torch.tensor([[1, 2], [-1, 3], [4, 0], [1, 2**31 - 1], [0, 1]], dtype=torch.int32, device=device)
+    lens = torch.tensor([99, 32, 32, 32, -5], dtype=torch.int32, device=device)
+    base = torch.full((5, 40, 2, 64), 5.0, dtype=torch.float16, device=device)
+    outs = [base.transpose(1, 2), base.clone().transpose(1, 2)]
+    native.kv_cache_load(*outs, x, x, None, None, table, lens)
+    want = torch.full((5, 2, 40, 64), 5.0, dtype=torch.float16, device=device)
+    want[0, :, :16], want[0, :, 16:32], want[1, :, 16:32], want[2, :, 16:32], want[3, :, :16] = x[1], x[2], x[3], x[0], x[1]
+    assert same_bits(outs[0], want) and same_bits(outs[1], want)
+
+
+def test_a_row_read_back_is_within_half_a_step(device):
+    """Store and load in turn: |back - x| is at most half a code's step, plus the output's rounding."""
+
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(50, 2, 128, generator=gen).to(torch.bfloat16).to(device)
+    slots = torch.randperm(64, generator=gen)[:50]
+    for dtype, relative, absolute in ((E4M3, 2.0**-4, 2.0**-10), (torch.int8, 0.0, 0.5)):
+        caches, scales = empty_cache(64, 2, 1, 128, dtype, device)
+        native.kv_cache_store(*caches, *scales, x, x, slots.to(device))
+        outs = [torch.zeros(1, 2, 50, 128, dtype=torch.bfloat16, device=device) for _ in range(2)]
+        native.kv_cache_load(*outs, *caches, *scales, slots.to(torch.int32).to(device)[None],
+                             torch.tensor([50], dtype=torch.int32, device=device))
+        true, back = f64(x).transpose(1, 0, 2), f64(outs[1])[0]
+        size = abs(true).max(-1, keepdims=True) / LARGEST[dtype]
+        bound = relative * abs(true) + absolute * size
+        assert (abs(back - true) <= bound + HALF[torch.bfloat16] * (abs(true) + bound)).all()
+
+
+def test_empty_calls(device):
+    z = dict(dtype=torch.bfloat16, device=device)
+    caches = [torch.zeros(2, 1, 16, 64, **z) for _ in range(2)]
+    none = torch.zeros(0, 1, 64, **z)
+    native.kv_cache_store(*caches, None, None, none, none, torch.zeros(0, dtype=torch.int64, device=device))
+    out = torch.zeros(0, 1, 5, 64, **z)
+    native.kv_cache_load(out, out, *caches, None, None, torch.zeros(0, 1, dtype=torch.int32, device=device),
+                         torch.zeros(0, dtype=torch.int32, device=device))
+    out = torch.ones(1, 1, 5, 64, **z)
+    native.kv_cache_load(out, out.clone(), *caches, None, None, torch.zeros(1, 0, dtype=torch.int32, device=device),
+                         torch.ones(1, dtype=torch.int32, device=device))
+    assert (out == 1).all()
