@@ -1,0 +1,707 @@
+// Attention over a paged cache (tree_attn.h) for few rows per request and key head: decoding steps and small
+// trees. A row is a (token, query head) of the key head's group, so a step of four query heads per key
+// head fills a quarter of a 16-row matrix block and reads each key once for all four.
+//
+// Such a call is bound by reading keys and values. As in flash_attn_decode.h each of a workgroup's four waves
+// walks its own steps of 32 or 64 keys with its own running maximum and sums: S^T = K Q^T (v_mfma_f32_16x16x32, operand A 16 keys x 32 d from K's rows,
+// operand B up to two blocks of 16 rows), P in registers straight to O^T += V^T P^T, no LDS until the end.
+//
+// Work is shared out in rounds (one step of each wave) of all requests, heads and blocks of rows in one line, an
+// equal range of it to each workgroup whatever the requests' lengths, which only the device knows: each
+// workgroup sums the requests' rounds by itself. A range that covers an item (request, head, block of rows) writes
+// its rows; others leave O, maximum and sum in 32 bits, and tree_attn_join_kernel joins them in
+// the order of the ranges.
+//
+// 8-bit caches: codes are widened to 16 bits (exact for both types) for the products; a key's scale multiplies
+// its scores, a value's its weights. Weights are rounded to 16 bits with that scale in them, so the running
+// maximum is of s + log2(value's scale): weights of at most 1, whatever the scales' sizes. The sum of weights stays in 32 bits.
+//
+// Weights of 16-bit caches are rounded to 16 bits, as in the flash attention kernels, and summed as rounded.
+#pragma once
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "common.h"
+#include "flash_attn_mfma.h"
+#include "kv_cache.h"
+#include "lds_dma.h"  // Int
+#include "tree_attn.h"
+
+namespace kg_gfx950 {
+
+namespace treer {
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr float kMinMax = -3.0e38f;  // the lowest running maximum: scores of -inf weigh nothing beside it
+// keys of a wave's step: 16 KiB of K and V rows, or what the registers hold (8 KiB of 8-bit heads of 64,
+// and of 128 with two blocks of rows; 32 KiB of 16-bit heads of 256)
+template <typename C, int D, int kNQ>
+constexpr int step_keys() { return (sizeof(C) == 2 && D >= 128) || D == 256 || (D == 128 && kNQ == 2) ? 32 : 64; }
+
+// A 16-bit pair of two 8-bit codes.
+template <typename Tag, typename C>
+struct Widen;
+template <>
+struct Widen<Bf16Tag, E4m3> {
+  template <bool kHigh>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHigh));
+  }
+};
+template <>
+struct Widen<F16Tag, E4m3> {
+  template <bool kHigh>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHigh));
+  }
+};
+template <typename Tag>
+struct Widen<Tag, int8_t> {
+  template <bool kHigh>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    const int a = (int)(w << (kHigh ? 8 : 24)) >> 24, b = (int)(w << (kHigh ? 0 : 16)) >> 24;
+    return Half16<Tag>::pack2((float)a, (float)b);
+  }
+};
+// 8 codes to 8 16-bit elements
+template <typename Tag, typename C>
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
+  using W = Widen<Tag, C>;
+  return u32x4{W::template pair<false>(lo), W::template pair<true>(lo), W::template pair<false>(hi), W::template pair<true>(hi)};
+}
+
+// a lane's columns of a V row
+template <int kDwords, typename C>
+__device__ __forceinline__ void load_v(uint32_t (&v)[kDwords], const C* p) {
+  if constexpr (kDwords == 1) {
+    v[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (kDwords == 2) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    v[0] = x[0], v[1] = x[1];
+  } else {
+#pragma unroll
+    for (int q = 0; q < kDwords; q += 4) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p) + 4 * q);
+      v[q] = x[0], v[q + 1] = x[1], v[q + 2] = x[2], v[q + 3] = x[3];
+    }
+  }
+}
+
+template <typename C>
+constexpr bool kScaled = CacheElem<C>::kScaled;
+template <>
+inline constexpr bool kScaled<uint16_t> = false;
+}  // namespace treer
+
+// A workgroup's share of the work: `units` of request b are its items times their rounds.
+struct TreeShare {
+  int first, last;  // [first, last) of all units
+  int b, base;      // the request that `first` lies in, and the units before it
+  int total;
+};
+struct TreeSplit {
+  int grid;       // workgroups the units are shared among
+  int block;      // rows of an item
+  int round;      // keys of a round; 0: items are not split, a unit is an item
+  float* partial; // 2 grid records of `block` rows x (width + 2): O, maximum (log2 units), sum
+  int width;
+};
+__device__ __forceinline__ int tree_rounds(const TreeRequest& r, int round) {
+  return round == 0 ? 1 : max((r.keys + round - 1) / round, 1);
+}
+__device__ __forceinline__ int tree_blocks(const TreeRequest& r, int group, int block) {
+  return (r.count * group + block - 1) / block;
+}
+__device__ __forceinline__ int tree_units(const TreeArgs& a, const TreeSplit& s, int b) {
+  if (b >= a.batch) return 0;
+  const TreeRequest r = tree_request(a, b);
+  return r.count == 0 ? 0 : a.heads * tree_blocks(r, a.group, s.block) * tree_rounds(r, s.round);
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(v, o, 64);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+// Workgroup w of those that have work takes the units from bound(w) up to bound(w + 1), at least one.
+__device__ __forceinline__ int share_bound(int w, const TreeSplit& s, int total) {
+  const int grid = min(s.grid, total);
+  return w >= grid ? total : (int)((long long)w * total / grid);
+}
+
+__device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, const TreeSplit& s, int w) {
+  const int lane = threadIdx.x & 63;
+  TreeShare t;
+  t.total = 0;
+  const int mine = tree_units(a, s, lane);
+  const int upto = wave_scan(mine, lane);
+  t.total = __builtin_amdgcn_readlane(upto, 63);
+  for (int b0 = 64; b0 < a.batch; b0 += 64)
+    t.total += __builtin_amdgcn_readlane(wave_scan(tree_units(a, s, b0 + lane), lane), 63);
+  t.first = share_bound(w, s, t.total);
+  t.last = share_bound(w + 1, s, t.total);
+  // the first request that ends behind `first`
+  t.b = a.batch;
+  t.base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int own = b0 == 0 ? mine : tree_units(a, s, b0 + lane);
+    const int end = t.base + (b0 == 0 ? upto : wave_scan(own, lane));
+    const unsigned long long behind = __builtin_amdgcn_ballot_w64(end > t.first);
+    if (behind != 0) {
+      const int x = __builtin_ctzll(behind);
+      t.b = b0 + x;
+      t.base = __builtin_amdgcn_readlane(end, x) - __builtin_amdgcn_readlane(own, x);
+      break;
+    }
+    t.base = __builtin_amdgcn_readlane(end, 63);
+  }
+  return t;
+}
+
+// C: uint16_t (elements of Tag), E4m3 or int8_t. D: 64, 128 or 256, heads of d <= D elements, d % 16 == 0. kNQ: blocks of 16
+// rows. kPage16: pages of a multiple of 16 tokens, so that 16 keys share one.
+template <typename Tag, typename C, int D, int kNQ, bool kPage16>
+__global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_rows_kernel(TreeArgs a, TreeSplit split) {
+  using namespace treer;
+  using H = Half16<Tag>;
+  constexpr bool kS = kScaled<C>;
+  constexpr int kES = sizeof(C);
+  constexpr int kStep = step_keys<C, D, kNQ>();
+  constexpr int NC = kStep / 32, NKB = kStep / 16;  // chunks of 32, blocks of 16 keys
+  constexpr int NDS = D / 32;                       // 32-deep steps of S^T
+  constexpr int NE = D / 16;                        // columns of V per lane, blocks of O^T
+  constexpr int kRows = 16 * kNQ;
+  constexpr int NKW = kS ? D / 64 : NDS;            // 16-byte pieces of a K row per lane
+  constexpr int NVW = NE * kES / 4;                 // dwords of a V row per lane
+  __shared__ float o_lds[kWaves][kRows][D];
+  __shared__ float ml_lds[kWaves][kRows][2];
+  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? kWaves : 1][2][kStep];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, lr = lane >> 4;
+
+  TreeShare share = tree_share(a, split, blockIdx.x);
+  const int own_first = share.first;
+
+  while (share.first < share.last && share.b < a.batch) {
+    const TreeRequest r = tree_request(a, share.b);
+    const int rounds = tree_rounds(r, split.round), blocks = tree_blocks(r, a.group, kRows);
+    const int units = r.count == 0 ? 0 : a.heads * blocks * rounds;
+    const int local = share.first - share.base;
+    if (local >= units) {
+      share.base += units;
+      ++share.b;
+      continue;
+    }
+    const int item = local / rounds, round0 = local - item * rounds;
+    const int round1 = min(rounds, round0 + share.last - share.first);
+    const int h = item / blocks, row0 = (item - h * blocks) * kRows;
+    const bool whole_item = round0 == 0 && round1 == rounds;
+    const int item_rows = min(r.count * a.group - row0, kRows);
+    const bool starts_here = share.first == own_first;
+    share.first += round1 - round0;
+
+    // keys of this range; of a chain only those that its last token sees
+    constexpr int kRound = kStep * kWaves;
+    int key_lo = split.round == 0 ? 0 : round0 * kRound;
+    int key_hi = split.round == 0 ? r.keys : min(r.keys, round1 * kRound);
+    if (a.words < 0) key_hi = (int)min((long long)key_hi, (long long)r.context + (row0 + item_rows - 1) / a.group + 1);
+    key_lo = __builtin_amdgcn_readfirstlane(key_lo);
+    key_hi = __builtin_amdgcn_readfirstlane(key_hi);
+
+    // this lane's rows: token of the request and query head
+    int tok[kNQ];
+    unsigned long long first_word[kNQ];  // of the token's mask
+    u32x4 qf[kNQ][NDS];
+#pragma unroll
+    for (int x = 0; x < kNQ; ++x) {
+      const int row = row0 + 16 * x + l16;
+      tok[x] = row / a.group;
+      const bool real = 16 * x + l16 < item_rows;
+      first_word[x] = real && a.words > 0 ? (unsigned long long)a.mask[(long long)(r.first + tok[x]) * a.mask_0] : 0ull;
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + (real ? r.first + tok[x] : 0) * a.q_token +
+                          ((long long)h * a.group + (row - tok[x] * a.group)) * a.q_head;
+#pragma unroll
+      for (int s = 0; s < NDS; ++s) {
+        // 8-bit rows: 16 bytes of a lane are the 8 d of two steps
+        const int d = kS ? 64 * (s >> 1) + 16 * lr + 8 * (s & 1) : 32 * s + 8 * lr;
+        qf[x][s] = real && d < a.d ? ld16(q + d) : u32x4{0, 0, 0, 0};
+      }
+    }
+    const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
+    const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
+    const int* table = a.table + share.b * a.table_0;
+
+    // Page of key `lane` of a step (-1: none, or a key past the range) and its offset there.
+    struct Place {
+      int page, offset;
+    };
+    auto place = [&](int key0) __attribute__((always_inline)) {
+      const int key = key0 + (lane & (kStep - 1));
+      Place p = {-1, 0};
+      if (key < key_hi) {
+        const int n = div_page(key, a.div);
+        p.page = table[n * a.table_1];
+        p.offset = key - n * a.page_size;
+      }
+      return p;
+    };
+    auto checked = [&](Place p) __attribute__((always_inline)) {
+      const bool there = p.page >= 0 && p.page < a.pages;
+      return Place{there ? p.page : -1, there ? p.offset : 0};
+    };
+
+    // Rows of a step. What is not there is read from page 0 instead, whose rows exist, and dropped later.
+    u32x4 k[NKB][NKW];
+    uint32_t v[NC][8][NVW];
+    float ks = 0.f, vs = 0.f;  // of key `lane` of the step
+    auto load_k = [&](const Place& p) __attribute__((always_inline)) {
+      if constexpr (kS) {
+        ks = a.k_scale[(long long)max(p.page, 0) * a.ks_page + h * a.ks_head + (long long)p.offset * a.ks_row];
+        vs = a.v_scale[(long long)max(p.page, 0) * a.vs_page + h * a.vs_head + (long long)p.offset * a.vs_row];
+      }
+      // (a lane's d past the head's end: its first ones)
+      auto piece = [&](const C* row, int kb, int s) __attribute__((always_inline)) {
+        const int d = (kS ? 16 : 8) * lr + (kS ? 64 : 32) * s;
+        k[kb][s] = ld16(row + (d < a.d ? d : 0));
+      };
+      if constexpr (kPage16) {
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {  // 16 keys on one page
+          const int page = __builtin_amdgcn_readlane(p.page, 16 * kb), offset = __builtin_amdgcn_readlane(p.offset, 16 * kb);
+          const C* row = kc + ((long long)max(page, 0) * a.k_page + (long long)offset * a.k_row);
+#pragma unroll
+          for (int s = 0; s < NKW; ++s) piece(row + (uint32_t)(l16 * (int)a.k_row), kb, s);
+        }
+      } else {  // each lane's own row, handed to the lanes that read it
+        const long long at = (long long)max(p.page, 0) * a.k_page + (long long)p.offset * a.k_row;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+          const C* row = kc + __shfl(at, 16 * kb + l16, 64);
+#pragma unroll
+          for (int s = 0; s < NKW; ++s) piece(row, kb, s);
+        }
+      }
+    };
+    const int v_col = NE * l16 < a.d ? NE * l16 : 0;
+    auto load_v_rows = [&](const Place& p) __attribute__((always_inline)) {
+      if constexpr (kPage16) {
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+          const int page = __builtin_amdgcn_readlane(p.page, 16 * kb), offset = __builtin_amdgcn_readlane(p.offset, 16 * kb);
+          const C* row = vc + ((long long)max(page, 0) * a.v_page + (long long)offset * a.v_row);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            load_v(v[kb >> 1][(kb & 1) * 4 + x], row + (uint32_t)((4 * lr + x) * (int)a.v_row + v_col));
+        }
+      } else {
+        const long long at = (long long)max(p.page, 0) * a.v_page + (long long)p.offset * a.v_row;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            load_v(v[kb >> 1][(kb & 1) * 4 + x], vc + __shfl(at, 16 * kb + 4 * lr + x, 64) + v_col);
+      }
+    };
+
+    f32x4 o[kNQ][NE];
+    f32x4 l_run[kNQ];  // scaled caches: element 0, this lane's keys alone
+    float m_run[kNQ];
+#pragma unroll
+    for (int x = 0; x < kNQ; ++x) {
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      l_run[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[x] = kMinMax;
+    }
+    const u32x4 ones = {H::kOnePair, H::kOnePair, H::kOnePair, H::kOnePair};
+
+    // This wave's steps: key_lo + kStep (wave + 4 i). A step reads its rows and waits for them; eight to twelve waves of a CU
+    // keep it reading (kept across steps, the rows took twice the registers in copies). The next step's pages are
+    // looked up ahead of the rows, since loads return in order.
+    constexpr int kStride = kStep * kWaves;
+    int key = key_lo + kStep * wave;
+    Place p = checked(place(key));
+    // One step. plain: one of the context, every key of it there; `there`: bits of those that are.
+    auto step = [&](auto plain_tag, unsigned long long there) __attribute__((always_inline)) {
+      constexpr bool kPlain = decltype(plain_tag)::value != 0;
+      const Place next = place(key + kStride);
+      load_k(p);
+      load_v_rows(p);
+      // ---- scores in log2 units; lane: row l16, keys 16 kb + 4 lr + i ----
+      if (a.d != D) {
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int s = 0; s < NKW; ++s)
+            if ((kS ? 16 : 8) * lr + (kS ? 64 : 32) * s >= a.d) k[kb][s] = u32x4{0, 0, 0, 0};
+      }
+      f32x4 sc[kNQ][NKB];
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x) sc[x][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NDS; ++s) {
+          u32x4 kf;
+          if constexpr (kS) kf = widen8<Tag, C>(k[kb][s >> 1][(s & 1) * 2], k[kb][s >> 1][(s & 1) * 2 + 1]);
+          else kf = k[kb][s];
+#pragma unroll
+          for (int x = 0; x < kNQ; ++x) sc[x][kb] = H::mfma16(kf, qf[x][s], sc[x][kb]);
+        }
+      }
+      if constexpr (kS) {
+        sc_lds[wave][0][lane & (kStep - 1)] = ks * a.scale_log2;
+        // (a NaN passes; a scale of 0 has codes of 0, so any weight does)
+        sc_lds[wave][1][lane & (kStep - 1)] = __builtin_amdgcn_logf(nan_max(vs, 0x1p-100f));
+      }
+      f32x4 lv[kS ? NKB : 1];
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        f32x4 f = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+        if constexpr (kS) {
+          f = *reinterpret_cast<const f32x4*>(&sc_lds[wave][0][16 * kb + 4 * lr]);
+          lv[kb] = *reinterpret_cast<const f32x4*>(&sc_lds[wave][1][16 * kb + 4 * lr]);
+        }
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[x][kb][i] *= f[i];
+      }
+      // ---- what is not seen ----
+      const uint32_t there_lo = (uint32_t)(there >> (4 * lr)), there_hi = (uint32_t)(there >> 32 >> (4 * lr));
+      uint32_t seen[kNQ];  // bit 4 kb + i: this lane's row sees its key
+      if constexpr (!kPlain) {
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x) {
+          seen[x] = 0;
+#pragma unroll 1
+          for (int n = 0; n < 4 * NKB; ++n) {
+            const int in_step = 16 * (n >> 2) + (n & 3), draft = key + 4 * lr + in_step - r.context;
+            bool s = ((in_step < 32 ? there_lo : there_hi) >> (in_step & 31) & 1u) != 0;
+            if (s && draft >= 0) {
+              if (a.words < 0) s = draft <= tok[x];
+              else if (draft < 64) s = (first_word[x] >> draft & 1ull) != 0;
+              else s = 16 * x + l16 < item_rows && tree_sees(a, r.first + tok[x], tok[x], draft);
+            }
+            seen[x] |= (s ? 1u : 0u) << n;
+          }
+#pragma unroll
+          for (int n = 0; n < 4 * NKB; ++n)
+            if (!(seen[x] >> n & 1u)) sc[x][n >> 2][n & 3] = -INFINITY;
+        }
+      }
+      // ---- weights: keys 32 c + 4 lr + 0..3, then + 16 ----
+      u32x4 pp[kNQ][NC];
+#pragma unroll
+      for (int x = 0; x < kNQ; ++x) {
+        auto weighed = [&](int n) __attribute__((always_inline)) {
+          if constexpr (kS) {  // (a scale of a key that is not seen may be anything)
+            const float s = (float)sc[x][n >> 2][n & 3] + (float)lv[n >> 2][n & 3];
+            return kPlain || (seen[x] >> n & 1u) ? s : -INFINITY;
+          } else return (float)sc[x][n >> 2][n & 3];
+        };
+        float mx = weighed(0);
+#pragma unroll
+        for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(n));
+        float mx2 = mx;
+        fa::rows4_combine<true>(mx, mx2);
+        const float m_new = nan_max(m_run[x], mx);
+        if (__builtin_amdgcn_ballot_w64(m_new > m_run[x] || m_new != m_new)) {
+          const float alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
+          m_run[x] = m_new;
+          l_run[x] *= alpha;
+#pragma unroll
+          for (int e = 0; e < NE; ++e) o[x][e] *= alpha;
+        }
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run[x]);
+            if constexpr (kS) l_run[x][0] += __builtin_amdgcn_exp2f((float)sc[x][kb][i] - m_run[x]);
+          }
+          pp[x][kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
+          pp[x][kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);
+        }
+        if constexpr (!kS) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) l_run[x] = H::mfma16(ones, pp[x][c], l_run[x]);
+        }
+      }
+      // ---- O^T += V^T P^T ----
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        uint32_t row16[8][NE / 2];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+#pragma unroll
+          for (int q = 0; q < NE / 2; ++q) {
+            if constexpr (kS)
+              row16[n][q] = (q & 1) ? Widen<Tag, C>::template pair<true>(v[c][n][q >> 1])
+                                    : Widen<Tag, C>::template pair<false>(v[c][n][q >> 1]);
+            else row16[n][q] = v[c][n][q];
+          }
+          if constexpr (!kPlain) {
+            const int in_step = 32 * c + (n < 4 ? n : 12 + n);
+            if (!((in_step < 32 ? there_lo : there_hi) >> (in_step & 31) & 1u)) {
+#pragma unroll
+              for (int q = 0; q < NE / 2; ++q) row16[n][q] = 0;
+            }
+          }
+        }
+        // Column e of this lane's 8 rows; low, high: v_perm_b32 bytes of the low or the high halves of two dwords.
+        constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
+        auto column = [&](int e, uint32_t low, uint32_t high) __attribute__((always_inline)) {
+          u32x4 vt;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            vt[q] = __builtin_amdgcn_perm(row16[2 * q + 1][e >> 1], row16[2 * q][e >> 1], (e & 1) ? high : low);
+          return vt;
+        };
+        // A weight of 0 does not take an infinity or NaN out of a sum: where a step that some rows do not see in
+        // full holds one, every row gets a pass of its own with zeros in place of the keys that it does not see.
+        bool apart = false;
+        if constexpr (!kPlain) {
+          uint32_t carry = 0;  // an exponent of ones carries into its sign bit
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int q = 0; q < NE / 2; ++q) carry |= (row16[n][q] & H::kExpPair) + H::kExpUnitPair;
+          apart = __builtin_amdgcn_ballot_w64((carry & 0x80008000u) != 0) != 0;
+        }
+        if (!apart) {
+#pragma unroll
+          for (int e = 0; e < NE; ++e) {
+            const u32x4 vt = column(e, kLow, kHigh);
+#pragma unroll
+            for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vt, pp[x][c], o[x][e]);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < kNQ; ++x)
+#pragma unroll 1
+            for (int q = 0; q < 16; ++q) {
+              // (opaque: all columns, kept in registers across this loop, cost the common path as many)
+              uint32_t low = kLow, high = kHigh;
+              asm volatile("" : "+s"(low), "+s"(high));
+              // row q's bits of the keys whose values this lane holds
+              const uint32_t bits = (uint32_t)__shfl((int)seen[x], (lane & 48) + q, 64) >> (8 * c);
+              u32x4 mask;
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                mask[y] = (bits >> (2 * y) & 1u ? 0xffffu : 0u) | (bits >> (2 * y + 1) & 1u ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int e = 0; e < NE; ++e) {
+                const f32x4 sum = H::mfma16(column(e, low, high) & mask, pp[x][c], o[x][e]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[x][e][i] = l16 == q ? (float)sum[i] : (float)o[x][e][i];
+                __builtin_amdgcn_sched_barrier(0);
+              }
+            }
+        }
+      }
+      p = checked(next);
+      key += kStride;
+    };
+    // Steps of the context whose keys are all there; from the first other one on
+    // (drafted tokens, the range's end, pages that do not exist) a loop that looks at each key.
+    unsigned long long there = 0;
+#pragma unroll 1
+    for (;;) {
+      there = __builtin_amdgcn_ballot_w64(p.page >= 0);
+      if (~there != 0 || key + kStep > r.context) break;
+      step(Int<1>{}, there);
+    }
+#pragma unroll 1
+    while (key < key_hi) {
+      step(Int<0>{}, there);
+      there = __builtin_amdgcn_ballot_w64(p.page >= 0);
+    }
+
+    // ---- join the waves ----
+#pragma unroll
+    for (int x = 0; x < kNQ; ++x) {
+      if constexpr (kS) {
+        float l0 = l_run[x][0], l1 = l0;
+        fa::rows4_combine<false>(l0, l1);
+        l_run[x][0] = l0;
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o_lds[wave][16 * x + l16][NE * (4 * lr + i) + e] = o[x][e][i];
+      if (lr == 0) {
+        ml_lds[wave][16 * x + l16][0] = m_run[x];
+        ml_lds[wave][16 * x + l16][1] = l_run[x][0];
+      }
+    }
+    __syncthreads();
+    float* record = split.partial + ((long long)2 * blockIdx.x + (starts_here ? 0 : 1)) * kRows * (D + 2);
+    for (int y = tid; y < item_rows * (D / 2); y += kThreads) {
+      const int n = y / (D / 2), d = 2 * (y - n * (D / 2));
+      if (d >= a.d) continue;
+      float m = ml_lds[0][n][0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) m = nan_max(m, ml_lds[w][n][0]);
+      float l = 0.f, v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ml_lds[w][n][0] - m);
+        l += f * ml_lds[w][n][1];
+        v0 += f * o_lds[w][n][d];
+        v1 += f * o_lds[w][n][d + 1];
+      }
+      if (whole_item) {
+        const int row = row0 + n, token = row / a.group;
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + (r.first + token) * a.o_token +
+                        ((long long)h * a.group + (row - token * a.group)) * a.o_head + d;
+        *reinterpret_cast<uint32_t*>(out) = H::pack2(l != 0.f ? v0 * inv : 0.f, l != 0.f ? v1 * inv : 0.f);
+      } else {
+        float* p = record + (long long)n * (D + 2);
+        *reinterpret_cast<f32x2*>(p + d) = f32x2{v0, v1};
+        if (d == 0) *reinterpret_cast<f32x2*>(p + D) = f32x2{m, l};
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// One wave per (token, query head): the records of its item joined, where several ranges share it.
+template <typename Tag, int D>
+__global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs a, TreeSplit split) {
+  const int lane = threadIdx.x & 63;
+  const long long id = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= (long long)a.tokens * a.heads_q) return;
+  const int t = (int)(id / a.heads_q), hq = (int)(id - (long long)t * a.heads_q);
+  // its request (the last one that starts at or before it), the units before that, and all units
+  int owner = -1, base = 0, total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    const unsigned long long at = __builtin_amdgcn_ballot_w64(b < a.batch && a.starts[b * a.start_stride] <= t);
+    const int upto = wave_scan(tree_units(a, split, b), lane);
+    if (at != 0) {
+      const int x = 63 - __builtin_clzll(at);
+      owner = b0 + x;
+      base = total + (x > 0 ? __builtin_amdgcn_readlane(upto, x - 1) : 0);
+    }
+    total += __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (owner < 0) return;
+  const TreeRequest r = tree_request(a, owner);
+  const int j = t - r.first;
+  if (j < 0 || j >= r.count) return;
+  const int h = hq / a.group, row = j * a.group + (hq - h * a.group);
+  const int rounds = tree_rounds(r, split.round), blocks = tree_blocks(r, a.group, split.block);
+  const int begin = base + (h * blocks + row / split.block) * rounds, end = begin + rounds;
+  // the workgroup whose range holds unit u
+  const int grid = min(split.grid, total);
+  auto holder = [&](int u) { return (int)((((long long)u + 1) * grid - 1) / total); };
+  const int w0 = max(holder(begin), 0), w1 = min(holder(end - 1), grid - 1);
+  if (w0 >= w1) return;  // one range: the row is written
+  auto record = [&](int w) {
+    const int slot = 2 * w + (share_bound(w, split, total) >= begin ? 0 : 1);
+    return split.partial + ((long long)slot * split.block + row % split.block) * (D + 2);
+  };
+  constexpr int NE = D / 64;
+  float m = treer::kMinMax;
+  for (int w = w0 + lane; w <= w1; w += 64) m = nan_max(m, record(w)[D]);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) m = nan_max(m, __shfl_xor(m, s, 64));
+  float l = 0.f, o[NE];
+#pragma unroll
+  for (int e = 0; e < NE; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int w = w0; w <= w1; ++w) {
+    const float* p = record(w);
+    const float f = __builtin_amdgcn_exp2f(p[D] - m);
+    l += f * p[D + 1];
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+      if (lane + 64 * e < a.d) o[e] += f * p[lane + 64 * e];
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.o_token + hq * a.o_head;
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+    if (lane + 64 * e < a.d) out[lane + 64 * e] = (uint16_t)(Half16<Tag>::pack2(l != 0.f ? o[e] * inv : 0.f, 0.f) & 0xffffu);
+}
+
+// ---- host ----
+
+// What the kernel takes: 16-bit queries, heads of a multiple of 16 up to 256, rows of 16-byte pieces.
+inline bool tree_rows_takes(const TreeArgs& a, int cache_bytes) {
+  auto whole = [&](const void* p, std::initializer_list<long long> strides, int bytes, int unit) {
+    bool ok = (uintptr_t)p % unit == 0;
+    for (long long s : strides) ok = ok && s * bytes % unit == 0;
+    return ok;
+  };
+  return a.d % 16 == 0 && a.d <= 256 && whole(a.q, {a.q_token, a.q_head}, 2, 16) && whole(a.out, {a.o_token, a.o_head}, 2, 4) &&
+         whole(a.k, {a.k_page, a.k_head, a.k_row}, cache_bytes, 16) && whole(a.v, {a.v_page, a.v_head, a.v_row}, cache_bytes, 16) &&
+         a.k_row <= 1 << 24 && a.v_row <= 1 << 24 && a.pages > 0;
+}
+
+// Shares of a call: as many workgroups as run at once, or as there can be units (the table's reach bounds a
+// request's keys, the batch's tokens its blocks of rows).
+struct TreePlan {
+  int width, blocks16;  // padded head, 16-row blocks of an item
+  TreeSplit split;
+  bool join;
+  size_t bytes;
+};
+inline TreePlan tree_rows_plan(const TreeArgs& a, int cache_bytes, bool may_split) {
+  TreePlan p;
+  p.width = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
+  const long long rows = ((long long)a.tokens + a.batch - 1) / a.batch * a.group;  // of a request and key head, on average
+  p.blocks16 = rows <= 16 || p.width == 256 || a.page_size % 16 != 0 ? 1 : 2;
+  p.split.block = 16 * p.blocks16;
+  p.split.width = p.width;
+  const int step = (cache_bytes == 2 && p.width >= 128) || p.width == 256 || (p.width == 128 && p.blocks16 == 2) ? 32 : 64;
+  const long long round = (long long)step * treer::kWaves, reach = (long long)a.per * a.page_size;
+  const long long items = a.heads * ((long long)a.tokens * a.group / p.split.block + a.batch);
+  const long long units = items * std::max(1ll, (reach + round - 1) / round);
+  may_split = may_split && reach > round && units < 0x7fffffffLL;
+  p.split.round = may_split ? (int)round : 0;
+  p.split.grid = (int)std::min<long long>(may_split ? units : items, p.width == 256 ? 256 : 512);
+  p.join = may_split;
+  p.split.partial = nullptr;
+  p.bytes = may_split ? (size_t)2 * p.split.grid * p.split.block * (p.width + 2) * sizeof(float) : 0;
+  return p;
+}
+
+template <typename Tag, typename C>
+hipError_t launch_tree_rows(const TreeArgs& a, const TreePlan& p, hipStream_t stream) {
+#define KG_TREE_ROWS(WIDTH, NQ, PAGE16)                                                                                  \
+  hipLaunchKernelGGL((tree_attn_rows_kernel<Tag, C, WIDTH, NQ, PAGE16>), dim3(p.split.grid), dim3(treer::kThreads), 0, stream, \
+                     a, p.split)
+  const bool page16 = a.page_size % 16 == 0;
+  if (p.width == 256) {
+    if (page16) KG_TREE_ROWS(256, 1, true);
+    else KG_TREE_ROWS(256, 1, false);
+  } else if (p.width == 128) {
+    if (!page16) KG_TREE_ROWS(128, 1, false);
+    else if (p.blocks16 == 1) KG_TREE_ROWS(128, 1, true);
+    else KG_TREE_ROWS(128, 2, true);
+  } else {
+    if (!page16) KG_TREE_ROWS(64, 1, false);
+    else if (p.blocks16 == 1) KG_TREE_ROWS(64, 1, true);
+    else KG_TREE_ROWS(64, 2, true);
+  }
+#undef KG_TREE_ROWS
+  if (p.join) {
+    const unsigned grid = (unsigned)(((long long)a.tokens * a.heads_q + 3) / 4);
+    if (p.width == 256) hipLaunchKernelGGL((tree_attn_join_kernel<Tag, 256>), dim3(grid), dim3(256), 0, stream, a, p.split);
+    else if (p.width == 128) hipLaunchKernelGGL((tree_attn_join_kernel<Tag, 128>), dim3(grid), dim3(256), 0, stream, a, p.split);
+    else hipLaunchKernelGGL((tree_attn_join_kernel<Tag, 64>), dim3(grid), dim3(256), 0, stream, a, p.split);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace kg_gfx950
