@@ -16,7 +16,7 @@
 #include "gemm_packed.h"
 #include "gemm_quad.h"
 #include "gemm_skinny.h"
-#include "tree_attn_rows.h"
+#include "tree_attn_launch.h"
 
 #ifdef KG_INSTANTIATE
 #define KG_INSTANCE template
@@ -183,18 +183,18 @@ KG_NHWC_INSTANCE(F16Tag)
 #undef KG_NHWC_INSTANCE
 #endif
 
-#define KG_TREE_ROWS_INSTANCE(TAG, C) KG_INSTANCE hipError_t launch_tree_rows<TAG, C>(const TreeArgs&, const TreePlan&, hipStream_t);
+#define KG_TREE_INSTANCE(TAG, C) KG_INSTANCE hipError_t launch_tree<TAG, C>(const TreeArgs&, const TreePlan&, hipStream_t);
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_TREE_BF16)
-KG_TREE_ROWS_INSTANCE(Bf16Tag, uint16_t)
-KG_TREE_ROWS_INSTANCE(Bf16Tag, E4m3)
-KG_TREE_ROWS_INSTANCE(Bf16Tag, int8_t)
+KG_TREE_INSTANCE(Bf16Tag, uint16_t)
+KG_TREE_INSTANCE(Bf16Tag, E4m3)
+KG_TREE_INSTANCE(Bf16Tag, int8_t)
 #endif
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_TREE_F16)
-KG_TREE_ROWS_INSTANCE(F16Tag, uint16_t)
-KG_TREE_ROWS_INSTANCE(F16Tag, E4m3)
-KG_TREE_ROWS_INSTANCE(F16Tag, int8_t)
+KG_TREE_INSTANCE(F16Tag, uint16_t)
+KG_TREE_INSTANCE(F16Tag, E4m3)
+KG_TREE_INSTANCE(F16Tag, int8_t)
 #endif
-#undef KG_TREE_ROWS_INSTANCE
+#undef KG_TREE_INSTANCE
 
 }  // namespace kg_gfx950
 

@@ -19,13 +19,11 @@
 // Weights of 16-bit caches are rounded to 16 bits, as in the flash attention kernels, and summed as rounded.
 #pragma once
 
-#include <algorithm>
-#include <initializer_list>
+#include <type_traits>
 
 #include "common.h"
 #include "flash_attn_mfma.h"
 #include "kv_cache.h"
-#include "lds_dma.h"  // Int
 #include "tree_attn.h"
 
 namespace kg_gfx950 {
@@ -88,6 +86,14 @@ __device__ __forceinline__ void load_v(uint32_t (&v)[kDwords], const C* p) {
   }
 }
 
+// A pair of 16-bit elements with zeros in place of infinities and NaN; `found` gets a bit for each.
+template <typename H>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t& found) {
+  const uint32_t bad = ((w & H::kExpPair) + H::kExpUnitPair) & 0x80008000u;  // an exponent of ones carries
+  found |= bad;
+  return w & ~((bad >> 15) * 0xffffu);
+}
+
 template <typename C>
 constexpr bool kScaled = CacheElem<C>::kScaled;
 template <>
@@ -100,11 +106,12 @@ struct TreeShare {
   int b, base;      // the request that `first` lies in, and the units before it
   int total;
 };
+constexpr int kTreePad = 4;  // of a record's rows: maximum and sum, on 16-byte rows
 struct TreeSplit {
   int grid;       // workgroups the units are shared among
   int block;      // rows of an item
   int round;      // keys of a round; 0: items are not split, a unit is an item
-  float* partial; // 2 grid records of `block` rows x (width + 2): O, maximum (log2 units), sum
+  float* partial; // 2 grid records of `block` rows x (width + kTreePad): O, maximum (log2 units), sum
   int width;
 };
 __device__ __forceinline__ int tree_rounds(const TreeRequest& r, int round) {
@@ -161,9 +168,36 @@ __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, const TreeSpl
   return t;
 }
 
+// A weight of 0 does not take an infinity or NaN out of a sum, and only some rows see a drafted token: where values are
+// not finite, the products run on zeros in their place and this adds them to the rows that see them (times a
+// weight they would be the same). One key of a step after another, from memory: row l16's elements d_of(e, i).
+// seen: bit 4 (n / 16) + n % 4 of the lane of row l16 and keys 4 (l / 16) + 0..3 is key n's.
+template <typename Tag, typename C, int kKeys, int NE, typename DOf>
+__device__ __forceinline__ void tree_add_nonfinite(const TreeArgs& a, f32x4 (&o)[NE], uint32_t seen, int page, int offset, int h,
+                                                   int lane, DOf d_of) {
+#pragma unroll 1
+  for (int n = 0; n < kKeys; ++n) {
+    const int at_page = __shfl(page, n, 64), at_offset = __shfl(offset, n, 64);
+    const uint32_t bits = (uint32_t)__shfl((int)seen, 16 * ((n & 15) >> 2) + (lane & 15), 64);
+    if (at_page < 0 || !(bits >> (4 * (n >> 4) + (n & 3)) & 1u)) continue;
+    const C* v = static_cast<const C*>(a.v) + at_page * a.v_page + h * a.v_head + at_offset * a.v_row;
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = d_of(e, i);
+        if (d >= a.d) continue;
+        float x;
+        if constexpr (sizeof(C) == 1) x = CacheElem<C>::load(v + d);
+        else x = Half16<Tag>::to_float(v[d]);
+        if (!__builtin_isfinite(x)) o[e][i] += x;
+      }
+  }
+}
+
 // C: uint16_t (elements of Tag), E4m3 or int8_t. D: 64, 128 or 256, heads of d <= D elements, d % 16 == 0. kNQ: blocks of 16
-// rows. kPage16: pages of a multiple of 16 tokens, so that 16 keys share one.
-template <typename Tag, typename C, int D, int kNQ, bool kPage16>
+// rows. Pages of a multiple of 16 tokens, so that 16 keys share one.
+template <typename Tag, typename C, int D, int kNQ>
 __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_rows_kernel(TreeArgs a, TreeSplit split) {
   using namespace treer;
   using H = Half16<Tag>;
@@ -270,42 +304,22 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
         const int d = (kS ? 16 : 8) * lr + (kS ? 64 : 32) * s;
         k[kb][s] = ld16(row + (d < a.d ? d : 0));
       };
-      if constexpr (kPage16) {
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {  // 16 keys on one page
-          const int page = __builtin_amdgcn_readlane(p.page, 16 * kb), offset = __builtin_amdgcn_readlane(p.offset, 16 * kb);
-          const C* row = kc + ((long long)max(page, 0) * a.k_page + (long long)offset * a.k_row);
+      for (int kb = 0; kb < NKB; ++kb) {  // 16 keys on one page
+        const int page = __builtin_amdgcn_readlane(p.page, 16 * kb), offset = __builtin_amdgcn_readlane(p.offset, 16 * kb);
+        const C* row = kc + ((long long)max(page, 0) * a.k_page + (long long)offset * a.k_row);
 #pragma unroll
-          for (int s = 0; s < NKW; ++s) piece(row + (uint32_t)(l16 * (int)a.k_row), kb, s);
-        }
-      } else {  // each lane's own row, handed to the lanes that read it
-        const long long at = (long long)max(p.page, 0) * a.k_page + (long long)p.offset * a.k_row;
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-          const C* row = kc + __shfl(at, 16 * kb + l16, 64);
-#pragma unroll
-          for (int s = 0; s < NKW; ++s) piece(row, kb, s);
-        }
+        for (int s = 0; s < NKW; ++s) piece(row + (uint32_t)(l16 * (int)a.k_row), kb, s);
       }
     };
     const int v_col = NE * l16 < a.d ? NE * l16 : 0;
     auto load_v_rows = [&](const Place& p) __attribute__((always_inline)) {
-      if constexpr (kPage16) {
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-          const int page = __builtin_amdgcn_readlane(p.page, 16 * kb), offset = __builtin_amdgcn_readlane(p.offset, 16 * kb);
-          const C* row = vc + ((long long)max(page, 0) * a.v_page + (long long)offset * a.v_row);
+      for (int kb = 0; kb < NKB; ++kb) {
+        const int page = __builtin_amdgcn_readlane(p.page, 16 * kb), offset = __builtin_amdgcn_readlane(p.offset, 16 * kb);
+        const C* row = vc + ((long long)max(page, 0) * a.v_page + (long long)offset * a.v_row);
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            load_v(v[kb >> 1][(kb & 1) * 4 + x], row + (uint32_t)((4 * lr + x) * (int)a.v_row + v_col));
-        }
-      } else {
-        const long long at = (long long)max(p.page, 0) * a.v_page + (long long)p.offset * a.v_row;
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            load_v(v[kb >> 1][(kb & 1) * 4 + x], vc + __shfl(at, 16 * kb + 4 * lr + x, 64) + v_col);
+        for (int x = 0; x < 4; ++x) load_v(v[kb >> 1][(kb & 1) * 4 + x], row + (uint32_t)((4 * lr + x) * (int)a.v_row + v_col));
       }
     };
 
@@ -327,12 +341,14 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
     constexpr int kStride = kStep * kWaves;
     int key = key_lo + kStep * wave;
     Place p = checked(place(key));
-    // One step. plain: one of the context, every key of it there; `there`: bits of those that are.
-    auto step = [&](auto plain_tag, unsigned long long there) __attribute__((always_inline)) {
-      constexpr bool kPlain = decltype(plain_tag)::value != 0;
+#pragma unroll 1
+    for (; key < key_hi; key += kStride) {
       const Place next = place(key + kStride);
       load_k(p);
       load_v_rows(p);
+      // plain: a step of the context, every key of it there; `there`: bits of those that are
+      const unsigned long long there = __builtin_amdgcn_ballot_w64(p.page >= 0);
+      const bool plain = ~there == 0 && key + kStep <= r.context;
       // ---- scores in log2 units; lane: row l16, keys 16 kb + 4 lr + i ----
       if (a.d != D) {
 #pragma unroll
@@ -341,7 +357,7 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           for (int s = 0; s < NKW; ++s)
             if ((kS ? 16 : 8) * lr + (kS ? 64 : 32) * s >= a.d) k[kb][s] = u32x4{0, 0, 0, 0};
       }
-      f32x4 sc[kNQ][NKB];
+      f32x4 sc[kNQ][NKB], y[kS ? kNQ : 1][NKB];  // y: with the values' scales
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
 #pragma unroll
@@ -360,23 +376,25 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
         // (a NaN passes; a scale of 0 has codes of 0, so any weight does)
         sc_lds[wave][1][lane & (kStep - 1)] = __builtin_amdgcn_logf(nan_max(vs, 0x1p-100f));
       }
-      f32x4 lv[kS ? NKB : 1];
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
-        f32x4 f = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+        f32x4 f = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2}, lv;
         if constexpr (kS) {
           f = *reinterpret_cast<const f32x4*>(&sc_lds[wave][0][16 * kb + 4 * lr]);
-          lv[kb] = *reinterpret_cast<const f32x4*>(&sc_lds[wave][1][16 * kb + 4 * lr]);
+          lv = *reinterpret_cast<const f32x4*>(&sc_lds[wave][1][16 * kb + 4 * lr]);
         }
 #pragma unroll
         for (int x = 0; x < kNQ; ++x)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[x][kb][i] *= f[i];
+          for (int i = 0; i < 4; ++i) {
+            sc[x][kb][i] *= f[i];
+            if constexpr (kS) y[x][kb][i] = sc[x][kb][i] + lv[i];
+          }
       }
       // ---- what is not seen ----
-      const uint32_t there_lo = (uint32_t)(there >> (4 * lr)), there_hi = (uint32_t)(there >> 32 >> (4 * lr));
-      uint32_t seen[kNQ];  // bit 4 kb + i: this lane's row sees its key
-      if constexpr (!kPlain) {
+      uint32_t seen[kNQ], found = 0;  // bit 4 kb + i: this lane's row sees its key
+      if (!plain) {
+        const uint32_t there_lo = (uint32_t)(there >> (4 * lr)), there_hi = (uint32_t)(there >> 32 >> (4 * lr));
 #pragma unroll
         for (int x = 0; x < kNQ; ++x) {
           seen[x] = 0;
@@ -393,18 +411,38 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           }
 #pragma unroll
           for (int n = 0; n < 4 * NKB; ++n)
-            if (!(seen[x] >> n & 1u)) sc[x][n >> 2][n & 3] = -INFINITY;
+            if (!(seen[x] >> n & 1u)) {
+              sc[x][n >> 2][n & 3] = -INFINITY;
+              if constexpr (kS) y[x][n >> 2][n & 3] = -INFINITY;
+            }
         }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int in_step = 32 * c + (n < 4 ? n : 12 + n);
+            const bool here = ((in_step < 32 ? there_lo : there_hi) >> (in_step & 31) & 1u) != 0;
+#pragma unroll
+            for (int q = 0; q < NVW; ++q) {
+              uint32_t w = here ? v[c][n][q] : 0;
+              if constexpr (!kS) {
+                w = finite_pair<H>(w, found);
+              } else if constexpr (std::is_same<C, E4m3>::value) {  // NaN: all ones below the sign
+                const uint32_t bad = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                found |= bad;
+                w &= ~((bad >> 7) * 0xffu);
+              }
+              v[c][n][q] = w;
+            }
+          }
       }
       // ---- weights: keys 32 c + 4 lr + 0..3, then + 16 ----
       u32x4 pp[kNQ][NC];
 #pragma unroll
       for (int x = 0; x < kNQ; ++x) {
         auto weighed = [&](int n) __attribute__((always_inline)) {
-          if constexpr (kS) {  // (a scale of a key that is not seen may be anything)
-            const float s = (float)sc[x][n >> 2][n & 3] + (float)lv[n >> 2][n & 3];
-            return kPlain || (seen[x] >> n & 1u) ? s : -INFINITY;
-          } else return (float)sc[x][n >> 2][n & 3];
+          if constexpr (kS) return (float)y[x][n >> 2][n & 3];
+          else return (float)sc[x][n >> 2][n & 3];
         };
         float mx = weighed(0);
 #pragma unroll
@@ -440,7 +478,7 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
       for (int c = 0; c < NC; ++c) {
         uint32_t row16[8][NE / 2];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
+        for (int n = 0; n < 8; ++n)
 #pragma unroll
           for (int q = 0; q < NE / 2; ++q) {
             if constexpr (kS)
@@ -448,81 +486,22 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
                                     : Widen<Tag, C>::template pair<false>(v[c][n][q >> 1]);
             else row16[n][q] = v[c][n][q];
           }
-          if constexpr (!kPlain) {
-            const int in_step = 32 * c + (n < 4 ? n : 12 + n);
-            if (!((in_step < 32 ? there_lo : there_hi) >> (in_step & 31) & 1u)) {
 #pragma unroll
-              for (int q = 0; q < NE / 2; ++q) row16[n][q] = 0;
-            }
-          }
-        }
-        // Column e of this lane's 8 rows; low, high: v_perm_b32 bytes of the low or the high halves of two dwords.
-        constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
-        auto column = [&](int e, uint32_t low, uint32_t high) __attribute__((always_inline)) {
-          u32x4 vt;
+        for (int e = 0; e < NE; ++e) {
+          u32x4 vt;  // column e of this lane's 8 rows
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            vt[q] = __builtin_amdgcn_perm(row16[2 * q + 1][e >> 1], row16[2 * q][e >> 1], (e & 1) ? high : low);
-          return vt;
-        };
-        // A weight of 0 does not take an infinity or NaN out of a sum: where a step that some rows do not see in
-        // full holds one, every row gets a pass of its own with zeros in place of the keys that it does not see.
-        bool apart = false;
-        if constexpr (!kPlain) {
-          uint32_t carry = 0;  // an exponent of ones carries into its sign bit
+            vt[q] = (e & 1) ? hi_halves(row16[2 * q][e >> 1], row16[2 * q + 1][e >> 1])
+                            : lo_halves(row16[2 * q][e >> 1], row16[2 * q + 1][e >> 1]);
 #pragma unroll
-          for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int q = 0; q < NE / 2; ++q) carry |= (row16[n][q] & H::kExpPair) + H::kExpUnitPair;
-          apart = __builtin_amdgcn_ballot_w64((carry & 0x80008000u) != 0) != 0;
-        }
-        if (!apart) {
-#pragma unroll
-          for (int e = 0; e < NE; ++e) {
-            const u32x4 vt = column(e, kLow, kHigh);
-#pragma unroll
-            for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vt, pp[x][c], o[x][e]);
-          }
-        } else {
-#pragma unroll
-          for (int x = 0; x < kNQ; ++x)
-#pragma unroll 1
-            for (int q = 0; q < 16; ++q) {
-              // (opaque: all columns, kept in registers across this loop, cost the common path as many)
-              uint32_t low = kLow, high = kHigh;
-              asm volatile("" : "+s"(low), "+s"(high));
-              // row q's bits of the keys whose values this lane holds
-              const uint32_t bits = (uint32_t)__shfl((int)seen[x], (lane & 48) + q, 64) >> (8 * c);
-              u32x4 mask;
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                mask[y] = (bits >> (2 * y) & 1u ? 0xffffu : 0u) | (bits >> (2 * y + 1) & 1u ? 0xffff0000u : 0u);
-#pragma unroll
-              for (int e = 0; e < NE; ++e) {
-                const f32x4 sum = H::mfma16(column(e, low, high) & mask, pp[x][c], o[x][e]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[x][e][i] = l16 == q ? (float)sum[i] : (float)o[x][e][i];
-                __builtin_amdgcn_sched_barrier(0);
-              }
-            }
+          for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vt, pp[x][c], o[x][e]);
         }
       }
+      if (!plain && __builtin_amdgcn_ballot_w64(found != 0) != 0)
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x)
+          tree_add_nonfinite<Tag, C, kStep>(a, o[x], seen[x], p.page, p.offset, h, lane, [&](int e, int i) { return NE * (4 * lr + i) + e; });
       p = checked(next);
-      key += kStride;
-    };
-    // Steps of the context whose keys are all there; from the first other one on
-    // (drafted tokens, the range's end, pages that do not exist) a loop that looks at each key.
-    unsigned long long there = 0;
-#pragma unroll 1
-    for (;;) {
-      there = __builtin_amdgcn_ballot_w64(p.page >= 0);
-      if (~there != 0 || key + kStep > r.context) break;
-      step(Int<1>{}, there);
-    }
-#pragma unroll 1
-    while (key < key_hi) {
-      step(Int<0>{}, there);
-      there = __builtin_amdgcn_ballot_w64(p.page >= 0);
     }
 
     // ---- join the waves ----
@@ -543,7 +522,7 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
       }
     }
     __syncthreads();
-    float* record = split.partial + ((long long)2 * blockIdx.x + (starts_here ? 0 : 1)) * kRows * (D + 2);
+    float* record = split.partial + ((long long)2 * blockIdx.x + (starts_here ? 0 : 1)) * kRows * (D + kTreePad);
     for (int y = tid; y < item_rows * (D / 2); y += kThreads) {
       const int n = y / (D / 2), d = 2 * (y - n * (D / 2));
       if (d >= a.d) continue;
@@ -565,7 +544,7 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
                         ((long long)h * a.group + (row - token * a.group)) * a.o_head + d;
         *reinterpret_cast<uint32_t*>(out) = H::pack2(l != 0.f ? v0 * inv : 0.f, l != 0.f ? v1 * inv : 0.f);
       } else {
-        float* p = record + (long long)n * (D + 2);
+        float* p = record + (long long)n * (D + kTreePad);
         *reinterpret_cast<f32x2*>(p + d) = f32x2{v0, v1};
         if (d == 0) *reinterpret_cast<f32x2*>(p + D) = f32x2{m, l};
       }
@@ -574,18 +553,24 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
   }
 }
 
-// One wave per (token, query head): the records of its item joined, where several ranges share it.
-template <typename Tag, int D>
+// kWaves waves per (token, query head): the records of its item joined, where several ranges share it. A wave takes
+// every kWaves-th record.
+template <typename Tag, int D, int kWaves>
 __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs a, TreeSplit split) {
+  constexpr int NE = D / 64, kPerGroup = 4 / kWaves;
+  __shared__ float o_lds[4][D];
+  __shared__ float ml_lds[4][2];
   const int lane = threadIdx.x & 63;
-  const long long id = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = wave % kWaves;
+  const long long id = (long long)blockIdx.x * kPerGroup + wave / kWaves;
   if (id >= (long long)a.tokens * a.heads_q) return;
   const int t = (int)(id / a.heads_q), hq = (int)(id - (long long)t * a.heads_q);
   // its request (the last one that starts at or before it), the units before that, and all units
   int owner = -1, base = 0, total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int b = b0 + lane;
-    const unsigned long long at = __builtin_amdgcn_ballot_w64(b < a.batch && a.starts[b * a.start_stride] <= t);
+    const unsigned long long at = __builtin_amdgcn_ballot_w64(b < a.batch && a.starts[min(b, a.batch) * a.start_stride] <= t);
     const int upto = wave_scan(tree_units(a, split, b), lane);
     if (at != 0) {
       const int x = 63 - __builtin_clzll(at);
@@ -606,102 +591,68 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs a, TreeSpl
   auto holder = [&](int u) { return (int)((((long long)u + 1) * grid - 1) / total); };
   const int w0 = max(holder(begin), 0), w1 = min(holder(end - 1), grid - 1);
   if (w0 >= w1) return;  // one range: the row is written
-  auto record = [&](int w) {
-    const int slot = 2 * w + (share_bound(w, split, total) >= begin ? 0 : 1);
-    return split.partial + ((long long)slot * split.block + row % split.block) * (D + 2);
-  };
-  constexpr int NE = D / 64;
-  float m = treer::kMinMax;
-  for (int w = w0 + lane; w <= w1; w += 64) m = nan_max(m, record(w)[D]);
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) m = nan_max(m, __shfl_xor(m, s, 64));
-  float l = 0.f, o[NE];
+  // an item that begins inside a workgroup's range is that workgroup's second record
+  const int first_slot = 2 * w0 + (share_bound(w0, split, total) >= begin ? 0 : 1);
+  const float* rows = split.partial + (long long)(row % split.block) * (D + kTreePad);
+  const long long pitch = (long long)split.block * (D + kTreePad);
+  float m = treer::kMinMax, l = 0.f, o[NE];
 #pragma unroll
   for (int e = 0; e < NE; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int w = w0; w <= w1; ++w) {
-    const float* p = record(w);
-    const float f = __builtin_amdgcn_exp2f(p[D] - m);
-    l += f * p[D + 1];
+  // 64 records at a time: lane i has the maximum and sum of record i
+  for (int x0 = w0 + part; x0 <= w1; x0 += 64 * kWaves) {
+    const int w = x0 + kWaves * lane;
+    float mw = treer::kMinMax, lw = 0.f;
+    if (w <= w1) {
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(rows + (w == w0 ? first_slot : 2 * w) * pitch + D);
+      mw = ml[0], lw = ml[1];
+    }
+    float top = mw;
 #pragma unroll
-    for (int e = 0; e < NE; ++e)
-      if (lane + 64 * e < a.d) o[e] += f * p[lane + 64 * e];
+    for (int s = 32; s > 0; s >>= 1) top = nan_max(top, __shfl_xor(top, s, 64));
+    const float m_new = nan_max(m, top), alpha = __builtin_amdgcn_exp2f(m - m_new);
+    const float f = __builtin_amdgcn_exp2f(mw - m_new);  // (0 past the last record, or of sums of 0)
+    l = l * alpha + wave_sum(f * lw);
+    m = m_new;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o[e] *= alpha;
+    const int count = min(64, (w1 - x0) / kWaves + 1);
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) {
+      const int v = x0 + kWaves * i;
+      const float* p = rows + (v == w0 ? first_slot : 2 * v) * pitch;
+      const float g = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+        if (lane + 64 * e < a.d) o[e] += g * p[lane + 64 * e];
+    }
+  }
+  if constexpr (kWaves > 1) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o_lds[wave][lane + 64 * e] = o[e];
+    if (lane == 0) ml_lds[wave][0] = m, ml_lds[wave][1] = l;
+    __syncthreads();
+    if (part != 0) return;
+    const int from = wave;
+    float top = m;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = nan_max(top, ml_lds[from + w][0]);
+    const float own = __builtin_amdgcn_exp2f(m - top);
+    l *= own;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o[e] *= own;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(ml_lds[from + w][0] - top);
+      l += f * ml_lds[from + w][1];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[e] += f * o_lds[from + w][lane + 64 * e];
+    }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
   uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.o_token + hq * a.o_head;
 #pragma unroll
   for (int e = 0; e < NE; ++e)
     if (lane + 64 * e < a.d) out[lane + 64 * e] = (uint16_t)(Half16<Tag>::pack2(l != 0.f ? o[e] * inv : 0.f, 0.f) & 0xffffu);
-}
-
-// ---- host ----
-
-// What the kernel takes: 16-bit queries, heads of a multiple of 16 up to 256, rows of 16-byte pieces.
-inline bool tree_rows_takes(const TreeArgs& a, int cache_bytes) {
-  auto whole = [&](const void* p, std::initializer_list<long long> strides, int bytes, int unit) {
-    bool ok = (uintptr_t)p % unit == 0;
-    for (long long s : strides) ok = ok && s * bytes % unit == 0;
-    return ok;
-  };
-  return a.d % 16 == 0 && a.d <= 256 && whole(a.q, {a.q_token, a.q_head}, 2, 16) && whole(a.out, {a.o_token, a.o_head}, 2, 4) &&
-         whole(a.k, {a.k_page, a.k_head, a.k_row}, cache_bytes, 16) && whole(a.v, {a.v_page, a.v_head, a.v_row}, cache_bytes, 16) &&
-         a.k_row <= 1 << 24 && a.v_row <= 1 << 24 && a.pages > 0;
-}
-
-// Shares of a call: as many workgroups as run at once, or as there can be units (the table's reach bounds a
-// request's keys, the batch's tokens its blocks of rows).
-struct TreePlan {
-  int width, blocks16;  // padded head, 16-row blocks of an item
-  TreeSplit split;
-  bool join;
-  size_t bytes;
-};
-inline TreePlan tree_rows_plan(const TreeArgs& a, int cache_bytes, bool may_split) {
-  TreePlan p;
-  p.width = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
-  const long long rows = ((long long)a.tokens + a.batch - 1) / a.batch * a.group;  // of a request and key head, on average
-  p.blocks16 = rows <= 16 || p.width == 256 || a.page_size % 16 != 0 ? 1 : 2;
-  p.split.block = 16 * p.blocks16;
-  p.split.width = p.width;
-  const int step = (cache_bytes == 2 && p.width >= 128) || p.width == 256 || (p.width == 128 && p.blocks16 == 2) ? 32 : 64;
-  const long long round = (long long)step * treer::kWaves, reach = (long long)a.per * a.page_size;
-  const long long items = a.heads * ((long long)a.tokens * a.group / p.split.block + a.batch);
-  const long long units = items * std::max(1ll, (reach + round - 1) / round);
-  may_split = may_split && reach > round && units < 0x7fffffffLL;
-  p.split.round = may_split ? (int)round : 0;
-  p.split.grid = (int)std::min<long long>(may_split ? units : items, p.width == 256 ? 256 : 512);
-  p.join = may_split;
-  p.split.partial = nullptr;
-  p.bytes = may_split ? (size_t)2 * p.split.grid * p.split.block * (p.width + 2) * sizeof(float) : 0;
-  return p;
-}
-
-template <typename Tag, typename C>
-hipError_t launch_tree_rows(const TreeArgs& a, const TreePlan& p, hipStream_t stream) {
-#define KG_TREE_ROWS(WIDTH, NQ, PAGE16)                                                                                  \
-  hipLaunchKernelGGL((tree_attn_rows_kernel<Tag, C, WIDTH, NQ, PAGE16>), dim3(p.split.grid), dim3(treer::kThreads), 0, stream, \
-                     a, p.split)
-  const bool page16 = a.page_size % 16 == 0;
-  if (p.width == 256) {
-    if (page16) KG_TREE_ROWS(256, 1, true);
-    else KG_TREE_ROWS(256, 1, false);
-  } else if (p.width == 128) {
-    if (!page16) KG_TREE_ROWS(128, 1, false);
-    else if (p.blocks16 == 1) KG_TREE_ROWS(128, 1, true);
-    else KG_TREE_ROWS(128, 2, true);
-  } else {
-    if (!page16) KG_TREE_ROWS(64, 1, false);
-    else if (p.blocks16 == 1) KG_TREE_ROWS(64, 1, true);
-    else KG_TREE_ROWS(64, 2, true);
-  }
-#undef KG_TREE_ROWS
-  if (p.join) {
-    const unsigned grid = (unsigned)(((long long)a.tokens * a.heads_q + 3) / 4);
-    if (p.width == 256) hipLaunchKernelGGL((tree_attn_join_kernel<Tag, 256>), dim3(grid), dim3(256), 0, stream, a, p.split);
-    else if (p.width == 128) hipLaunchKernelGGL((tree_attn_join_kernel<Tag, 128>), dim3(grid), dim3(256), 0, stream, a, p.split);
-    else hipLaunchKernelGGL((tree_attn_join_kernel<Tag, 64>), dim3(grid), dim3(256), 0, stream, a, p.split);
-  }
-  return hipGetLastError();
 }
 
 }  // namespace kg_gfx950

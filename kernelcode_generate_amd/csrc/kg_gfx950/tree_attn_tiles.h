@@ -1,0 +1,384 @@
+// Attention over a paged cache (tree_attn.h) for many rows per request and key head: trees of drafted tokens,
+// pieces of prompts; and for pages of no multiple of 16 tokens.
+//
+// Sharing of the work, weights, scales and joining are those of tree_attn_rows.h. Here the four waves of a workgroup take
+// different rows (16 or 32 each) and the same keys: tiles of 64 (32 for heads of 256) go through registers, where 8-bit
+// codes are widened once for all rows, into one of two LDS stages as 16-bit [key][d]; the next tile's rows are
+// in flight under the current one's products, with one barrier per tile. K fragments are one ds_read_b128 per 16 keys x 32 d
+// (16-byte chunk c of row r at c ^ (r % 16): 16 rows hit distinct banks), V^T fragments two ds_read_b64_tr_b16 per 16 d x 32
+// keys in the key order that P's lanes hold (chunk pairs at pair ^ (r % 8): the 8 rows of half a wave do).
+#pragma once
+
+#include "common.h"
+#include "flash_attn_mfma.h"
+#include "kv_cache.h"
+#include "lds_dma.h"
+#include "tree_attn.h"
+#include "tree_attn_rows.h"
+
+namespace kg_gfx950 {
+
+namespace treet {
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+template <int D>
+constexpr int tile_keys() { return D == 256 ? 32 : 64; }
+// byte address of 16-byte chunk c of row r within a [rows][D] 16-bit tile
+template <int D>
+__device__ __forceinline__ uint32_t k_at(int r, int c) {
+  return r * D * 2 + 16 * (D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15));
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_at(int r, int c) {
+  return r * D * 2 + 16 * (D == 64 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * (r & 7)));
+}
+}  // namespace treet
+
+template <typename Tag, typename C, int D, int kNQ>
+__global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(TreeArgs a, TreeSplit split) {
+  using namespace treet;
+  using treer::kMinMax;
+  using H = Half16<Tag>;
+  constexpr bool kS = treer::kScaled<C>;
+  constexpr int kES = sizeof(C);
+  constexpr int kTile = tile_keys<D>();
+  constexpr int NC = kTile / 32, NKB = kTile / 16;
+  constexpr int NDS = D / 32, NE = D / 16;
+  constexpr int kWaveRows = 16 * kNQ, kRows = kWaves * kWaveRows;
+  constexpr int kPerRow = D * kES / 16;              // 16-byte pieces of a row
+  constexpr int kPieces = kTile * kPerRow / kThreads;  // of a thread, K and V each
+  constexpr int kRowStep = kThreads / kPerRow;       // rows between a thread's pieces
+  constexpr int kStage = kTile * D * 2;              // bytes of one tile
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kStage];  // K, V of stage 0, K, V of stage 1
+  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? 2 : 1][2][kTile];
+  __shared__ int found_lds[3];  // whether tile t has values that are not finite, at t % 3
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, lr = lane >> 4;
+  const uint32_t lds0 = lds_addr(lds);
+  const int piece_row = tid / kPerRow, piece = tid % kPerRow;
+  const bool piece_in = piece * 16 / kES < a.d;
+
+  TreeShare share = tree_share(a, split, blockIdx.x);
+  const int own_first = share.first;
+
+  while (share.first < share.last && share.b < a.batch) {
+    const TreeRequest r = tree_request(a, share.b);
+    const int rounds = tree_rounds(r, split.round), blocks = tree_blocks(r, a.group, kRows);
+    const int units = r.count == 0 ? 0 : a.heads * blocks * rounds;
+    const int local = share.first - share.base;
+    if (local >= units) {
+      share.base += units;
+      ++share.b;
+      continue;
+    }
+    const int item = local / rounds, round0 = local - item * rounds;
+    const int round1 = min(rounds, round0 + share.last - share.first);
+    const int h = item / blocks, row0 = (item - h * blocks) * kRows;
+    const bool whole_item = round0 == 0 && round1 == rounds;
+    const int item_rows = min(r.count * a.group - row0, kRows);
+    const bool starts_here = share.first == own_first;
+    share.first += round1 - round0;
+
+    int key_lo = split.round == 0 ? 0 : round0 * kTile;
+    int key_hi = split.round == 0 ? r.keys : min(r.keys, round1 * kTile);
+    if (a.words < 0) key_hi = (int)min((long long)key_hi, (long long)r.context + (row0 + item_rows - 1) / a.group + 1);
+    key_lo = __builtin_amdgcn_readfirstlane(key_lo);
+    key_hi = __builtin_amdgcn_readfirstlane(key_hi);
+
+    // this wave's rows: lane l16 of block x
+    const int wave_rows = min(item_rows - wave * kWaveRows, kWaveRows);  // (may be none)
+    int tok[kNQ];
+    unsigned long long first_word[kNQ];
+    u32x4 qf[kNQ][NDS];
+#pragma unroll
+    for (int x = 0; x < kNQ; ++x) {
+      const bool real = 16 * x + l16 < wave_rows;
+      const int row = row0 + wave * kWaveRows + 16 * x + l16;
+      tok[x] = row / a.group;
+      first_word[x] = real && a.words > 0 ? (unsigned long long)a.mask[(long long)(r.first + tok[x]) * a.mask_0] : 0ull;
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + (real ? r.first + tok[x] : 0) * a.q_token +
+                          ((long long)h * a.group + (row - tok[x] * a.group)) * a.q_head;
+#pragma unroll
+      for (int s = 0; s < NDS; ++s) qf[x][s] = real && 32 * s + 8 * lr < a.d ? ld16(q + 32 * s + 8 * lr) : u32x4{0, 0, 0, 0};
+    }
+    const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
+    const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
+    const int* table = a.table + share.b * a.table_0;
+
+    // Page of key `lane` of a tile (-1: none, or a key past the range) and its offset there.
+    struct Place {
+      int page, offset;
+    };
+    auto place = [&](int key0) __attribute__((always_inline)) {
+      const int key = key0 + (lane & (kTile - 1));
+      Place p = {-1, 0};
+      if (key < key_hi) {
+        const int n = div_page(key, a.div);
+        p.page = table[n * a.table_1];
+        p.offset = key - n * a.page_size;
+      }
+      return p;
+    };
+    auto checked = [&](Place p) __attribute__((always_inline)) {
+      const bool there = p.page >= 0 && p.page < a.pages;
+      return Place{there ? p.page : -1, there ? p.offset : 0};
+    };
+
+    // A tile's rows on their way: what is not there (a key, or d past the head's end) is read from a row that is, and written
+    // as zeros.
+    u32x4 kr[kPieces], vr[kPieces];
+    uint32_t row_there = 0;
+    float ks = 0.f, vs = 0.f;
+    auto load = [&](const Place& p) __attribute__((always_inline)) {
+      row_there = 0;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int n = piece_row + kRowStep * i;
+        const int page = __shfl(p.page, n, 64), offset = __shfl(p.offset, n, 64);
+        row_there |= (page >= 0 ? 1u : 0u) << i;
+        const int d = piece_in ? piece * (16 / kES) : 0;
+        kr[i] = ld16(kc + (long long)max(page, 0) * a.k_page + (long long)offset * a.k_row + d);
+        vr[i] = ld16(vc + (long long)max(page, 0) * a.v_page + (long long)offset * a.v_row + d);
+      }
+      if constexpr (kS) {
+        if (tid < kTile) {
+          ks = a.k_scale[(long long)max(p.page, 0) * a.ks_page + h * a.ks_head + (long long)p.offset * a.ks_row];
+          vs = a.v_scale[(long long)max(p.page, 0) * a.vs_page + h * a.vs_head + (long long)p.offset * a.vs_row];
+        }
+      }
+    };
+    auto put = [&](uint32_t at, u32x4 x) __attribute__((always_inline)) {
+      *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = x;
+    };
+    // sift: a tile that not every row sees in full: values that are not finite are left out (tree_add_nonfinite)
+    auto store = [&](int stage, const Place& p, bool sift, int at) __attribute__((always_inline)) {
+      uint32_t found = 0;
+      const uint32_t kb = lds0 + stage * 2 * kStage, vb = kb + kStage;
+      auto put_v = [&](uint32_t to, u32x4 x) __attribute__((always_inline)) {
+        if (sift) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[q] = treer::finite_pair<H>(x[q], found);
+        }
+        put(to, x);
+      };
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int n = piece_row + kRowStep * i;
+        const bool there = piece_in && (row_there >> i & 1u);
+        const u32x4 k = there ? kr[i] : u32x4{0, 0, 0, 0}, v = there ? vr[i] : u32x4{0, 0, 0, 0};
+        if constexpr (kS) {
+          put(kb + k_at<D>(n, 2 * piece), treer::widen8<Tag, C>(k[0], k[1]));
+          put(kb + k_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(k[2], k[3]));
+          put_v(vb + v_at<D>(n, 2 * piece), treer::widen8<Tag, C>(v[0], v[1]));
+          put_v(vb + v_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(v[2], v[3]));
+        } else {
+          put(kb + k_at<D>(n, piece), k);
+          put_v(vb + v_at<D>(n, piece), v);
+        }
+      }
+      if (found != 0) found_lds[at] = 1;
+      if constexpr (kS) {
+        if (tid < kTile) {
+          sc_lds[stage][0][tid] = p.page >= 0 ? ks * a.scale_log2 : 0.f;
+          // (a NaN passes; a scale of 0 has codes of 0, so any weight does)
+          sc_lds[stage][1][tid] = p.page >= 0 ? __builtin_amdgcn_logf(nan_max(vs, 0x1p-100f)) : 0.f;
+        }
+      }
+    };
+
+    f32x4 o[kNQ][NE];
+    f32x4 l_run[kNQ];
+    float m_run[kNQ];
+#pragma unroll
+    for (int x = 0; x < kNQ; ++x) {
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      l_run[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[x] = kMinMax;
+    }
+    const u32x4 ones = {H::kOnePair, H::kOnePair, H::kOnePair, H::kOnePair};
+
+    // V^T of block e, keys 32 c + 4 lr + 0..3 and + 16, of column d = 16 e + l16
+    auto v_frag = [&](int stage, int c, int e) __attribute__((always_inline)) {
+      const uint32_t vb = lds0 + stage * 2 * kStage + kStage;
+      const int n = 32 * c + 4 * lr + (l16 >> 2), d = 16 * e + 4 * (l16 & 3);
+      const uint32_t at = vb + v_at<D>(n, d >> 3) + (d & 7) * 2;  // row n + 16: the same swizzle
+      const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at);
+      const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(uintptr_t)(at + 16 * D * 2));
+      const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+      return u32x4{w0[0], w0[1], w1[0], w1[1]};
+    };
+    // plain: a tile of the context, every key of it there; `there`: bits of those that are (placed at p); found: the
+    // tile had values that are not finite
+    auto compute = [&](int stage, int key, unsigned long long there, const Place& p, bool found) __attribute__((always_inline)) {
+      const bool plain = ~there == 0 && key + kTile <= r.context;
+      const uint32_t kbase = lds0 + stage * 2 * kStage;
+      f32x4 sc[kNQ][NKB], y[kS ? kNQ : 1][NKB];  // y: with the values' scales
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x) sc[x][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NDS; ++s) {
+          const u32x4 kf = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(kbase + k_at<D>(16 * kb + l16, 4 * s + lr));
+#pragma unroll
+          for (int x = 0; x < kNQ; ++x) sc[x][kb] = H::mfma16(kf, qf[x][s], sc[x][kb]);
+        }
+      }
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        f32x4 f = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2}, lv;
+        if constexpr (kS) {
+          f = *reinterpret_cast<const f32x4*>(&sc_lds[stage][0][16 * kb + 4 * lr]);
+          lv = *reinterpret_cast<const f32x4*>(&sc_lds[stage][1][16 * kb + 4 * lr]);
+        }
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sc[x][kb][i] *= f[i];
+            if constexpr (kS) y[x][kb][i] = sc[x][kb][i] + lv[i];
+          }
+      }
+      uint32_t seen[kNQ];  // bit 4 kb + i: this lane's row sees its key
+      if (!plain) {
+        const uint32_t there_lo = (uint32_t)(there >> (4 * lr)), there_hi = (uint32_t)(there >> 32 >> (4 * lr));
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x) {
+          seen[x] = 0;
+#pragma unroll 1
+          for (int n = 0; n < 4 * NKB; ++n) {
+            const int in_tile = 16 * (n >> 2) + (n & 3), draft = key + 4 * lr + in_tile - r.context;
+            bool s = ((in_tile < 32 ? there_lo : there_hi) >> (in_tile & 31) & 1u) != 0;
+            if (s && draft >= 0) {
+              if (a.words < 0) s = draft <= tok[x];
+              else if (draft < 64) s = (first_word[x] >> draft & 1ull) != 0;
+              else s = 16 * x + l16 < wave_rows && tree_sees(a, r.first + tok[x], tok[x], draft);
+            }
+            seen[x] |= (s ? 1u : 0u) << n;
+          }
+#pragma unroll
+          for (int n = 0; n < 4 * NKB; ++n)
+            if (!(seen[x] >> n & 1u)) {
+              sc[x][n >> 2][n & 3] = -INFINITY;
+              if constexpr (kS) y[x][n >> 2][n & 3] = -INFINITY;
+            }
+        }
+      }
+      u32x4 pp[kNQ][NC];
+#pragma unroll
+      for (int x = 0; x < kNQ; ++x) {
+        auto weighed = [&](int n) __attribute__((always_inline)) {
+          if constexpr (kS) return (float)y[x][n >> 2][n & 3];
+          else return (float)sc[x][n >> 2][n & 3];
+        };
+        float mx = weighed(0);
+#pragma unroll
+        for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(n));
+        float mx2 = mx;
+        fa::rows4_combine<true>(mx, mx2);
+        const float m_new = nan_max(m_run[x], mx);
+        if (__builtin_amdgcn_ballot_w64(m_new > m_run[x] || m_new != m_new)) {
+          const float alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
+          m_run[x] = m_new;
+          l_run[x] *= alpha;
+#pragma unroll
+          for (int e = 0; e < NE; ++e) o[x][e] *= alpha;
+        }
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run[x]);
+            if constexpr (kS) l_run[x][0] += __builtin_amdgcn_exp2f((float)sc[x][kb][i] - m_run[x]);
+          }
+          pp[x][kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
+          pp[x][kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);
+        }
+        if constexpr (!kS) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) l_run[x] = H::mfma16(ones, pp[x][c], l_run[x]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          const u32x4 vt = v_frag(stage, c, e);
+#pragma unroll
+          for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vt, pp[x][c], o[x][e]);
+        }
+      if (!plain && found)
+#pragma unroll
+        for (int x = 0; x < kNQ; ++x)
+          tree_add_nonfinite<Tag, C, kTile>(a, o[x], seen[x], p.page, p.offset, h, lane, [&](int e, int i) { return 16 * e + 4 * lr + i; });
+    };
+
+    // ---- the tiles ----
+    auto drafts = [&](int key) __attribute__((always_inline)) { return key + kTile > r.context; };
+    if (tid < 3) found_lds[tid] = 0;
+    Place p = checked(place(key_lo)), p1 = place(key_lo + kTile);
+    load(p);
+    __syncthreads();
+    store(0, p, drafts(key_lo), 0);
+    __syncthreads();
+    int stage = 0, at = 0;  // at: the tile's number % 3
+#pragma unroll 1
+    for (int key = key_lo; key < key_hi; key += kTile) {
+      const bool more = key + kTile < key_hi;
+      const Place p2 = place(key + 2 * kTile);  // (before the rows: loads return in order)
+      p1 = checked(p1);
+      if (more) load(p1);
+      const int at1 = at == 2 ? 0 : at + 1;
+      if (tid == 0) found_lds[at1 == 2 ? 0 : at1 + 1] = 0;  // read a tile ago, written in the next turn
+      if (wave_rows > 0)
+        compute(stage, key, __builtin_amdgcn_ballot_w64(p.page >= 0), p, drafts(key) && found_lds[at] != 0);
+      stage ^= 1;
+      at = at1;
+      if (more) store(stage, p1, drafts(key + kTile), at);
+      p = p1;
+      p1 = p2;
+      __syncthreads();
+    }
+
+    // ---- this wave's rows: lane l16 holds row l16 of block x, d = 16 e + 4 lr + 0..3 ----
+    float* record = split.partial + ((long long)2 * blockIdx.x + (starts_here ? 0 : 1)) * kRows * (D + kTreePad);
+#pragma unroll
+    for (int x = 0; x < kNQ; ++x) {
+      float l = l_run[x][0];
+      if constexpr (kS) {
+        float l1 = l;
+        fa::rows4_combine<false>(l, l1);
+      }
+      if (16 * x + l16 >= wave_rows) continue;
+      const int n = wave * kWaveRows + 16 * x + l16;
+      if (whole_item) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + (r.first + tok[x]) * a.o_token +
+                        ((long long)h * a.group + (row0 + n - tok[x] * a.group)) * a.o_head;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          const int d = 16 * e + 4 * lr;
+          if (d >= a.d) continue;
+          u32x2 w = {0, 0};
+          if (l != 0.f) w = u32x2{H::pack2(o[x][e][0] * inv, o[x][e][1] * inv), H::pack2(o[x][e][2] * inv, o[x][e][3] * inv)};
+          *reinterpret_cast<uint32_t*>(out + d) = w[0];
+          *reinterpret_cast<uint32_t*>(out + d + 2) = w[1];
+        }
+      } else {
+        float* rec = record + (long long)n * (D + kTreePad);
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+          if (16 * e + 4 * lr < a.d) *reinterpret_cast<f32x4*>(rec + 16 * e + 4 * lr) = o[x][e];
+        if (lr == 0) *reinterpret_cast<f32x2*>(rec + D) = f32x2{m_run[x], l};
+      }
+    }
+  }
+}
+
+}  // namespace kg_gfx950

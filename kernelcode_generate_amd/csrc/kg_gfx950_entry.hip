@@ -1526,23 +1526,23 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
   a.div = page_div((int)kv.page_size);
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   if (tokens * heads_q > 0x7fffffffLL) return fail(kUnsupported, "tree_attention: %lld rows exceed the grid limit", tokens * heads_q);
-  if (q.dtype != KG_DTYPE_F32 && tree_rows_takes(a, (int)element_bytes(kv.dtype))) {
-    TreePlan plan = tree_rows_plan(a, (int)element_bytes(kv.dtype), true);
+  if (q.dtype != KG_DTYPE_F32 && tree_matrix_takes(a, (int)element_bytes(kv.dtype))) {
+    TreePlan plan = tree_plan(a, (int)element_bytes(kv.dtype), true, kSplitMaxWorkspace);
     SplitLease lease;  // held until both kernels are enqueued
     if (plan.join) {
       lease = split_workspace(plan.bytes, g_stream);
-      if (lease.ptr == nullptr) plan = tree_rows_plan(a, (int)element_bytes(kv.dtype), false);
+      if (lease.ptr == nullptr) plan = tree_plan(a, (int)element_bytes(kv.dtype), false, 0);
     }
     plan.split.partial = static_cast<float*>(lease.ptr);
     auto launch = [&](auto tag) {
       using Tag = decltype(tag);
-      return kv.dtype == KG_DTYPE_E4M3 ? launch_tree_rows<Tag, E4m3>(a, plan, g_stream)
-             : kv.dtype == KG_DTYPE_I8 ? launch_tree_rows<Tag, int8_t>(a, plan, g_stream)
-                                       : launch_tree_rows<Tag, uint16_t>(a, plan, g_stream);
+      return kv.dtype == KG_DTYPE_E4M3 ? launch_tree<Tag, E4m3>(a, plan, g_stream)
+             : kv.dtype == KG_DTYPE_I8 ? launch_tree<Tag, int8_t>(a, plan, g_stream)
+                                       : launch_tree<Tag, uint16_t>(a, plan, g_stream);
     };
     const hipError_t e = q.dtype == KG_DTYPE_BF16 ? launch(Bf16Tag{}) : launch(F16Tag{});
-    if (e != hipSuccess) return fail(kHipFailure, "tree_attention(rows): %s", hipGetErrorString(e));
-    return finish_launch("tree_attention(rows)");
+    if (e != hipSuccess) return fail(kHipFailure, "tree_attention(mfma): %s", hipGetErrorString(e));
+    return finish_launch("tree_attention(mfma)");
   }
   return with_kv_types(q.dtype, kv.dtype, [&](auto t, auto c) {
     hipLaunchKernelGGL((tree_attn_any_kernel<decltype(t), decltype(c)>), dim3((unsigned)(tokens * heads_q)), dim3(256), 0, g_stream, a);
