@@ -7,8 +7,12 @@
 // infinity or NaN in a row makes its scale one, and the whole row reads back as NaN. Read back: code s,
 // rounded once to the output's type.
 //
-// kv_store_any_kernel, kv_load_any_kernel: any D and strides, one wave per row.
+// kv_store_kernel, kv_load_kernel: rows of whole 16-byte pieces (8 elements a lane), bound by their bytes: 4096 tokens of 8
+// heads of 128 bf16 to e4m3 STORE_US, back LOAD_US. kv_store_any_kernel, kv_load_any_kernel: any D and
+// alignment, one wave per row.
 #pragma once
+
+#include <type_traits>
 
 #include "common.h"
 
@@ -81,6 +85,7 @@ struct KvStoreArgs {
   long long slot_stride;
   int tokens, heads, d, page_size;
   long long total_slots;
+  PageDiv by_heads;
 };
 
 // page and offset of a slot inside the cache
@@ -157,6 +162,165 @@ __global__ __launch_bounds__(256) void kv_load_any_kernel(KvLoadArgs a) {
     for (int d = lane; d < a.d; d += 64) Elem<Dst>::store(y + d, CacheElem<C>::load(c + d) * scale);
   } else {
     for (int d = lane; d < a.d; d += 64) y[d] = c[d];
+  }
+}
+
+// Eight elements of a row, as a lane of the kernels below holds them.
+template <typename T>
+struct Eight {  // bf16, f16
+  using Tag = typename std::conditional<std::is_same<T, __bf16>::value, Bf16Tag, F16Tag>::type;
+  static __device__ __forceinline__ void load(const T* p, float (&x)[8]) {
+    const u32x4 w = ld16(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = w[i];
+      x[2 * i] = Half16<Tag>::to_float(u & 0xffffu);
+      x[2 * i + 1] = Half16<Tag>::to_float(u >> 16);
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&x)[8]) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = Half16<Tag>::pack2(x[2 * i], x[2 * i + 1]);
+    st16(p, w);
+  }
+};
+template <>
+struct Eight<float> {
+  static __device__ __forceinline__ void load(const float* p, float (&x)[8]) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&x)[8]) {
+    *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+  }
+};
+template <>
+struct Eight<E4m3> {
+  static __device__ __forceinline__ void load(const E4m3* p, float (&x)[8]) {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int u = (int)w[i];
+      x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(u, 0);
+      x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(u, 1);
+      x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(u, 2);
+      x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(u, 3);
+    }
+  }
+  static __device__ __forceinline__ void store(E4m3* p, const float (&x)[8]) {
+    u32x2 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+      w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], lo, true);
+    }
+    st8(p, w);
+  }
+};
+template <>
+struct Eight<int8_t> {
+  static __device__ __forceinline__ void load(const int8_t* p, float (&x)[8]) {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)((int)(w[i >> 2] << (24 - 8 * (i & 3))) >> 24);
+  }
+  static __device__ __forceinline__ void store(int8_t* p, const float (&x)[8]) {
+    u32x2 w = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)(int)__builtin_rintf(x[i]) & 0xffu) << (8 * (i & 3));
+    st8(p, w);
+  }
+};
+
+// scaled_code of eight elements: x / scale by the scale's inverse, which is rounded, as the quotient is, to nearest: a product within
+// 1.5 steps, and two corrections by the exact remainder, of which the second lands on the rounded quotient
+// (5 instructions for a division's 11). Quotients under 2^-12, whose remainders may underflow, are codes of 0 either way.
+template <typename C>
+__device__ __forceinline__ void scaled_codes(float (&x)[8], float scale) {
+  if (scale >= 0x1p-60f && scale <= 0x1p60f) {
+    const float inverse = 1.f / scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float q = x[i] * inverse;
+      q = __builtin_fmaf(__builtin_fmaf(-q, scale, x[i]), inverse, q);
+      q = __builtin_fmaf(__builtin_fmaf(-q, scale, x[i]), inverse, q);
+      x[i] = fminf(fmaxf(q, -CacheElem<C>::kLargest), CacheElem<C>::kLargest);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = scaled_code<C>(x[i], scale);
+  }
+}
+
+// kLanes lanes per row (D <= 8 kLanes), 256 / kLanes rows per workgroup; blockIdx.y: K, V.
+template <typename Src, typename C, int kLanes>
+__global__ __launch_bounds__(256) void kv_store_kernel(KvStoreArgs a) {
+  const KvSide& s = a.side[blockIdx.y];
+  const int part = threadIdx.x % kLanes;
+  const int r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (r >= a.tokens * a.heads) return;
+  const int t = div_page(r, a.by_heads), h = r - t * a.heads;
+  const long long slot = a.slots[t * a.slot_stride];
+  const bool in = 8 * part < a.d;
+  float x[8];
+  const Src* src = static_cast<const Src*>(s.rows) + t * s.r0 + h * s.r1 + (in ? 8 * part : 0);
+  Eight<Src>::load(src, x);
+  if (slot < 0 || slot >= a.total_slots) return;  // not written
+  long long page;
+  int offset;
+  split_slot(slot, a.page_size, &page, &offset);
+  C* c = static_cast<C*>(s.cache) + page * s.page + h * s.head + offset * s.row + 8 * part;
+  if constexpr (CacheElem<C>::kScaled) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = nan_max(top, __builtin_fabsf(x[i]));  // (lanes past the row repeat its first elements)
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = nan_max(top, __shfl_xor(top, o, 64));
+    const float scale = top * CacheElem<C>::kInverse;
+    scaled_codes<C>(x, scale);
+    if (part == 0) s.scale[page * s.s_page + h * s.s_head + offset * s.s_row] = scale;
+  }
+  if (in) Eight<C>::store(c, x);
+}
+
+// Four rows per lane group, their reads in flight together; blockIdx.x: blocks of rows of a sequence and head.
+template <typename C, typename Dst, int kLanes>
+__global__ __launch_bounds__(256) void kv_load_kernel(KvLoadArgs a) {
+  constexpr int kRows = 256 / kLanes, kTurns = 4;
+  const KvSide& s = a.side[blockIdx.z];
+  const int part = threadIdx.x % kLanes;
+  const int b = blockIdx.y / a.heads, h = blockIdx.y - b * a.heads;
+  const int first = blockIdx.x * (kRows * kTurns) + threadIdx.x / kLanes;
+  const int len = min(a.lens[b * a.len_stride], a.reach);
+  if (blockIdx.x * (kRows * kTurns) >= len) return;
+  const bool in = 8 * part < a.d;
+  const C* src[kTurns];
+  float scale[kTurns];
+  bool there[kTurns];
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int i = first + u * kRows, p = div_page(i, a.div);
+    there[u] = in && i < len && p < a.per;
+    const long long page = there[u] ? a.table[b * a.table_stride0 + p * a.table_stride1] : -1;
+    there[u] = page >= 0 && page < a.pages;
+    const int offset = i - p * a.page_size;
+    src[u] = static_cast<const C*>(s.cache) + (there[u] ? page * s.page + h * s.head + offset * s.row + 8 * part : 0);
+    if constexpr (CacheElem<C>::kScaled)
+      scale[u] = there[u] ? s.scale[page * s.s_page + h * s.s_head + offset * s.s_row] : 0.f;
+  }
+  float x[kTurns][8];
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) Eight<C>::load(src[u], x[u]);  // (row 0 of page 0 where there is none)
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    if (!there[u]) continue;
+    if constexpr (CacheElem<C>::kScaled)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[u][e] *= scale[u];
+    Eight<Dst>::store(static_cast<Dst*>(s.rows) + b * s.r0 + h * s.r1 + (long long)(first + u * kRows) * s.r2 + 8 * part, x[u]);
   }
 }
 

@@ -32,6 +32,9 @@ struct TreePlan {
 };
 // Shares of a call: as many workgroups as run at once, or as there can be units (the table's reach bounds a
 // request's keys, the batch's tokens its blocks of rows).
+inline long long tree_items(const TreeArgs& a, int block) {  // at most
+  return a.heads * ((long long)a.tokens * a.group / block + a.batch);
+}
 inline TreePlan tree_plan(const TreeArgs& a, int cache_bytes, bool may_split, long long most_bytes) {
   TreePlan p;
   p.width = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
@@ -43,7 +46,7 @@ inline TreePlan tree_plan(const TreeArgs& a, int cache_bytes, bool may_split, lo
   const long long round = p.tiles ? (p.width == 256 ? 32 : 64)
                                   : ((cache_bytes == 2 && p.width >= 128) || p.width == 256 ? 32 : 64) * treer::kWaves;
   const long long reach = (long long)a.per * a.page_size;
-  const long long items = a.heads * ((long long)a.tokens * a.group / p.split.block + a.batch);
+  const long long items = tree_items(a, p.split.block);
   const long long units = items * std::max(1ll, (reach + round - 1) / round);
   may_split = may_split && reach > round && units < 0x7fffffffLL;
   p.split.round = may_split ? (int)round : 0;
@@ -77,19 +80,19 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream)
 #undef KG_TREE_TILES
 #undef KG_TREE_ROWS
   if (p.join) {
-    // four waves per row while that many rows do not fill the chip
-    const long long rows = (long long)a.tokens * a.heads_q;
-#define KG_TREE_JOIN(WIDTH, WAVES)                                                                                          \
-  hipLaunchKernelGGL((tree_attn_join_kernel<Tag, WIDTH, WAVES>), dim3((unsigned)((rows * WAVES + 3) / 4)), dim3(256), 0, stream, a, \
-                     p.split)
+    const long long quads = tree_items(a, p.split.block) * (p.split.block / kTreeJoinRows);  // of rows
+    const bool few = quads <= 512;
+#define KG_TREE_JOIN(WIDTH, WAVES)                                                                                       \
+  hipLaunchKernelGGL((tree_attn_join_kernel<Tag, WIDTH, WAVES>), dim3((unsigned)((quads * WAVES + 3) / 4)), dim3(256), 0, \
+                     stream, a, p.split)
     if (p.width == 256) {
-      if (rows <= 4096) KG_TREE_JOIN(256, 4);
+      if (few) KG_TREE_JOIN(256, 4);
       else KG_TREE_JOIN(256, 1);
     } else if (p.width == 128) {
-      if (rows <= 4096) KG_TREE_JOIN(128, 4);
+      if (few) KG_TREE_JOIN(128, 4);
       else KG_TREE_JOIN(128, 1);
     } else {
-      if (rows <= 4096) KG_TREE_JOIN(64, 4);
+      if (few) KG_TREE_JOIN(64, 4);
       else KG_TREE_JOIN(64, 1);
     }
 #undef KG_TREE_JOIN

@@ -136,7 +136,15 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
 // Workgroup w of those that have work takes the units from bound(w) up to bound(w + 1), at least one.
 __device__ __forceinline__ int share_bound(int w, const TreeSplit& s, int total) {
   const int grid = min(s.grid, total);
-  return w >= grid ? total : (int)((long long)w * total / grid);
+  if (w >= grid) return total;
+  if (total <= 1 << 22) return (int)((uint32_t)w * (uint32_t)total / (uint32_t)grid);  // (grids have at most 512)
+  return (int)((long long)w * total / grid);
+}
+// The workgroup whose range holds unit u.
+__device__ __forceinline__ int share_of(int u, const TreeSplit& s, int total) {
+  const int grid = min(s.grid, total);
+  if (total <= 1 << 22) return (int)((((uint32_t)u + 1) * (uint32_t)grid - 1) / (uint32_t)total);
+  return (int)((((long long)u + 1) * grid - 1) / total);
 }
 
 __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, const TreeSplit& s, int w) {
@@ -553,106 +561,127 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
   }
 }
 
-// kWaves waves per (token, query head): the records of its item joined, where several ranges share it. A wave takes
-// every kWaves-th record.
+// The records of the items that several ranges share, joined: a wave takes four consecutive rows of an item, a lane four
+// columns. (A wave per row spent most of its time on finding its item: 14 us for 3104 rows of 8 records each, 8 now.)
+// kWaves: 4 where few rows have many records (32 rows of 64: 34 us with one wave each, 14 with four): they take every
+// fourth record of the same rows.
+constexpr int kTreeJoinRows = 4;
 template <typename Tag, int D, int kWaves>
 __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs a, TreeSplit split) {
-  constexpr int NE = D / 64, kPerGroup = 4 / kWaves;
-  __shared__ float o_lds[4][D];
-  __shared__ float ml_lds[4][2];
+  constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes;                    // lanes of a row, rows of a load
+  constexpr int kLoads = kTreeJoinRows / kAtOnce < 1 ? 1 : kTreeJoinRows / kAtOnce;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = wave % kWaves;
-  const long long id = (long long)blockIdx.x * kPerGroup + wave / kWaves;
-  if (id >= (long long)a.tokens * a.heads_q) return;
-  const int t = (int)(id / a.heads_q), hq = (int)(id - (long long)t * a.heads_q);
-  // its request (the last one that starts at or before it), the units before that, and all units
-  int owner = -1, base = 0, total = 0;
+  const int turn = wave % kWaves;
+  const long long id = (long long)blockIdx.x * (4 / kWaves) + wave / kWaves;
+  const int parts = split.block / kTreeJoinRows;
+  const int item = (int)(id / parts), part = (int)(id - (long long)item * parts);
+  // the request of this item, the items and units before it, and all units
+  int owner = -1, items = 0, base = 0, total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int b = b0 + lane;
-    const unsigned long long at = __builtin_amdgcn_ballot_w64(b < a.batch && a.starts[min(b, a.batch) * a.start_stride] <= t);
-    const int upto = wave_scan(tree_units(a, split, b), lane);
-    if (at != 0) {
-      const int x = 63 - __builtin_clzll(at);
-      owner = b0 + x;
-      base = total + (x > 0 ? __builtin_amdgcn_readlane(upto, x - 1) : 0);
+    int own_items = 0, own_units = 0;
+    if (b < a.batch) {
+      const TreeRequest r = tree_request(a, b);
+      own_items = r.count == 0 ? 0 : a.heads * tree_blocks(r, a.group, split.block);
+      own_units = own_items * tree_rounds(r, split.round);
+    }
+    const int upto_items = wave_scan(own_items, lane), upto = wave_scan(own_units, lane);
+    if (owner < 0) {
+      const unsigned long long behind = __builtin_amdgcn_ballot_w64(items + upto_items > item);
+      if (behind != 0) {
+        const int x = __builtin_ctzll(behind);
+        owner = b0 + x;
+        items += __builtin_amdgcn_readlane(upto_items, x) - __builtin_amdgcn_readlane(own_items, x);
+        base = total + __builtin_amdgcn_readlane(upto, x) - __builtin_amdgcn_readlane(own_units, x);
+      } else {
+        items += __builtin_amdgcn_readlane(upto_items, 63);
+      }
     }
     total += __builtin_amdgcn_readlane(upto, 63);
   }
   if (owner < 0) return;
   const TreeRequest r = tree_request(a, owner);
-  const int j = t - r.first;
-  if (j < 0 || j >= r.count) return;
-  const int h = hq / a.group, row = j * a.group + (hq - h * a.group);
   const int rounds = tree_rounds(r, split.round), blocks = tree_blocks(r, a.group, split.block);
-  const int begin = base + (h * blocks + row / split.block) * rounds, end = begin + rounds;
-  // the workgroup whose range holds unit u
-  const int grid = min(split.grid, total);
-  auto holder = [&](int u) { return (int)((((long long)u + 1) * grid - 1) / total); };
-  const int w0 = max(holder(begin), 0), w1 = min(holder(end - 1), grid - 1);
-  if (w0 >= w1) return;  // one range: the row is written
+  const int begin = base + (item - items) * rounds;
+  const int w0 = share_of(begin, split, total), w1 = share_of(begin + rounds - 1, split, total);
+  if (w0 >= w1) return;  // one range: its rows are written
+  const int h = (item - items) / blocks, row0 = ((item - items) - h * blocks) * split.block + part * kTreeJoinRows;
+  const int item_rows = r.count * a.group - row0;  // from this wave's first row on
+  if (item_rows <= 0) return;
   // an item that begins inside a workgroup's range is that workgroup's second record
   const int first_slot = 2 * w0 + (share_bound(w0, split, total) >= begin ? 0 : 1);
-  const float* rows = split.partial + (long long)(row % split.block) * (D + kTreePad);
   const long long pitch = (long long)split.block * (D + kTreePad);
-  float m = treer::kMinMax, l = 0.f, o[NE];
+  const int sub = lane / kLanes, col = 4 * (lane % kLanes);
+  const float* rows = split.partial + (long long)(part * kTreeJoinRows + sub) * (D + kTreePad);
+  float m[kLoads], l[kLoads];
+  f32x4 o[kLoads];
 #pragma unroll
-  for (int e = 0; e < NE; ++e) o[e] = 0.f;
-  // 64 records at a time: lane i has the maximum and sum of record i
-  for (int x0 = w0 + part; x0 <= w1; x0 += 64 * kWaves) {
-    const int w = x0 + kWaves * lane;
-    float mw = treer::kMinMax, lw = 0.f;
-    if (w <= w1) {
-      const f32x2 ml = *reinterpret_cast<const f32x2*>(rows + (w == w0 ? first_slot : 2 * w) * pitch + D);
-      mw = ml[0], lw = ml[1];
+  for (int x = 0; x < kLoads; ++x) {
+    m[x] = treer::kMinMax;
+    l[x] = 0.f;
+    o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  constexpr int kAhead = kWaves == 1 ? 4 : 8;
+  for (int v0 = w0 + turn; v0 <= w1; v0 += kWaves * kAhead) {
+    f32x4 ov[kAhead][kLoads];
+    f32x2 ml[kAhead][kLoads];
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      const int w = min(v0 + kWaves * y, w1);
+      const float* rec = rows + (w == w0 ? first_slot : 2 * w) * pitch;
+#pragma unroll
+      for (int x = 0; x < kLoads; ++x) {  // (rows past the item's are in the record's bounds)
+        ov[y][x] = *reinterpret_cast<const f32x4*>(rec + x * kAtOnce * (D + kTreePad) + col);
+        ml[y][x] = *reinterpret_cast<const f32x2*>(rec + x * kAtOnce * (D + kTreePad) + D);
+      }
     }
-    float top = mw;
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) top = nan_max(top, __shfl_xor(top, s, 64));
-    const float m_new = nan_max(m, top), alpha = __builtin_amdgcn_exp2f(m - m_new);
-    const float f = __builtin_amdgcn_exp2f(mw - m_new);  // (0 past the last record, or of sums of 0)
-    l = l * alpha + wave_sum(f * lw);
-    m = m_new;
+    for (int y = 0; y < kAhead; ++y) {
+      if (v0 + kWaves * y > w1) break;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) o[e] *= alpha;
-    const int count = min(64, (w1 - x0) / kWaves + 1);
-#pragma unroll 8
-    for (int i = 0; i < count; ++i) {
-      const int v = x0 + kWaves * i;
-      const float* p = rows + (v == w0 ? first_slot : 2 * v) * pitch;
-      const float g = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
-#pragma unroll
-      for (int e = 0; e < NE; ++e)
-        if (lane + 64 * e < a.d) o[e] += g * p[lane + 64 * e];
+      for (int x = 0; x < kLoads; ++x) {
+        const float m_new = nan_max(m[x], ml[y][x][0]);
+        const float f = __builtin_amdgcn_exp2f(m[x] - m_new), g = __builtin_amdgcn_exp2f(ml[y][x][0] - m_new);
+        m[x] = m_new;
+        l[x] = l[x] * f + ml[y][x][1] * g;
+        o[x] = o[x] * f + ov[y][x] * g;
+      }
     }
   }
-  if constexpr (kWaves > 1) {
+  if constexpr (kWaves > 1) {  // (all waves of a group are here: what they returned on is the same for them)
+    __shared__ f32x4 o_lds[4][kLoads][64];
+    __shared__ f32x2 ml_lds[4][kLoads][64];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) o_lds[wave][lane + 64 * e] = o[e];
-    if (lane == 0) ml_lds[wave][0] = m, ml_lds[wave][1] = l;
+    for (int x = 0; x < kLoads; ++x) o_lds[wave][x][lane] = o[x], ml_lds[wave][x][lane] = f32x2{m[x], l[x]};
     __syncthreads();
-    if (part != 0) return;
-    const int from = wave;
-    float top = m;
+    if (turn != 0) return;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = nan_max(top, ml_lds[from + w][0]);
-    const float own = __builtin_amdgcn_exp2f(m - top);
-    l *= own;
+    for (int w = 1; w < kWaves; ++w)
 #pragma unroll
-    for (int e = 0; e < NE; ++e) o[e] *= own;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(ml_lds[from + w][0] - top);
-      l += f * ml_lds[from + w][1];
-#pragma unroll
-      for (int e = 0; e < NE; ++e) o[e] += f * o_lds[from + w][lane + 64 * e];
-    }
+      for (int x = 0; x < kLoads; ++x) {
+        const f32x2 ml = ml_lds[wave + w][x][lane];
+        const float m_new = nan_max(m[x], ml[0]);
+        const float f = __builtin_amdgcn_exp2f(m[x] - m_new), g = __builtin_amdgcn_exp2f(ml[0] - m_new);
+        m[x] = m_new;
+        l[x] = l[x] * f + ml[1] * g;
+        o[x] = o[x] * f + o_lds[wave + w][x][lane] * g;
+      }
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.o_token + hq * a.o_head;
 #pragma unroll
-  for (int e = 0; e < NE; ++e)
-    if (lane + 64 * e < a.d) out[lane + 64 * e] = (uint16_t)(Half16<Tag>::pack2(l != 0.f ? o[e] * inv : 0.f, 0.f) & 0xffffu);
+  for (int x = 0; x < kLoads; ++x) {
+    const int n = x * kAtOnce + sub;
+    if (n >= item_rows || n >= kTreeJoinRows || col >= a.d) continue;
+    const int row = row0 + n, token = row / a.group;
+    const float inv = l[x] != 0.f ? 1.f / l[x] : 0.f;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (r.first + token) * a.o_token +
+                    ((long long)h * a.group + (row - token * a.group)) * a.o_head + col;
+    u32x2 w = {0, 0};
+    if (l[x] != 0.f)
+      w = u32x2{Half16<Tag>::pack2(o[x][0] * inv, o[x][1] * inv), Half16<Tag>::pack2(o[x][2] * inv, o[x][3] * inv)};
+    *reinterpret_cast<uint32_t*>(out) = w[0];
+    *reinterpret_cast<uint32_t*>(out + 2) = w[1];
+  }
 }
 
 }  // namespace kg_gfx950

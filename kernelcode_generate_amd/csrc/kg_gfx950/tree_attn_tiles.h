@@ -218,16 +218,25 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
       const bool plain = ~there == 0 && key + kTile <= r.context;
       const uint32_t kbase = lds0 + stage * 2 * kStage;
       f32x4 sc[kNQ][NKB], y[kS ? kNQ : 1][NKB];  // y: with the values' scales
+      // a block's fragments are read under the products of the block before
+      u32x4 kf[2][NDS];
+      auto read_k = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < NDS; ++s)
+          kf[kb & 1][s] = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(kbase + k_at<D>(16 * kb + l16, 4 * s + lr));
+      };
+      read_k(0);
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
+        if (kb + 1 < NKB) read_k(kb + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < kNQ; ++x) sc[x][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < NDS; ++s) {
-          const u32x4 kf = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(kbase + k_at<D>(16 * kb + l16, 4 * s + lr));
+        for (int s = 0; s < NDS; ++s)
 #pragma unroll
-          for (int x = 0; x < kNQ; ++x) sc[x][kb] = H::mfma16(kf, qf[x][s], sc[x][kb]);
-        }
+          for (int x = 0; x < kNQ; ++x) sc[x][kb] = H::mfma16(kf[kb & 1][s], qf[x][s], sc[x][kb]);
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
@@ -269,6 +278,12 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
             }
         }
       }
+      u32x4 vf[2][4];
+      auto read_v = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) vf[g & 1][u] = v_frag(stage, (4 * g + u) / NE, (4 * g + u) % NE);
+      };
+      read_v(0);
       u32x4 pp[kNQ][NC];
 #pragma unroll
       for (int x = 0; x < kNQ; ++x) {
@@ -305,14 +320,20 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
           for (int c = 0; c < NC; ++c) l_run[x] = H::mfma16(ones, pp[x][c], l_run[x]);
         }
       }
+      // groups of four V fragments, read under the products of the group before (the first under the softmax)
+      constexpr int kGroups = NC * NE / 4;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int g = 0; g < kGroups; ++g) {
+        if (g + 1 < kGroups) read_v(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          const u32x4 vt = v_frag(stage, c, e);
+        for (int u = 0; u < 4; ++u) {
+          const int c = (4 * g + u) / NE, e = (4 * g + u) % NE;
 #pragma unroll
-          for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vt, pp[x][c], o[x][e]);
+          for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vf[g & 1][u], pp[x][c], o[x][e]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if (!plain && found)
 #pragma unroll
         for (int x = 0; x < kNQ; ++x)

@@ -1364,6 +1364,20 @@ KvSide kv_side(const KvSlots& kv, int x, const Mem& rows) {
                 s.stride[0], s.stride[1], s.stride[2], rows.stride[0], rows.stride[1], rows.stride[2]};
 }
 
+// Whether the rows of a view start at multiples of `unit` bytes.
+bool rows_aligned(const Mem& m, long long unit) {
+  const long long es = element_bytes(m.dtype);
+  bool ok = (uintptr_t)m.data % unit == 0;
+  for (int i = 0; i + 1 < m.rank; ++i) ok = ok && (m.shape[i] <= 1 || m.stride[i] * es % unit == 0);
+  return ok;
+}
+// Rows that the kernels of eight elements a lane take, of caches and of dense rows.
+bool kv_in_eights(const KvSlots& kv, const Mem* rows) {
+  bool ok = kv.d % 8 == 0;
+  for (int x = 0; x < 2; ++x) ok = ok && rows_aligned(kv.cache[x], kv.scaled() ? 8 : 16) && rows_aligned(rows[x], 16);
+  return ok;
+}
+
 // Calls f(type of the dense rows, type of the cache's elements): the same, or 8 bits.
 template <typename F>
 int with_kv_types(int dtype, int cache, F&& f) {
@@ -1407,6 +1421,19 @@ int kv_cache_store_impl(const KgArgSlot* args, unsigned long long n) {
   a.page_size = (int)kv.page_size;
   a.total_slots = kv.pages * kv.page_size;
   const long long items = 2 * tokens * kv.heads;
+  a.by_heads = page_div((int)kv.heads);
+  if (kv_in_eights(kv, rows) && items / 2 < 0x7fffffffLL)
+    return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
+#define KG_KV_STORE(LANES)                                                                                             \
+  hipLaunchKernelGGL((kv_store_kernel<decltype(t), decltype(c), LANES>), dim3((unsigned)cdiv(items / 2 * LANES, 256), 2), \
+                     dim3(256), 0, g_stream, a)
+      if (kv.d <= 64) KG_KV_STORE(8);
+      else if (kv.d <= 128) KG_KV_STORE(16);
+      else if (kv.d <= 256) KG_KV_STORE(32);
+      else KG_KV_STORE(64);
+#undef KG_KV_STORE
+      return finish_launch("kv_cache_store");
+    });
   if (cdiv(items, 4) > 0x7fffffffLL) return fail(kUnsupported, "kv_cache_store: %lld rows exceed the grid limit", items);
   return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
     hipLaunchKernelGGL((kv_store_any_kernel<decltype(t), decltype(c)>), dim3((unsigned)cdiv(items, 4)), dim3(256), 0, g_stream, a);
@@ -1454,6 +1481,18 @@ int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
   a.reach = (int)reach;
   a.pages = kv.pages;
   a.div = page_div((int)kv.page_size);
+  if (kv_in_eights(kv, rows) && batch * kv.heads <= 65535)
+    return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
+#define KG_KV_LOAD(LANES)                                                                                                \
+  hipLaunchKernelGGL((kv_load_kernel<decltype(c), decltype(t), LANES>),                                                  \
+                     dim3((unsigned)cdiv(reach * LANES, 1024), (unsigned)(batch * kv.heads), 2), dim3(256), 0, g_stream, a)
+      if (kv.d <= 64) KG_KV_LOAD(8);
+      else if (kv.d <= 128) KG_KV_LOAD(16);
+      else if (kv.d <= 256) KG_KV_LOAD(32);
+      else KG_KV_LOAD(64);
+#undef KG_KV_LOAD
+      return finish_launch("kv_cache_load");
+    });
   if (batch * kv.heads > 0x7fffffffLL || cdiv(2 * batch * kv.heads, 4) > 0x7fffffffLL / reach)
     return fail(kUnsupported, "kv_cache_load: %lld x %lld rows exceed the grid limit", batch * kv.heads, reach);
   return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
