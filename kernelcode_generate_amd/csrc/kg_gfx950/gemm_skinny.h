@@ -17,6 +17,7 @@
 // have no tile at N = 4096: two workgroups on one tile's K would need partials in HBM.
 #pragma once
 
+#include "adapter.h"
 #include "common.h"
 #include "conv2d_igemm.h"  // F32Tag, IgElem
 
@@ -117,11 +118,13 @@ struct Step<F32Tag> {
 };
 }  // namespace gemms
 
-template <typename Tag, int kMT>  // kMT: 16-row blocks of a workgroup
+// kMT: 16-row blocks of a workgroup. kAdapters: 16-bit calls with low-rank adapters beside rhs (adapter.h), whose k the waves
+// take turns with behind their own.
+template <typename Tag, int kMT, bool kAdapters>
 __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
     const typename convg::IgElem<Tag>::T* __restrict__ A, const typename convg::IgElem<Tag>::T* __restrict__ B,
     typename convg::IgElem<Tag>::T* __restrict__ C, const void* __restrict__ bias, int bias_kind, int M, int N, int K,
-    long long lda, long long ldb, long long ldc) {
+    long long lda, long long ldb, long long ldc, AdapterPart part) {
   using namespace gemms;
   using E = convg::IgElem<Tag>;
   using T = typename E::T;
@@ -209,6 +212,70 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
       S::mac(p, acc);
     }
 
+  if constexpr (kAdapters) {
+    // lane s: the s-th distinct adapter of the block's rows
+    int own = lane < kRows && lane < rows ? part.index[(long long)(m0 + lane) * part.index_stride] : -1;
+    if (own >= part.count) own = -1;
+    int of_row[kMT], listed = -1, slots = 0;
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) of_row[i] = __shfl(own, 16 * i + l16, 64);
+    for (unsigned long long left = __builtin_amdgcn_ballot_w64(own >= 0); left != 0; ++slots) {
+      const int l = __builtin_amdgcn_readlane(own, __builtin_ctzll(left));
+      left &= ~__builtin_amdgcn_ballot_w64(own == l);
+      if (lane == slots) listed = l;
+    }
+    const int pieces = part.rank / 8, total_pieces = slots * pieces;
+    f32x4 low[kMT][2];
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) low[i][0] = low[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = wave; 4 * s < total_pieces; s += kWaves) {
+      const int piece = 4 * s + lg, slot = div_page(piece, part.by_pieces), r0 = 8 * (piece - slot * pieces);
+      const int l = __shfl(listed, min(slot, 63), 64);
+      const bool there = piece < total_pieces;
+      Regs& f = r[0][0];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        f.b[e] = there ? S::load_b(reinterpret_cast<const char*>(part.b + l * part.b_l + (r0 + e) * part.b_r + min(n0 + 2 * l16, N - 2)))
+                       : 0u;
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+        f.a[i] = there && of_row[i] == l ? ld16(part.t + (long long)(m0 + 16 * i + l16) * part.rank + r0) : u32x4{0, 0, 0, 0};
+      S::mac(f, low);
+    }
+    bool spoilt = false;
+#pragma unroll
+    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) spoilt |= !__builtin_isfinite((float)low[i][0][e]) || !__builtin_isfinite((float)low[i][1][e]);
+    if (__builtin_amdgcn_ballot_w64(spoilt) != 0) {
+      // this wave's pieces again, each row over its own adapter's
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = 16 * i + 4 * lg + e, l_row = __shfl(own, m & 63, 64), n = min(n0 + 2 * l16, N - 2);
+          float v0 = 0.f, v1 = 0.f;
+#pragma unroll 1
+          for (int s = wave; 4 * s < total_pieces; s += kWaves)
+#pragma unroll 1
+            for (int piece = 4 * s; piece < min(4 * s + 4, total_pieces); ++piece) {
+              const int slot = piece / pieces, r0 = 8 * (piece - slot * pieces), l = __builtin_amdgcn_readlane(listed, slot);
+              if (l_row != l) continue;
+              const uint16_t *t = part.t + (long long)(m0 + m) * part.rank, *b = part.b + l * part.b_l + n;
+#pragma unroll 1
+              for (int q = r0; q < r0 + 8; ++q) {
+                v0 = __builtin_fmaf(Half16<Tag>::to_float(t[q]), Half16<Tag>::to_float(b[q * part.b_r]), v0);
+                v1 = __builtin_fmaf(Half16<Tag>::to_float(t[q]), Half16<Tag>::to_float(b[q * part.b_r + 1]), v1);
+              }
+            }
+          low[i][0][e] = v0;
+          low[i][1][e] = v1;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) acc[i][0] += low[i][0], acc[i][1] += low[i][1];
+  }
+
   // lane holds C[m = 16 i + 4 lg + e][columns 2 l16, 2 l16 + 1]
 #pragma unroll
   for (int i = 0; i < kMT; ++i)
@@ -256,16 +323,16 @@ inline int gemm_skinny_rows(long long M, long long N) {
 }
 
 // bias_kind: 0 none, 1 fp32, 2 16-bit.
-template <typename Tag>
+template <typename Tag, bool kAdapters>
 hipError_t launch_gemm_skinny(const void* A, const void* B, void* C, const void* bias, int bias_kind, int M, int N, int K,
-                              long long lda, long long ldb, long long ldc, hipStream_t stream) {
+                              long long lda, long long ldb, long long ldc, const AdapterPart& part, hipStream_t stream) {
   using T = typename convg::IgElem<Tag>::T;
   const long long tiles = ((long long)N + gemms::kCols - 1) / gemms::kCols;
 #define KG_GEMM_SKINNY(MT)                                                                                             \
-  hipLaunchKernelGGL((gemm_skinny_kernel<Tag, MT>), dim3((unsigned)(tiles * ((M + 16 * MT - 1) / (16 * MT)))),         \
+  hipLaunchKernelGGL((gemm_skinny_kernel<Tag, MT, kAdapters>), dim3((unsigned)(tiles * ((M + 16 * MT - 1) / (16 * MT)))), \
                      dim3(gemms::kWaves * 64), 0, stream,                                                              \
                      static_cast<const T*>(A), static_cast<const T*>(B), static_cast<T*>(C), bias, bias_kind, M, N, K, \
-                     lda, ldb, ldc)
+                     lda, ldb, ldc, part)
   if (gemm_skinny_rows(M, N) == 16) KG_GEMM_SKINNY(1);
   else KG_GEMM_SKINNY(2);
 #undef KG_GEMM_SKINNY

@@ -46,13 +46,16 @@ KG_GEMM_PIPE_INSTANCES(F16Tag, 256, true)
 #endif
 
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_GEMM_MID)
-#define KG_GEMM_MID_INSTANCE(TAG, ST, RAG)                                                                             \
-  KG_INSTANCE hipError_t launch_gemm_mid<TAG, ST, RAG>(const uint16_t*, const uint16_t*, uint16_t*, const void*, int, int, \
-                                                       int, int, long long, long long, long long, hipStream_t);
-#define KG_GEMM_MID_INSTANCES(TAG)                                      \
-  KG_GEMM_MID_INSTANCE(TAG, 2, false) KG_GEMM_MID_INSTANCE(TAG, 2, true) \
-  KG_GEMM_MID_INSTANCE(TAG, 3, false) KG_GEMM_MID_INSTANCE(TAG, 3, true) \
-  KG_GEMM_MID_INSTANCE(TAG, 4, false) KG_GEMM_MID_INSTANCE(TAG, 4, true)
+#define KG_GEMM_MID_INSTANCE(TAG, ST, RAG, ADAPTERS)                                                                     \
+  KG_INSTANCE hipError_t launch_gemm_mid<TAG, ST, RAG, ADAPTERS>(const uint16_t*, const uint16_t*, uint16_t*, const void*, int, \
+                                                                 int, int, int, long long, long long, long long,           \
+                                                                 const AdapterPart&, hipStream_t);
+#define KG_GEMM_MID_INSTANCES(TAG)                                                    \
+  KG_GEMM_MID_INSTANCE(TAG, 2, false, false) KG_GEMM_MID_INSTANCE(TAG, 2, true, false) \
+  KG_GEMM_MID_INSTANCE(TAG, 3, false, false) KG_GEMM_MID_INSTANCE(TAG, 3, true, false) \
+  KG_GEMM_MID_INSTANCE(TAG, 4, false, false) KG_GEMM_MID_INSTANCE(TAG, 4, true, false) \
+  KG_GEMM_MID_INSTANCE(TAG, 2, false, true) KG_GEMM_MID_INSTANCE(TAG, 2, true, true)   \
+  KG_GEMM_MID_INSTANCE(TAG, 4, false, true) KG_GEMM_MID_INSTANCE(TAG, 4, true, true)
 KG_GEMM_MID_INSTANCES(Bf16Tag)
 KG_GEMM_MID_INSTANCES(F16Tag)
 #undef KG_GEMM_MID_INSTANCES
@@ -60,12 +63,14 @@ KG_GEMM_MID_INSTANCES(F16Tag)
 #endif
 
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_GEMM_SKINNY)
-#define KG_GEMM_SKINNY_INSTANCE(TAG)                                                                                     \
-  KG_INSTANCE hipError_t launch_gemm_skinny<TAG>(const void*, const void*, void*, const void*, int, int, int, int,       \
-                                                 long long, long long, long long, hipStream_t);
-KG_GEMM_SKINNY_INSTANCE(F32Tag)
-KG_GEMM_SKINNY_INSTANCE(Bf16Tag)
-KG_GEMM_SKINNY_INSTANCE(F16Tag)
+#define KG_GEMM_SKINNY_INSTANCE(TAG, ADAPTERS)                                                                          \
+  KG_INSTANCE hipError_t launch_gemm_skinny<TAG, ADAPTERS>(const void*, const void*, void*, const void*, int, int, int, int, \
+                                                           long long, long long, long long, const AdapterPart&, hipStream_t);
+KG_GEMM_SKINNY_INSTANCE(F32Tag, false)
+KG_GEMM_SKINNY_INSTANCE(Bf16Tag, false)
+KG_GEMM_SKINNY_INSTANCE(F16Tag, false)
+KG_GEMM_SKINNY_INSTANCE(Bf16Tag, true)
+KG_GEMM_SKINNY_INSTANCE(F16Tag, true)
 #undef KG_GEMM_SKINNY_INSTANCE
 #endif
 

@@ -550,8 +550,8 @@ int launch_gemm_mfma(const Mem& out, const Mem& lhs, const Mem& rhs, const Mem& 
     const int depth = staged ? stages : gemm_mid_stages(K);
     const bool edges = M % gemmm::kT || N % gemmm::kT || K % gemmm::kBK;
 #define KG_GEMM_MID(ST)                                                                                                   \
-  (edges ? launch_gemm_mid<Tag, ST, true>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, g_stream)                       \
-         : launch_gemm_mid<Tag, ST, false>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, g_stream))
+  (edges ? launch_gemm_mid<Tag, ST, true, false>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, AdapterPart{}, g_stream) \
+         : launch_gemm_mid<Tag, ST, false, false>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, AdapterPart{}, g_stream))
     const hipError_t e = depth == 2 ? KG_GEMM_MID(2) : depth == 3 ? KG_GEMM_MID(3) : KG_GEMM_MID(4);
 #undef KG_GEMM_MID
     if (e != hipSuccess) return fail(kHipFailure, "matmul(mfma-mid): %s", hipGetErrorString(e));
@@ -794,8 +794,8 @@ int matmul_impl(const KgArgSlot* args, unsigned long long n) {
     const int bias_kind = !bias.present ? 0 : (bias.dtype == KG_DTYPE_F32 ? 1 : 2);
     const void* bp = bias.present ? bias.data : nullptr;
 #define KG_GEMM_SKINNY(TAG)                                                                                         \
-  launch_gemm_skinny<TAG>(lhs.data, rhs.data, out.data, bp, bias_kind, m, nn, k, lhs.stride[0], rhs.stride[0], \
-                          out.stride[0], g_stream)
+  launch_gemm_skinny<TAG, false>(lhs.data, rhs.data, out.data, bp, bias_kind, m, nn, k, lhs.stride[0], rhs.stride[0], \
+                                 out.stride[0], AdapterPart{}, g_stream)
     const hipError_t e = f32                          ? KG_GEMM_SKINNY(F32Tag)
                          : out.dtype == KG_DTYPE_BF16 ? KG_GEMM_SKINNY(Bf16Tag)
                                                       : KG_GEMM_SKINNY(F16Tag);
@@ -1589,6 +1589,33 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
   });
 }
 
+// The projection with its adapters in one pass over the output (adapter.h).
+template <typename Tag>
+int launch_adapter_matmul(const AdapterArgs& p, int bias_kind, char* ws) {
+  uint16_t* t = reinterpret_cast<uint16_t*>(ws + kAdapterHeader);
+  const unsigned blocks = (unsigned)cdiv(p.m, 16);
+  const unsigned at_once = (unsigned)std::min(16u, std::max(1u, 512u / blocks));  // of a block's adapters
+  hipLaunchKernelGGL((adapter_low_kernel<Tag>), dim3(blocks, at_once, (unsigned)cdiv(p.rank, 64)), dim3(512), 0, g_stream, p, t,
+                     reinterpret_cast<uint32_t*>(ws));
+  const AdapterPart part{t, reinterpret_cast<const uint16_t*>(ws), static_cast<const uint16_t*>(p.b), p.index, p.b_l, p.b_r,
+                         p.index_stride, p.rank, p.count, page_div(p.rank / 8)};
+  hipError_t e;
+  if (gemm_skinny_pays(p.m, p.n, p.k, false, true, true)) {
+    e = launch_gemm_skinny<Tag, true>(p.x, p.w, p.out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream);
+  } else {
+    const bool edges = p.m % gemmm::kT || p.n % gemmm::kT || p.k % gemmm::kBK;
+    const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.w);
+    uint16_t* out = static_cast<uint16_t*>(p.out);
+#define KG_ADAPTER_MID(ST, RAG) \
+  launch_gemm_mid<Tag, ST, RAG, true>(x, w, out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream)
+    if (gemm_mid_stages(p.k) == 2) e = edges ? KG_ADAPTER_MID(2, true) : KG_ADAPTER_MID(2, false);
+    else e = edges ? KG_ADAPTER_MID(4, true) : KG_ADAPTER_MID(4, false);
+#undef KG_ADAPTER_MID
+  }
+  if (e != hipSuccess) return fail(kHipFailure, "adapter_matmul(mfma): %s", hipGetErrorString(e));
+  return finish_launch("adapter_matmul(mfma)");
+}
+
 int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   if (args == nullptr) return fail(kInvalid, "ordered_args is null");
   if (n != 8) return fail(kInvalid, "adapter_matmul expects 8 slots, got %llu", n);
@@ -1632,6 +1659,16 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   p.a_l = a.stride[0], p.a_k = a.stride[1], p.b_l = b.stride[0], p.b_r = b.stride[1];
   p.index_stride = index.stride[0], p.scale_stride = scale.stride[0];
   p.m = (int)M, p.n = (int)N, p.k = (int)K, p.rank = (int)rank, p.count = (int)count;
+  const bool mfma = adapters && out.dtype != KG_DTYPE_F32 && K > 0 && K % 8 == 0 && N % 8 == 0 && rank % 8 == 0 &&
+                    w.stride[1] == 1 && (!bias.present || bias.stride[0] == 1 || N == 1) && rows_aligned(out, 16) &&
+                    rows_aligned(x, 16) && rows_aligned(w, 16) && rows_aligned(b, 16) && rows_aligned(a, 4) &&
+                    x.stride[0] <= kMaxPipeLd && w.stride[0] <= kMaxPipeLd;
+  if (mfma) {
+    const SplitLease lease = split_workspace(kAdapterHeader + (size_t)(M * rank) * 2, g_stream);  // held until both kernels are enqueued
+    const int bias_kind = !bias.present ? 0 : bias.dtype == KG_DTYPE_F32 ? 1 : 2;
+    if (char* ws = static_cast<char*>(lease.ptr))
+      return out.dtype == KG_DTYPE_BF16 ? launch_adapter_matmul<Bf16Tag>(p, bias_kind, ws) : launch_adapter_matmul<F16Tag>(p, bias_kind, ws);
+  }
   if ((rc = matmul_impl(args, 4)) || !adapters) return rc;
   return with_kv_types(out.dtype, out.dtype, [&](auto t, auto) {
     hipLaunchKernelGGL((adapter_add_kernel<decltype(t)>), dim3((unsigned)M), dim3(256), 0, g_stream, p);
