@@ -3,11 +3,11 @@
 // an index outside 0..L-1 is a row without one.
 //
 // 16-bit calls of whole 16-byte rows: adapter_low_kernel writes t = scale x A, rounded to the operands' type as
-// a 16-bit layer's output is, to a workspace [M, R]; then the projection's kernels (gemm_skinny.h, gemm_mid.h) take the
-// adapters as further k behind their own: the distinct adapters of a tile's rows, one after the other, R values
-// each, t's rows in the slots of their adapter and zeros in the others. These products have accumulators of their own: a
-// value of B that is not finite, times the zeros of rows that do not use it, would be NaN in them, so where such a sum
-// is not finite it is taken again over the row's own adapter alone.
+// a 16-bit layer's output is, to a workspace [M, R]; then the projection's kernels (gemm_skinny.h, gemm_mid.h, gemm_quad.h)
+// take the adapters as further k behind their own: the distinct adapters of a tile's rows, one after the other, R
+// values each, t's rows in the slots of their adapter and zeros in the others. A value of B that is not finite, times
+// the zeros of rows that do not use it, would be NaN in them: the products run on zeros in place of such values, and
+// where there were any each output adds those of its own row's adapter (adapter_nonfinite).
 //
 // adapter_add_kernel: any types and strides, one workgroup per row: t = scale x A in 32 bits, then
 // out += t B, on an output that holds the projection already (matmul's kernels). A 16-bit output is
@@ -16,6 +16,7 @@
 
 #include "common.h"
 #include "kv_cache.h"  // PageDiv
+#include "lds_dma.h"   // Int
 
 namespace kg_gfx950 {
 
@@ -84,27 +85,104 @@ struct AdapterPart {
 };
 constexpr size_t kAdapterHeader = 256;  // bytes of the workspace before t
 
-// sum_r t[m, r] B[l, r, n], for sums that another row's values have spoilt
+// The sum of t[m, r] B[l, r, n] over the B that are not finite, l row m's adapter.
 template <typename H>
-__device__ __forceinline__ float adapter_alone(const AdapterPart& p, int m, int n) {
+__device__ __forceinline__ float adapter_nonfinite(const AdapterPart& p, int m, int n) {
   const int l = p.index[m * p.index_stride];
   if (l < 0 || l >= p.count) return 0.f;
   const uint16_t *t = p.t + (long long)m * p.rank, *b = p.b + l * p.b_l + n;
   float sum = 0.f;
 #pragma unroll 1
-  for (int r = 0; r < p.rank; ++r) sum = __builtin_fmaf(H::to_float(t[r]), H::to_float(b[r * p.b_r]), sum);
+  for (int r = 0; r < p.rank; ++r) {
+    const float x = H::to_float(b[r * p.b_r]);
+    if (!__builtin_isfinite(x)) sum = __builtin_fmaf(H::to_float(t[r]), x, sum);
+  }
   return sum;
 }
 
-// t = scale x A of 16 rows and up to 64 columns (blockIdx.z) per workgroup: its eight waves share K in steps of
+// The values of B that are not finite, added to outputs that a wave has written: kRows rows from m0, kLanes lanes of 8
+// columns from n0 per row, a lane those that it wrote itself. (What is added is not finite, so the output's rounding
+// does not matter. In the epilogues' own loops it cost the products their registers.)
+template <typename H, int kRows, int kLanes>
+__device__ __forceinline__ void adapter_add_nonfinite(const AdapterPart& p, uint16_t* C, long long ldc, int m0, int n0, int M, int N,
+                                                      int lane) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  const int n = n0 + 8 * (lane % kLanes);
+#pragma unroll 1
+  for (int r = lane / kLanes; r < kRows; r += 64 / kLanes) {
+    const int m = m0 + r;
+    if (m >= M || n >= N) continue;
+#pragma unroll 1
+    for (int u = 0; u < 8; ++u) {
+      const float x = adapter_nonfinite<H>(p, m, n + u);
+      uint16_t* out = C + (long long)m * ldc + n + u;
+      if (x != 0.f) *out = (uint16_t)H::from_float(H::to_float(*out) + x);
+    }
+  }
+}
+
+// The adapters of a tile of kRows rows from m0: row_lds[i] row i's (-1: none), slot_lds[s] the s-th distinct one in the
+// order of their first rows. Every wave of the workgroup writes the same. Returns the number of distinct ones.
+template <int kRows>
+__device__ __forceinline__ int adapter_slots(const AdapterPart& p, int m0, int M, int lane, int* row_lds, int* slot_lds) {
+  constexpr int kParts = kRows / 64;
+  int own[kParts];
+  unsigned long long left[kParts], any = 0;
+#pragma unroll
+  for (int u = 0; u < kParts; ++u) {
+    const int m = m0 + 64 * u + lane;
+    own[u] = m < M ? p.index[m * p.index_stride] : -1;
+    if (own[u] < 0 || own[u] >= p.count) own[u] = -1;
+    row_lds[64 * u + lane] = own[u];
+    left[u] = __builtin_amdgcn_ballot_w64(own[u] >= 0);
+    any |= left[u];
+  }
+  int slots = 0;
+  while (any != 0) {
+    int l = -1;
+#pragma unroll
+    for (int u = 0; u < kParts; ++u)
+      if (l < 0 && left[u] != 0) l = __builtin_amdgcn_readlane(own[u], __builtin_ctzll(left[u]));
+    any = 0;
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+      left[u] &= ~__builtin_amdgcn_ballot_w64(own[u] == l);
+      any |= left[u];
+    }
+    slot_lds[slots++] = l;
+  }
+  return slots;
+}
+
+// Where the 16 bytes of a tile's row (t) or of a k-row's columns (B) of an eight-k piece lie; null: zeros.
+__device__ __forceinline__ const uint16_t* adapter_t(const AdapterPart& p, int piece, int pieces, int slots, const int* slot_lds, int l,
+                                                     int m) {
+  const int slot = div_page(piece, p.by_pieces);
+  return slot < slots && slot_lds[slot] == l ? p.t + (long long)m * p.rank + 8 * (piece - slot * pieces) : nullptr;
+}
+__device__ __forceinline__ const uint16_t* adapter_b(const AdapterPart& p, int piece, int pieces, int slots, const int* slot_lds, int k,
+                                                     int n) {
+  const int slot = div_page(piece, p.by_pieces);
+  return slot < slots ? p.b + slot_lds[slot] * p.b_l + (8 * (piece - slot * pieces) + k) * p.b_r + n : nullptr;
+}
+// 16 bytes of B from there to LDS, zeros in place of what is not finite; `found` gets bits for that.
+template <typename H>
+__device__ __forceinline__ void adapter_put(u32x4 x, uint32_t to, uint32_t& found) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) x[q] = finite_pair<H>(x[q], found);
+  *(__attribute__((address_space(3))) u32x4*)(uintptr_t)to = x;
+}
+
+// t = scale x A of 16 rows and up to 64 columns (blockIdx.z) per workgroup: its sixteen waves share K in steps of
 // 32, lanes hold two columns of A by eight k as in gemm_skinny.h, one sum over the waves through LDS. A workgroup takes every
 // gridDim.y-th of its rows' distinct adapters and stores the rows that use it: few rows have many adapters
 // (gridDim.y workgroups read them at once), many rows few. 16 x 4096, 16 adapters of rank 16: LOW_STEP us; 4096 x 4096 in
 // runs: LOW_PROMPTS us, the reading of x.
+constexpr int kAdapterLowThreads = 1024, kAdapterLowCols = 64;
 template <typename Tag>
-__global__ __launch_bounds__(512) void adapter_low_kernel(AdapterArgs a, uint16_t* __restrict__ t, uint32_t* __restrict__ zeros) {
+__global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(AdapterArgs a, uint16_t* __restrict__ t, uint32_t* __restrict__ zeros) {
   using H = Half16<Tag>;
-  constexpr int kWaves = 8, kCols = 64;
+  constexpr int kWaves = kAdapterLowThreads / 64, kCols = kAdapterLowCols;
   __shared__ float red[kWaves][16][kCols];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -117,7 +195,7 @@ __global__ __launch_bounds__(512) void adapter_low_kernel(AdapterArgs a, uint16_
   if (lane < rows) own = a.index[(m0 + lane) * a.index_stride];
   if (own >= a.count) own = -1;
   const uint16_t* x = static_cast<const uint16_t*>(a.x) + (m0 + min(l16, rows - 1)) * a.ldx + 8 * lg;
-  const int steps = (a.k + 31) / 32;
+  const int full = a.k / 32;
   unsigned long long left = __builtin_amdgcn_ballot_w64(own >= 0);
   for (int slot = 0; left != 0; ++slot) {
     const int l = __builtin_amdgcn_readlane(own, __builtin_ctzll(left));
@@ -128,46 +206,75 @@ __global__ __launch_bounds__(512) void adapter_low_kernel(AdapterArgs a, uint16_
     f32x4 acc[2][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[j][0] = acc[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = wave; s < steps; s += kWaves) {
-      const int k = 32 * s + 8 * lg;  // (K is a multiple of 8)
-      const bool in = k < a.k;
-      const u32x4 xf = in ? ld16(x + 32 * s) : u32x4{0, 0, 0, 0};
+    // columns past the rank repeat the first ones and are dropped
+    const uint16_t* a_row = A + (long long)(8 * lg) * a.a_k;
+    const int col0 = 2 * l16 < cols ? 2 * l16 : 0, col1 = 32 + 2 * l16 < cols ? 32 + 2 * l16 : 0;
+    auto product = [&](u32x4 xf, const uint32_t (&w)[8], int j) __attribute__((always_inline)) {
+      u32x4 even, odd;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (32 * j >= cols) break;
-        const bool there = in && 32 * j + 2 * l16 < cols;
-        uint32_t w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e] = there ? *reinterpret_cast<const uint32_t*>(A + (long long)(k + e) * a.a_k + 32 * j + 2 * l16) : 0u;
-        u32x4 even, odd;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          even[q] = lo_halves(w[2 * q], w[2 * q + 1]);
-          odd[q] = hi_halves(w[2 * q], w[2 * q + 1]);
-        }
-        acc[j][0] = H::mfma16(xf, even, acc[j][0]);
-        acc[j][1] = H::mfma16(xf, odd, acc[j][1]);
+      for (int q = 0; q < 4; ++q) {
+        even[q] = lo_halves(w[2 * q], w[2 * q + 1]);
+        odd[q] = hi_halves(w[2 * q], w[2 * q + 1]);
       }
+      acc[j][0] = H::mfma16(xf, even, acc[j][0]);
+      acc[j][1] = H::mfma16(xf, odd, acc[j][1]);
+    };
+    auto loop = [&](auto wide_tag) __attribute__((always_inline)) {
+      constexpr bool kWide = decltype(wide_tag)::value != 0;  // more than 32 columns
+#pragma unroll 2
+      for (int s0 = 2 * wave; s0 < full; s0 += 2 * kWaves) {  // 64 k: whole lines of x
+        u32x4 xf[2];
+        uint32_t w0[2][8], w1[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int s = min(s0 + u, full - 1);
+          xf[u] = ld16(x + 32 * s);
+          const uint16_t* row = a_row + (long long)(32 * s) * a.a_k;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            w0[u][e] = *reinterpret_cast<const uint32_t*>(row + e * a.a_k + col0);
+            if constexpr (kWide) w1[u][e] = *reinterpret_cast<const uint32_t*>(row + e * a.a_k + col1);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (s0 + u >= full) break;
+          product(xf[u], w0[u], 0);
+          if constexpr (kWide) product(xf[u], w1[u], 1);
+        }
+      }
+    };
+    if (cols > 32) loop(Int<1>{});
+    else loop(Int<0>{});
+    if (full * 32 < a.k && wave == kWaves - 1) {  // the last K % 32 (a multiple of 8): zeros in both operands
+      const bool in = 32 * full + 8 * lg < a.k;
+      const u32x4 xf = in ? ld16(x + 32 * full) : u32x4{0, 0, 0, 0};
+      uint32_t w0[8], w1[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t* row = a_row + (long long)(32 * full + e) * a.a_k;
+        w0[e] = in ? *reinterpret_cast<const uint32_t*>(row + col0) : 0u;
+        w1[e] = in ? *reinterpret_cast<const uint32_t*>(row + col1) : 0u;
+      }
+      product(xf, w0, 0);
+      product(xf, w1, 1);
     }
     __syncthreads();  // the sums of the adapter before are read
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        red[wave][4 * lg + e][32 * j + 2 * l16] = acc[j][0][e];
-        red[wave][4 * lg + e][32 * j + 2 * l16 + 1] = acc[j][1][e];
-      }
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x2*>(&red[wave][4 * lg + e][32 * j + 2 * l16]) = f32x2{acc[j][0][e], acc[j][1][e]};
     __syncthreads();
     const float scale = a.scale ? a.scale[l * a.scale_stride] : 1.f;
-    for (int y = tid; y < 16 * kCols / 2; y += 512) {
-      const int m = y / (kCols / 2), c = 2 * (y % (kCols / 2));
-      if (c >= cols || !(users >> m & 1ull)) continue;
-      float v0 = 0.f, v1 = 0.f;
+    if (tid < 16 * kCols / 2) {
+      const int m = tid / (kCols / 2), c = 2 * (tid % (kCols / 2));
+      if (c < cols && (users >> m & 1ull)) {
+        f32x2 sum = {0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) v0 += red[w][m][c], v1 += red[w][m][c + 1];
-      *reinterpret_cast<uint32_t*>(t + (long long)(m0 + m) * a.rank + c0 + c) = H::pack2(v0 * scale, v1 * scale);
+        for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x2*>(&red[w][m][c]);
+        *reinterpret_cast<uint32_t*>(t + (long long)(m0 + m) * a.rank + c0 + c) = H::pack2(sum[0] * scale, sum[1] * scale);
+      }
     }
   }
 }

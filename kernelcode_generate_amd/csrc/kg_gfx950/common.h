@@ -107,6 +107,14 @@ __device__ __forceinline__ uint32_t hi_halves(uint32_t x, uint32_t y) {
   return __builtin_amdgcn_perm(y, x, 0x07060302u);
 }
 
+// A pair of 16-bit elements with zeros in place of infinities and NaN; `found` gets a bit for each.
+template <typename H>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t& found) {
+  const uint32_t bad = ((w & H::kExpPair) + H::kExpUnitPair) & 0x80008000u;  // an exponent of ones carries
+  found |= bad;
+  return w & ~((bad >> 15) * 0xffffu);
+}
+
 // Transpose an 8x8 block of 16-bit elements held as 8 rows of 16 bytes.
 // in[r] holds row r (8 elements, element e in dword e/2, half e%2).
 // out[c] holds column c: element r of column c = in[r] element c.

@@ -34,8 +34,7 @@ __device__ __forceinline__ int a_swz(int row) { return (row >> 1) & 7; }
 
 // kRagged: M % 128, N % 128 or K % 64 non-zero: copies through buffer loads that land zeros
 // outside the matrices, and stores only inside.
-// kAdapters: low-rank adapters beside rhs (adapter.h): further slices of 64 k after the K loop's, kStages read at once,
-// into accumulators of their own.
+// kAdapters: low-rank adapters beside rhs (adapter.h): further slices of 64 k after the K loop's, kStages read at once.
 template <typename Tag, int kBias, int kStages, bool kRagged, bool kAdapters>
 __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mid_kernel(
     const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, uint16_t* __restrict__ C,
@@ -46,6 +45,7 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
   constexpr int kPieces = 8;  // copies per wave and slice: 4 lhs (8 rows each), 4 rhs (4 k-rows each)
   __shared__ __attribute__((aligned(1024))) char lds[kStages * 2 * kOperand];
   __shared__ int slot_lds[kAdapters ? kT : 1], row_lds[kAdapters ? kT : 1];  // adapters of the tile's slots and rows
+  __shared__ int found_lds;  // whether there are values of B that are not finite
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -141,28 +141,10 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
     if (st < nk)
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) issue_piece(st, st, p);
-  // The tile's distinct adapters, in the order of their first rows (each wave finds and writes the same).
-  int pieces = 0, total_pieces = 0;
+  int slots = 0;
   if constexpr (kAdapters) {
-    int own[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int m = m0 + 64 * u + lane;
-      own[u] = m < M ? part.index[m * part.index_stride] : -1;
-      if (own[u] < 0 || own[u] >= part.count) own[u] = -1;
-      row_lds[64 * u + lane] = own[u];
-    }
-    int slots = 0;
-    unsigned long long left[2] = {__builtin_amdgcn_ballot_w64(own[0] >= 0), __builtin_amdgcn_ballot_w64(own[1] >= 0)};
-    while ((left[0] | left[1]) != 0) {
-      const int l = left[0] != 0 ? __builtin_amdgcn_readlane(own[0], __builtin_ctzll(left[0]))
-                                 : __builtin_amdgcn_readlane(own[1], __builtin_ctzll(left[1]));
-      left[0] &= ~__builtin_amdgcn_ballot_w64(own[0] == l);
-      left[1] &= ~__builtin_amdgcn_ballot_w64(own[1] == l);
-      slot_lds[slots++] = l;
-    }
-    pieces = part.rank / 8;
-    total_pieces = slots * pieces;
+    if (tid == 0) found_lds = 0;
+    slots = adapter_slots<kT>(part, m0, M, lane, row_lds, slot_lds);
   }
   {
     const int younger = min(kStages, nk) - 1;
@@ -229,38 +211,34 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
   for (; kt + 2 * kStages <= nk; kt += kStages) turn(kt, Int<1>{});
   for (; kt < nk; kt += kStages) turn(kt, Int<0>{});
 
+  bool nonfinite = false;
   if constexpr (kAdapters) {
-    // A slice of the adapters' k, from wherever its eight-k pieces lie; zeros where a row uses another adapter.
-    auto issue_adapters = [&](int slice, int stage) __attribute__((always_inline)) {
-      const uint32_t dst = lds0 + stage * kStage + wave * 4096;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int row = (wave * 4 + p) * 8 + (lane >> 3);
-        const int piece = 8 * slice + ((lane & 7) ^ a_swz(row)), slot = div_page(piece, part.by_pieces);
-        const bool there = piece < total_pieces && slot_lds[min(slot, kT - 1)] == row_lds[row];
-        g2lds16_m(there ? part.t + (long long)(m0 + row) * part.rank + 8 * (piece - slot * pieces) : part.zeros, dst + p * 1024);
-      }
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int k = (wave * 4 + p) * 4 + (lane >> 4), bc = 8 * ((lane & 15) ^ b_mask(k));
-        const int piece = 8 * slice + (k >> 3), slot = div_page(piece, part.by_pieces);
-        const bool there = piece < total_pieces && n0 + bc < N;
-        const int l = slot_lds[min(slot, kT - 1)];
-        g2lds16_m(there ? part.b + l * part.b_l + (8 * (piece - slot * pieces) + (k & 7)) * part.b_r + n0 + bc : part.zeros,
-                  dst + kOperand + p * 1024);
-      }
-    };
-    f32x4 low[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; 8 * first < total_pieces; first += kStages) {
-      const int slices = min(kStages, (total_pieces + 7) / 8 - first);
+    const int pieces = part.rank / 8, slices = (slots * pieces + 7) / 8;
+    uint32_t found = 0;
+    for (int first = 0; first < slices; first += kStages) {
+      const int count = min(kStages, slices - first);
       wait_and_barrier<0>();  // the stages are read
-      for (int s = 0; s < slices; ++s) issue_adapters(first + s, s);
+      for (int s = 0; s < count; ++s) {
+        const uint32_t dst = lds0 + s * kStage + wave * 4096;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int row = (wave * 4 + p) * 8 + (lane >> 3);
+          const uint16_t* from = adapter_t(part, 8 * (first + s) + ((lane & 7) ^ a_swz(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
+          g2lds16_m(from ? from : part.zeros, dst + p * 1024);
+        }
+        u32x4 b[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int k = (wave * 4 + p) * 4 + (lane >> 4), bc = 8 * ((lane & 15) ^ b_mask(k));
+          const uint16_t* from = n0 + bc < N ? adapter_b(part, 8 * (first + s) + (k >> 3), pieces, slots, slot_lds, k & 7, n0 + bc) : nullptr;
+          b[p] = ld16(from ? from : part.zeros);
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p) adapter_put<H>(b[p], dst + kOperand + p * 1024 + lane * 16, found);
+      }
+      if (found != 0) found_lds = 1;
       wait_and_barrier<0>();
-      for (int s = 0; s < slices; ++s)
+      for (int s = 0; s < count; ++s)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
@@ -268,31 +246,10 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) low[i][j] = H::mfma16(fr[0].b[j], fr[0].a[i], low[i][j]);
+            for (int j = 0; j < 4; ++j) acc[i][j] = H::mfma16(fr[0].b[j], fr[0].a[i], acc[i][j]);
         }
     }
-    bool spoilt = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) spoilt |= !__builtin_isfinite((float)low[i][j][e]);
-    if (spoilt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int m = m0 + wm * 64 + 16 * i + l16, n = n0 + wn * 64 + 16 * j + 4 * lg + e;
-            if (!__builtin_isfinite((float)low[i][j][e])) low[i][j][e] = m < M && n < N ? adapter_alone<H>(part, m, n) : 0.f;
-          }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] += low[i][j];
+    nonfinite = found_lds != 0;
   }
 
   // ---- epilogue: lane holds C[m = l16][n = 4 lg .. +3] of each block. Each wave packs its quarter
@@ -329,6 +286,9 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
     const int m = m0 + wm * 64 + r, n = n0 + wn * 64 + 8 * c;
     if (kRagged && (m >= M || n >= N)) continue;
     __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(C + (long long)m * ldc + n));
+  }
+  if constexpr (kAdapters) {
+    if (nonfinite) adapter_add_nonfinite<H, 64, 8>(part, C, ldc, m0 + wm * 64, n0 + wn * 64, M, N, lane);
   }
 }
 

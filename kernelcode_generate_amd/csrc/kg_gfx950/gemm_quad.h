@@ -22,6 +22,7 @@
 // shorter launches than write-back stores at C2's shape).
 #pragma once
 
+#include "adapter.h"
 #include "common.h"
 #include "gemm.h"
 #include "lds_dma.h"
@@ -56,10 +57,11 @@ constexpr int kBPieces = 4;    // rhs copies per wave per slice (2 k-rows each)
 constexpr int kDefaultStages = 4;
 }  // namespace gemmq
 
-template <typename Tag, int kBias, int kStages, bool kExact, int kTM>
+// kAdapters: low-rank adapters beside rhs (adapter.h): further slices of 32 k after the K loop's, kStages read at once.
+template <typename Tag, int kBias, int kStages, bool kExact, int kTM, bool kAdapters>
 __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
     const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, uint16_t* __restrict__ C,
-    const void* __restrict__ bias, int M, int N, int K, long long lda, long long ldb, long long ldc) {
+    const void* __restrict__ bias, int M, int N, int K, long long lda, long long ldb, long long ldc, AdapterPart part) {
   using namespace gemmq;
   using gemmp::a_mask;
   using gemmp::a_slot;
@@ -80,6 +82,8 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
   static_assert(kCopyGap >= 4 && 2 * kReads <= kMfmas, "slots");
   __shared__ u32x4 lds_a[kStages][kVecsA];
   __shared__ u32x4 lds_b[kStages][kVecsB];
+  __shared__ int slot_lds[kAdapters ? kTM : 1], row_lds[kAdapters ? kTM : 1];  // adapters of the tile's slots and rows
+  __shared__ int found_lds;  // whether there are values of B that are not finite
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -183,6 +187,11 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
     if (st < ktiles)
 #pragma unroll
       for (int piece = 0; piece < kPieces; ++piece) issue_piece(st, st, piece);
+  int slots = 0;
+  if constexpr (kAdapters) {
+    if (tid == 0) found_lds = 0;
+    slots = adapter_slots<kTM>(part, m0, M, lane, row_lds, slot_lds);
+  }
   {
     const int younger = min(kStages - 1, ktiles - 1);
     if (younger >= 4) wait_and_barrier<4 * kPieces>();
@@ -266,6 +275,46 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
     for (; kt < ktiles; kt += U) unrolled(kt, Int<0>{});
   }
 
+  bool nonfinite = false;
+  if constexpr (kAdapters) {
+    const int pieces = part.rank / 8, slices = (slots * pieces + 3) / 4;
+    uint32_t found = 0;
+    for (int first = 0; first < slices; first += kStages) {
+      const int count = min(kStages, slices - first);
+      wait_and_barrier<0>();  // the stages are read
+      for (int s = 0; s < count; ++s) {
+#pragma unroll
+        for (int p = 0; p < kAPieces; ++p) {
+          const int row = (wave * kAPieces + p) * 16 + (lane >> 2);
+          const uint16_t* from =
+              adapter_t(part, 4 * (first + s) + ((lane & 3) ^ a_mask(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
+          g2lds16_m(from ? from : part.zeros, lds_a0 + s * kStageA + (wave * kAPieces + p) * 1024);
+        }
+        u32x4 b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = (wave * 4 + i) * 2 + (lane >> 5), bc = 8 * ((lane & 31) ^ b_mask(k));
+          const uint16_t* from = adapter_b(part, 4 * (first + s) + (k >> 3), pieces, slots, slot_lds, k & 7, n0 + bc);
+          b[i] = ld16(from ? from : part.zeros);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) adapter_put<H>(b[i], lds_b0 + s * kStageB + (wave * 4 + i) * 1024 + lane * 16, found);
+      }
+      if (found != 0) found_lds = 1;
+      wait_and_barrier<0>();
+#pragma unroll 1
+      for (int s = 0; s < count; ++s) {
+#pragma unroll
+        for (int x = 0; x < kReads; ++x) read_step(s, fr[0], x);
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mfma16_tied<Tag>(acc[i][j], fr[0].b[j], fr[0].a[i]);
+      }
+    }
+    nonfinite = found_lds != 0;
+  }
+
   // Epilogue: lane l holds C[m][n .. n+3] of block (i, j) (m = row block + l % 16, n = column
   // block + 4 (l / 16)). Stored as is, every store instruction would write 32-byte pieces of
   // 16 rows; instead each wave packs P row blocks at a time (bias added, rounded once) into an
@@ -322,19 +371,23 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
       __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(C + (long long)m * ldc + n0 + wn * 128 + 8 * c));
     }
   }
+  if constexpr (kAdapters) {
+    if (nonfinite) adapter_add_nonfinite<H, WM, 16>(part, C, ldc, m0 + wm * WM, n0 + wn * 128, M, N, lane);
+  }
 }
 
 // One launch of gemm_quad_kernel over (M/kTM) x (N/256) workgroups. bias_kind: 0 none,
 // 1 fp32, 2 16-bit.
-template <typename Tag, int kStages, int kTM>
+template <typename Tag, int kStages, int kTM, bool kAdapters>
 hipError_t launch_gemm_quad(const uint16_t* A, const uint16_t* B, uint16_t* C, const void* bias, int bias_kind, int M,
-                            int N, int K, long long lda, long long ldb, long long ldc, hipStream_t stream) {
+                            int N, int K, long long lda, long long ldb, long long ldc, const AdapterPart& part,
+                            hipStream_t stream) {
   const int grid = (M / kTM) * (N / gemmq::kT);
   const int ktiles = K / gemmq::kBK;
   const bool exact = kStages % 2 == 0 && ktiles % kStages == 0 && ktiles >= 2 * kStages;
 #define KG_GEMM_QUAD(BIAS, EXACT)                                                                                   \
-  hipLaunchKernelGGL((gemm_quad_kernel<Tag, BIAS, kStages, EXACT, kTM>), dim3(grid), dim3(gemmq::kThreads), 0, stream, A, \
-                     B, C, bias, M, N, K, lda, ldb, ldc)
+  hipLaunchKernelGGL((gemm_quad_kernel<Tag, BIAS, kStages, EXACT, kTM, kAdapters>), dim3(grid), dim3(gemmq::kThreads), 0, \
+                     stream, A, B, C, bias, M, N, K, lda, ldb, ldc, part)
   if constexpr (kStages % 2 == 0) {
     if (exact) {
       if (bias_kind == 0) KG_GEMM_QUAD(0, true);

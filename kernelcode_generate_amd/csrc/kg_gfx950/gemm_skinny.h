@@ -224,56 +224,45 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
       left &= ~__builtin_amdgcn_ballot_w64(own == l);
       if (lane == slots) listed = l;
     }
-    const int pieces = part.rank / 8, total_pieces = slots * pieces;
-    f32x4 low[kMT][2];
-#pragma unroll
-    for (int i = 0; i < kMT; ++i) low[i][0] = low[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int pieces = part.rank / 8, total_pieces = slots * pieces, n = min(n0 + 2 * l16, N - 2);
     for (int s = wave; 4 * s < total_pieces; s += kWaves) {
       const int piece = 4 * s + lg, slot = div_page(piece, part.by_pieces), r0 = 8 * (piece - slot * pieces);
       const int l = __shfl(listed, min(slot, 63), 64);
       const bool there = piece < total_pieces;
       Regs& f = r[0][0];
+      uint32_t found = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        f.b[e] = there ? S::load_b(reinterpret_cast<const char*>(part.b + l * part.b_l + (r0 + e) * part.b_r + min(n0 + 2 * l16, N - 2)))
-                       : 0u;
+        f.b[e] = there ? S::load_b(reinterpret_cast<const char*>(part.b + l * part.b_l + (r0 + e) * part.b_r + n)) : 0u;
 #pragma unroll
       for (int i = 0; i < kMT; ++i)
         f.a[i] = there && of_row[i] == l ? ld16(part.t + (long long)(m0 + 16 * i + l16) * part.rank + r0) : u32x4{0, 0, 0, 0};
-      S::mac(f, low);
-    }
-    bool spoilt = false;
 #pragma unroll
-    for (int i = 0; i < kMT; ++i)
+      for (int e = 0; e < 8; ++e) f.b[e] = finite_pair<Half16<Tag>>(f.b[e], found);
+      S::mac(f, acc);
+      if (__builtin_amdgcn_ballot_w64(found != 0) != 0) {  // this step's values that are not finite
 #pragma unroll
-      for (int e = 0; e < 4; ++e) spoilt |= !__builtin_isfinite((float)low[i][0][e]) || !__builtin_isfinite((float)low[i][1][e]);
-    if (__builtin_amdgcn_ballot_w64(spoilt) != 0) {
-      // this wave's pieces again, each row over its own adapter's
+        for (int i = 0; i < kMT; ++i)
 #pragma unroll
-      for (int i = 0; i < kMT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int m = 16 * i + 4 * lg + e, l_row = __shfl(own, m & 63, 64), n = min(n0 + 2 * l16, N - 2);
-          float v0 = 0.f, v1 = 0.f;
+          for (int e = 0; e < 4; ++e) {
+            const int m = 16 * i + 4 * lg + e, of_m = __shfl(own, m & 63, 64);
 #pragma unroll 1
-          for (int s = wave; 4 * s < total_pieces; s += kWaves)
+            for (int x = 4 * s; x < min(4 * s + 4, total_pieces); ++x) {
+              const int at = x / pieces, l_x = __builtin_amdgcn_readlane(listed, at);
+              if (of_m != l_x) continue;
+              const uint16_t* t = part.t + (long long)(m0 + m) * part.rank + 8 * (x - at * pieces);
+              const uint16_t* b = part.b + l_x * part.b_l + 8 * (x - at * pieces) * part.b_r + n;
 #pragma unroll 1
-            for (int piece = 4 * s; piece < min(4 * s + 4, total_pieces); ++piece) {
-              const int slot = piece / pieces, r0 = 8 * (piece - slot * pieces), l = __builtin_amdgcn_readlane(listed, slot);
-              if (l_row != l) continue;
-              const uint16_t *t = part.t + (long long)(m0 + m) * part.rank, *b = part.b + l * part.b_l + n;
-#pragma unroll 1
-              for (int q = r0; q < r0 + 8; ++q) {
-                v0 = __builtin_fmaf(Half16<Tag>::to_float(t[q]), Half16<Tag>::to_float(b[q * part.b_r]), v0);
-                v1 = __builtin_fmaf(Half16<Tag>::to_float(t[q]), Half16<Tag>::to_float(b[q * part.b_r + 1]), v1);
+              for (int q = 0; q < 8; ++q) {
+                const float tq = Half16<Tag>::to_float(t[q]), b0 = Half16<Tag>::to_float(b[q * part.b_r]),
+                            b1 = Half16<Tag>::to_float(b[q * part.b_r + 1]);
+                if (!__builtin_isfinite(b0)) acc[i][0][e] = __builtin_fmaf(tq, b0, (float)acc[i][0][e]);
+                if (!__builtin_isfinite(b1)) acc[i][1][e] = __builtin_fmaf(tq, b1, (float)acc[i][1][e]);
               }
             }
-          low[i][0][e] = v0;
-          low[i][1][e] = v1;
-        }
+          }
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kMT; ++i) acc[i][0] += low[i][0], acc[i][1] += low[i][1];
   }
 
   // lane holds C[m = 16 i + 4 lg + e][columns 2 l16, 2 l16 + 1]

@@ -45,22 +45,28 @@ KG_GEMM_PIPE_INSTANCES(F16Tag, 256, true)
 #undef KG_GEMM_PIPE_INSTANCE
 #endif
 
-#if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_GEMM_MID)
 #define KG_GEMM_MID_INSTANCE(TAG, ST, RAG, ADAPTERS)                                                                     \
   KG_INSTANCE hipError_t launch_gemm_mid<TAG, ST, RAG, ADAPTERS>(const uint16_t*, const uint16_t*, uint16_t*, const void*, int, \
                                                                  int, int, int, long long, long long, long long,           \
                                                                  const AdapterPart&, hipStream_t);
-#define KG_GEMM_MID_INSTANCES(TAG)                                                    \
-  KG_GEMM_MID_INSTANCE(TAG, 2, false, false) KG_GEMM_MID_INSTANCE(TAG, 2, true, false) \
-  KG_GEMM_MID_INSTANCE(TAG, 3, false, false) KG_GEMM_MID_INSTANCE(TAG, 3, true, false) \
-  KG_GEMM_MID_INSTANCE(TAG, 4, false, false) KG_GEMM_MID_INSTANCE(TAG, 4, true, false) \
-  KG_GEMM_MID_INSTANCE(TAG, 2, false, true) KG_GEMM_MID_INSTANCE(TAG, 2, true, true)   \
-  KG_GEMM_MID_INSTANCE(TAG, 4, false, true) KG_GEMM_MID_INSTANCE(TAG, 4, true, true)
-KG_GEMM_MID_INSTANCES(Bf16Tag)
-KG_GEMM_MID_INSTANCES(F16Tag)
+#define KG_GEMM_MID_INSTANCES(TAG, ST, ADAPTERS) \
+  KG_GEMM_MID_INSTANCE(TAG, ST, false, ADAPTERS) KG_GEMM_MID_INSTANCE(TAG, ST, true, ADAPTERS)
+#if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_GEMM_MID)
+KG_GEMM_MID_INSTANCES(Bf16Tag, 2, false)
+KG_GEMM_MID_INSTANCES(Bf16Tag, 3, false)
+KG_GEMM_MID_INSTANCES(Bf16Tag, 4, false)
+KG_GEMM_MID_INSTANCES(F16Tag, 2, false)
+KG_GEMM_MID_INSTANCES(F16Tag, 3, false)
+KG_GEMM_MID_INSTANCES(F16Tag, 4, false)
+#endif
+#if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_ADAPTER_MID)
+KG_GEMM_MID_INSTANCES(Bf16Tag, 2, true)
+KG_GEMM_MID_INSTANCES(Bf16Tag, 4, true)
+KG_GEMM_MID_INSTANCES(F16Tag, 2, true)
+KG_GEMM_MID_INSTANCES(F16Tag, 4, true)
+#endif
 #undef KG_GEMM_MID_INSTANCES
 #undef KG_GEMM_MID_INSTANCE
-#endif
 
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_GEMM_SKINNY)
 #define KG_GEMM_SKINNY_INSTANCE(TAG, ADAPTERS)                                                                          \
@@ -74,19 +80,26 @@ KG_GEMM_SKINNY_INSTANCE(F16Tag, true)
 #undef KG_GEMM_SKINNY_INSTANCE
 #endif
 
+#define KG_GEMM_QUAD_INSTANCE(TAG, ST, TM, ADAPTERS)                                                                       \
+  KG_INSTANCE hipError_t launch_gemm_quad<TAG, ST, TM, ADAPTERS>(const uint16_t*, const uint16_t*, uint16_t*, const void*, int, \
+                                                                 int, int, int, long long, long long, long long,           \
+                                                                 const AdapterPart&, hipStream_t);
+#define KG_GEMM_QUAD_INSTANCES(ST, TM, ADAPTERS) \
+  KG_GEMM_QUAD_INSTANCE(Bf16Tag, ST, TM, ADAPTERS) KG_GEMM_QUAD_INSTANCE(F16Tag, ST, TM, ADAPTERS)
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_GEMM_QUAD)
-#define KG_GEMM_QUAD_INSTANCE(TAG, ST, TM)                                                                              \
-  KG_INSTANCE hipError_t launch_gemm_quad<TAG, ST, TM>(const uint16_t*, const uint16_t*, uint16_t*, const void*, int, int, \
-                                                       int, int, long long, long long, long long, hipStream_t);
-#define KG_GEMM_QUAD_INSTANCES(TAG, TM) \
-  KG_GEMM_QUAD_INSTANCE(TAG, 2, TM) KG_GEMM_QUAD_INSTANCE(TAG, 3, TM) KG_GEMM_QUAD_INSTANCE(TAG, 4, TM)
-KG_GEMM_QUAD_INSTANCES(Bf16Tag, 256)
-KG_GEMM_QUAD_INSTANCES(Bf16Tag, 128)
-KG_GEMM_QUAD_INSTANCES(F16Tag, 256)
-KG_GEMM_QUAD_INSTANCES(F16Tag, 128)
+KG_GEMM_QUAD_INSTANCES(2, 256, false)
+KG_GEMM_QUAD_INSTANCES(3, 256, false)
+KG_GEMM_QUAD_INSTANCES(4, 256, false)
+KG_GEMM_QUAD_INSTANCES(2, 128, false)
+KG_GEMM_QUAD_INSTANCES(3, 128, false)
+KG_GEMM_QUAD_INSTANCES(4, 128, false)
+#endif
+#if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_ADAPTER_QUAD)
+KG_GEMM_QUAD_INSTANCES(4, 256, true)
+KG_GEMM_QUAD_INSTANCES(4, 128, true)
+#endif
 #undef KG_GEMM_QUAD_INSTANCES
 #undef KG_GEMM_QUAD_INSTANCE
-#endif
 
 // The persistent attention form: its own translation unit; every other one, the attention
 // family's included, sees `extern template` declarations (ahead of the attention launchers

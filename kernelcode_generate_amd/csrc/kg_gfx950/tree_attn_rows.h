@@ -86,14 +86,6 @@ __device__ __forceinline__ void load_v(uint32_t (&v)[kDwords], const C* p) {
   }
 }
 
-// A pair of 16-bit elements with zeros in place of infinities and NaN; `found` gets a bit for each.
-template <typename H>
-__device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t& found) {
-  const uint32_t bad = ((w & H::kExpPair) + H::kExpUnitPair) & 0x80008000u;  // an exponent of ones carries
-  found |= bad;
-  return w & ~((bad >> 15) * 0xffffu);
-}
-
 template <typename C>
 constexpr bool kScaled = CacheElem<C>::kScaled;
 template <>

@@ -160,7 +160,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
       auto put_v = [&](uint32_t to, u32x4 x) __attribute__((always_inline)) {
         if (sift) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = treer::finite_pair<H>(x[q], found);
+          for (int q = 0; q < 4; ++q) x[q] = finite_pair<H>(x[q], found);
         }
         put(to, x);
       };

