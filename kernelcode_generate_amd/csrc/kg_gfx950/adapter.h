@@ -2,12 +2,13 @@
 //   out[m] = x[m] W + bias + scale[l] (x[m] A[l]) B[l],    A [L, K, R], B [L, R, N];
 // an index outside 0..L-1 is a row without one.
 //
-// 16-bit calls of whole 16-byte rows: adapter_low_kernel writes t = scale x A, rounded to the operands' type as
-// a 16-bit layer's output is, to a workspace [M, R]; then the projection's kernels (gemm_skinny.h, gemm_mid.h, gemm_quad.h)
-// take the adapters as further k behind their own: the distinct adapters of a tile's rows, one after the other, R
+// 16-bit calls of whole 16-byte rows: adapter_low_kernel writes t = scale x A in 32 bits, as sums over ranges of K, to a
+// workspace; then the projection's kernels (gemm_skinny.h,
+// gemm_mid.h, gemm_quad.h, gemm.h) take the adapters as further k behind their own: the distinct adapters of a tile's rows, one after the other, R
 // values each, t's rows in the slots of their adapter and zeros in the others. A value of B that is not finite, times
 // the zeros of rows that do not use it, would be NaN in them: the products run on zeros in place of such values, and
-// where there were any each output adds those of its own row's adapter (adapter_nonfinite).
+// where there were any each output adds those of its own row's adapter (adapter_nonfinite). For the products t is
+// rounded to the operands' type, as the output of a 16-bit layer would be.
 //
 // adapter_add_kernel: any types and strides, one workgroup per row: t = scale x A in 32 bits, then
 // out += t B, on an output that holds the projection already (matmul's kernels). A 16-bit output is
@@ -75,27 +76,46 @@ __global__ __launch_bounds__(256) void adapter_add_kernel(AdapterArgs p) {
   }
 }
 
-// The adapters' part of a projection, for its kernels: t [M, rank] 16-bit behind 16 bytes of zeros.
+// The adapters' part of a projection, for its kernels. sums: t as [splits, M, rank] sums over ranges of K; zeros: 16 bytes of zeros.
 struct AdapterPart {
-  const uint16_t *t, *zeros, *b;
+  const float* sums;
+  const uint16_t *zeros, *b;
   const int* index;
-  long long b_l, b_r, index_stride;
-  int rank, count;  // rank % 8 == 0
-  PageDiv by_pieces;  // division by rank / 8
+  long long split_pitch, b_l, b_r, index_stride;  // split_pitch: M rank
+  int splits, rank, count;                        // rank % 8 == 0
+  PageDiv by_pieces;                              // division by rank / 8
 };
-constexpr size_t kAdapterHeader = 256;  // bytes of the workspace before t
+// Eight elements of t from `at` on, rounded.
+constexpr int kAdapterMaxSplits = 8;
+template <typename H>
+__device__ __forceinline__ u32x4 adapter_t8(const AdapterPart& p, const float* at) {
+  f32x4 a = *reinterpret_cast<const f32x4*>(at), b = *reinterpret_cast<const f32x4*>(at + 4);
+#pragma unroll
+  for (int y = 1; y < kAdapterMaxSplits; ++y) {  // (unrolled: the reads are in flight together)
+    if (y >= p.splits) break;
+    a += *reinterpret_cast<const f32x4*>(at + y * p.split_pitch);
+    b += *reinterpret_cast<const f32x4*>(at + y * p.split_pitch + 4);
+  }
+  return u32x4{H::pack2(a[0], a[1]), H::pack2(a[2], a[3]), H::pack2(b[0], b[1]), H::pack2(b[2], b[3])};
+}
+constexpr size_t kAdapterHeader = 256;  // bytes of the workspace before the sums: zeros
 
 // The sum of t[m, r] B[l, r, n] over the B that are not finite, l row m's adapter.
 template <typename H>
 __device__ __forceinline__ float adapter_nonfinite(const AdapterPart& p, int m, int n) {
   const int l = p.index[m * p.index_stride];
   if (l < 0 || l >= p.count) return 0.f;
-  const uint16_t *t = p.t + (long long)m * p.rank, *b = p.b + l * p.b_l + n;
+  const float* t = p.sums + (long long)m * p.rank;
+  const uint16_t* b = p.b + l * p.b_l + n;
   float sum = 0.f;
 #pragma unroll 1
   for (int r = 0; r < p.rank; ++r) {
     const float x = H::to_float(b[r * p.b_r]);
-    if (!__builtin_isfinite(x)) sum = __builtin_fmaf(H::to_float(t[r]), x, sum);
+    if (__builtin_isfinite(x)) continue;
+    float tr = 0.f;
+#pragma unroll 1
+    for (int y = 0; y < p.splits; ++y) tr += t[y * p.split_pitch + r];
+    sum = __builtin_fmaf(tr, x, sum);
   }
   return sum;
 }
@@ -117,6 +137,27 @@ __device__ __forceinline__ void adapter_add_nonfinite(const AdapterPart& p, uint
       const float x = adapter_nonfinite<H>(p, m, n + u);
       uint16_t* out = C + (long long)m * ldc + n + u;
       if (x != 0.f) *out = (uint16_t)H::from_float(H::to_float(*out) + x);
+    }
+  }
+}
+
+// The same for the epilogues whose lanes hold 4 columns of a row in each of kM x kN blocks of 16 x 16: outputs
+// (pitch ldc) or, before they are summed, fp32 partial sums.
+template <typename H, int kM, int kN, typename T>
+__device__ __forceinline__ void adapter_add_nonfinite_blocks(const AdapterPart& p, T* C, long long ldc, int m0, int n0, int M, int N,
+                                                             int lane) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll 1
+  for (int i = 0; i < kM * kN; ++i) {
+    const int m = m0 + 16 * (i / kN) + (lane & 15), n = n0 + 16 * (i % kN) + 4 * (lane >> 4);
+    if (m >= M || n >= N) continue;
+#pragma unroll 1
+    for (int u = 0; u < 4; ++u) {
+      const float x = adapter_nonfinite<H>(p, m, n + u);
+      T* out = C + (long long)m * ldc + n + u;
+      if (x == 0.f) continue;
+      if constexpr (sizeof(T) == 4) *out += x;
+      else *out = (T)H::from_float(H::to_float(*out) + x);
     }
   }
 }
@@ -154,16 +195,22 @@ __device__ __forceinline__ int adapter_slots(const AdapterPart& p, int m0, int M
   return slots;
 }
 
-// Where the 16 bytes of a tile's row (t) or of a k-row's columns (B) of an eight-k piece lie; null: zeros.
-__device__ __forceinline__ const uint16_t* adapter_t(const AdapterPart& p, int piece, int pieces, int slots, const int* slot_lds, int l,
-                                                     int m) {
+// Where a tile's row of t, or a k-row's columns of B, of an eight-k piece lie; null: zeros.
+__device__ __forceinline__ const float* adapter_t(const AdapterPart& p, int piece, int pieces, int slots, const int* slot_lds, int l,
+                                                  int m) {
   const int slot = div_page(piece, p.by_pieces);
-  return slot < slots && slot_lds[slot] == l ? p.t + (long long)m * p.rank + 8 * (piece - slot * pieces) : nullptr;
+  return slot < slots && slot_lds[slot] == l ? p.sums + (long long)m * p.rank + 8 * (piece - slot * pieces) : nullptr;
 }
 __device__ __forceinline__ const uint16_t* adapter_b(const AdapterPart& p, int piece, int pieces, int slots, const int* slot_lds, int k,
                                                      int n) {
   const int slot = div_page(piece, p.by_pieces);
   return slot < slots ? p.b + slot_lds[slot] * p.b_l + (8 * (piece - slot * pieces) + k) * p.b_r + n : nullptr;
+}
+template <typename H>
+__device__ __forceinline__ void adapter_put_t(const AdapterPart& p, const float* from, uint32_t to) {
+  u32x4 x = {0, 0, 0, 0};
+  if (from) x = adapter_t8<H>(p, from);
+  *(__attribute__((address_space(3))) u32x4*)(uintptr_t)to = x;
 }
 // 16 bytes of B from there to LDS, zeros in place of what is not finite; `found` gets bits for that.
 template <typename H>
@@ -173,108 +220,117 @@ __device__ __forceinline__ void adapter_put(u32x4 x, uint32_t to, uint32_t& foun
   *(__attribute__((address_space(3))) u32x4*)(uintptr_t)to = x;
 }
 
-// t = scale x A of 16 rows and up to 64 columns (blockIdx.z) per workgroup: its sixteen waves share K in steps of
-// 32, lanes hold two columns of A by eight k as in gemm_skinny.h, one sum over the waves through LDS. A workgroup takes every
+// t = scale x A of 16 rows and up to 64 columns (blockIdx.z) per workgroup, whose four waves share a range of K (blockIdx.x)
+// in pieces of 64 and end in one sum through LDS. A step of 32 k is one 16-byte load per lane of x and one of each 16 columns of A (rows
+// of k, 32 bytes), which turn through a wave's own 1 KiB of LDS into MFMA operands (ds_read_b64_tr_b16; rows with
+// bit 3 set half a bank row apart); as many steps as registers hold are in flight at once. (Columns loaded as
+// pairs straight into operands took eight loads a step, 10 us for the first call below.) A workgroup takes every
 // gridDim.y-th of its rows' distinct adapters and stores the rows that use it: few rows have many adapters
-// (gridDim.y workgroups read them at once), many rows few. 16 x 4096, 16 adapters of rank 16: LOW_STEP us; 4096 x 4096 in
-// runs: LOW_PROMPTS us, the reading of x.
-constexpr int kAdapterLowThreads = 1024, kAdapterLowCols = 64;
+// (gridDim.y workgroups read them at once), many rows few. Few rows also share out K over up to eight workgroups: one CU reads
+// some 16 bytes a clock. 16 x 4096, 16 adapters of rank 16: 5.4 us
+// (one workgroup of 16 waves over all of K: 10); 4096 x 4096 in runs: 13.4 us, 2.5 TB/s of x (16.7).
+constexpr int kAdapterLowThreads = 256, kAdapterLowCols = 64;
 template <typename Tag>
-__global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(AdapterArgs a, uint16_t* __restrict__ t, uint32_t* __restrict__ zeros) {
+__global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(AdapterArgs a, uint32_t* __restrict__ zeros,
+                                                                          float* __restrict__ sums, int splits) {
   using H = Half16<Tag>;
   constexpr int kWaves = kAdapterLowThreads / 64, kCols = kAdapterLowCols;
-  __shared__ float red[kWaves][16][kCols];
+  static_assert(kAdapterLowThreads == 4 * kCols, "a thread per column and four rows in the sum over the waves");
+  __shared__ __attribute__((aligned(16))) float red[kWaves][kCols][16 + 4];
+  __shared__ __attribute__((aligned(1024))) char turn[kWaves * 1024];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
-  const int m0 = blockIdx.x * 16, rows = min(a.m - m0, 16), c0 = blockIdx.z * kCols;
+  const int split = blockIdx.x % splits, m0 = blockIdx.x / splits * 16, rows = min(a.m - m0, 16), c0 = blockIdx.z * kCols;
   const int cols = min(a.rank - c0, kCols);
+  // this range's K, as a product of its own (ranges of whole pieces of 64)
+  const int range = ((a.k + 63) / 64 + splits - 1) / splits * 64;
+  const int k_begin = split * range, k_end = min(a.k - k_begin, range);
   if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && tid < 4) zeros[tid] = 0;
 
   int own = -1;  // adapter of row `lane`
   if (lane < rows) own = a.index[(m0 + lane) * a.index_stride];
   if (own >= a.count) own = -1;
-  const uint16_t* x = static_cast<const uint16_t*>(a.x) + (m0 + min(l16, rows - 1)) * a.ldx + 8 * lg;
-  const int full = a.k / 32;
+  const uint16_t* x = static_cast<const uint16_t*>(a.x) + (m0 + min(l16, rows - 1)) * a.ldx + k_begin + 8 * lg;
+  // this lane's part of 32 rows of 16 columns, and its read addresses (k-rows 8 lg + 0..3, then + 4)
+  const int k_row = lane >> 1, half = lane & 1;
+  auto turned = [](int k) { return (k * 32) ^ ((k & 8) << 4); };
+  const uint32_t turn0 = lds_addr(turn) + wave * 1024;
+  const uint32_t put_at = turn0 + turned(k_row) + 16 * half;
+  const uint32_t get_at = turn0 + turned(8 * lg + (l16 >> 2)) + 8 * (l16 & 3);
+  const int steps = (k_end + 31) / 32;
   unsigned long long left = __builtin_amdgcn_ballot_w64(own >= 0);
   for (int slot = 0; left != 0; ++slot) {
     const int l = __builtin_amdgcn_readlane(own, __builtin_ctzll(left));
     const unsigned long long users = __builtin_amdgcn_ballot_w64(own == l);
     left &= ~users;
     if (slot % gridDim.y != blockIdx.y) continue;
-    const uint16_t* A = static_cast<const uint16_t*>(a.a) + l * a.a_l + c0;
-    f32x4 acc[2][2];
+    const float scale = a.scale ? a.scale[l * a.scale_stride] : 1.f;
+    const uint16_t* A = static_cast<const uint16_t*>(a.a) + l * a.a_l + c0 + (long long)(k_begin + k_row) * a.a_k;
+    f32x4 acc[4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[j][0] = acc[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // columns past the rank repeat the first ones and are dropped
-    const uint16_t* a_row = A + (long long)(8 * lg) * a.a_k;
-    const int col0 = 2 * l16 < cols ? 2 * l16 : 0, col1 = 32 + 2 * l16 < cols ? 32 + 2 * l16 : 0;
-    auto product = [&](u32x4 xf, const uint32_t (&w)[8], int j) __attribute__((always_inline)) {
-      u32x4 even, odd;
+    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto loop = [&](auto blocks_tag) __attribute__((always_inline)) {
+      constexpr int kBlocks = decltype(blocks_tag)::value;  // of 16 columns
+      constexpr int kAhead = 4;                             // steps in flight
+      // columns past the rank repeat the first ones and are dropped
+      int col[kBlocks];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        even[q] = lo_halves(w[2 * q], w[2 * q + 1]);
-        odd[q] = hi_halves(w[2 * q], w[2 * q + 1]);
-      }
-      acc[j][0] = H::mfma16(xf, even, acc[j][0]);
-      acc[j][1] = H::mfma16(xf, odd, acc[j][1]);
-    };
-    auto loop = [&](auto wide_tag) __attribute__((always_inline)) {
-      constexpr bool kWide = decltype(wide_tag)::value != 0;  // more than 32 columns
-#pragma unroll 2
-      for (int s0 = 2 * wave; s0 < full; s0 += 2 * kWaves) {  // 64 k: whole lines of x
-        u32x4 xf[2];
-        uint32_t w0[2][8], w1[2][8];
+      for (int j = 0; j < kBlocks; ++j) col[j] = 16 * j + 8 * half < cols ? 16 * j + 8 * half : 0;
+      // step i of this wave: two consecutive ones of every four pairs, whole 128-byte lines of x
+      auto step_of = [&](int i) { return 2 * (wave + kWaves * (i >> 1)) + (i & 1); };
+      for (int i0 = 0; step_of(i0) < steps; i0 += kAhead) {
+        u32x4 xf[kAhead], af[kAhead][kBlocks];
+        if (k_end % 32 == 0) {  // (steps past the last repeat it and are not used)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int s = min(s0 + u, full - 1);
-          xf[u] = ld16(x + 32 * s);
-          const uint16_t* row = a_row + (long long)(32 * s) * a.a_k;
+          for (int u = 0; u < kAhead; ++u) {
+            const int k = min(32 * step_of(i0 + u), k_end - 32);
+            xf[u] = ld16(x + k);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            w0[u][e] = *reinterpret_cast<const uint32_t*>(row + e * a.a_k + col0);
-            if constexpr (kWide) w1[u][e] = *reinterpret_cast<const uint32_t*>(row + e * a.a_k + col1);
+            for (int j = 0; j < kBlocks; ++j) af[u][j] = ld16(A + (long long)k * a.a_k + col[j]);
+          }
+        } else {  // past K (a multiple of 8): zeros, in both operands
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int k = 32 * step_of(i0 + u);
+            xf[u] = k + 8 * lg < k_end ? ld16(x + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < kBlocks; ++j)
+              af[u][j] = k + k_row < k_end ? ld16(A + (long long)k * a.a_k + col[j]) : u32x4{0, 0, 0, 0};
           }
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (s0 + u >= full) break;
-          product(xf[u], w0[u], 0);
-          if constexpr (kWide) product(xf[u], w1[u], 1);
+        for (int u = 0; u < kAhead; ++u) {
+          if (step_of(i0 + u) >= steps) break;
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) {
+            // (a wave's LDS operations run in order: the reads of the block before are done)
+            *(__attribute__((address_space(3))) u32x4*)(uintptr_t)put_at = af[u][j];
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)get_at);
+            const s16x4 v1 =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(get_at ^ 128));
+            const u32x2 lo = __builtin_bit_cast(u32x2, v0), hi = __builtin_bit_cast(u32x2, v1);
+            acc[j] = H::mfma16(xf[u], u32x4{lo[0], lo[1], hi[0], hi[1]}, acc[j]);
+          }
         }
       }
     };
-    if (cols > 32) loop(Int<1>{});
-    else loop(Int<0>{});
-    if (full * 32 < a.k && wave == kWaves - 1) {  // the last K % 32 (a multiple of 8): zeros in both operands
-      const bool in = 32 * full + 8 * lg < a.k;
-      const u32x4 xf = in ? ld16(x + 32 * full) : u32x4{0, 0, 0, 0};
-      uint32_t w0[8], w1[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint16_t* row = a_row + (long long)(32 * full + e) * a.a_k;
-        w0[e] = in ? *reinterpret_cast<const uint32_t*>(row + col0) : 0u;
-        w1[e] = in ? *reinterpret_cast<const uint32_t*>(row + col1) : 0u;
-      }
-      product(xf, w0, 0);
-      product(xf, w1, 1);
-    }
+    if (cols > 32) loop(Int<4>{});
+    else if (cols > 16) loop(Int<2>{});
+    else loop(Int<1>{});
     __syncthreads();  // the sums of the adapter before are read
+    // column-major: a lane's four rows in one write
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(&red[wave][16 * j + l16][4 * lg]) = acc[j];
+    __syncthreads();
+    const int c = tid % kCols, r0 = 4 * (tid / kCols);
+    if (c < cols) {
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x4*>(&red[w][c][r0]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<f32x2*>(&red[wave][4 * lg + e][32 * j + 2 * l16]) = f32x2{acc[j][0][e], acc[j][1][e]};
-    __syncthreads();
-    const float scale = a.scale ? a.scale[l * a.scale_stride] : 1.f;
-    if (tid < 16 * kCols / 2) {
-      const int m = tid / (kCols / 2), c = 2 * (tid % (kCols / 2));
-      if (c < cols && (users >> m & 1ull)) {
-        f32x2 sum = {0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x2*>(&red[w][m][c]);
-        *reinterpret_cast<uint32_t*>(t + (long long)(m0 + m) * a.rank + c0 + c) = H::pack2(sum[0] * scale, sum[1] * scale);
-      }
+        if (users >> (r0 + e) & 1ull) sums[((long long)split * a.m + m0 + r0 + e) * a.rank + c0 + c] = sum[e] * scale;
     }
   }
 }

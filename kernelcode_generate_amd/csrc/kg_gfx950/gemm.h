@@ -10,6 +10,7 @@
 //   4x4 outputs per thread, fp32 FMA accumulation in k order.
 #pragma once
 
+#include "adapter.h"
 #include "common.h"
 #include "lds_dma.h"
 
@@ -59,11 +60,13 @@ struct StageIdx {
 };
 }  // namespace gemmp
 
-template <typename Tag, int kBias, int kTM, int kStages, bool kRagged>
+// kAdapters: low-rank adapters beside rhs (adapter.h): further slices of 32 k after the K loop's (the first K range's), kStages
+// read at once.
+template <typename Tag, int kBias, int kTM, int kStages, bool kRagged, bool kAdapters>
 __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
     const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, uint16_t* __restrict__ C,
     const void* __restrict__ bias, int M, int N, int K, long long lda, long long ldb, long long ldc,
-    float* __restrict__ partial, int k_chunk) {
+    float* __restrict__ partial, int k_chunk, AdapterPart part) {
   using namespace gemmp;
   using H = Half16<Tag>;
   static_assert(kTM == 256 || kTM == 128, "tile height");
@@ -86,6 +89,8 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
   constexpr int kAVecs = kTM * kBK / 8;     // u32x4 per lhs stage
   __shared__ u32x4 lds_a[kStages][kAVecs];
   __shared__ u32x4 lds_b[kStages][kBVecs];
+  __shared__ int slot_lds[kAdapters ? kTM : 1], row_lds[kAdapters ? kTM : 1];  // adapters of the tile's slots and rows
+  __shared__ int found_lds;  // whether there are values of B that are not finite
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -211,6 +216,11 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
     if (st < ktiles)
 #pragma unroll
       for (int piece = 0; piece < kPieces; ++piece) issue_piece(st, st, piece);
+  int slots = 0;
+  if constexpr (kAdapters) {
+    if (tid == 0) found_lds = 0;
+    if (blockIdx.y == 0) slots = adapter_slots<kTM>(part, m0, M, lane, row_lds, slot_lds);
+  }
   {
     const int younger = min(kStages - 1, ktiles - 1);
     if (younger >= 3) wait_and_barrier<3 * kPieces>();
@@ -299,6 +309,48 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
   for (; kt + U + kStages <= ktiles; kt += U) unrolled(kt, StageIdx<1>{});  // every slice refills its stage
   for (; kt < ktiles; kt += U) unrolled(kt, StageIdx<0>{});
 
+  bool nonfinite = false;
+  if constexpr (kAdapters) {
+    const int pieces = part.rank / 8, slices = (slots * pieces + 3) / 4;
+    uint32_t found = 0;
+    for (int first = 0; first < slices; first += kStages) {
+      const int count = min(kStages, slices - first);
+      wait_and_barrier<0>();  // the stages are read
+      for (int s = 0; s < count; ++s) {
+#pragma unroll
+        for (int p = 0; p < AP; ++p) {
+          const int row = (wave * AP + p) * 16 + (lane >> 2);
+          const float* from =
+              adapter_t(part, 4 * (first + s) + ((lane & 3) ^ a_mask(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
+          adapter_put_t<H>(part, from, lds_a0 + s * kAStage + (wave * AP + p) * 1024 + lane * 16);
+        }
+        u32x4 b[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int k = (wave * 2 + i) * 2 + (lane >> 5), bc = 8 * ((lane & 31) ^ b_mask(k));
+          const uint16_t* from = n0 + bc < N ? adapter_b(part, 4 * (first + s) + (k >> 3), pieces, slots, slot_lds, k & 7, n0 + bc) : nullptr;
+          b[i] = ld16(from ? from : part.zeros);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) adapter_put<H>(b[i], lds_b0 + s * kBStage + (wave * 2 + i) * 1024 + lane * 16, found);
+      }
+      if (found != 0) found_lds = 1;
+      wait_and_barrier<0>();
+#pragma unroll 1
+      for (int s = 0; s < count; ++s) {
+#pragma unroll
+        for (int x = 0; x < NRX; ++x) read_x(s, fr[0], x);
+#pragma unroll
+        for (int x = 0; x < MH; ++x) fy[x] = read_a(s, MH + x);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = H::mfma16(fr[0].b[j], i < MH ? fr[0].a[i % MH] : fy[i % MH], acc[i][j]);
+      }
+    }
+    nonfinite = found_lds != 0;
+  }
+
   // Epilogue: lane l holds C[m][n .. n+3] of block (ib, nb): m = row block + l % 16, n = column
   // block + 4 (l / 16).
   auto out_value = [&](int i, int j, int n) -> u32x2 {  // bias added, rounded once
@@ -321,7 +373,7 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
     packed[1] = H::pack2(v2, v3);
     return packed;
   };
-  if (!kRagged && k_chunk == 0) {
+  if (!kRagged && !kAdapters && k_chunk == 0) {
     // Whole tiles: each wave packs P row blocks at a time into an LDS region of its own,
     // [16P rows][64 columns], and writes them back as whole 128-byte row segments (16 bytes
     // per lane, 8 rows per instruction) instead of 32-byte pieces of 16 rows. 16-byte chunk c
@@ -369,6 +421,13 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
         }
         st8(C + (long long)m * ldc + n, out_value(i, j, n));
       }
+    }
+  }
+  if constexpr (kAdapters) {
+    if (nonfinite) {
+      const int m = m0 + wm * (kTM / 2), n = n0 + wn * 64;
+      if (k_chunk > 0) adapter_add_nonfinite_blocks<H, MB, 4>(part, partial, N, m, n, M, N, lane);
+      else adapter_add_nonfinite_blocks<H, MB, 4>(part, C, ldc, m, n, M, N, lane);
     }
   }
 }
@@ -495,13 +554,13 @@ __global__ __launch_bounds__(256) void gemm_simt_kernel(const TA* __restrict__ A
 // One launch of gemm_pipe_kernel (grid x splits workgroups; splits > 1: fp32 partials of
 // k_chunk-deep K chunks into `partial`, reduced by gemm_splitk_reduce_kernel afterwards).
 // bias_kind: 0 none, 1 fp32, 2 16-bit.
-template <typename Tag, int kTM, int kStages, bool kRagged>
+template <typename Tag, int kTM, int kStages, bool kRagged, bool kAdapters>
 hipError_t launch_gemm_pipe(const uint16_t* A, const uint16_t* B, uint16_t* C, const void* bias, int bias_kind, int M,
                             int N, int K, long long lda, long long ldb, long long ldc, float* partial, int k_chunk,
-                            int grid, int splits, hipStream_t stream) {
+                            int grid, int splits, const AdapterPart& part, hipStream_t stream) {
 #define KG_GEMM_PIPE(BIAS)                                                                                             \
-  hipLaunchKernelGGL((gemm_pipe_kernel<Tag, BIAS, kTM, kStages, kRagged>), dim3(grid, splits), dim3(gemmp::kThreads), 0, \
-                     stream, A, B, C, bias, M, N, K, lda, ldb, ldc, partial, k_chunk)
+  hipLaunchKernelGGL((gemm_pipe_kernel<Tag, BIAS, kTM, kStages, kRagged, kAdapters>), dim3(grid, splits), \
+                     dim3(gemmp::kThreads), 0, stream, A, B, C, bias, M, N, K, lda, ldb, ldc, partial, k_chunk, part)
   if (bias_kind == 0) KG_GEMM_PIPE(0);
   else if (bias_kind == 1) KG_GEMM_PIPE(1);
   else KG_GEMM_PIPE(2);

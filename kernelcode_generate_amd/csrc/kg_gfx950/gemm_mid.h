@@ -223,8 +223,8 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           const int row = (wave * 4 + p) * 8 + (lane >> 3);
-          const uint16_t* from = adapter_t(part, 8 * (first + s) + ((lane & 7) ^ a_swz(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
-          g2lds16_m(from ? from : part.zeros, dst + p * 1024);
+          const float* from = adapter_t(part, 8 * (first + s) + ((lane & 7) ^ a_swz(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
+          adapter_put_t<H>(part, from, dst + p * 1024 + lane * 16);
         }
         u32x4 b[4];
 #pragma unroll

@@ -286,9 +286,9 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
 #pragma unroll
         for (int p = 0; p < kAPieces; ++p) {
           const int row = (wave * kAPieces + p) * 16 + (lane >> 2);
-          const uint16_t* from =
+          const float* from =
               adapter_t(part, 4 * (first + s) + ((lane & 3) ^ a_mask(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
-          g2lds16_m(from ? from : part.zeros, lds_a0 + s * kStageA + (wave * kAPieces + p) * 1024);
+          adapter_put_t<H>(part, from, lds_a0 + s * kStageA + (wave * kAPieces + p) * 1024 + lane * 16);
         }
         u32x4 b[4];
 #pragma unroll

@@ -235,8 +235,11 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
       for (int e = 0; e < 8; ++e)
         f.b[e] = there ? S::load_b(reinterpret_cast<const char*>(part.b + l * part.b_l + (r0 + e) * part.b_r + n)) : 0u;
 #pragma unroll
-      for (int i = 0; i < kMT; ++i)
-        f.a[i] = there && of_row[i] == l ? ld16(part.t + (long long)(m0 + 16 * i + l16) * part.rank + r0) : u32x4{0, 0, 0, 0};
+      for (int i = 0; i < kMT; ++i) {
+        f.a[i] = u32x4{0, 0, 0, 0};
+        if (there && of_row[i] == l)
+          f.a[i] = adapter_t8<Half16<Tag>>(part, part.sums + (long long)(m0 + 16 * i + l16) * part.rank + r0);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) f.b[e] = finite_pair<Half16<Tag>>(f.b[e], found);
       S::mac(f, acc);
@@ -250,11 +253,13 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
             for (int x = 4 * s; x < min(4 * s + 4, total_pieces); ++x) {
               const int at = x / pieces, l_x = __builtin_amdgcn_readlane(listed, at);
               if (of_m != l_x) continue;
-              const uint16_t* t = part.t + (long long)(m0 + m) * part.rank + 8 * (x - at * pieces);
+              const float* t = part.sums + (long long)(m0 + m) * part.rank + 8 * (x - at * pieces);
               const uint16_t* b = part.b + l_x * part.b_l + 8 * (x - at * pieces) * part.b_r + n;
 #pragma unroll 1
               for (int q = 0; q < 8; ++q) {
-                const float tq = Half16<Tag>::to_float(t[q]), b0 = Half16<Tag>::to_float(b[q * part.b_r]),
+                float tq = 0.f;
+                for (int y = 0; y < part.splits; ++y) tq += t[y * part.split_pitch + q];
+                const float b0 = Half16<Tag>::to_float(b[q * part.b_r]),
                             b1 = Half16<Tag>::to_float(b[q * part.b_r + 1]);
                 if (!__builtin_isfinite(b0)) acc[i][0][e] = __builtin_fmaf(tq, b0, (float)acc[i][0][e]);
                 if (!__builtin_isfinite(b1)) acc[i][1][e] = __builtin_fmaf(tq, b1, (float)acc[i][1][e]);

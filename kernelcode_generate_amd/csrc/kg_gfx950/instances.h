@@ -26,13 +26,15 @@
 
 namespace kg_gfx950 {
 
+#define KG_GEMM_PIPE_INSTANCE(TAG, TM, ST, RAG, ADAPTERS)                                                                  \
+  KG_INSTANCE hipError_t launch_gemm_pipe<TAG, TM, ST, RAG, ADAPTERS>(                                                     \
+      const uint16_t*, const uint16_t*, uint16_t*, const void*, int, int, int, int, long long, long long, long long, float*, int, \
+      int, int, const AdapterPart&, hipStream_t);
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_GEMM)
-#define KG_GEMM_PIPE_INSTANCE(TAG, TM, ST, RAG)                                                                          \
-  KG_INSTANCE hipError_t launch_gemm_pipe<TAG, TM, ST, RAG>(const uint16_t*, const uint16_t*, uint16_t*, const void*, int, \
-                                                            int, int, int, long long, long long, long long, float*, int,  \
-                                                            int, int, hipStream_t);
-#define KG_GEMM_PIPE_INSTANCES(TAG, TM, RAG) \
-  KG_GEMM_PIPE_INSTANCE(TAG, TM, 2, RAG) KG_GEMM_PIPE_INSTANCE(TAG, TM, 3, RAG) KG_GEMM_PIPE_INSTANCE(TAG, TM, 4, RAG)
+#define KG_GEMM_PIPE_INSTANCES(TAG, TM, RAG)       \
+  KG_GEMM_PIPE_INSTANCE(TAG, TM, 2, RAG, false) \
+  KG_GEMM_PIPE_INSTANCE(TAG, TM, 3, RAG, false) \
+  KG_GEMM_PIPE_INSTANCE(TAG, TM, 4, RAG, false)
 KG_GEMM_PIPE_INSTANCES(Bf16Tag, 128, false)
 KG_GEMM_PIPE_INSTANCES(Bf16Tag, 128, true)
 KG_GEMM_PIPE_INSTANCES(Bf16Tag, 256, false)
@@ -42,8 +44,14 @@ KG_GEMM_PIPE_INSTANCES(F16Tag, 128, true)
 KG_GEMM_PIPE_INSTANCES(F16Tag, 256, false)
 KG_GEMM_PIPE_INSTANCES(F16Tag, 256, true)
 #undef KG_GEMM_PIPE_INSTANCES
-#undef KG_GEMM_PIPE_INSTANCE
 #endif
+#if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_ADAPTER_PIPE)
+KG_GEMM_PIPE_INSTANCE(Bf16Tag, 128, 4, true, true)
+KG_GEMM_PIPE_INSTANCE(Bf16Tag, 256, 4, true, true)
+KG_GEMM_PIPE_INSTANCE(F16Tag, 128, 4, true, true)
+KG_GEMM_PIPE_INSTANCE(F16Tag, 256, 4, true, true)
+#endif
+#undef KG_GEMM_PIPE_INSTANCE
 
 #define KG_GEMM_MID_INSTANCE(TAG, ST, RAG, ADAPTERS)                                                                     \
   KG_INSTANCE hipError_t launch_gemm_mid<TAG, ST, RAG, ADAPTERS>(const uint16_t*, const uint16_t*, uint16_t*, const void*, int, \

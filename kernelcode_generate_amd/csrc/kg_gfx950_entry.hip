@@ -521,6 +521,18 @@ bool gemm_mid_pays(long long M, long long N, long long K) {
 int gemm_mid_stages(long long K) { return K <= 1024 ? 2 : 4; }
 
 template <typename Tag>
+void launch_splitk_reduce(const float* partial, int splits, uint16_t* C, const void* bias, int bias_kind, int M, int N, long long ldc) {
+  const int grid = (int)cdiv((long long)M * (N / 4), kSplitReduceThreads);
+#define KG_SPLITK_REDUCE(BIAS)                                                                                          \
+  hipLaunchKernelGGL((gemm_splitk_reduce_kernel<Tag, BIAS>), dim3(grid), dim3(kSplitReduceThreads), 0, g_stream, partial, \
+                     splits, C, bias, M, N, ldc)
+  if (bias_kind == 0) KG_SPLITK_REDUCE(0);
+  else if (bias_kind == 1) KG_SPLITK_REDUCE(1);
+  else KG_SPLITK_REDUCE(2);
+#undef KG_SPLITK_REDUCE
+}
+
+template <typename Tag>
 int launch_gemm_mfma(const Mem& out, const Mem& lhs, const Mem& rhs, const Mem& bias, int M, int N, int K,
                      int stages, bool staged) {
   const uint16_t* A = static_cast<const uint16_t*>(lhs.data);
@@ -572,8 +584,8 @@ int launch_gemm_mfma(const Mem& out, const Mem& lhs, const Mem& rhs, const Mem& 
     return finish_launch("matmul(mfma-quad)");
   }
 #define KG_GEMM_PIPE(TM, ST, RAG)                                                                          \
-  e = launch_gemm_pipe<Tag, TM, ST, RAG>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, partial, k_chunk, grid, splits, \
-                                         g_stream)
+  e = launch_gemm_pipe<Tag, TM, ST, RAG, false>(A, B, C, bp, bias_kind, M, N, K, lda, ldb, ldc, partial, k_chunk, grid, splits, \
+                                                AdapterPart{}, g_stream)
 #define KG_GEMM_PIPE_DEPTH(TM, RAG)                  \
   if (stages == 2) { KG_GEMM_PIPE(TM, 2, RAG); }      \
   else if (stages == 3) { KG_GEMM_PIPE(TM, 3, RAG); } \
@@ -588,16 +600,7 @@ int launch_gemm_mfma(const Mem& out, const Mem& lhs, const Mem& rhs, const Mem& 
 #undef KG_GEMM_PIPE
   if (e != hipSuccess) return fail(kHipFailure, "matmul(mfma-pipe): %s", hipGetErrorString(e));
   if (splits > 1) {
-    const int rgrid = (int)cdiv((long long)M * (N / 4), kSplitReduceThreads);
-    if (bias_kind == 0)
-      hipLaunchKernelGGL((gemm_splitk_reduce_kernel<Tag, 0>), dim3(rgrid), dim3(kSplitReduceThreads), 0, g_stream, partial, splits, C, bp,
-                         M, N, ldc);
-    else if (bias_kind == 1)
-      hipLaunchKernelGGL((gemm_splitk_reduce_kernel<Tag, 1>), dim3(rgrid), dim3(kSplitReduceThreads), 0, g_stream, partial, splits, C, bp,
-                         M, N, ldc);
-    else
-      hipLaunchKernelGGL((gemm_splitk_reduce_kernel<Tag, 2>), dim3(rgrid), dim3(kSplitReduceThreads), 0, g_stream, partial, splits, C, bp,
-                         M, N, ldc);
+    launch_splitk_reduce<Tag>(partial, splits, C, bp, bias_kind, M, N, ldc);
     return finish_launch("matmul(mfma-pipe-splitk)");
   }
   return finish_launch(ragged ? "matmul(mfma-pipe-ragged)" : "matmul(mfma-pipe)");
@@ -1599,41 +1602,74 @@ bool adapter_skinny_pays(long long M, long long N, long long K) {
   return 4000 + rounds * 3 * K < 6700 + mid * cdiv(K, gemmm::kBK) * 450;
 }
 
-// The projection with its adapters in one pass over the output (adapter.h).
+// The form of a 16-bit projection with adapters (adapter.h), matmul's own where it has one of that call, and the memory
+// between its launches: zeros and t's sums, then the partial sums of a split K.
+struct AdapterPlan {
+  enum { kSkinny, kMid, kQuad, kPipe } form;
+  long long tile_rows, chunk;
+  int splits;      // of the projection's K
+  int at_once;     // distinct adapters of 16 rows that are read at once for t
+  int low_splits;  // of t's K
+  size_t low_bytes, bytes;
+};
+AdapterPlan adapter_plan(const AdapterArgs& p) {
+  const long long M = p.m, N = p.n, K = p.k;
+  AdapterPlan a{AdapterPlan::kPipe, pipe_tile_m(M, N), K, 1, 1, 1, 0, 0};
+  const long long low = cdiv(M, 16) * cdiv(p.rank, kAdapterLowCols);  // workgroups of t, of an adapter and all of K
+  a.at_once = (int)std::min(std::min(16ll, (long long)std::min(p.m, p.count)), std::max(1ll, 512 / low));
+  // 64 k for each of a workgroup's four waves at least, and some two workgroups a compute unit: more splits are more
+  // sums for every reader (1024 workgroups: 256 x 4096 x 4096 47 us, 512: 41, 256: 39; x 512 rows in runs 39, 40, 43)
+  a.low_splits = (int)std::max(1ll, std::min(std::min<long long>(K / 256, kAdapterMaxSplits), 512 / (low * a.at_once)));
+  a.low_bytes = (size_t)cdiv(kAdapterHeader + (long long)a.low_splits * M * p.rank * 4, 256) * 256;
+  if (adapter_skinny_pays(M, N, K)) {
+    a.form = AdapterPlan::kSkinny;
+  } else if (gemm_mid_pays(M, N, K)) {
+    a.form = AdapterPlan::kMid;
+  } else {
+    a.splits = pipe_splits(M, N, K, &a.chunk);
+    if (a.low_bytes + (size_t)a.splits * M * N * sizeof(float) > (size_t)kSplitMaxWorkspace) a.splits = 1;
+    if (a.splits == 1 && pipe_aligned(M, N, K) && (a.tile_rows == 256 || cdiv(M, 128) * cdiv(N, gemmp::kBN) >= kNumCUs))
+      a.form = AdapterPlan::kQuad;
+  }
+  a.bytes = a.low_bytes + (a.splits > 1 ? (size_t)a.splits * M * N * sizeof(float) : 0);
+  return a;
+}
+
 template <typename Tag>
-int launch_adapter_matmul(const AdapterArgs& p, int bias_kind, char* ws) {
-  uint16_t* t = reinterpret_cast<uint16_t*>(ws + kAdapterHeader);
-  const unsigned blocks = (unsigned)cdiv(p.m, 16);
-  const unsigned at_once = (unsigned)std::min(16u, std::max(1u, 512u / blocks));  // of a block's adapters
-  hipLaunchKernelGGL((adapter_low_kernel<Tag>), dim3(blocks, at_once, (unsigned)cdiv(p.rank, kAdapterLowCols)),
-                     dim3(kAdapterLowThreads), 0, g_stream, p, t,
-                     reinterpret_cast<uint32_t*>(ws));
-  const AdapterPart part{t, reinterpret_cast<const uint16_t*>(ws), static_cast<const uint16_t*>(p.b), p.index, p.b_l, p.b_r,
-                         p.index_stride, p.rank, p.count, page_div(p.rank / 8)};
-  hipError_t e;
-  const long long tm = pipe_tile_m(p.m, p.n);
-  long long chunk = p.k;
-  // whole tiles that fill the chip, as in matmul
-  const bool quad = !gemm_mid_pays(p.m, p.n, p.k) && pipe_aligned(p.m, p.n, p.k) && pipe_splits(p.m, p.n, p.k, &chunk) == 1 &&
-                    (tm == 256 || cdiv(p.m, tm) * cdiv(p.n, gemmp::kBN) >= kNumCUs);
-  if (adapter_skinny_pays(p.m, p.n, p.k)) {
-    e = launch_gemm_skinny<Tag, true>(p.x, p.w, p.out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream);
-  } else if (quad) {
-    const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.w);
-    uint16_t* out = static_cast<uint16_t*>(p.out);
+int launch_adapter_matmul(const AdapterArgs& p, const AdapterPlan& plan, int bias_kind, char* ws) {
+  float* sums = reinterpret_cast<float*>(ws + kAdapterHeader);
+  hipLaunchKernelGGL((adapter_low_kernel<Tag>),
+                     dim3((unsigned)(cdiv(p.m, 16) * plan.low_splits), (unsigned)plan.at_once, (unsigned)cdiv(p.rank, kAdapterLowCols)),
+                     dim3(kAdapterLowThreads), 0, g_stream, p, reinterpret_cast<uint32_t*>(ws), sums, plan.low_splits);
+  const AdapterPart part{sums, reinterpret_cast<const uint16_t*>(ws), static_cast<const uint16_t*>(p.b), p.index, (long long)p.m * p.rank,
+                         p.b_l, p.b_r, p.index_stride, plan.low_splits, p.rank, p.count, page_div(p.rank / 8)};
+  const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.w);
+  uint16_t* out = static_cast<uint16_t*>(p.out);
+  hipError_t e = hipSuccess;
+  if (plan.form == AdapterPlan::kSkinny) {
+    e = launch_gemm_skinny<Tag, true>(x, w, out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream);
+  } else if (plan.form == AdapterPlan::kQuad) {
 #define KG_ADAPTER_QUAD(TM) \
   launch_gemm_quad<Tag, 4, TM, true>(x, w, out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream)
-    e = tm == 256 ? KG_ADAPTER_QUAD(256) : KG_ADAPTER_QUAD(128);
+    e = plan.tile_rows == 256 ? KG_ADAPTER_QUAD(256) : KG_ADAPTER_QUAD(128);
 #undef KG_ADAPTER_QUAD
-  } else {
+  } else if (plan.form == AdapterPlan::kMid) {
     const bool edges = p.m % gemmm::kT || p.n % gemmm::kT || p.k % gemmm::kBK;
-    const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.w);
-    uint16_t* out = static_cast<uint16_t*>(p.out);
 #define KG_ADAPTER_MID(ST, RAG) \
   launch_gemm_mid<Tag, ST, RAG, true>(x, w, out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, part, g_stream)
     if (gemm_mid_stages(p.k) == 2) e = edges ? KG_ADAPTER_MID(2, true) : KG_ADAPTER_MID(2, false);
     else e = edges ? KG_ADAPTER_MID(4, true) : KG_ADAPTER_MID(4, false);
 #undef KG_ADAPTER_MID
+  } else {
+    float* partial = plan.splits > 1 ? reinterpret_cast<float*>(ws + plan.low_bytes) : nullptr;
+    const int grid = (int)(cdiv(p.m, plan.tile_rows) * cdiv(p.n, gemmp::kBN)), chunk = plan.splits > 1 ? (int)plan.chunk : 0;
+#define KG_ADAPTER_PIPE(TM)                                                                                                  \
+  launch_gemm_pipe<Tag, TM, 4, true, true>(x, w, out, p.bias, bias_kind, p.m, p.n, p.k, p.ldx, p.ldw, p.ldo, partial, chunk, grid, \
+                                           plan.splits, part, g_stream)
+    e = plan.tile_rows == 256 ? KG_ADAPTER_PIPE(256) : KG_ADAPTER_PIPE(128);
+#undef KG_ADAPTER_PIPE
+    if (e == hipSuccess && plan.splits > 1)
+      launch_splitk_reduce<Tag>(partial, plan.splits, out, p.bias, bias_kind, p.m, p.n, p.ldo);
   }
   if (e != hipSuccess) return fail(kHipFailure, "adapter_matmul(mfma): %s", hipGetErrorString(e));
   return finish_launch("adapter_matmul(mfma)");
@@ -1684,13 +1720,16 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   p.m = (int)M, p.n = (int)N, p.k = (int)K, p.rank = (int)rank, p.count = (int)count;
   const bool mfma = adapters && out.dtype != KG_DTYPE_F32 && K > 0 && K % 8 == 0 && N % 8 == 0 && rank % 8 == 0 &&
                     w.stride[1] == 1 && (!bias.present || bias.stride[0] == 1 || N == 1) && rows_aligned(out, 16) &&
-                    rows_aligned(x, 16) && rows_aligned(w, 16) && rows_aligned(b, 16) && rows_aligned(a, 4) &&
+                    rows_aligned(x, 16) && rows_aligned(w, 16) && rows_aligned(b, 16) && rows_aligned(a, 16) &&
                     x.stride[0] <= kMaxPipeLd && w.stride[0] <= kMaxPipeLd;
-  if (mfma && kAdapterHeader + (size_t)(M * rank) * 2 <= (size_t)kSplitMaxWorkspace) {
-    const SplitLease lease = split_workspace(kAdapterHeader + (size_t)(M * rank) * 2, g_stream);  // held until both kernels are enqueued
+  if (mfma) {
+    const AdapterPlan plan = adapter_plan(p);
+    SplitLease lease;  // held until the kernels are enqueued
+    if (plan.bytes <= (size_t)kSplitMaxWorkspace) lease = split_workspace(plan.bytes, g_stream);
     const int bias_kind = !bias.present ? 0 : bias.dtype == KG_DTYPE_F32 ? 1 : 2;
     if (char* ws = static_cast<char*>(lease.ptr))
-      return out.dtype == KG_DTYPE_BF16 ? launch_adapter_matmul<Bf16Tag>(p, bias_kind, ws) : launch_adapter_matmul<F16Tag>(p, bias_kind, ws);
+      return out.dtype == KG_DTYPE_BF16 ? launch_adapter_matmul<Bf16Tag>(p, plan, bias_kind, ws)
+                                        : launch_adapter_matmul<F16Tag>(p, plan, bias_kind, ws);
   }
   if ((rc = matmul_impl(args, 4)) || !adapters) return rc;
   return with_kv_types(out.dtype, out.dtype, [&](auto t, auto) {
