@@ -185,8 +185,16 @@ def dtype_code_of(value: Any) -> int:
     return code
 
 
+_MEMORY_KINDS: set[type] = set()  # classes whose objects are memory arguments (looked up once: a shape is made by asking)
+
+
 def _is_memory(value: Any) -> bool:
-    return hasattr(value, "data_ptr") and hasattr(value, "shape") and hasattr(value, "stride")
+    if type(value) in _MEMORY_KINDS:
+        return True
+    if hasattr(value, "data_ptr") and hasattr(value, "shape") and hasattr(value, "stride"):
+        _MEMORY_KINDS.add(type(value))
+        return True
+    return False
 
 
 # A KgArgSlot is eight 64-bit words (the 32-bit fields are padded to one each), so a call's
@@ -202,32 +210,34 @@ def _float_bits(value: float) -> int:
     return _unpack_int64(_pack_double(value))[0]
 
 
-def _pack_slots(args: Sequence[Any]) -> tuple[array, int]:
-    """(packed words, their address) for ``args`` (tensors / None / int / float)."""
+def _slot_words(args: Sequence[Any], address: int) -> list[int]:
+    """The words of ``args`` (tensors / None / int / float), to lie at ``address``."""
 
     words: list[int] = []
     tail: list[int] = []  # shapes and strides of the memory slots
-    memory: list[tuple[int, int]] = []  # (slot, rank rounded up to 1) of each
+    at = address + 8 * _SLOT_WORDS * max(len(args), 1)  # of the next ones
     for position, arg in enumerate(args):
         kind = type(arg)
         if arg is None:
-            words += (KG_ARG_MEMORY, 0, 0, 0, 1, 0, 0, 0)
+            words += (KG_ARG_MEMORY, 0, at, at + 8, 1, 0, 0, 0)
             tail += (0, 1)
-            memory.append((position, 1))
+            at += 16
         elif kind is int:
             words += (KG_ARG_INT, 0, 0, 0, 0, 0, arg, 0)
         elif kind is float:
             words += (KG_ARG_FLOAT, 0, 0, 0, 0, 0, 0, _float_bits(arg))
-        elif _is_memory(arg):  # (no number has a data_ptr)
-            dims, strides = arg.shape, arg.stride()
+        elif kind in _MEMORY_KINDS or _is_memory(arg):  # (no number has a data_ptr)
+            dims = arg.shape
             rank = len(dims)
-            words += (KG_ARG_MEMORY, int(arg.data_ptr()), 0, 0, rank, dtype_code_of(arg), 0, 0)
+            code = _DTYPE_CODE_OF.get(arg.dtype) or dtype_code_of(arg)
+            words += (KG_ARG_MEMORY, arg.data_ptr(), at, at + 8 * (rank or 1), rank, code, 0, 0)
             if rank:
                 tail += dims
-                tail += strides
+                tail += arg.stride()
+                at += 16 * rank
             else:
                 tail += (0, 0)
-            memory.append((position, rank or 1))
+                at += 16
         elif isinstance(arg, bool):
             raise NativeLibraryError(f"bool runtime arg at position {position} is not supported", -1)
         elif isinstance(arg, Integral):
@@ -238,25 +248,42 @@ def _pack_slots(args: Sequence[Any]) -> tuple[array, int]:
             raise NativeLibraryError(f"unsupported runtime arg at position {position}: {type(arg).__name__}", -1)
     if not words:
         words = [0] * _SLOT_WORDS
-    at = len(words)
     words += tail
+    return words
+
+
+def _put_words(words: list[int], to: array) -> None:
+    pack = _PACKERS.get(len(words))
+    if pack is None:
+        pack = _PACKERS[len(words)] = struct.Struct(f"{len(words)}q").pack_into
     try:
-        packed = array("q", words)
-    except OverflowError:  # an integer beyond a C long long: its low 64 bits
-        packed = array("q", [(w + _INT64) % (2 * _INT64) - _INT64 for w in words])
-    address = packed.buffer_info()[0]
-    for slot, rank in memory:
-        shape = address + 8 * at
-        packed[_SLOT_WORDS * slot + 2] = shape
-        packed[_SLOT_WORDS * slot + 3] = shape + 8 * rank
-        at += 2 * rank
-    return packed, address
+        pack(to, 0, *words)
+    except struct.error:  # an integer beyond a C long long: its low 64 bits
+        pack(to, 0, *((w + _INT64) % (2 * _INT64) - _INT64 for w in words))
+
+
+_PACKERS: dict[int, Any] = {}  # number of words -> their packing
+
+
+# Memory for the words of a call, and its address, while no call uses it. Taken and given back by a list's own pop and
+# append, so that calls of two threads, or of a signal handler amid another, never have the same.
+_CALL_WORDS = 512
+_FREE_WORDS: list[tuple[array, int]] = []
+
+
+def _take_words() -> tuple[array, int]:
+    try:
+        return _FREE_WORDS.pop()
+    except IndexError:
+        packed = array("q", bytes(8 * _CALL_WORDS))
+        return packed, packed.buffer_info()[0]
 
 
 def marshal_slots(args: Sequence[Any]) -> tuple[ctypes.Array, list[Any]]:
     """Build the C slot array for ``args`` (tensors / None / int / float)."""
 
-    packed, _ = _pack_slots(args)
+    packed = array("q", bytes(8 * len(_slot_words(args, 0))))
+    _put_words(_slot_words(args, packed.buffer_info()[0]), packed)
     slots = (KgArgSlot * max(len(args), 1)).from_buffer(packed)
     return slots, [packed, slots, *args]
 
@@ -266,12 +293,18 @@ def call_entry(entry_point: str, args: Sequence[Any], *, check: bool = True) -> 
 
     lib = load_library()
     fn = _ADDRESS_CALLS.get(entry_point)
-    packed, address = _pack_slots(args)
-    if fn is not None:
-        status = fn(address, len(args))
-    else:
-        slots = (KgArgSlot * max(len(args), 1)).from_buffer(packed)
-        status = int(getattr(lib, entry_point)(slots, ctypes.c_ulonglong(len(args))))
+    own = _take_words()
+    try:
+        words = _slot_words(args, own[1])
+        if fn is not None and len(words) <= _CALL_WORDS:
+            _put_words(words, own[0])
+            status = fn(own[1], len(args))
+        else:
+            slots, keepalive = marshal_slots(args)
+            status = int(getattr(lib, entry_point)(slots, ctypes.c_ulonglong(len(args))))
+            del keepalive
+    finally:
+        _FREE_WORDS.append(own)
     if check and status != 0:
         detail = lib.kg_gfx950_last_error().decode("utf-8", "replace")
         raise NativeLibraryError(f"{entry_point} returned {status}: {detail}", status)
