@@ -19,7 +19,7 @@ inline bool tree_matrix_takes(const TreeArgs& a, int cache_bytes) {
   };
   return a.d % 16 == 0 && a.d <= 256 && whole(a.q, {a.q_token, a.q_head}, 2, 16) && whole(a.out, {a.o_token, a.o_head}, 2, 4) &&
          whole(a.k, {a.k_page, a.k_head, a.k_row}, cache_bytes, 16) && whole(a.v, {a.v_page, a.v_head, a.v_row}, cache_bytes, 16) &&
-         a.k_row <= 1 << 24 && a.v_row <= 1 << 24 && a.pages > 0;
+         a.k_row <= 1 << 24 && a.v_row <= 1 << 24 && a.pages > 0 && a.per > 0;
 }
 
 struct TreePlan {
@@ -81,18 +81,23 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream)
 #undef KG_TREE_ROWS
   if (p.join) {
     const long long quads = tree_items(a, p.split.block) * (p.split.block / kTreeJoinRows);  // of rows
-    const bool few = quads <= 512;
-#define KG_TREE_JOIN(WIDTH, WAVES)                                                                                       \
-  hipLaunchKernelGGL((tree_attn_join_kernel<Tag, WIDTH, WAVES>), dim3((unsigned)((quads * WAVES + 3) / 4)), dim3(256), 0, \
-                     stream, a, p.split)
+    // of an item, if the ranges are about as many as the workgroups
+    const bool many = p.split.grid / std::max(1ll, tree_items(a, p.split.block)) >= 16, few = quads <= 512;
+#define KG_TREE_JOIN(WIDTH, WAVES)                                                                                      \
+  hipLaunchKernelGGL((tree_attn_join_kernel<Tag, WIDTH, WAVES>),                                                        \
+                     dim3((unsigned)((quads * WAVES + tree_join_waves(WAVES) - 1) / tree_join_waves(WAVES))),           \
+                     dim3(64 * tree_join_waves(WAVES)), 0, stream, a, p.split)
     if (p.width == 256) {
-      if (few) KG_TREE_JOIN(256, 4);
+      if (few && many) KG_TREE_JOIN(256, 8);
+      else if (few) KG_TREE_JOIN(256, 4);
       else KG_TREE_JOIN(256, 1);
     } else if (p.width == 128) {
-      if (few) KG_TREE_JOIN(128, 4);
+      if (few && many) KG_TREE_JOIN(128, 16);
+      else if (few) KG_TREE_JOIN(128, 4);
       else KG_TREE_JOIN(128, 1);
     } else {
-      if (few) KG_TREE_JOIN(64, 4);
+      if (few && many) KG_TREE_JOIN(64, 16);
+      else if (few) KG_TREE_JOIN(64, 4);
       else KG_TREE_JOIN(64, 1);
     }
 #undef KG_TREE_JOIN

@@ -168,6 +168,37 @@ __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, const TreeSpl
   return t;
 }
 
+// Keys key + 0..63 that a row sees of those there are (bit n: key + n), its token j of the request, whose mask begins with
+// `first`. At once for a tile: a loop over the keys took 18 us of 176 at 2 x 512 tokens behind 4096.
+__device__ __forceinline__ unsigned long long tree_visible(const TreeArgs& a, const TreeRequest& r, bool row, int j,
+                                                           unsigned long long first, int key) {
+  const int before = r.context - key;  // the first of them are the context's
+  if (before >= 64) return ~0ull;
+  const int draft = max(-before, 0);  // the next one's number
+  unsigned long long seen = 0;
+  if (a.words < 0) {
+    const int n = j + 1 - draft;
+    if (n > 0) seen = n >= 64 ? ~0ull : (1ull << n) - 1;
+  } else {
+    const int w = draft >> 6, shift = draft & 63;
+    auto word = [&](int i) __attribute__((always_inline)) {
+      if (i == 0) return first;
+      return row && i < a.words ? (unsigned long long)a.mask[(r.first + j) * a.mask_0 + i * a.mask_1] : 0ull;
+    };
+    seen = word(w) >> shift;
+    if (shift != 0) seen |= word(w + 1) << (64 - shift);
+  }
+  return before <= 0 ? seen : seen << before | ((1ull << before) - 1);
+}
+// Of those the ones that exist and lie with this lane: bit 4 kb + i is key 16 kb + 4 lr + i.
+template <int NKB>
+__device__ __forceinline__ uint32_t tree_lane_keys(unsigned long long keys, int lr) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int kb = 0; kb < NKB; ++kb) bits |= ((uint32_t)(keys >> (16 * kb) >> (4 * lr)) & 0xfu) << (4 * kb);
+  return bits;
+}
+
 // A weight of 0 does not take an infinity or NaN out of a sum, and only some rows see a drafted token: where values are
 // not finite, the products run on zeros in their place and this adds them to the rows that see them (times a
 // weight they would be the same). One key of a step after another, from memory: row l16's elements d_of(e, i).
@@ -397,18 +428,7 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
         const uint32_t there_lo = (uint32_t)(there >> (4 * lr)), there_hi = (uint32_t)(there >> 32 >> (4 * lr));
 #pragma unroll
         for (int x = 0; x < kNQ; ++x) {
-          seen[x] = 0;
-#pragma unroll 1
-          for (int n = 0; n < 4 * NKB; ++n) {
-            const int in_step = 16 * (n >> 2) + (n & 3), draft = key + 4 * lr + in_step - r.context;
-            bool s = ((in_step < 32 ? there_lo : there_hi) >> (in_step & 31) & 1u) != 0;
-            if (s && draft >= 0) {
-              if (a.words < 0) s = draft <= tok[x];
-              else if (draft < 64) s = (first_word[x] >> draft & 1ull) != 0;
-              else s = 16 * x + l16 < item_rows && tree_sees(a, r.first + tok[x], tok[x], draft);
-            }
-            seen[x] |= (s ? 1u : 0u) << n;
-          }
+          seen[x] = tree_lane_keys<NKB>(there & tree_visible(a, r, 16 * x + l16 < item_rows, tok[x], first_word[x], key), lr);
 #pragma unroll
           for (int n = 0; n < 4 * NKB; ++n)
             if (!(seen[x] >> n & 1u)) {
@@ -555,17 +575,19 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
 
 // The records of the items that several ranges share, joined: a wave takes four consecutive rows of an item, a lane four
 // columns. (A wave per row spent most of its time on finding its item: 14 us for 3104 rows of 8 records each, 8 now.)
-// kWaves: 4 where few rows have many records (32 rows of 64: 34 us with one wave each, 14 with four): they take every
-// fourth record of the same rows.
+// kWaves: more where few rows have many records (32 rows of 64: 34 us with one wave each, 13 with four, 10 with 16): they
+// take every kWaves-th record of the same rows.
 constexpr int kTreeJoinRows = 4;
+__host__ __device__ constexpr int tree_join_waves(int waves) { return waves > 4 ? waves : 4; }  // of a workgroup
 template <typename Tag, int D, int kWaves>
-__global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs a, TreeSplit split) {
+__global__ __launch_bounds__(64 * tree_join_waves(kWaves)) void tree_attn_join_kernel(TreeArgs a, TreeSplit split) {
   constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes;                    // lanes of a row, rows of a load
   constexpr int kLoads = kTreeJoinRows / kAtOnce < 1 ? 1 : kTreeJoinRows / kAtOnce;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int turn = wave % kWaves;
-  const long long id = (long long)blockIdx.x * (4 / kWaves) + wave / kWaves;
+  constexpr int kAll = tree_join_waves(kWaves);
+  const long long id = (long long)blockIdx.x * (kAll / kWaves) + wave / kWaves;
   const int parts = split.block / kTreeJoinRows;
   const int item = (int)(id / parts), part = (int)(id - (long long)item * parts);
   // the request of this item, the items and units before it, and all units
@@ -614,7 +636,7 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs a, TreeSpl
     l[x] = 0.f;
     o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  constexpr int kAhead = kWaves == 1 ? 4 : 8;
+  constexpr int kAhead = kWaves == 4 ? 8 : 4;
   for (int v0 = w0 + turn; v0 <= w1; v0 += kWaves * kAhead) {
     f32x4 ov[kAhead][kLoads];
     f32x2 ml[kAhead][kLoads];
@@ -642,8 +664,8 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(TreeArgs a, TreeSpl
     }
   }
   if constexpr (kWaves > 1) {  // (all waves of a group are here: what they returned on is the same for them)
-    __shared__ f32x4 o_lds[4][kLoads][64];
-    __shared__ f32x2 ml_lds[4][kLoads][64];
+    __shared__ f32x4 o_lds[kAll][kLoads][64];
+    __shared__ f32x2 ml_lds[kAll][kLoads][64];
 #pragma unroll
     for (int x = 0; x < kLoads; ++x) o_lds[wave][x][lane] = o[x], ml_lds[wave][x][lane] = f32x2{m[x], l[x]};
     __syncthreads();

@@ -2,11 +2,16 @@
 // pieces of prompts; and for pages of no multiple of 16 tokens.
 //
 // Sharing of the work, weights, scales and joining are those of tree_attn_rows.h. Here the four waves of a workgroup take
-// different rows (16 or 32 each) and the same keys: tiles of 64 (32 for heads of 256) go through registers, where 8-bit
-// codes are widened once for all rows, into one of two LDS stages as 16-bit [key][d]; the next tile's rows are
-// in flight under the current one's products, with one barrier per tile. K fragments are one ds_read_b128 per 16 keys x 32 d
+// different rows (16 or 32 each) and the same keys: tiles of 64 (32 for heads of 256) in one of two LDS stages as 16-bit
+// [key][d], the next one on its way under the current one's products, with one barrier per tile. 16-bit rows are copied there by the
+// loads; 8-bit codes go through registers, where they are widened once for all rows. K fragments are one ds_read_b128 per 16 keys x 32 d
 // (16-byte chunk c of row r at c ^ (r % 16): 16 rows hit distinct banks), V^T fragments two ds_read_b64_tr_b16 per 16 d x 32
 // keys in the key order that P's lanes hold (chunk pairs at pair ^ (r % 8): the 8 rows of half a wave do).
+//
+// Measured, heads of 128 in 8 groups of 4: 2 x 512 rows behind 4096 in bf16 144 us with the join, 507 TFLOP/s (654 behind
+// 16384); with rows through registers, which spilled, and a loop over the keys of tiles with drafts, 185. 8 x 16 rows behind 16384: bf16
+// 114 us, 4.75 TB/s of rows; e4m3 104 us, bound by each wave's chain of widening, products and softmax, not by bytes (two tiles
+// in flight: 110; eight waves with half the keys each, in 128 registers: 162).
 #pragma once
 
 #include "common.h"
@@ -32,6 +37,7 @@ template <int D>
 __device__ __forceinline__ uint32_t v_at(int r, int c) {
   return r * D * 2 + 16 * (D == 64 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * (r & 7)));
 }
+__device__ const char kZeros[512] = {};  // the row of a key that is not there
 }  // namespace treet
 
 template <typename Tag, typename C, int D, int kNQ>
@@ -108,27 +114,58 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
     const int* table = a.table + share.b * a.table_0;
 
-    // Page of key `lane` of a tile (-1: none, or a key past the range) and its offset there.
+    // Page of key `lane` of a tile (-1: none, or a key past the range), its offset there, and its rows: a lane's 64-bit
+    // products for its key and not for each piece it copies (158 -> 146 us at 2 x 512 rows behind 4096).
     struct Place {
       int page, offset;
+      unsigned long long k, v;
     };
-    auto place = [&](int key0) __attribute__((always_inline)) {
-      const int key = key0 + (lane & (kTile - 1));
-      Place p = {-1, 0};
-      if (key < key_hi) {
-        const int n = div_page(key, a.div);
-        p.page = table[n * a.table_1];
-        p.offset = key - n * a.page_size;
-      }
+    auto place = [&](int first) __attribute__((always_inline)) {
+      const int key = first + (lane & (kTile - 1)), n = div_page(max(min(key, key_hi - 1), 0), a.div);
+      Place p = {table[n * a.table_1], key - n * a.page_size, 0, 0};
+      if (key >= key_hi) p.page = -1;
       return p;
     };
     auto checked = [&](Place p) __attribute__((always_inline)) {
       const bool there = p.page >= 0 && p.page < a.pages;
-      return Place{there ? p.page : -1, there ? p.offset : 0};
+      const unsigned long long k = (unsigned long long)(kc + p.page * a.k_page + (long long)p.offset * (int)a.k_row);
+      const unsigned long long v = (unsigned long long)(vc + p.page * a.v_page + (long long)p.offset * (int)a.v_row);
+      const unsigned long long zeros = (unsigned long long)&kZeros;
+      return Place{there ? p.page : -1, there ? p.offset : 0, there ? k : zeros, there ? v : zeros};
+    };
+    auto row_of = [&](unsigned long long p, int n) __attribute__((always_inline)) {  // key n's
+      return (unsigned long long)(uint32_t)__shfl((int)(p >> 32), n, 64) << 32 | (uint32_t)__shfl((int)p, n, 64);
     };
 
-    // A tile's rows on their way: what is not there (a key, or d past the head's end) is read from a row that is, and written
-    // as zeros.
+    // 16-bit rows: copied to LDS by the load itself, a wave's 1 KiB at a time; d past the head's end comes from kZeros.
+    // Lane l's 16 bytes land at 16 l, so it takes the chunk that the swizzle puts there.
+    auto copy = [&](int stage, const Place& p) __attribute__((always_inline)) {
+      const uint32_t kb = lds0 + stage * 2 * kStage + wave * 1024, vb = kb + kStage;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int n = piece_row + kRowStep * i;
+        const uint32_t ck = k_at<D>(n, piece) - n * D * 2, cv = v_at<D>(n, piece) - n * D * 2;  // bytes in the row
+        const unsigned long long k = row_of(p.k, n), v = row_of(p.v, n), zeros = (unsigned long long)&kZeros;
+        g2lds16_m(reinterpret_cast<const char*>(((int)ck < 2 * a.d ? k : zeros) + ck), kb + i * kThreads * 16);
+        g2lds16_m(reinterpret_cast<const char*>(((int)cv < 2 * a.d ? v : zeros) + cv), vb + i * kThreads * 16);
+      }
+    };
+    // A tile that not every row sees in full: values that are not finite are left out of the products (tree_add_nonfinite).
+    auto sift = [&](int stage, int at) __attribute__((always_inline)) {
+      uint32_t found = 0;
+#pragma unroll
+      for (int i = 0; i < kStage / (kThreads * 16); ++i) {
+        const auto to = (__attribute__((address_space(3))) u32x4*)(uintptr_t)(lds0 + (2 * stage + 1) * kStage + (i * kThreads + tid) * 16);
+        u32x4 x = *to;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = finite_pair<H>(x[q], found);
+        *to = x;
+      }
+      if (found != 0) found_lds[at] = 1;
+    };
+
+    // 8-bit rows: through registers, where they are widened. What is not there is read from a row that is, and written as
+    // zeros.
     u32x4 kr[kPieces], vr[kPieces];
     uint32_t row_there = 0;
     float ks = 0.f, vs = 0.f;
@@ -139,31 +176,20 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
         const int n = piece_row + kRowStep * i;
         const int page = __shfl(p.page, n, 64), offset = __shfl(p.offset, n, 64);
         row_there |= (page >= 0 ? 1u : 0u) << i;
-        const int d = piece_in ? piece * (16 / kES) : 0;
+        const int d = piece_in ? piece * 16 : 0;
         kr[i] = ld16(kc + (long long)max(page, 0) * a.k_page + (long long)offset * a.k_row + d);
         vr[i] = ld16(vc + (long long)max(page, 0) * a.v_page + (long long)offset * a.v_row + d);
       }
       if constexpr (kS) {
-        if (tid < kTile) {
-          ks = a.k_scale[(long long)max(p.page, 0) * a.ks_page + h * a.ks_head + (long long)p.offset * a.ks_row];
-          vs = a.v_scale[(long long)max(p.page, 0) * a.vs_page + h * a.vs_head + (long long)p.offset * a.vs_row];
-        }
+        ks = a.k_scale[(long long)max(p.page, 0) * a.ks_page + h * a.ks_head + (long long)p.offset * a.ks_row];
+        vs = a.v_scale[(long long)max(p.page, 0) * a.vs_page + h * a.vs_head + (long long)p.offset * a.vs_row];
       }
     };
     auto put = [&](uint32_t at, u32x4 x) __attribute__((always_inline)) {
       *(__attribute__((address_space(3))) u32x4*)(uintptr_t)at = x;
     };
-    // sift: a tile that not every row sees in full: values that are not finite are left out (tree_add_nonfinite)
-    auto store = [&](int stage, const Place& p, bool sift, int at) __attribute__((always_inline)) {
-      uint32_t found = 0;
+    auto store = [&](int stage, const Place& p) __attribute__((always_inline)) {
       const uint32_t kb = lds0 + stage * 2 * kStage, vb = kb + kStage;
-      auto put_v = [&](uint32_t to, u32x4 x) __attribute__((always_inline)) {
-        if (sift) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = finite_pair<H>(x[q], found);
-        }
-        put(to, x);
-      };
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int n = piece_row + kRowStep * i;
@@ -172,20 +198,14 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
         if constexpr (kS) {
           put(kb + k_at<D>(n, 2 * piece), treer::widen8<Tag, C>(k[0], k[1]));
           put(kb + k_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(k[2], k[3]));
-          put_v(vb + v_at<D>(n, 2 * piece), treer::widen8<Tag, C>(v[0], v[1]));
-          put_v(vb + v_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(v[2], v[3]));
-        } else {
-          put(kb + k_at<D>(n, piece), k);
-          put_v(vb + v_at<D>(n, piece), v);
+          put(vb + v_at<D>(n, 2 * piece), treer::widen8<Tag, C>(v[0], v[1]));
+          put(vb + v_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(v[2], v[3]));
         }
       }
-      if (found != 0) found_lds[at] = 1;
-      if constexpr (kS) {
-        if (tid < kTile) {
-          sc_lds[stage][0][tid] = p.page >= 0 ? ks * a.scale_log2 : 0.f;
-          // (a NaN passes; a scale of 0 has codes of 0, so any weight does)
-          sc_lds[stage][1][tid] = p.page >= 0 ? __builtin_amdgcn_logf(nan_max(vs, 0x1p-100f)) : 0.f;
-        }
+      if (tid < kTile) {
+        sc_lds[stage][0][tid] = p.page >= 0 ? ks * a.scale_log2 : 0.f;
+        // (a NaN passes; a scale of 0 has codes of 0, so any weight does)
+        sc_lds[stage][1][tid] = p.page >= 0 ? __builtin_amdgcn_logf(nan_max(vs, 0x1p-100f)) : 0.f;
       }
     };
 
@@ -255,21 +275,9 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
       }
       uint32_t seen[kNQ];  // bit 4 kb + i: this lane's row sees its key
       if (!plain) {
-        const uint32_t there_lo = (uint32_t)(there >> (4 * lr)), there_hi = (uint32_t)(there >> 32 >> (4 * lr));
 #pragma unroll
         for (int x = 0; x < kNQ; ++x) {
-          seen[x] = 0;
-#pragma unroll 1
-          for (int n = 0; n < 4 * NKB; ++n) {
-            const int in_tile = 16 * (n >> 2) + (n & 3), draft = key + 4 * lr + in_tile - r.context;
-            bool s = ((in_tile < 32 ? there_lo : there_hi) >> (in_tile & 31) & 1u) != 0;
-            if (s && draft >= 0) {
-              if (a.words < 0) s = draft <= tok[x];
-              else if (draft < 64) s = (first_word[x] >> draft & 1ull) != 0;
-              else s = 16 * x + l16 < wave_rows && tree_sees(a, r.first + tok[x], tok[x], draft);
-            }
-            seen[x] |= (s ? 1u : 0u) << n;
-          }
+          seen[x] = tree_lane_keys<NKB>(there & tree_visible(a, r, 16 * x + l16 < wave_rows, tok[x], first_word[x], key), lr);
 #pragma unroll
           for (int n = 0; n < 4 * NKB; ++n)
             if (!(seen[x] >> n & 1u)) {
@@ -342,29 +350,44 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
 
     // ---- the tiles ----
     auto drafts = [&](int key) __attribute__((always_inline)) { return key + kTile > r.context; };
+    // the copies or stores of a tile are done, in every wave
+    auto landed = [&](int stage, int key, int at) __attribute__((always_inline)) {
+      if constexpr (kS) __syncthreads();
+      else wait_and_barrier<0>();
+      if constexpr (!std::is_same_v<C, int8_t>) {
+        if (key < key_hi && drafts(key)) {
+          sift(stage, at);
+          __syncthreads();
+        }
+      }
+    };
     if (tid < 3) found_lds[tid] = 0;
     Place p = checked(place(key_lo)), p1 = place(key_lo + kTile);
-    load(p);
+    if constexpr (kS) load(p);
     __syncthreads();
-    store(0, p, drafts(key_lo), 0);
-    __syncthreads();
+    if constexpr (kS) store(0, p);
+    else copy(0, p);
+    landed(0, key_lo, 0);
     int stage = 0, at = 0;  // at: the tile's number % 3
 #pragma unroll 1
     for (int key = key_lo; key < key_hi; key += kTile) {
       const bool more = key + kTile < key_hi;
       const Place p2 = place(key + 2 * kTile);  // (before the rows: loads return in order)
       p1 = checked(p1);
-      if (more) load(p1);
+      if constexpr (kS) load(p1);  // (also past the last: the wait for p2 behind a branch would be for every load)
+      else if (more) copy(stage ^ 1, p1);
       const int at1 = at == 2 ? 0 : at + 1;
       if (tid == 0) found_lds[at1 == 2 ? 0 : at1 + 1] = 0;  // read a tile ago, written in the next turn
       if (wave_rows > 0)
         compute(stage, key, __builtin_amdgcn_ballot_w64(p.page >= 0), p, drafts(key) && found_lds[at] != 0);
       stage ^= 1;
       at = at1;
-      if (more) store(stage, p1, drafts(key + kTile), at);
+      if constexpr (kS) {
+        if (more) store(stage, p1);
+      }
+      landed(stage, key + kTile, at);
       p = p1;
       p1 = p2;
-      __syncthreads();
     }
 
     // ---- this wave's rows: lane l16 holds row l16 of block x, d = 16 e + 4 lr + 0..3 ----
