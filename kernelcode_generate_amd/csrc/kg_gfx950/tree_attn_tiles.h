@@ -391,7 +391,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     }
 
     // ---- this wave's rows: lane l16 holds row l16 of block x, d = 16 e + 4 lr + 0..3 ----
-    float* record = split.partial + ((long long)2 * blockIdx.x + (starts_here ? 0 : 1)) * kRows * (D + kTreePad);
+    float* record = split.partial + ((long long)2 * share.w + (starts_here ? 0 : 1)) * kRows * (D + kTreePad);
 #pragma unroll
     for (int x = 0; x < kNQ; ++x) {
       float l = l_run[x][0];
