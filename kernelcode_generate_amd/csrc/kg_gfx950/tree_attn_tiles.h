@@ -249,14 +249,12 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
         if (kb + 1 < NKB) read_k(kb + 1);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < kNQ; ++x) sc[x][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < NDS; ++s)
 #pragma unroll
           for (int x = 0; x < kNQ; ++x) sc[x][kb] = H::mfma16(kf[kb & 1][s], qf[x][s], sc[x][kb]);
-        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
@@ -333,14 +331,12 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         if (g + 1 < kGroups) read_v(g + 1);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int c = (4 * g + u) / NE, e = (4 * g + u) % NE;
 #pragma unroll
           for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vf[g & 1][u], pp[x][c], o[x][e]);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
       if (!plain && found)
 #pragma unroll
