@@ -45,6 +45,12 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int b) {
   return r;
 }
 
+// Elements before row `offset` of a page that is there, for strides below 2^32: two multiply-adds (eight multiplications of the
+// general product are four cycles each).
+__device__ __forceinline__ unsigned long long tree_row(int page, int offset, long long page_stride, long long row_stride) {
+  return (unsigned long long)(uint32_t)page * (uint32_t)page_stride + (unsigned long long)(uint32_t)offset * (uint32_t)row_stride;
+}
+
 // Whether token j of a request (batch row t) sees the drafted token i >= 0.
 __device__ __forceinline__ bool tree_sees(const TreeArgs& a, int t, int j, int i) {
   if (a.words < 0) return i <= j;

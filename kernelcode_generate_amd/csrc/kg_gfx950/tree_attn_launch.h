@@ -10,13 +10,18 @@
 
 namespace kg_gfx950 {
 
-// What they take: 16-bit queries, heads of a multiple of 16 up to 256, rows of 16-byte pieces.
+// What they take: 16-bit queries, heads of a multiple of 16 up to 256, rows of 16-byte pieces, strides of tree_row.
 inline bool tree_matrix_takes(const TreeArgs& a, int cache_bytes) {
   auto whole = [&](const void* p, std::initializer_list<long long> strides, int bytes, int unit) {
     bool ok = (uintptr_t)p % unit == 0;
     for (long long s : strides) ok = ok && s * bytes % unit == 0;
     return ok;
   };
+  for (long long s : {a.k_page, a.v_page})
+    if (s > 0xffffffffLL) return false;
+  if (a.k_scale != nullptr)
+    for (long long s : {a.ks_page, a.ks_row, a.vs_page, a.vs_row})
+      if (s > 0xffffffffLL) return false;
   return a.d % 16 == 0 && a.d <= 256 && whole(a.q, {a.q_token, a.q_head}, 2, 16) && whole(a.out, {a.o_token, a.o_head}, 2, 4) &&
          whole(a.k, {a.k_page, a.k_head, a.k_row}, cache_bytes, 16) && whole(a.v, {a.v_page, a.v_head, a.v_row}, cache_bytes, 16) &&
          a.k_row <= 1 << 24 && a.v_row <= 1 << 24 && a.pages > 0 && a.per > 0;

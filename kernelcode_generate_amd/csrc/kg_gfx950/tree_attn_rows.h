@@ -305,6 +305,8 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
     }
     const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
     const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
+    const float* k_scale = kS ? a.k_scale + h * a.ks_head : nullptr;
+    const float* v_scale = kS ? a.v_scale + h * a.vs_head : nullptr;
     const int* table = a.table + share.b * a.table_0;
 
     // Page of key `lane` of a step (-1: none, or a key past the range) and its offset there.
@@ -332,8 +334,8 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
     float ks = 0.f, vs = 0.f;  // of key `lane` of the step
     auto load_k = [&](const Place& p) __attribute__((always_inline)) {
       if constexpr (kS) {
-        ks = a.k_scale[(long long)max(p.page, 0) * a.ks_page + h * a.ks_head + (long long)p.offset * a.ks_row];
-        vs = a.v_scale[(long long)max(p.page, 0) * a.vs_page + h * a.vs_head + (long long)p.offset * a.vs_row];
+        ks = k_scale[tree_row(max(p.page, 0), p.offset, a.ks_page, a.ks_row)];
+        vs = v_scale[tree_row(max(p.page, 0), p.offset, a.vs_page, a.vs_row)];
       }
       // (a lane's d past the head's end: its first ones)
       auto piece = [&](const C* row, int kb, int s) __attribute__((always_inline)) {

@@ -112,6 +112,8 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     }
     const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
     const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
+    const float* k_scale = kS ? a.k_scale + h * a.ks_head : nullptr;
+    const float* v_scale = kS ? a.v_scale + h * a.vs_head : nullptr;
     const int* table = a.table + share.b * a.table_0;
 
     // Page of key `lane` of a tile (-1: none, or a key past the range), its offset there, and its rows: a lane's 64-bit
@@ -128,8 +130,8 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     };
     auto checked = [&](Place p) __attribute__((always_inline)) {
       const bool there = p.page >= 0 && p.page < a.pages;
-      const unsigned long long k = (unsigned long long)(kc + p.page * a.k_page + (long long)p.offset * (int)a.k_row);
-      const unsigned long long v = (unsigned long long)(vc + p.page * a.v_page + (long long)p.offset * (int)a.v_row);
+      const unsigned long long k = (unsigned long long)(kc + tree_row(p.page, p.offset, a.k_page, a.k_row));
+      const unsigned long long v = (unsigned long long)(vc + tree_row(p.page, p.offset, a.v_page, a.v_row));
       const unsigned long long zeros = (unsigned long long)&kZeros;
       return Place{there ? p.page : -1, there ? p.offset : 0, there ? k : zeros, there ? v : zeros};
     };
@@ -177,12 +179,12 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
         const int page = __shfl(p.page, n, 64), offset = __shfl(p.offset, n, 64);
         row_there |= (page >= 0 ? 1u : 0u) << i;
         const int d = piece_in ? piece * 16 : 0;
-        kr[i] = ld16(kc + (long long)max(page, 0) * a.k_page + (long long)offset * a.k_row + d);
-        vr[i] = ld16(vc + (long long)max(page, 0) * a.v_page + (long long)offset * a.v_row + d);
+        kr[i] = ld16(kc + tree_row(max(page, 0), offset, a.k_page, a.k_row) + d);
+        vr[i] = ld16(vc + tree_row(max(page, 0), offset, a.v_page, a.v_row) + d);
       }
       if constexpr (kS) {
-        ks = a.k_scale[(long long)max(p.page, 0) * a.ks_page + h * a.ks_head + (long long)p.offset * a.ks_row];
-        vs = a.v_scale[(long long)max(p.page, 0) * a.vs_page + h * a.vs_head + (long long)p.offset * a.vs_row];
+        ks = k_scale[tree_row(max(p.page, 0), p.offset, a.ks_page, a.ks_row)];
+        vs = v_scale[tree_row(max(p.page, 0), p.offset, a.vs_page, a.vs_row)];
       }
     };
     auto put = [&](uint32_t at, u32x4 x) __attribute__((always_inline)) {
