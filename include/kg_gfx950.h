@@ -21,7 +21,7 @@
  * and element strides. Kernels allocate nothing per call, with one exception: calls that need
  * memory between their launches (fp32 partial sums of a K split over workgroups, packed operands
  * of matmuls with unaligned rows, a conv's channel-last copy, partial outputs of split attention
- * keys) take it from a workspace held per (device, stream) for the life of the process (at most
+ * keys, the low-rank sums of projections with adapters) take it from a workspace held per (device, stream) for the life of the process (at most
  * 64 MiB, for 8 streams per device), allocated on the first such call on that stream and
  * reallocated when a later one needs more. While a stream records a HIP graph such calls take a
  * buffer that belongs to the graph instead: it is allocated during the recording, lives as long as
@@ -165,7 +165,7 @@ int kg_gfx950_kv_cache_load_entry(const KgArgSlot* ordered_args, unsigned long l
  * i <= j: a decoding step (one token), a chain of drafts, a piece of a prompt. Query head h reads key head h / (Hq / heads).
  * Rows that see nothing get zeros; rows of no request are left as they are. Positions past P * page_size and
  * pages outside 0 .. pages - 1 are not seen. What is not seen has no influence, infinities and NaN included. q, out:
- * f32, f16 or bf16; of a cache that is not in 8 bits, its type. P * page_size < 2^31. out must not overlap q.
+ * f32, f16 or bf16; of a cache that is not in 8 bits, its type. P * page_size <= 2^31 - 4096. out must not overlap q.
  */
 int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
 

@@ -10,7 +10,11 @@
 
 namespace kg_gfx950 {
 
-// What they take: 16-bit queries, heads of a multiple of 16 up to 256, rows of 16-byte pieces, strides of tree_row.
+inline long long tree_items(const TreeArgs& a, int block) {  // at most, where `starts` ascend
+  return a.heads * ((long long)a.tokens * a.group / block + std::min(a.batch, a.tokens));
+}
+// What they take: 16-bit queries, heads of a multiple of 16 up to 256, rows of 16-byte pieces, strides of tree_row, sums of
+// units in 31 bits.
 inline bool tree_matrix_takes(const TreeArgs& a, int cache_bytes) {
   auto whole = [&](const void* p, std::initializer_list<long long> strides, int bytes, int unit) {
     bool ok = (uintptr_t)p % unit == 0;
@@ -22,6 +26,7 @@ inline bool tree_matrix_takes(const TreeArgs& a, int cache_bytes) {
   if (a.k_scale != nullptr)
     for (long long s : {a.ks_page, a.ks_row, a.vs_page, a.vs_row})
       if (s > 0xffffffffLL) return false;
+  if ((long long)a.tokens * a.heads_q > kTreeMostUnits || tree_items(a, 16) > kTreeMostUnits) return false;
   return a.d % 16 == 0 && a.d <= 256 && whole(a.q, {a.q_token, a.q_head}, 2, 16) && whole(a.out, {a.o_token, a.o_head}, 2, 4) &&
          whole(a.k, {a.k_page, a.k_head, a.k_row}, cache_bytes, 16) && whole(a.v, {a.v_page, a.v_head, a.v_row}, cache_bytes, 16) &&
          a.k_row <= 1 << 24 && a.v_row <= 1 << 24 && a.pages > 0 && a.per > 0;
@@ -37,9 +42,6 @@ struct TreePlan {
 };
 // Shares of a call: as many workgroups as run at once, or as there can be units (the table's reach bounds a
 // request's keys, the batch's tokens its blocks of rows).
-inline long long tree_items(const TreeArgs& a, int block) {  // at most
-  return a.heads * ((long long)a.tokens * a.group / block + a.batch);
-}
 inline TreePlan tree_plan(const TreeArgs& a, int cache_bytes, bool may_split, long long most_bytes) {
   TreePlan p;
   p.width = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
@@ -53,7 +55,7 @@ inline TreePlan tree_plan(const TreeArgs& a, int cache_bytes, bool may_split, lo
   const long long reach = (long long)a.per * a.page_size;
   const long long items = tree_items(a, p.split.block);
   const long long units = items * std::max(1ll, (reach + round - 1) / round);
-  may_split = may_split && reach > round && units < 0x7fffffffLL;
+  may_split = may_split && reach > round && units < kTreeMostUnits && items * p.split.block / kTreeJoinRows < 0x7fffffffLL;
   p.split.round = may_split ? (int)round : 0;
   p.split.grid = (int)std::min<long long>(may_split ? units : items, p.width == 256 ? 256 : 512);
   const long long record = 2ll * p.split.block * (p.width + kTreePad) * (long long)sizeof(float);

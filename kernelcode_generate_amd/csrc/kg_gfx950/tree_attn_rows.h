@@ -118,11 +118,15 @@ __device__ __forceinline__ int tree_units(const TreeArgs& a, const TreeSplit& s,
   const TreeRequest r = tree_request(a, b);
   return r.count == 0 ? 0 : a.heads * tree_blocks(r, a.group, s.block) * tree_rounds(r, s.round);
 }
+// Sums of units, up to the most there are where `starts` ascend: others than that may repeat the tokens, and their requests
+// past the limit have no units (a request's own are below it by the host's checks).
+constexpr int kTreeMostUnits = 1 << 30;
+__device__ __forceinline__ int tree_sum(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)kTreeMostUnits); }
 __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int x = __shfl_up(v, o, 64);
-    if (lane >= o) v += x;
+    if (lane >= o) v = tree_sum(v, x);
   }
   return v;
 }
@@ -150,7 +154,7 @@ __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, const TreeSpl
   const int upto = wave_scan(mine, lane);
   t.total = __builtin_amdgcn_readlane(upto, 63);
   for (int b0 = 64; b0 < a.batch; b0 += 64)
-    t.total += __builtin_amdgcn_readlane(wave_scan(tree_units(a, s, b0 + lane), lane), 63);
+    t.total = tree_sum(t.total, __builtin_amdgcn_readlane(wave_scan(tree_units(a, s, b0 + lane), lane), 63));
   const int eighth = min(s.grid, t.total) >> 3;
   t.w = id < 8 * eighth ? (id & 7) * eighth + (id >> 3) : id;
   t.first = share_bound(t.w, s, t.total);
@@ -160,7 +164,7 @@ __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, const TreeSpl
   t.base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int own = b0 == 0 ? mine : tree_units(a, s, b0 + lane);
-    const int end = t.base + (b0 == 0 ? upto : wave_scan(own, lane));
+    const int end = tree_sum(t.base, b0 == 0 ? upto : wave_scan(own, lane));
     const unsigned long long behind = __builtin_amdgcn_ballot_w64(end > t.first);
     if (behind != 0) {
       const int x = __builtin_ctzll(behind);
@@ -264,7 +268,7 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
     const int units = r.count == 0 ? 0 : a.heads * blocks * rounds;
     const int local = share.first - share.base;
     if (local >= units) {
-      share.base += units;
+      share.base = tree_sum(share.base, units);
       ++share.b;
       continue;
     }
@@ -609,17 +613,17 @@ __global__ __launch_bounds__(64 * tree_join_waves(kWaves)) void tree_attn_join_k
     }
     const int upto_items = wave_scan(own_items, lane), upto = wave_scan(own_units, lane);
     if (owner < 0) {
-      const unsigned long long behind = __builtin_amdgcn_ballot_w64(items + upto_items > item);
+      const unsigned long long behind = __builtin_amdgcn_ballot_w64(tree_sum(items, upto_items) > item);
       if (behind != 0) {
         const int x = __builtin_ctzll(behind);
         owner = b0 + x;
-        items += __builtin_amdgcn_readlane(upto_items, x) - __builtin_amdgcn_readlane(own_items, x);
-        base = total + __builtin_amdgcn_readlane(upto, x) - __builtin_amdgcn_readlane(own_units, x);
+        items = tree_sum(items, __builtin_amdgcn_readlane(upto_items, x)) - __builtin_amdgcn_readlane(own_items, x);
+        base = tree_sum(total, __builtin_amdgcn_readlane(upto, x)) - __builtin_amdgcn_readlane(own_units, x);
       } else {
-        items += __builtin_amdgcn_readlane(upto_items, 63);
+        items = tree_sum(items, __builtin_amdgcn_readlane(upto_items, 63));
       }
     }
-    total += __builtin_amdgcn_readlane(upto, 63);
+    total = tree_sum(total, __builtin_amdgcn_readlane(upto, 63));
   }
   if (owner < 0) return;
   const TreeRequest r = tree_request(a, owner);

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     const int units = r.count == 0 ? 0 : a.heads * blocks * rounds;
     const int local = share.first - share.base;
     if (local >= units) {
-      share.base += units;
+      share.base = tree_sum(share.base, units);
       ++share.b;
       continue;
     }

@@ -1287,8 +1287,14 @@ int read_view(const KgArgSlot* slots, int idx, int rank, unsigned types, bool al
   return kOk;
 }
 
+bool no_elements(const Mem& m) {  // (extents of axes without a stride may have any product)
+  bool none = false;
+  for (int i = 0; i < m.rank; ++i) none = none || m.shape[i] == 0;
+  return none;
+}
+
 int check_view(const Mem& m, const char* name) {
-  if (!m.present || m.numel() == 0) return kOk;
+  if (!m.present || no_elements(m)) return kOk;
   if (m.data == nullptr) return fail(kInvalid, "%s: memory slot has no data", name);
   hipPointerAttribute_t attr;
   if (hipPointerGetAttributes(&attr, m.data) != hipSuccess || attr.type != hipMemoryTypeDevice) {
@@ -1468,7 +1474,7 @@ int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
   if ((rc = check_view(rows[0], "k_out")) || (rc = check_view(rows[1], "v_out")) || (rc = check_kv(kv)) ||
       (rc = check_view(table, "page_table")) || (rc = check_view(lens, "lengths")))
     return rc;
-  if (rows[0].numel() == 0 || table.shape[1] == 0) return finish_launch("kv_cache_load(empty)");
+  if (no_elements(rows[0]) || table.shape[1] == 0) return finish_launch("kv_cache_load(empty)");
   KvLoadArgs a;
   for (int x = 0; x < 2; ++x) a.side[x] = kv_side(kv, x, rows[x]);
   a.table = static_cast<const int*>(table.data);
@@ -1505,6 +1511,9 @@ int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
   });
 }
 
+// Positions of a request: the kernels' steps, and the pages looked up ahead of them, stay in 31 bits.
+constexpr long long kTreeMostKeys = (1ll << 31) - 4096;
+
 int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
   if (args == nullptr) return fail(kInvalid, "ordered_args is null");
   if (n != 11) return fail(kInvalid, "tree_attention expects 11 slots, got %llu", n);
@@ -1535,12 +1544,12 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
     return fail(kInvalid, "tree_attention: starts must have %lld values, got %lld", batch + 1, starts.shape[0]);
   if (mask.present && mask.shape[0] != tokens)
     return fail(kInvalid, "tree_attention: mask has %lld rows for %lld tokens", mask.shape[0], tokens);
-  if (table.shape[1] * kv.page_size > 0x7fffffffLL)
+  if (table.shape[1] * kv.page_size > kTreeMostKeys)
     return fail(kUnsupported, "tree_attention: a page table of %lld x %lld tokens exceeds int32", table.shape[1], kv.page_size);
   if ((rc = check_view(out, "out")) || (rc = check_view(q, "q")) || (rc = check_kv(kv)) || (rc = check_view(table, "page_table")) ||
       (rc = check_view(lens, "context_lens")) || (rc = check_view(starts, "starts")) || (rc = check_view(mask, "mask")))
     return rc;
-  if (out.numel() == 0 || batch == 0) return finish_launch("tree_attention(empty)");
+  if (no_elements(out) || batch == 0) return finish_launch("tree_attention(empty)");
   TreeArgs a;
   a.q = q.data;
   a.out = out.data;
@@ -1723,13 +1732,31 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
                     rows_aligned(x, 16) && rows_aligned(w, 16) && rows_aligned(b, 16) && rows_aligned(a, 16) &&
                     x.stride[0] <= kMaxPipeLd && w.stride[0] <= kMaxPipeLd;
   if (mfma) {
-    const AdapterPlan plan = adapter_plan(p);
+    // pieces of whole 256-row tiles whose sums fit the workspace (262144 rows of rank 64: two)
+    const long long most = ((long long)kSplitMaxWorkspace - kAdapterHeader - 256) / (rank * 4) / 256 * 256;
+    const long long rows = cdiv(cdiv(M, cdiv(M, most)), 256) * 256;
+    auto piece = [&](long long m0) {
+      AdapterArgs part = p;
+      part.x = static_cast<const uint16_t*>(p.x) + m0 * p.ldx;
+      part.out = static_cast<uint16_t*>(p.out) + m0 * p.ldo;
+      part.index = p.index + m0 * p.index_stride;
+      part.m = (int)std::min(rows, M - m0);
+      return part;
+    };
+    const size_t bytes = std::max(adapter_plan(piece(0)).bytes, adapter_plan(piece((M - 1) / rows * rows)).bytes);
     SplitLease lease;  // held until the kernels are enqueued
-    if (plan.bytes <= (size_t)kSplitMaxWorkspace) lease = split_workspace(plan.bytes, g_stream);
+    if (bytes <= (size_t)kSplitMaxWorkspace) lease = split_workspace(bytes, g_stream);
     const int bias_kind = !bias.present ? 0 : bias.dtype == KG_DTYPE_F32 ? 1 : 2;
-    if (char* ws = static_cast<char*>(lease.ptr))
-      return out.dtype == KG_DTYPE_BF16 ? launch_adapter_matmul<Bf16Tag>(p, plan, bias_kind, ws)
-                                        : launch_adapter_matmul<F16Tag>(p, plan, bias_kind, ws);
+    if (char* ws = static_cast<char*>(lease.ptr)) {
+      for (long long m0 = 0; m0 < M; m0 += rows) {
+        const AdapterArgs part = piece(m0);
+        const AdapterPlan plan = adapter_plan(part);
+        if ((rc = out.dtype == KG_DTYPE_BF16 ? launch_adapter_matmul<Bf16Tag>(part, plan, bias_kind, ws)
+                                             : launch_adapter_matmul<F16Tag>(part, plan, bias_kind, ws)))
+          return rc;
+      }
+      return kOk;
+    }
   }
   if ((rc = matmul_impl(args, 4)) || !adapters) return rc;
   return with_kv_types(out.dtype, out.dtype, [&](auto t, auto) {

@@ -149,3 +149,11 @@ def test_empty_calls(device):
     native.adapter_matmul(out, torch.zeros(3, 0, **z), torch.zeros(0, 16, **z), torch.full((16,), 2.0, device=device), torch.zeros(1, 0, 8, **z),
                           torch.ones(1, 8, 16, **z), torch.zeros(3, dtype=torch.int32, device=device))
     assert (f64(out) == 2).all()
+
+
+@pytest.mark.parametrize("model,m,rank", [(BF16, 66000, 512), (F16, 40001, 448)])
+def test_rows_whose_sums_exceed_the_workspace(device, model, m, rank):
+    """32-bit sums of m x rank values are more than the workspace holds: the rows go in pieces."""
+
+    call = Call(m, 64, 64, 3, rank, model, order="sorted")
+    call.check(call.run(device))

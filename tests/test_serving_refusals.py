@@ -159,3 +159,24 @@ def test_other_entries_take_no_8_bit_memory():
     x = torch.zeros(4, 4, dtype=torch.int8)
     with pytest.raises(native.NativeLibraryError, match="unsupported dtype_code 7"):
         native.matmul(x, x, x)
+
+
+def test_axes_without_strides_are_elements():
+    """Extents whose product is a multiple of 2^64 are no empty tensor: the memory behind them is checked."""
+
+    cache = native.TensorSpec((2**30, 2**4, 2**26, 64), "bfloat16", (0, 0, 0, 1))
+    refused("load", load_args, -1, "k_out: data is not a device pointer",
+            **{x: native.TensorSpec((2**30, 2**4, 2**26, 64), "bfloat16", (0, 0, 0, 1)) for x in ("k_out", "v_out")},
+            k_cache=cache, v_cache=cache, page_table=native.TensorSpec((2**30, 1), "int32", (0, 0)),
+            lengths=native.TensorSpec((2**30,), "int32", (0,)))
+    rows = native.TensorSpec((2**30, 2**30, 64), "bfloat16", (0, 0, 1))
+    refused("tree", tree_args, -1, "out: data is not a device pointer", out=rows, q=rows)
+
+
+def test_the_most_positions_of_a_request():
+    """Past 2^31 - 4096 the kernels' steps and the pages looked up ahead would leave 32 bits."""
+
+    for columns, page, text in ((2**27 - 256, 16, "not a device pointer"), (2**27 - 255, 16, "exceeds int32")):
+        caches = [torch.zeros(1, 2, page, 64, dtype=torch.bfloat16) for _ in range(2)]
+        refused("tree", tree_args, -1 if text.startswith("not") else -3, text, k_cache=caches[0], v_cache=caches[1],
+                page_table=torch.zeros(2, 1, dtype=torch.int32).expand(2, columns))
