@@ -14,7 +14,7 @@
 //
 // 8-bit caches: codes are widened to 16 bits (exact for both types) for the products; a key's scale multiplies
 // its scores, a value's its weights. Weights are rounded to 16 bits with that scale in them, so the running
-// maximum is of s + log2(value's scale): weights of at most 1, whatever the scales' sizes. The sum of weights stays in 32 bits.
+// maximum is of s + log2(value's scale): weights of at most 2^8, whatever the scales' sizes. The sum of weights stays in 32 bits.
 //
 // Weights of 16-bit caches are rounded to 16 bits, as in the flash attention kernels, and summed as rounded.
 #pragma once
@@ -32,6 +32,9 @@ namespace treer {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kMinMax = -3.0e38f;  // the lowest running maximum: scores of -inf weigh nothing beside it
+// The running maximum (log2 units) is raised by scores beyond it by more than this: weights are at most 2^8, and sums
+// are rescaled a few times and not at every other tile. Weights and their sum have the same maximum, so the result does not depend on it.
+constexpr float kSlack = 8.f;
 // keys of a wave's step: 16 KiB of K and V rows, or what the registers hold (8 KiB of 8-bit heads of 64,
 // and of 128 with two blocks of rows; 32 KiB of 16-bit heads of 256)
 template <typename C, int D, int kNQ>
@@ -480,10 +483,10 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
         for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(n));
         float mx2 = mx;
         fa::rows4_combine<true>(mx, mx2);
-        const float m_new = nan_max(m_run[x], mx);
-        if (__builtin_amdgcn_ballot_w64(m_new > m_run[x] || m_new != m_new)) {
-          const float alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
-          m_run[x] = m_new;
+        const bool raise = !(mx <= m_run[x] + kSlack);  // (a NaN too)
+        if (__builtin_amdgcn_ballot_w64(raise)) {
+          const float alpha = raise ? __builtin_amdgcn_exp2f(m_run[x] - mx) : 1.f;
+          m_run[x] = raise ? mx : m_run[x];
           l_run[x] *= alpha;
 #pragma unroll
           for (int e = 0; e < NE; ++e) o[x][e] *= alpha;

@@ -37,6 +37,17 @@ template <int D>
 __device__ __forceinline__ uint32_t v_at(int r, int c) {
   return r * D * 2 + 16 * (D == 64 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * (r & 7)));
 }
+// A query pair for scores that are multiplied by |scale|, or 1 where scale is 0: their products are -1 or 0 times
+// those of the pair (0 times what is not finite: NaN). A positive factor leaves the largest score the largest.
+template <typename H>
+__device__ __forceinline__ uint32_t with_sign(uint32_t w, float scale) {
+  uint32_t bad = 0;
+  if (scale == 0.f) {
+    const uint32_t finite = finite_pair<H>(w, bad);
+    return (w ^ finite) | (bad >> 15);
+  }
+  return scale < 0.f ? w ^ 0x80008000u : w;
+}
 __device__ const char kZeros[512] = {};  // the row of a key that is not there
 }  // namespace treet
 
@@ -44,6 +55,7 @@ template <typename Tag, typename C, int D, int kNQ>
 __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(TreeArgs a, TreeSplit split) {
   using namespace treet;
   using treer::kMinMax;
+  using treer::kSlack;
   using H = Half16<Tag>;
   constexpr bool kS = treer::kScaled<C>;
   constexpr int kES = sizeof(C);
@@ -109,7 +121,13 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
                           ((long long)h * a.group + (row - tok[x] * a.group)) * a.q_head;
 #pragma unroll
       for (int s = 0; s < NDS; ++s) qf[x][s] = real && 32 * s + 8 * lr < a.d ? ld16(q + 32 * s + 8 * lr) : u32x4{0, 0, 0, 0};
+      if constexpr (!kS)
+#pragma unroll
+        for (int s = 0; s < NDS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qf[x][s][i] = treet::with_sign<H>(qf[x][s][i], a.scale_log2);
     }
+    const float scale = a.scale_log2 == 0.f ? 1.f : __builtin_fabsf(a.scale_log2);
     const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
     const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
     const float* k_scale = kS ? a.k_scale + h * a.ks_head : nullptr;
@@ -143,14 +161,23 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     // Lane l's 16 bytes land at 16 l, so it takes the chunk that the swizzle puts there.
     auto copy = [&](int stage, const Place& p) __attribute__((always_inline)) {
       const uint32_t kb = lds0 + stage * 2 * kStage + wave * 1024, vb = kb + kStage;
+      auto pieces = [&](auto padded) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int n = piece_row + kRowStep * i;
-        const uint32_t ck = k_at<D>(n, piece) - n * D * 2, cv = v_at<D>(n, piece) - n * D * 2;  // bytes in the row
-        const unsigned long long k = row_of(p.k, n), v = row_of(p.v, n), zeros = (unsigned long long)&kZeros;
-        g2lds16_m(reinterpret_cast<const char*>(((int)ck < 2 * a.d ? k : zeros) + ck), kb + i * kThreads * 16);
-        g2lds16_m(reinterpret_cast<const char*>(((int)cv < 2 * a.d ? v : zeros) + cv), vb + i * kThreads * 16);
-      }
+        for (int i = 0; i < kPieces; ++i) {
+          const int n = piece_row + kRowStep * i;
+          const uint32_t ck = k_at<D>(n, piece) - n * D * 2, cv = v_at<D>(n, piece) - n * D * 2;  // bytes in the row
+          unsigned long long k = row_of(p.k, n), v = row_of(p.v, n);
+          if constexpr (decltype(padded)::value != 0) {
+            const unsigned long long zeros = (unsigned long long)&kZeros;
+            k = (int)ck < 2 * a.d ? k : zeros;
+            v = (int)cv < 2 * a.d ? v : zeros;
+          }
+          g2lds16_m(reinterpret_cast<const char*>(k + ck), kb + i * kThreads * 16);
+          g2lds16_m(reinterpret_cast<const char*>(v + cv), vb + i * kThreads * 16);
+        }
+      };
+      if (a.d == D) pieces(Int<0>{});
+      else pieces(Int<1>{});
     };
     // A tile that not every row sees in full: values that are not finite are left out of the products (tree_add_nonfinite).
     auto sift = [&](int stage, int at) __attribute__((always_inline)) {
@@ -259,20 +286,18 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
           for (int x = 0; x < kNQ; ++x) sc[x][kb] = H::mfma16(kf[kb & 1][s], qf[x][s], sc[x][kb]);
       }
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        f32x4 f = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2}, lv;
+      for (int kb = 0; kb < NKB; ++kb)
         if constexpr (kS) {
-          f = *reinterpret_cast<const f32x4*>(&sc_lds[stage][0][16 * kb + 4 * lr]);
-          lv = *reinterpret_cast<const f32x4*>(&sc_lds[stage][1][16 * kb + 4 * lr]);
+          const f32x4 f = *reinterpret_cast<const f32x4*>(&sc_lds[stage][0][16 * kb + 4 * lr]);
+          const f32x4 lv = *reinterpret_cast<const f32x4*>(&sc_lds[stage][1][16 * kb + 4 * lr]);
+#pragma unroll
+          for (int x = 0; x < kNQ; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              sc[x][kb][i] *= f[i];
+              y[x][kb][i] = sc[x][kb][i] + lv[i];
+            }
         }
-#pragma unroll
-        for (int x = 0; x < kNQ; ++x)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[x][kb][i] *= f[i];
-            if constexpr (kS) y[x][kb][i] = sc[x][kb][i] + lv[i];
-          }
-      }
       uint32_t seen[kNQ];  // bit 4 kb + i: this lane's row sees its key
       if (!plain) {
 #pragma unroll
@@ -302,12 +327,13 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
         float mx = weighed(0);
 #pragma unroll
         for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(n));
+        if constexpr (!kS) mx *= scale;
         float mx2 = mx;
         fa::rows4_combine<true>(mx, mx2);
-        const float m_new = nan_max(m_run[x], mx);
-        if (__builtin_amdgcn_ballot_w64(m_new > m_run[x] || m_new != m_new)) {
-          const float alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
-          m_run[x] = m_new;
+        const bool raise = !(mx <= m_run[x] + kSlack);  // (a NaN too)
+        if (__builtin_amdgcn_ballot_w64(raise)) {
+          const float alpha = raise ? __builtin_amdgcn_exp2f(m_run[x] - mx) : 1.f;
+          m_run[x] = raise ? mx : m_run[x];
           l_run[x] *= alpha;
 #pragma unroll
           for (int e = 0; e < NE; ++e) o[x][e] *= alpha;
@@ -317,7 +343,8 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run[x]);
+            if constexpr (kS) w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run[x]);
+            else w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(weighed(4 * kb + i), scale, -m_run[x]));
             if constexpr (kS) l_run[x][0] += __builtin_amdgcn_exp2f((float)sc[x][kb][i] - m_run[x]);
           }
           pp[x][kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
