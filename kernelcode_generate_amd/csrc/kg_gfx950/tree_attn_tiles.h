@@ -8,10 +8,12 @@
 // (16-byte chunk c of row r at c ^ (r % 16): 16 rows hit distinct banks), V^T fragments two ds_read_b64_tr_b16 per 16 d x 32
 // keys in the key order that P's lanes hold (chunk pairs at pair ^ (r % 8): the 8 rows of half a wave do).
 //
-// Measured, heads of 128 in 8 groups of 4: 2 x 512 rows behind 4096 in bf16 144 us with the join, 507 TFLOP/s (654 behind
-// 16384); with rows through registers, which spilled, and a loop over the keys of tiles with drafts, 185. 8 x 16 rows behind 16384: bf16
-// 114 us, 4.75 TB/s of rows; e4m3 104 us, bound by each wave's chain of widening, products and softmax, not by bytes (two tiles
-// in flight: 110; eight waves with half the keys each, in 128 registers: 162).
+// Measured, heads of 128 in 8 groups of 4: 2 x 512 rows behind 4096 in bf16 136 us with the join, 538 TFLOP/s (674 behind
+// 16384); with rows through registers, which spilled, and a loop over the keys of tiles with drafts, 185. Two waves a SIMD
+// issue vector instructions for 3000 of the 6500 cycles that two tiles of 128 rows take, MFMAs fill 2200, reads of LDS 2000: a
+// tile's scores taken under the exponentials of the one before (33 registers more, spilled) took 151. 8 x 16 rows behind
+// 16384: bf16 115 us, 4.7 TB/s of rows; e4m3 96 us, bound by each wave's chain of widening, products and softmax, not by bytes (two
+// tiles in flight: 6 % longer; eight waves with half the keys each, in 128 registers: 56 %).
 #pragma once
 
 #include "common.h"
@@ -261,9 +263,9 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
       const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
       return u32x4{w0[0], w0[1], w1[0], w1[1]};
     };
-    // plain: a tile of the context, every key of it there; `there`: bits of those that are (placed at p); found: the
+    // plain: a tile of the context, every key of it there; `there`: bits of those that are; found: the
     // tile had values that are not finite
-    auto compute = [&](int stage, int key, unsigned long long there, const Place& p, bool found) __attribute__((always_inline)) {
+    auto compute = [&](int stage, int key, unsigned long long there, bool found) __attribute__((always_inline)) {
       const bool plain = ~there == 0 && key + kTile <= r.context;
       const uint32_t kbase = lds0 + stage * 2 * kStage;
       f32x4 sc[kNQ][NKB], y[kS ? kNQ : 1][NKB];  // y: with the values' scales
@@ -317,16 +319,15 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
         for (int u = 0; u < 4; ++u) vf[g & 1][u] = v_frag(stage, (4 * g + u) / NE, (4 * g + u) % NE);
       };
       read_v(0);
-      u32x4 pp[kNQ][NC];
+      auto weighed = [&](int x, int n) __attribute__((always_inline)) {
+        if constexpr (kS) return (float)y[x][n >> 2][n & 3];
+        else return (float)sc[x][n >> 2][n & 3];
+      };
 #pragma unroll
       for (int x = 0; x < kNQ; ++x) {
-        auto weighed = [&](int n) __attribute__((always_inline)) {
-          if constexpr (kS) return (float)y[x][n >> 2][n & 3];
-          else return (float)sc[x][n >> 2][n & 3];
-        };
-        float mx = weighed(0);
+        float mx = weighed(x, 0);
 #pragma unroll
-        for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(n));
+        for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(x, n));
         if constexpr (!kS) mx *= scale;
         float mx2 = mx;
         fa::rows4_combine<true>(mx, mx2);
@@ -338,13 +339,17 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
 #pragma unroll
           for (int e = 0; e < NE; ++e) o[x][e] *= alpha;
         }
+      }
+      u32x4 pp[kNQ][NC];
+#pragma unroll
+      for (int x = 0; x < kNQ; ++x) {
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) {
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if constexpr (kS) w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run[x]);
-            else w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(weighed(4 * kb + i), scale, -m_run[x]));
+            if constexpr (kS) w[i] = __builtin_amdgcn_exp2f(weighed(x, 4 * kb + i) - m_run[x]);
+            else w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(weighed(x, 4 * kb + i), scale, -m_run[x]));
             if constexpr (kS) l_run[x][0] += __builtin_amdgcn_exp2f((float)sc[x][kb][i] - m_run[x]);
           }
           pp[x][kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
@@ -367,10 +372,12 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
           for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vf[g & 1][u], pp[x][c], o[x][e]);
         }
       }
-      if (!plain && found)
+      if (!plain && found) {
+        const Place p = checked(place(key));
 #pragma unroll
         for (int x = 0; x < kNQ; ++x)
           tree_add_nonfinite<Tag, C, kTile>(a, o[x], seen[x], p.page, p.offset, h, lane, [&](int e, int i) { return 16 * e + 4 * lr + i; });
+      }
     };
 
     // ---- the tiles ----
@@ -388,6 +395,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     };
     if (tid < 3) found_lds[tid] = 0;
     Place p = checked(place(key_lo)), p1 = place(key_lo + kTile);
+    unsigned long long there = __builtin_amdgcn_ballot_w64(p.page >= 0);
     if constexpr (kS) load(p);
     __syncthreads();
     if constexpr (kS) store(0, p);
@@ -404,14 +412,14 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
       const int at1 = at == 2 ? 0 : at + 1;
       if (tid == 0) found_lds[at1 == 2 ? 0 : at1 + 1] = 0;  // read a tile ago, written in the next turn
       if (wave_rows > 0)
-        compute(stage, key, __builtin_amdgcn_ballot_w64(p.page >= 0), p, drafts(key) && found_lds[at] != 0);
+        compute(stage, key, there, drafts(key) && found_lds[at] != 0);
       stage ^= 1;
       at = at1;
       if constexpr (kS) {
         if (more) store(stage, p1);
       }
       landed(stage, key + kTile, at);
-      p = p1;
+      there = __builtin_amdgcn_ballot_w64(p1.page >= 0);
       p1 = p2;
     }
 
