@@ -221,14 +221,14 @@ __device__ __forceinline__ void adapter_put(u32x4 x, uint32_t to, uint32_t& foun
 }
 
 // t = scale x A of 16 rows and up to 64 columns (blockIdx.z) per workgroup, whose four waves share a range of K (blockIdx.x)
-// in pieces of 64 and end in one sum through LDS. A step of 32 k is one 16-byte load per lane of x and one of each 16 columns of A (rows
-// of k, 32 bytes), which turn through a wave's own 1 KiB of LDS into MFMA operands (ds_read_b64_tr_b16; rows with
-// bit 3 set half a bank row apart); as many steps as registers hold are in flight at once. (Columns loaded as
-// pairs straight into operands took eight loads a step, 10 us for the first call below.) A workgroup takes every
-// gridDim.y-th of its rows' distinct adapters and stores the rows that use it: few rows have many adapters
-// (gridDim.y workgroups read them at once), many rows few. Few rows also share out K over up to eight workgroups: one CU reads
-// some 16 bytes a clock. 16 x 4096, 16 adapters of rank 16: 5.4 us
-// (one workgroup of 16 waves over all of K: 10); 4096 x 4096 in runs: 13.4 us, 2.5 TB/s of x (16.7).
+// in pieces of 64 and end in one sum through LDS. A step of 32 k is one 16-byte load per lane of x and one of each 16 columns
+// of A (rows of k, 32 bytes), which turn through 1 KiB of a wave's own LDS each into MFMA operands (ds_read_b64_tr_b16; rows with
+// bit 3 set half a bank row apart); four steps are in flight at once. (Eight, in twice the registers, took 2 us longer; columns loaded
+// as pairs straight into operands, eight loads a step, twice as long.) A workgroup takes every gridDim.y-th of its rows' distinct
+// adapters and stores the rows that use it: few rows have many adapters (gridDim.y workgroups read them at once), many rows
+// few. Few rows also share out K over up to eight workgroups: one CU reads some 16 bytes a clock. 16 x 4096, 16 adapters of
+// rank 16: 4-5 us (one workgroup of 16 waves over all of K: 10); 200 x 2048 of rank 64, mixed: 9.6; 4096 x 4096 in runs: 12.6 us,
+// 2.7 TB/s of x.
 constexpr int kAdapterLowThreads = 256, kAdapterLowCols = 64;
 template <typename Tag>
 __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(AdapterArgs a, uint32_t* __restrict__ zeros,
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(Adapter
   constexpr int kWaves = kAdapterLowThreads / 64, kCols = kAdapterLowCols;
   static_assert(kAdapterLowThreads == 4 * kCols, "a thread per column and four rows in the sum over the waves");
   __shared__ __attribute__((aligned(16))) float red[kWaves][kCols][16 + 4];
-  __shared__ __attribute__((aligned(1024))) char turn[kWaves * 1024];
+  __shared__ __attribute__((aligned(1024))) char turn[kWaves * 4096];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(Adapter
   // this lane's part of 32 rows of 16 columns, and its read addresses (k-rows 8 lg + 0..3, then + 4)
   const int k_row = lane >> 1, half = lane & 1;
   auto turned = [](int k) { return (k * 32) ^ ((k & 8) << 4); };
-  const uint32_t turn0 = lds_addr(turn) + wave * 1024;
+  const uint32_t turn0 = lds_addr(turn) + wave * 4096;
   const uint32_t put_at = turn0 + turned(k_row) + 16 * half;
   const uint32_t get_at = turn0 + turned(8 * lg + (l16 >> 2)) + 8 * (l16 & 3);
   const int steps = (k_end + 31) / 32;
@@ -279,40 +279,56 @@ __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(Adapter
       for (int j = 0; j < kBlocks; ++j) col[j] = 16 * j + 8 * half < cols ? 16 * j + 8 * half : 0;
       // step i of this wave: two consecutive ones of every four pairs, whole 128-byte lines of x
       auto step_of = [&](int i) { return 2 * (wave + kWaves * (i >> 1)) + (i & 1); };
-      for (int i0 = 0; step_of(i0) < steps; i0 += kAhead) {
-        u32x4 xf[kAhead], af[kAhead][kBlocks];
+      struct Batch {
+        u32x4 x[kAhead], a[kAhead][kBlocks];
+      };
+      auto load = [&](Batch& to, int i0) __attribute__((always_inline)) {
         if (k_end % 32 == 0) {  // (steps past the last repeat it and are not used)
 #pragma unroll
           for (int u = 0; u < kAhead; ++u) {
             const int k = min(32 * step_of(i0 + u), k_end - 32);
-            xf[u] = ld16(x + k);
+            to.x[u] = ld16(x + k);
 #pragma unroll
-            for (int j = 0; j < kBlocks; ++j) af[u][j] = ld16(A + (long long)k * a.a_k + col[j]);
+            for (int j = 0; j < kBlocks; ++j) to.a[u][j] = ld16(A + (long long)k * a.a_k + col[j]);
           }
         } else {  // past K (a multiple of 8): zeros, in both operands
 #pragma unroll
           for (int u = 0; u < kAhead; ++u) {
             const int k = 32 * step_of(i0 + u);
-            xf[u] = k + 8 * lg < k_end ? ld16(x + k) : u32x4{0, 0, 0, 0};
+            to.x[u] = k + 8 * lg < k_end ? ld16(x + k) : u32x4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < kBlocks; ++j)
-              af[u][j] = k + k_row < k_end ? ld16(A + (long long)k * a.a_k + col[j]) : u32x4{0, 0, 0, 0};
+              to.a[u][j] = k + k_row < k_end ? ld16(A + (long long)k * a.a_k + col[j]) : u32x4{0, 0, 0, 0};
           }
         }
+      };
+      auto multiply = [&](const Batch& from, int i0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           if (step_of(i0 + u) >= steps) break;
+          // (a wave's LDS operations run in order: the reads of the step before are done)
+          u32x4 f[kBlocks];
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j)
+            *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(put_at + 1024 * j) = from.a[u][j];
 #pragma unroll
           for (int j = 0; j < kBlocks; ++j) {
-            // (a wave's LDS operations run in order: the reads of the block before are done)
-            *(__attribute__((address_space(3))) u32x4*)(uintptr_t)put_at = af[u][j];
-            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)get_at);
+            const uint32_t at = get_at + 1024 * j;
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at);
             const s16x4 v1 =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(get_at ^ 128));
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(at ^ 128));
             const u32x2 lo = __builtin_bit_cast(u32x2, v0), hi = __builtin_bit_cast(u32x2, v1);
-            acc[j] = H::mfma16(xf[u], u32x4{lo[0], lo[1], hi[0], hi[1]}, acc[j]);
+            f[j] = u32x4{lo[0], lo[1], hi[0], hi[1]};
           }
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) acc[j] = H::mfma16(from.x[u], f[j], acc[j]);
         }
+      };
+      if (step_of(0) >= steps) return;
+      for (int i0 = 0; step_of(i0) < steps; i0 += kAhead) {
+        Batch batch;
+        load(batch, i0);
+        multiply(batch, i0);
       }
     };
     if (cols > 32) loop(Int<4>{});
