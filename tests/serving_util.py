@@ -82,12 +82,17 @@ def tree_oracle(q, k_cache, v_cache, k_scale, v_scale, table, context, starts, m
         key's scale and the call's), plus the argument of the exponential, |s_j - max| 2^-23, and 2^-22 for
         the exponential itself;
       - sums over n keys in any order and their joining: (n + 32) 2^-24 sum_j w_j (|V_j| + |O|).
-    A weight is at least the type's least subnormal's half off (2^-25 for fp16 weights of at most 1). A weight of up to
+    A weight is at least the type's least subnormal's half off (2^-25 for fp16 weights whose largest is 1 or more). Of a cache with
+    scales what is rounded is 2^(s_j + log2 c_j - max_i(s_i + log2 c_i)), c_j key j's value scale, against a sum of
+    2^(s_j - max_i(s_i + log2 c_i)): 2^-25 there is 2^-25 2^(max(s_i + log2 c_i) - max s_i) <= 2^-25 max c_i of a sum whose largest
+    term is 1, for each code: 2^-25 max c sum_j |code_j|, which is more than 2^-25 sum_j c_j |code_j| where scales differ (one
+    output of 16384: 2.92e-7 off, 2.55e-7 by the latter and all other terms). A weight of up to
     2^-25 so may round to 0, and 0 times an infinity is NaN by arithmetic: where an infinite value has such a weight (against
     the row's largest; e^-745 in 64 bits, where the oracle's own is 0), an infinite result may be NaN (allowed: infinity)."""
 
     u = HALF[q.dtype]
     keys, values = cache_values(k_cache, k_scale), cache_values(v_cache, v_scale)
+    value_codes, value_scales = f64(v_cache), None if v_scale is None else f64(v_scale)
     pages, heads, page_size, d = keys.shape
     qs, expected = f64(q), f64(out).copy()
     allowed = np.zeros_like(expected)
@@ -123,8 +128,13 @@ def tree_oracle(q, k_cache, v_cache, k_scale, v_scale, table, context, starts, m
                     e = 2 * (d + 4) * 2.0**-24 * abs(scale) * (np.abs(kk) @ np.abs(qs[t, h])) + np.abs(s - top) * 2.0**-23 + 2.0**-22
                     expected[t, h] = o
                     small = (np.exp(s - top) <= 2 * tiny)[:, None] & np.isinf(vv)
+                    lost = np.abs(vv).sum(0)
+                    if v_scale is not None:
+                        own = value_scales[at[seen], h // group, pos[seen] % page_size]
+                        codes = np.abs(value_codes[at[seen], h // group, pos[seen] % page_size]).sum(0)
+                        lost = np.maximum(lost, codes * np.abs(own).max())
                     allowed[t, h] = (u * np.abs(o) + (u + (len(s) + 32) * 2.0**-24) * spread + e.max() * spread
-                                     + tiny * np.abs(vv).sum(0) / max(total, 1.0) + tiny + 1e-30)
+                                     + tiny * lost / max(total, 1.0) + tiny + 1e-30)
                     allowed[t, h][np.isinf(o)] = 0.0
                     allowed[t, h][np.isinf(o) & small.any(0)] = np.inf
     return expected, allowed

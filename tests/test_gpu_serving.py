@@ -202,6 +202,56 @@ def test_recorded_steps(device, cache):
         native.set_launch_mode(True, None)
 
 
+@pytest.mark.parametrize("cache", [F16, torch.int8])
+def test_recorded_calls_read_their_lengths_anew(device, cache):
+    """One recorded pass of attention and adapters serves other lengths, pages, masks and adapters at each replay."""
+
+    layer = Layer(device, F16, cache, longest=2000)
+    layer.context = [0, 0, 0]
+    for counts in ([700, 1000, 300], [600, 40, 900]):
+        step = layer.step(counts, False, 3)
+        step.run()
+        layer.context = [c + n for c, n in zip(layer.context, counts)]
+    step = layer.step([8, 13, 11], True, 4)
+    step.run()
+    table, mask = layer.table.clone(), step.mask.clone()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+
+    def calls():
+        native.tree_attention(step.att, step.q, layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale, layer.table,
+                              step.context, step.starts, step.mask, D**-0.5)
+        native.adapter_matmul(step.out, step.att.view(-1, HIDDEN), layer.w_out, None, layer.a_out, layer.b_out, step.index,
+                              layer.adapter_scale)
+
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            native.set_launch_mode(False, stream.cuda_stream)
+            calls()
+        native.set_launch_mode(True, None)
+        for lens, starts in (([1300, 1040, 1200], [0, 8, 21, 32]), ([0, 1, 1999], [0, 1, 1, 30]), ([16, 0, 640], [0, 0, 32, 32]),
+                             ([700, 300, 20], [2, 9, 20, 25])):
+            step.context.copy_(torch.tensor(lens, dtype=torch.int32))
+            step.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+            layer.table.copy_(table.flip(0) if lens[0] == 16 else table)
+            step.mask.copy_(mask.flip(0) if lens[0] == 0 else mask)
+            step.index.copy_(step.index.roll(5))
+            step.att.fill_(3.0)
+            calls()
+            eager = step.results()[1:3]
+            step.att.fill_(3.0)
+            step.out.fill_(0.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            same(step.results()[1:3], eager, f"{lens}")
+            held = [None if x is None else x.cpu() for x in (layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale)]
+            expected, allowed = tree_oracle(step.q.cpu(), *held, layer.table.cpu(), lens, starts, step.mask.cpu(), D**-0.5,
+                                            torch.full_like(step.att, 3.0))
+            assert_rows(step.att, expected, allowed)
+    finally:
+        native.set_launch_mode(True, None)
+
+
 def test_threads_and_streams(device):
     """Two threads on one stream, and each on streams of its own: the bits of calls by themselves."""
 

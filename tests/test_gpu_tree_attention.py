@@ -301,3 +301,29 @@ def test_empty_calls(device):
     native.tree_attention(out, torch.zeros(3, 2, 64, **z), *caches, None, None, torch.zeros(1, 0, **i), torch.ones(1, **i),
                           torch.tensor([0, 3], **i))
     assert not out.any()  # a table without pages: nothing is seen
+
+
+@pytest.mark.parametrize("model,cache,counts", [(BF16, BF16, [3]), (F16, F16, [40, 3]), (BF16, E4M3, [30]), (F32, F32, [4])])
+def test_queries_that_are_not_finite(device, model, cache, counts):
+    """Rows with an infinity or NaN in their query are NaN, with a scale of 0 too; the others are what they are without them."""
+
+    for scale in (0.0, -0.5, 0.2):
+        call = Call([130] * len(counts), counts, 2, 2, 64, 16, model, cache, scale=scale)
+        clean = call.run(device)
+        call.check(clean)
+        call.q[0, 1, 5], call.q[1, 3, 60] = float("inf"), float("nan")
+        out = call.run(device)
+        assert torch.isnan(out[0, 1]).all() and torch.isnan(out[1, 3]).all(), scale
+        out[0, 1], out[1, 3] = clean[0, 1], clean[1, 3]
+        assert torch.equal(out, clean), scale
+
+
+def test_many_requests_of_many_rows(device):
+    """More requests than a wave has lanes, whose rows take the shared tiles."""
+
+    rng = random.Random(11)
+    context = [rng.choice((0, 1, 70, 200)) for _ in range(90)]
+    counts = [rng.choice((0, 5, 9, 18)) for _ in range(90)]
+    for model, cache in ((BF16, BF16), (F16, torch.int8)):
+        call = Call(context, counts, 1, 4, 64, 16, model, cache)
+        call.check(call.run(device))
