@@ -89,7 +89,7 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream)
   if (p.join) {
     const long long quads = tree_items(a, p.split.block) * (p.split.block / kTreeJoinRows);  // of rows
     // of an item, if the ranges are about as many as the workgroups
-    const bool many = p.split.grid / std::max(1ll, tree_items(a, p.split.block)) >= 16, few = quads <= 512;
+    const bool many = p.split.grid / std::max(1ll, tree_items(a, p.split.block)) >= 16, few = quads <= 4096;
 #define KG_TREE_JOIN(WIDTH, WAVES)                                                                                      \
   hipLaunchKernelGGL((tree_attn_join_kernel<Tag, WIDTH, WAVES>),                                                        \
                      dim3((unsigned)((quads * WAVES + tree_join_waves(WAVES) - 1) / tree_join_waves(WAVES))),           \

@@ -589,8 +589,8 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
 
 // The records of the items that several ranges share, joined: a wave takes four consecutive rows of an item, a lane four
 // columns. (A wave per row spent most of its time on finding its item: 14 us for 3104 rows of 8 records each, 8 now.)
-// kWaves: more where few rows have many records (32 rows of 64: 34 us with one wave each, 13 with four, 10 with 16): they
-// take every kWaves-th record of the same rows.
+// kWaves: more where few rows have many records, which take every kWaves-th record of the same rows (32 rows of 64 records: 34 us
+// with one wave each, 13 with four, 9 with 16; 512 rows of 4: 6.2, 4.7 with four; 4096 rows of 8: 8.2, 6.5; 34816 rows of 2: 11 with one).
 constexpr int kTreeJoinRows = 4;
 __host__ __device__ constexpr int tree_join_waves(int waves) { return waves > 4 ? waves : 4; }  // of a workgroup
 template <typename Tag, int D, int kWaves>
