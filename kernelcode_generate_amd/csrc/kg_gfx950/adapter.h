@@ -3,9 +3,9 @@
 // an index outside 0..L-1 is a row without one.
 //
 // 16-bit calls of whole 16-byte rows: adapter_low_kernel writes t = scale x A in 32 bits, as sums over ranges of K, to a
-// workspace; then the projection's kernels (gemm_skinny.h,
-// gemm_mid.h, gemm_quad.h, gemm.h) take the adapters as further k behind their own: the distinct adapters of a tile's rows, one after the other, R
-// values each, t's rows in the slots of their adapter and zeros in the others. A value of B that is not finite, times
+// workspace; then the projection's kernels (gemm_skinny.h, gemm_mid.h, gemm_quad.h, gemm.h) take the adapters as further k
+// behind their own: the distinct adapters of a tile's rows, one after the other, R values each, t's rows in the slots of
+// their adapter and zeros in the others. A value of B that is not finite, times
 // the zeros of rows that do not use it, would be NaN in them: the products run on zeros in place of such values, and
 // where there were any each output adds those of its own row's adapter (adapter_nonfinite). For the products t is
 // rounded to the operands' type, as the output of a 16-bit layer would be.

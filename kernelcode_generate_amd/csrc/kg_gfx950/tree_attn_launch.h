@@ -69,7 +69,7 @@ inline TreePlan tree_plan(const TreeArgs& a, int cache_bytes, bool may_split, lo
 template <typename Tag, typename C>
 hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream) {
 #define KG_TREE_ROWS(WIDTH) \
-  hipLaunchKernelGGL((tree_attn_rows_kernel<Tag, C, WIDTH, 1>), dim3(p.split.grid), dim3(treer::kThreads), 0, stream, a, p.split)
+  hipLaunchKernelGGL((tree_attn_rows_kernel<Tag, C, WIDTH>), dim3(p.split.grid), dim3(treer::kThreads), 0, stream, a, p.split)
 #define KG_TREE_TILES(WIDTH, NQ) \
   hipLaunchKernelGGL((tree_attn_tiles_kernel<Tag, C, WIDTH, NQ>), dim3(p.split.grid), dim3(treet::kThreads), 0, stream, a, p.split)
   if (p.width == 256) {
@@ -88,7 +88,7 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream)
 #undef KG_TREE_ROWS
   if (p.join) {
     const long long quads = tree_items(a, p.split.block) * (p.split.block / kTreeJoinRows);  // of rows
-    // of an item, if the ranges are about as many as the workgroups
+    // many: 16 records and more of an item, if all workgroups have work
     const bool many = p.split.grid / std::max(1ll, tree_items(a, p.split.block)) >= 16, few = quads <= 4096;
 #define KG_TREE_JOIN(WIDTH, WAVES)                                                                                      \
   hipLaunchKernelGGL((tree_attn_join_kernel<Tag, WIDTH, WAVES>),                                                        \

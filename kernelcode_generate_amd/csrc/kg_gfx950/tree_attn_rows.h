@@ -3,8 +3,9 @@
 // head fills a quarter of a 16-row matrix block and reads each key once for all four.
 //
 // Such a call is bound by reading keys and values. As in flash_attn_decode.h each of a workgroup's four waves
-// walks its own steps of 32 or 64 keys with its own running maximum and sums: S^T = K Q^T (v_mfma_f32_16x16x32, operand A 16 keys x 32 d from K's rows,
-// operand B up to two blocks of 16 rows), P in registers straight to O^T += V^T P^T, no LDS until the end.
+// walks its own steps of 32 or 64 keys with its own running maximum and sums: S^T = K Q^T (v_mfma_f32_16x16x32, operand A
+// 16 keys x 32 d from K's rows, operand B the 16 rows), P in registers straight to O^T += V^T P^T, no LDS until the end.
+// (A second block of rows per wave took twice the registers: more rows go through shared tiles, tree_attn_tiles.h.)
 //
 // Work is shared out in rounds (one step of each wave) of all requests, heads and blocks of rows in one line, an
 // equal range of it to each workgroup whatever the requests' lengths, which only the device knows: each
@@ -35,10 +36,10 @@ constexpr float kMinMax = -3.0e38f;  // the lowest running maximum: scores of -i
 // The running maximum (log2 units) is raised by scores beyond it by more than this: weights are at most 2^8, and sums
 // are rescaled a few times and not at every other tile. Weights and their sum have the same maximum, so the result does not depend on it.
 constexpr float kSlack = 8.f;
-// keys of a wave's step: 16 KiB of K and V rows, or what the registers hold (8 KiB of 8-bit heads of 64,
-// and of 128 with two blocks of rows; 32 KiB of 16-bit heads of 256)
-template <typename C, int D, int kNQ>
-constexpr int step_keys() { return (sizeof(C) == 2 && D >= 128) || D == 256 || (D == 128 && kNQ == 2) ? 32 : 64; }
+// keys of a wave's step: 16 KiB of K and V rows, or what the registers hold (8 KiB of 8-bit heads of 64;
+// 32 KiB of 16-bit heads of 256)
+template <typename C, int D>
+constexpr int step_keys() { return (sizeof(C) == 2 && D >= 128) || D == 256 ? 32 : 64; }
 
 // A 16-bit pair of two 8-bit codes.
 template <typename Tag, typename C>
@@ -238,19 +239,19 @@ __device__ __forceinline__ void tree_add_nonfinite(const TreeArgs& a, f32x4 (&o)
   }
 }
 
-// C: uint16_t (elements of Tag), E4m3 or int8_t. D: 64, 128 or 256, heads of d <= D elements, d % 16 == 0. kNQ: blocks of 16
-// rows. Pages of a multiple of 16 tokens, so that 16 keys share one.
-template <typename Tag, typename C, int D, int kNQ>
+// C: uint16_t (elements of Tag), E4m3 or int8_t. D: 64, 128 or 256, heads of d <= D elements, d % 16 == 0. Pages of a
+// multiple of 16 tokens, so that 16 keys share one.
+template <typename Tag, typename C, int D>
 __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_rows_kernel(TreeArgs a, TreeSplit split) {
   using namespace treer;
   using H = Half16<Tag>;
   constexpr bool kS = kScaled<C>;
   constexpr int kES = sizeof(C);
-  constexpr int kStep = step_keys<C, D, kNQ>();
+  constexpr int kStep = step_keys<C, D>();
   constexpr int NC = kStep / 32, NKB = kStep / 16;  // chunks of 32, blocks of 16 keys
   constexpr int NDS = D / 32;                       // 32-deep steps of S^T
   constexpr int NE = D / 16;                        // columns of V per lane, blocks of O^T
-  constexpr int kRows = 16 * kNQ;
+  constexpr int kRows = 16;
   constexpr int NKW = kS ? D / 64 : NDS;            // 16-byte pieces of a K row per lane
   constexpr int NVW = NE * kES / 4;                 // dwords of a V row per lane
   __shared__ float o_lds[kWaves][kRows][D];
@@ -292,23 +293,18 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
     key_hi = __builtin_amdgcn_readfirstlane(key_hi);
 
     // this lane's rows: token of the request and query head
-    int tok[kNQ];
-    unsigned long long first_word[kNQ];  // of the token's mask
-    u32x4 qf[kNQ][NDS];
+    u32x4 qf[NDS];
+    const int row = row0 + l16, tok = row / a.group;
+    const bool real = l16 < item_rows;
+    const unsigned long long first_word =  // of the token's mask
+        real && a.words > 0 ? (unsigned long long)a.mask[(long long)(r.first + tok) * a.mask_0] : 0ull;
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + (real ? r.first + tok : 0) * a.q_token +
+                        ((long long)h * a.group + (row - tok * a.group)) * a.q_head;
 #pragma unroll
-    for (int x = 0; x < kNQ; ++x) {
-      const int row = row0 + 16 * x + l16;
-      tok[x] = row / a.group;
-      const bool real = 16 * x + l16 < item_rows;
-      first_word[x] = real && a.words > 0 ? (unsigned long long)a.mask[(long long)(r.first + tok[x]) * a.mask_0] : 0ull;
-      const uint16_t* q = static_cast<const uint16_t*>(a.q) + (real ? r.first + tok[x] : 0) * a.q_token +
-                          ((long long)h * a.group + (row - tok[x] * a.group)) * a.q_head;
-#pragma unroll
-      for (int s = 0; s < NDS; ++s) {
-        // 8-bit rows: 16 bytes of a lane are the 8 d of two steps
-        const int d = kS ? 64 * (s >> 1) + 16 * lr + 8 * (s & 1) : 32 * s + 8 * lr;
-        qf[x][s] = real && d < a.d ? ld16(q + d) : u32x4{0, 0, 0, 0};
-      }
+    for (int s = 0; s < NDS; ++s) {
+      // 8-bit rows: 16 bytes of a lane are the 8 d of two steps
+      const int d = kS ? 64 * (s >> 1) + 16 * lr + 8 * (s & 1) : 32 * s + 8 * lr;
+      qf[s] = real && d < a.d ? ld16(q + d) : u32x4{0, 0, 0, 0};
     }
     const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
     const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
@@ -368,16 +364,11 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
       }
     };
 
-    f32x4 o[kNQ][NE];
-    f32x4 l_run[kNQ];  // scaled caches: element 0, this lane's keys alone
-    float m_run[kNQ];
+    f32x4 o[NE];
+    f32x4 l_run = {0.f, 0.f, 0.f, 0.f};  // scaled caches: element 0, this lane's keys alone
+    float m_run = kMinMax;
 #pragma unroll
-    for (int x = 0; x < kNQ; ++x) {
-#pragma unroll
-      for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-      l_run[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-      m_run[x] = kMinMax;
-    }
+    for (int e = 0; e < NE; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
     const u32x4 ones = {H::kOnePair, H::kOnePair, H::kOnePair, H::kOnePair};
 
     // This wave's steps: key_lo + kStep (wave + 4 i). A step reads its rows and waits for them; eight to twelve waves of a CU
@@ -402,18 +393,16 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           for (int s = 0; s < NKW; ++s)
             if ((kS ? 16 : 8) * lr + (kS ? 64 : 32) * s >= a.d) k[kb][s] = u32x4{0, 0, 0, 0};
       }
-      f32x4 sc[kNQ][NKB], y[kS ? kNQ : 1][NKB];  // y: with the values' scales
+      f32x4 sc[NKB], y[NKB];  // y: with the values' scales
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
-#pragma unroll
-        for (int x = 0; x < kNQ; ++x) sc[x][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < NDS; ++s) {
           u32x4 kf;
           if constexpr (kS) kf = widen8<Tag, C>(k[kb][s >> 1][(s & 1) * 2], k[kb][s >> 1][(s & 1) * 2 + 1]);
           else kf = k[kb][s];
-#pragma unroll
-          for (int x = 0; x < kNQ; ++x) sc[x][kb] = H::mfma16(kf, qf[x][s], sc[x][kb]);
+          sc[kb] = H::mfma16(kf, qf[s], sc[kb]);
         }
       }
       if constexpr (kS) {
@@ -429,27 +418,22 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           lv = *reinterpret_cast<const f32x4*>(&sc_lds[wave][1][16 * kb + 4 * lr]);
         }
 #pragma unroll
-        for (int x = 0; x < kNQ; ++x)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[x][kb][i] *= f[i];
-            if constexpr (kS) y[x][kb][i] = sc[x][kb][i] + lv[i];
-          }
+        for (int i = 0; i < 4; ++i) {
+          sc[kb][i] *= f[i];
+          if constexpr (kS) y[kb][i] = sc[kb][i] + lv[i];
+        }
       }
       // ---- what is not seen ----
-      uint32_t seen[kNQ], found = 0;  // bit 4 kb + i: this lane's row sees its key
+      uint32_t seen, found = 0;  // bit 4 kb + i: this lane's row sees its key
       if (!plain) {
         const uint32_t there_lo = (uint32_t)(there >> (4 * lr)), there_hi = (uint32_t)(there >> 32 >> (4 * lr));
+        seen = tree_lane_keys<NKB>(there & tree_visible(a, r, l16 < item_rows, tok, first_word, key), lr);
 #pragma unroll
-        for (int x = 0; x < kNQ; ++x) {
-          seen[x] = tree_lane_keys<NKB>(there & tree_visible(a, r, 16 * x + l16 < item_rows, tok[x], first_word[x], key), lr);
-#pragma unroll
-          for (int n = 0; n < 4 * NKB; ++n)
-            if (!(seen[x] >> n & 1u)) {
-              sc[x][n >> 2][n & 3] = -INFINITY;
-              if constexpr (kS) y[x][n >> 2][n & 3] = -INFINITY;
-            }
-        }
+        for (int n = 0; n < 4 * NKB; ++n)
+          if (!(seen >> n & 1u)) {
+            sc[n >> 2][n & 3] = -INFINITY;
+            if constexpr (kS) y[n >> 2][n & 3] = -INFINITY;
+          }
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -471,41 +455,38 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           }
       }
       // ---- weights: keys 32 c + 4 lr + 0..3, then + 16 ----
-      u32x4 pp[kNQ][NC];
+      u32x4 pp[NC];
+      auto weighed = [&](int n) __attribute__((always_inline)) {
+        if constexpr (kS) return (float)y[n >> 2][n & 3];
+        else return (float)sc[n >> 2][n & 3];
+      };
+      float mx = weighed(0);
 #pragma unroll
-      for (int x = 0; x < kNQ; ++x) {
-        auto weighed = [&](int n) __attribute__((always_inline)) {
-          if constexpr (kS) return (float)y[x][n >> 2][n & 3];
-          else return (float)sc[x][n >> 2][n & 3];
-        };
-        float mx = weighed(0);
+      for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(n));
+      float mx2 = mx;
+      fa::rows4_combine<true>(mx, mx2);
+      const bool raise = !(mx <= m_run + kSlack);  // (a NaN too)
+      if (__builtin_amdgcn_ballot_w64(raise)) {
+        const float alpha = raise ? __builtin_amdgcn_exp2f(m_run - mx) : 1.f;
+        m_run = raise ? mx : m_run;
+        l_run *= alpha;
 #pragma unroll
-        for (int n = 1; n < 4 * NKB; ++n) mx = nan_max(mx, weighed(n));
-        float mx2 = mx;
-        fa::rows4_combine<true>(mx, mx2);
-        const bool raise = !(mx <= m_run[x] + kSlack);  // (a NaN too)
-        if (__builtin_amdgcn_ballot_w64(raise)) {
-          const float alpha = raise ? __builtin_amdgcn_exp2f(m_run[x] - mx) : 1.f;
-          m_run[x] = raise ? mx : m_run[x];
-          l_run[x] *= alpha;
+        for (int e = 0; e < NE; ++e) o[e] *= alpha;
+      }
 #pragma unroll
-          for (int e = 0; e < NE; ++e) o[x][e] *= alpha;
+      for (int kb = 0; kb < NKB; ++kb) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run);
+          if constexpr (kS) l_run[0] += __builtin_amdgcn_exp2f((float)sc[kb][i] - m_run);
         }
+        pp[kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
+        pp[kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);
+      }
+      if constexpr (!kS) {
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-          float w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run[x]);
-            if constexpr (kS) l_run[x][0] += __builtin_amdgcn_exp2f((float)sc[x][kb][i] - m_run[x]);
-          }
-          pp[x][kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
-          pp[x][kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);
-        }
-        if constexpr (!kS) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) l_run[x] = H::mfma16(ones, pp[x][c], l_run[x]);
-        }
+        for (int c = 0; c < NC; ++c) l_run = H::mfma16(ones, pp[c], l_run);
       }
       // ---- O^T += V^T P^T ----
 #pragma unroll
@@ -527,33 +508,27 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           for (int q = 0; q < 4; ++q)
             vt[q] = (e & 1) ? hi_halves(row16[2 * q][e >> 1], row16[2 * q + 1][e >> 1])
                             : lo_halves(row16[2 * q][e >> 1], row16[2 * q + 1][e >> 1]);
-#pragma unroll
-          for (int x = 0; x < kNQ; ++x) o[x][e] = H::mfma16(vt, pp[x][c], o[x][e]);
+          o[e] = H::mfma16(vt, pp[c], o[e]);
         }
       }
       if (!plain && __builtin_amdgcn_ballot_w64(found != 0) != 0)
-#pragma unroll
-        for (int x = 0; x < kNQ; ++x)
-          tree_add_nonfinite<Tag, C, kStep>(a, o[x], seen[x], p.page, p.offset, h, lane, [&](int e, int i) { return NE * (4 * lr + i) + e; });
+        tree_add_nonfinite<Tag, C, kStep>(a, o, seen, p.page, p.offset, h, lane, [&](int e, int i) { return NE * (4 * lr + i) + e; });
       p = checked(next);
     }
 
     // ---- join the waves ----
+    if constexpr (kS) {
+      float l0 = l_run[0], l1 = l0;
+      fa::rows4_combine<false>(l0, l1);
+      l_run[0] = l0;
+    }
 #pragma unroll
-    for (int x = 0; x < kNQ; ++x) {
-      if constexpr (kS) {
-        float l0 = l_run[x][0], l1 = l0;
-        fa::rows4_combine<false>(l0, l1);
-        l_run[x][0] = l0;
-      }
+    for (int e = 0; e < NE; ++e)
 #pragma unroll
-      for (int e = 0; e < NE; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o_lds[wave][16 * x + l16][NE * (4 * lr + i) + e] = o[x][e][i];
-      if (lr == 0) {
-        ml_lds[wave][16 * x + l16][0] = m_run[x];
-        ml_lds[wave][16 * x + l16][1] = l_run[x][0];
-      }
+      for (int i = 0; i < 4; ++i) o_lds[wave][l16][NE * (4 * lr + i) + e] = o[e][i];
+    if (lr == 0) {
+      ml_lds[wave][l16][0] = m_run;
+      ml_lds[wave][l16][1] = l_run[0];
     }
     __syncthreads();
     float* record = split.partial + ((long long)2 * share.w + (starts_here ? 0 : 1)) * kRows * (D + kTreePad);
