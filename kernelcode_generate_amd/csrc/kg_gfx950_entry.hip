@@ -1431,7 +1431,7 @@ int kv_cache_store_impl(const KgArgSlot* args, unsigned long long n) {
   a.total_slots = kv.pages * kv.page_size;
   const long long items = 2 * tokens * kv.heads;
   a.by_heads = page_div((int)kv.heads);
-  if (kv_in_eights(kv, rows) && items / 2 < 0x7fffffffLL)
+  if (kv_in_eights(kv, rows) && items / 2 <= 0x7fffff00LL)  // (row numbers of the last workgroup stay in 31 bits)
     return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
 #define KG_KV_STORE(LANES)                                                                                             \
   hipLaunchKernelGGL((kv_store_kernel<decltype(t), decltype(c), LANES>), dim3((unsigned)cdiv(items / 2 * LANES, 256), 2), \
@@ -1474,7 +1474,7 @@ int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
   if ((rc = check_view(rows[0], "k_out")) || (rc = check_view(rows[1], "v_out")) || (rc = check_kv(kv)) ||
       (rc = check_view(table, "page_table")) || (rc = check_view(lens, "lengths")))
     return rc;
-  if (no_elements(rows[0]) || table.shape[1] == 0) return finish_launch("kv_cache_load(empty)");
+  if (no_elements(rows[0]) || table.shape[1] == 0 || kv.pages == 0) return finish_launch("kv_cache_load(empty)");
   KvLoadArgs a;
   for (int x = 0; x < 2; ++x) a.side[x] = kv_side(kv, x, rows[x]);
   a.table = static_cast<const int*>(table.data);
@@ -1490,7 +1490,7 @@ int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
   a.reach = (int)reach;
   a.pages = kv.pages;
   a.div = page_div((int)kv.page_size);
-  if (kv_in_eights(kv, rows) && batch * kv.heads <= 65535)
+  if (kv_in_eights(kv, rows) && batch * kv.heads <= 65535 && reach <= 0x7fffff00LL)
     return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
 #define KG_KV_LOAD(LANES)                                                                                                \
   hipLaunchKernelGGL((kv_load_kernel<decltype(c), decltype(t), LANES>),                                                  \

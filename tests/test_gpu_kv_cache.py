@@ -200,3 +200,23 @@ def test_empty_calls(device):
     native.kv_cache_load(out, out.clone(), *caches, None, None, torch.zeros(1, 0, dtype=torch.int32, device=device),
                          torch.ones(1, dtype=torch.int32, device=device))
     assert (out == 1).all()
+
+
+@pytest.mark.parametrize("cache", [torch.bfloat16, torch.int8])
+def test_a_cache_without_pages(device, cache):
+    """Nothing is written, nothing read, nothing seen, whatever the slots, lengths and tables say."""
+
+    bf16, i32 = dict(dtype=torch.bfloat16, device=device), dict(dtype=torch.int32, device=device)
+    caches = [torch.zeros(0, 2, 16, 64, dtype=cache, device=device) for _ in range(2)]
+    scales = [torch.zeros(0, 2, 16, device=device) if cache == torch.int8 else None for _ in range(2)]
+    rows = [torch.ones(3, 2, 64, **bf16) for _ in range(2)]
+    native.kv_cache_store(*caches, *scales, *rows, torch.arange(3, device=device))
+    outs = [torch.full((1, 2, 20, 64), 5.0, **bf16) for _ in range(2)]
+    table, lengths = torch.zeros(1, 2, **i32), torch.full((1,), 20, **i32)
+    native.kv_cache_load(*outs, *caches, *scales, table, lengths)
+    assert all((x == 5.0).all() for x in outs)
+    for tokens in (1, 40):
+        out = torch.full((tokens, 4, 64), 5.0, **bf16)
+        native.tree_attention(out, torch.ones(tokens, 4, 64, **bf16), *caches, *scales, table, lengths,
+                              torch.tensor([0, tokens], **i32))
+        assert not out.any()
