@@ -248,7 +248,8 @@ __device__ __forceinline__ void scaled_codes(float (&x)[8], float scale) {
       float q = x[i] * inverse;
       q = __builtin_fmaf(__builtin_fmaf(-q, scale, x[i]), inverse, q);
       q = __builtin_fmaf(__builtin_fmaf(-q, scale, x[i]), inverse, q);
-      x[i] = fminf(fmaxf(q, -CacheElem<C>::kLargest), CacheElem<C>::kLargest);
+      // (the corrections make a zero positive; its sign is the quotient's)
+      x[i] = __builtin_copysignf(fminf(fmaxf(q, -CacheElem<C>::kLargest), CacheElem<C>::kLargest), x[i]);
     }
   } else {
 #pragma unroll
