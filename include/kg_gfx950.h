@@ -135,7 +135,8 @@ int kg_gfx950_flash_attention_entry(const KgArgSlot* ordered_args, unsigned long
  *
  * Caches: k_cache, v_cache [pages, heads, page_size, D] (D 1..512, any page_size), f32, f16, bf16, or 8-bit
  * (i8, e4m3) with k_scale, v_scale f32 [pages, heads, page_size] (absent otherwise). An 8-bit element stands
- * for code x scale. Token i of a sequence lies on page page_table[b, i / page_size] at offset i % page_size.
+ * for code x scale, whatever the scale's sign and size; attention gives rows that see a value whose scale is not finite
+ * values that are not finite either. Token i of a sequence lies on page page_table[b, i / page_size] at offset i % page_size.
  */
 
 /*

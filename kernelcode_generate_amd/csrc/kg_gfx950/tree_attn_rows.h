@@ -15,7 +15,8 @@
 //
 // 8-bit caches: codes are widened to 16 bits (exact for both types) for the products; a key's scale multiplies
 // its scores, a value's its weights. Weights are rounded to 16 bits with that scale in them, so the running
-// maximum is of s + log2(value's scale): weights of at most 2^8, whatever the scales' sizes. The sum of weights stays in 32 bits.
+// maximum is of s + log2(value's scale): weights of at most 2^8, whatever the scales' sizes. The sum of weights, which has no scales
+// in it, stays in 32 bits, so the scale that counts there lies within 2^-80..2^80 (ValueScale).
 //
 // Weights of 16-bit caches are rounded to 16 bits, as in the flash attention kernels, and summed as rounded.
 #pragma once
@@ -89,6 +90,24 @@ __device__ __forceinline__ void load_v(uint32_t (&v)[kDwords], const C* p) {
     }
   }
 }
+
+// A value's scale, of any sign and size. What counts for the running maximum is its magnitude within 2^-80..2^80 (log_of its logarithm):
+// a sum of weights is then 2^-80..2^88 for each of up to 2^31 keys, with 46 bits or more below it that 32 bits hold. ratio_of, the scale
+// over that, multiplies the weight before it is rounded: 1 of all scales that are not odd, 0 of a scale of 0, and within 2^-69..2^48,
+// which bf16 holds. In fp16 a ratio ends at 2^7, so that weights stay finite: the result is infinite with it as without, unless
+// that key's weight is below some 2^-70.
+template <typename Tag>
+struct ValueScale {
+  static constexpr float kLeast = 0x1p-80f, kMost = 0x1p80f;
+  static __device__ __forceinline__ bool odd(float scale) { return !(scale >= kLeast && scale <= kMost); }
+  static __device__ __forceinline__ float within(float scale) { return fminf(fmaxf(__builtin_fabsf(scale), kLeast), kMost); }
+  // (NaN of a scale that is not finite: so are the rows that see the value)
+  static __device__ __forceinline__ float log_of(float scale) { return __builtin_amdgcn_logf(within(scale)) + (scale - scale); }
+  static __device__ __forceinline__ float ratio_of(float scale) {
+    const float r = scale / within(scale);
+    return std::is_same<Tag, F16Tag>::value ? fminf(fmaxf(r, -0x1p7f), 0x1p7f) : r;
+  }
+};
 
 template <typename C>
 constexpr bool kScaled = CacheElem<C>::kScaled;
@@ -256,7 +275,7 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
   constexpr int NVW = NE * kES / 4;                 // dwords of a V row per lane
   __shared__ float o_lds[kWaves][kRows][D];
   __shared__ float ml_lds[kWaves][kRows][2];
-  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? kWaves : 1][2][kStep];
+  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? kWaves : 1][3][kStep];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -405,10 +424,12 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           sc[kb] = H::mfma16(kf, qf[s], sc[kb]);
         }
       }
+      bool odd = false;  // whether there are values with a ratio
       if constexpr (kS) {
         sc_lds[wave][0][lane & (kStep - 1)] = ks * a.scale_log2;
-        // (a NaN passes; a scale of 0 has codes of 0, so any weight does)
-        sc_lds[wave][1][lane & (kStep - 1)] = __builtin_amdgcn_logf(nan_max(vs, 0x1p-100f));
+        sc_lds[wave][1][lane & (kStep - 1)] = ValueScale<Tag>::log_of(vs);
+        odd = __builtin_amdgcn_ballot_w64(ValueScale<Tag>::odd(vs)) != 0;
+        if (odd) sc_lds[wave][2][lane & (kStep - 1)] = ValueScale<Tag>::ratio_of(vs);
       }
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
@@ -480,6 +501,13 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
         for (int i = 0; i < 4; ++i) {
           w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run);
           if constexpr (kS) l_run[0] += __builtin_amdgcn_exp2f((float)sc[kb][i] - m_run);
+        }
+        if constexpr (kS) {
+          if (odd) {
+            const f32x4 ratio = *reinterpret_cast<const f32x4*>(&sc_lds[wave][2][16 * kb + 4 * lr]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = w[i] == 0.f ? 0.f : w[i] * ratio[i];  // (of a key that is not seen, whatever its scale)
+          }
         }
         pp[kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
         pp[kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);

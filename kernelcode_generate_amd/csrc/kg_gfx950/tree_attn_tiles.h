@@ -58,6 +58,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
   using namespace treet;
   using treer::kMinMax;
   using treer::kSlack;
+  using Scale = treer::ValueScale<Tag>;
   using H = Half16<Tag>;
   constexpr bool kS = treer::kScaled<C>;
   constexpr int kES = sizeof(C);
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
   constexpr int kRowStep = kThreads / kPerRow;       // rows between a thread's pieces
   constexpr int kStage = kTile * D * 2;              // bytes of one tile
   __shared__ __attribute__((aligned(1024))) char lds[4 * kStage];  // K, V of stage 0, K, V of stage 1
-  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? 2 : 1][2][kTile];
+  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? 2 : 1][3][kTile];
   __shared__ int found_lds[3];  // whether tile t has values that are not finite, at t % 3
 
   const int tid = threadIdx.x;
@@ -200,6 +201,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     u32x4 kr[kPieces], vr[kPieces];
     uint32_t row_there = 0;
     float ks = 0.f, vs = 0.f;
+    bool odd = false;  // whether the tile stored last has values with a ratio
     auto load = [&](const Place& p) __attribute__((always_inline)) {
       row_there = 0;
 #pragma unroll
@@ -235,9 +237,11 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
       }
       if (tid < kTile) {
         sc_lds[stage][0][tid] = p.page >= 0 ? ks * a.scale_log2 : 0.f;
-        // (a NaN passes; a scale of 0 has codes of 0, so any weight does)
-        sc_lds[stage][1][tid] = p.page >= 0 ? __builtin_amdgcn_logf(nan_max(vs, 0x1p-100f)) : 0.f;
+        sc_lds[stage][1][tid] = p.page >= 0 ? Scale::log_of(vs) : 0.f;
       }
+      // (every wave has the scales of all keys)
+      odd = __builtin_amdgcn_ballot_w64(p.page >= 0 && Scale::odd(vs)) != 0;
+      if (odd && tid < kTile) sc_lds[stage][2][tid] = p.page >= 0 ? Scale::ratio_of(vs) : 0.f;
     };
 
     f32x4 o[kNQ][NE];
@@ -351,6 +355,13 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
             if constexpr (kS) w[i] = __builtin_amdgcn_exp2f(weighed(x, 4 * kb + i) - m_run[x]);
             else w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(weighed(x, 4 * kb + i), scale, -m_run[x]));
             if constexpr (kS) l_run[x][0] += __builtin_amdgcn_exp2f((float)sc[x][kb][i] - m_run[x]);
+          }
+          if constexpr (kS) {
+            if (odd) {
+              const f32x4 ratio = *reinterpret_cast<const f32x4*>(&sc_lds[stage][2][16 * kb + 4 * lr]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = w[i] == 0.f ? 0.f : w[i] * ratio[i];  // (of a key that is not seen, whatever its scale)
+            }
           }
           pp[x][kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
           pp[x][kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);
