@@ -175,7 +175,9 @@ int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long 
  * (out[M, N], x[M, K], weight[K, N], bias[N] | absent, a[L, K, R], b[L, R, N], index[M] i32, scale[L] f32 | absent)
  * out[m] = x[m] weight + bias + scale[l] (x[m] a[l]) b[l], l = index[m]; an index outside 0 .. L - 1 is a row without an
  * adapter; an absent scale is 1. dtypes as matmul's, a and b the operands'. R <= 512. Adapters of unequal
- * rank are padded with zeros. out must not overlap an operand.
+ * rank are padded with zeros. out must not overlap an operand. Sums are held in 32 bits; 16-bit calls round scale[l] (x[m] a[l]) to
+ * their type for its product with b (f16: times a power of two for each row, so that none of it leaves the type's range at the top),
+ * or, where rows are not whole 16-byte pieces, the projection before the adapter's part is added.
  */
 int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
 

@@ -8,12 +8,16 @@
 // their adapter and zeros in the others. A value of B that is not finite, times
 // the zeros of rows that do not use it, would be NaN in them: the products run on zeros in place of such values, and
 // where there were any each output adds those of its own row's adapter (adapter_nonfinite). For the products t is
-// rounded to the operands' type, as the output of a 16-bit layer would be.
+// rounded to the operands' type, as the output of a 16-bit layer would be; for fp16, whose range a product of x, A and a scale
+// leaves at either end, as a row's t times a power of two that brings its largest near 2^12 (adapter_range): the row's sums are
+// scaled by it before the adapter's products, and back after them, both exact.
 //
 // adapter_add_kernel: any types and strides, one workgroup per row: t = scale x A in 32 bits, then
 // out += t B, on an output that holds the projection already (matmul's kernels). A 16-bit output is
 // so rounded twice, by half a step each time.
 #pragma once
+
+#include <type_traits>
 
 #include "common.h"
 #include "kv_cache.h"  // PageDiv
@@ -84,11 +88,28 @@ struct AdapterPart {
   long long split_pitch, b_l, b_r, index_stride;  // split_pitch: M rank
   int splits, rank, count;                        // rank % 8 == 0
   PageDiv by_pieces;                              // division by rank / 8
+  const float* tops;                              // fp16: [top_count, M], the largest of a row's sums in each part of them
+  int top_count, rows;                            // rows: M
 };
-// Eight elements of t from `at` on, rounded.
+template <typename H>
+constexpr bool kAdapterRanged = std::is_same<H, Half16<F16Tag>>::value;
+// The power of two for row m's t: its sums over ranges of K are below 2^12 with it, t, of up to 8 of them, below 2^15. At most 2^60,
+// which the projection's sums bear (of fp16 operands they stay below 2^50); what is smaller then is no fp16 value times any B.
+// Of infinite sums the least, so that finite ones beside them stay finite.
+__device__ __forceinline__ float adapter_range(const AdapterPart& p, int m) {
+  float top = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < p.top_count; ++i) top = fmaxf(top, p.tops[(long long)i * p.rows + m]);
+  const int exponent = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+  return __builtin_bit_cast(float, (uint32_t)(127 + max(min(11 - exponent, 60), -116)) << 23);
+}
+__device__ __forceinline__ float inverse_power(float power) {
+  return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, power));
+}
+// Eight elements of t from `at` on, times their row's power of two, rounded.
 constexpr int kAdapterMaxSplits = 8;
 template <typename H>
-__device__ __forceinline__ u32x4 adapter_t8(const AdapterPart& p, const float* at) {
+__device__ __forceinline__ u32x4 adapter_t8(const AdapterPart& p, const float* at, float range) {
   f32x4 a = *reinterpret_cast<const f32x4*>(at), b = *reinterpret_cast<const f32x4*>(at + 4);
 #pragma unroll
   for (int y = 1; y < kAdapterMaxSplits; ++y) {  // (unrolled: the reads are in flight together)
@@ -96,6 +117,7 @@ __device__ __forceinline__ u32x4 adapter_t8(const AdapterPart& p, const float* a
     a += *reinterpret_cast<const f32x4*>(at + y * p.split_pitch);
     b += *reinterpret_cast<const f32x4*>(at + y * p.split_pitch + 4);
   }
+  if constexpr (kAdapterRanged<H>) a *= range, b *= range;
   return u32x4{H::pack2(a[0], a[1]), H::pack2(a[2], a[3]), H::pack2(b[0], b[1]), H::pack2(b[2], b[3])};
 }
 constexpr size_t kAdapterHeader = 256;  // bytes of the workspace before the sums: zeros
@@ -195,6 +217,16 @@ __device__ __forceinline__ int adapter_slots(const AdapterPart& p, int m0, int M
   return slots;
 }
 
+// fp16: range_lds[i] the power of two of row i (1 without an adapter), after adapter_slots. Every wave writes the same.
+template <int kRows>
+__device__ __forceinline__ void adapter_ranges(const AdapterPart& p, int m0, int lane, const int* row_lds, float* range_lds) {
+#pragma unroll
+  for (int u = 0; u < kRows / 64; ++u) {
+    const int i = 64 * u + lane;
+    range_lds[i] = row_lds[i] >= 0 ? adapter_range(p, m0 + i) : 1.f;
+  }
+}
+
 // Where a tile's row of t, or a k-row's columns of B, of an eight-k piece lie; null: zeros.
 __device__ __forceinline__ const float* adapter_t(const AdapterPart& p, int piece, int pieces, int slots, const int* slot_lds, int l,
                                                   int m) {
@@ -207,9 +239,9 @@ __device__ __forceinline__ const uint16_t* adapter_b(const AdapterPart& p, int p
   return slot < slots ? p.b + slot_lds[slot] * p.b_l + (8 * (piece - slot * pieces) + k) * p.b_r + n : nullptr;
 }
 template <typename H>
-__device__ __forceinline__ void adapter_put_t(const AdapterPart& p, const float* from, uint32_t to) {
+__device__ __forceinline__ void adapter_put_t(const AdapterPart& p, const float* from, uint32_t to, float range) {
   u32x4 x = {0, 0, 0, 0};
-  if (from) x = adapter_t8<H>(p, from);
+  if (from) x = adapter_t8<H>(p, from, range);
   *(__attribute__((address_space(3))) u32x4*)(uintptr_t)to = x;
 }
 // 16 bytes of B from there to LDS, zeros in place of what is not finite; `found` gets bits for that.
@@ -232,7 +264,8 @@ __device__ __forceinline__ void adapter_put(u32x4 x, uint32_t to, uint32_t& foun
 constexpr int kAdapterLowThreads = 256, kAdapterLowCols = 64;
 template <typename Tag>
 __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(AdapterArgs a, uint32_t* __restrict__ zeros,
-                                                                          float* __restrict__ sums, int splits) {
+                                                                          float* __restrict__ sums, int splits,
+                                                                          float* __restrict__ tops) {
   using H = Half16<Tag>;
   constexpr int kWaves = kAdapterLowThreads / 64, kCols = kAdapterLowCols;
   static_assert(kAdapterLowThreads == 4 * kCols, "a thread per column and four rows in the sum over the waves");
@@ -339,14 +372,24 @@ __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(Adapter
 #pragma unroll
     for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(&red[wave][16 * j + l16][4 * lg]) = acc[j];
     __syncthreads();
-    const int c = tid % kCols, r0 = 4 * (tid / kCols);
+    const int c = tid % kCols, r0 = 4 * (tid / kCols);  // (a wave has all columns of four rows)
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     if (c < cols) {
-      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x4*>(&red[w][c][r0]);
+      sum *= scale;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (users >> (r0 + e) & 1ull) sums[((long long)split * a.m + m0 + r0 + e) * a.rank + c0 + c] = sum[e] * scale;
+        if (users >> (r0 + e) & 1ull) sums[((long long)split * a.m + m0 + r0 + e) * a.rank + c0 + c] = sum[e];
+    }
+    if constexpr (kAdapterRanged<H>) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float top = __builtin_fabsf(sum[e]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        if (lane == 0 && (users >> (r0 + e) & 1ull)) tops[((long long)split * gridDim.z + blockIdx.z) * a.m + m0 + r0 + e] = top;
+      }
     }
   }
 }

@@ -90,6 +90,8 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
   __shared__ u32x4 lds_a[kStages][kAVecs];
   __shared__ u32x4 lds_b[kStages][kBVecs];
   __shared__ int slot_lds[kAdapters ? kTM : 1], row_lds[kAdapters ? kTM : 1];  // adapters of the tile's slots and rows
+  constexpr bool kRanged = kAdapters && kAdapterRanged<H>;
+  __shared__ float range_lds[kRanged ? kTM : 1];
   __shared__ int found_lds;  // whether there are values of B that are not finite
 
   const int tid = threadIdx.x;
@@ -219,7 +221,10 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
   int slots = 0;
   if constexpr (kAdapters) {
     if (tid == 0) found_lds = 0;
-    if (blockIdx.y == 0) slots = adapter_slots<kTM>(part, m0, M, lane, row_lds, slot_lds);
+    if (blockIdx.y == 0) {
+      slots = adapter_slots<kTM>(part, m0, M, lane, row_lds, slot_lds);
+      if constexpr (kRanged) adapter_ranges<kTM>(part, m0, lane, row_lds, range_lds);
+    }
   }
   {
     const int younger = min(kStages - 1, ktiles - 1);
@@ -313,6 +318,16 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
   if constexpr (kAdapters) {
     const int pieces = part.rank / 8, slices = (slots * pieces + 3) / 4;
     uint32_t found = 0;
+    if constexpr (kRanged) {
+      if (slots > 0) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const float to = range_lds[wm * (kTM / 2) + 16 * i + l16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] *= to;
+        }
+      }
+    }
     for (int first = 0; first < slices; first += kStages) {
       const int count = min(kStages, slices - first);
       wait_and_barrier<0>();  // the stages are read
@@ -322,7 +337,7 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
           const int row = (wave * AP + p) * 16 + (lane >> 2);
           const float* from =
               adapter_t(part, 4 * (first + s) + ((lane & 3) ^ a_mask(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
-          adapter_put_t<H>(part, from, lds_a0 + s * kAStage + (wave * AP + p) * 1024 + lane * 16);
+          adapter_put_t<H>(part, from, lds_a0 + s * kAStage + (wave * AP + p) * 1024 + lane * 16, kRanged ? range_lds[row] : 1.f);
         }
         u32x4 b[2];
 #pragma unroll
@@ -346,6 +361,16 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
         for (int i = 0; i < MB; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] = H::mfma16(fr[0].b[j], i < MH ? fr[0].a[i % MH] : fy[i % MH], acc[i][j]);
+      }
+    }
+    if constexpr (kRanged) {
+      if (slots > 0) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const float to = inverse_power(range_lds[wm * (kTM / 2) + 16 * i + l16]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] *= to;
+        }
       }
     }
     nonfinite = found_lds != 0;

@@ -45,6 +45,8 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
   constexpr int kPieces = 8;  // copies per wave and slice: 4 lhs (8 rows each), 4 rhs (4 k-rows each)
   __shared__ __attribute__((aligned(1024))) char lds[kStages * 2 * kOperand];
   __shared__ int slot_lds[kAdapters ? kT : 1], row_lds[kAdapters ? kT : 1];  // adapters of the tile's slots and rows
+  constexpr bool kRanged = kAdapters && kAdapterRanged<H>;
+  __shared__ float range_lds[kRanged ? kT : 1];
   __shared__ int found_lds;  // whether there are values of B that are not finite
 
   const int tid = threadIdx.x;
@@ -145,6 +147,7 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
   if constexpr (kAdapters) {
     if (tid == 0) found_lds = 0;
     slots = adapter_slots<kT>(part, m0, M, lane, row_lds, slot_lds);
+    if constexpr (kRanged) adapter_ranges<kT>(part, m0, lane, row_lds, range_lds);
   }
   {
     const int younger = min(kStages, nk) - 1;
@@ -215,6 +218,16 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
   if constexpr (kAdapters) {
     const int pieces = part.rank / 8, slices = (slots * pieces + 7) / 8;
     uint32_t found = 0;
+    if constexpr (kRanged) {
+      if (slots > 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float to = range_lds[wm * 64 + 16 * i + l16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] *= to;
+        }
+      }
+    }
     for (int first = 0; first < slices; first += kStages) {
       const int count = min(kStages, slices - first);
       wait_and_barrier<0>();  // the stages are read
@@ -224,7 +237,7 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
         for (int p = 0; p < 4; ++p) {
           const int row = (wave * 4 + p) * 8 + (lane >> 3);
           const float* from = adapter_t(part, 8 * (first + s) + ((lane & 7) ^ a_swz(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
-          adapter_put_t<H>(part, from, dst + p * 1024 + lane * 16);
+          adapter_put_t<H>(part, from, dst + p * 1024 + lane * 16, kRanged ? range_lds[row] : 1.f);
         }
         u32x4 b[4];
 #pragma unroll
@@ -248,6 +261,16 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = H::mfma16(fr[0].b[j], fr[0].a[i], acc[i][j]);
         }
+    }
+    if constexpr (kRanged) {
+      if (slots > 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float to = inverse_power(range_lds[wm * 64 + 16 * i + l16]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] *= to;
+        }
+      }
     }
     nonfinite = found_lds != 0;
   }

@@ -83,6 +83,8 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
   __shared__ u32x4 lds_a[kStages][kVecsA];
   __shared__ u32x4 lds_b[kStages][kVecsB];
   __shared__ int slot_lds[kAdapters ? kTM : 1], row_lds[kAdapters ? kTM : 1];  // adapters of the tile's slots and rows
+  constexpr bool kRanged = kAdapters && kAdapterRanged<H>;
+  __shared__ float range_lds[kRanged ? kTM : 1];
   __shared__ int found_lds;  // whether there are values of B that are not finite
 
   const int tid = threadIdx.x;
@@ -191,6 +193,7 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
   if constexpr (kAdapters) {
     if (tid == 0) found_lds = 0;
     slots = adapter_slots<kTM>(part, m0, M, lane, row_lds, slot_lds);
+    if constexpr (kRanged) adapter_ranges<kTM>(part, m0, lane, row_lds, range_lds);
   }
   {
     const int younger = min(kStages - 1, ktiles - 1);
@@ -279,6 +282,20 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
   if constexpr (kAdapters) {
     const int pieces = part.rank / 8, slices = (slots * pieces + 3) / 4;
     uint32_t found = 0;
+    if constexpr (kRanged) {
+      if (slots > 0) {
+        mfma_drain();
+#pragma unroll
+        for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+          const float to = range_lds[wm * WM + 16 * i + l16];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[i][j] *= to;
+          mfma_order(acc[i]);  // (one block after another: all of them at once are more than the registers hold)
+        }
+      }
+    }
     for (int first = 0; first < slices; first += kStages) {
       const int count = min(kStages, slices - first);
       wait_and_barrier<0>();  // the stages are read
@@ -288,7 +305,7 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
           const int row = (wave * kAPieces + p) * 16 + (lane >> 2);
           const float* from =
               adapter_t(part, 4 * (first + s) + ((lane & 3) ^ a_mask(row)), pieces, slots, slot_lds, row_lds[row], m0 + row);
-          adapter_put_t<H>(part, from, lds_a0 + s * kStageA + (wave * kAPieces + p) * 1024 + lane * 16);
+          adapter_put_t<H>(part, from, lds_a0 + s * kStageA + (wave * kAPieces + p) * 1024 + lane * 16, kRanged ? range_lds[row] : 1.f);
         }
         u32x4 b[4];
 #pragma unroll
@@ -341,6 +358,10 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
       for (int j = 0; j < 8; ++j) {
         const int n = n0 + wn * 128 + j * 16 + 4 * lg;
         float v0 = acc[i][j][0], v1 = acc[i][j][1], v2 = acc[i][j][2], v3 = acc[i][j][3];
+        if constexpr (kRanged) {
+          const float back = inverse_power(range_lds[wm * WM + 16 * i + l16]);
+          v0 *= back, v1 *= back, v2 *= back, v3 *= back;
+        }
         if constexpr (kBias == 1) {
           const float* bp = static_cast<const float*>(bias);
           v0 += bp[n];

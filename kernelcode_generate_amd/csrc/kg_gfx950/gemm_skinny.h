@@ -219,6 +219,24 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
     int of_row[kMT], listed = -1, slots = 0;
 #pragma unroll
     for (int i = 0; i < kMT; ++i) of_row[i] = __shfl(own, 16 * i + l16, 64);
+    constexpr bool kRanged = kAdapterRanged<Half16<Tag>>;
+    float range = 1.f, range_of[kMT];  // of row `lane`, of this lane's rows of t
+    if constexpr (kRanged) {
+      if (own >= 0) range = adapter_range(part, m0 + lane);
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) {
+        range_of[i] = __shfl(range, 16 * i + l16, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float to = __shfl(range, 16 * i + 4 * lg + e, 64);
+          acc[i][0][e] *= to;
+          acc[i][1][e] *= to;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) range_of[i] = 1.f;
+    }
     for (unsigned long long left = __builtin_amdgcn_ballot_w64(own >= 0); left != 0; ++slots) {
       const int l = __builtin_amdgcn_readlane(own, __builtin_ctzll(left));
       left &= ~__builtin_amdgcn_ballot_w64(own == l);
@@ -238,7 +256,7 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
       for (int i = 0; i < kMT; ++i) {
         f.a[i] = u32x4{0, 0, 0, 0};
         if (there && of_row[i] == l)
-          f.a[i] = adapter_t8<Half16<Tag>>(part, part.sums + (long long)(m0 + 16 * i + l16) * part.rank + r0);
+          f.a[i] = adapter_t8<Half16<Tag>>(part, part.sums + (long long)(m0 + 16 * i + l16) * part.rank + r0, range_of[i]);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) f.b[e] = finite_pair<Half16<Tag>>(f.b[e], found);
@@ -267,6 +285,16 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
             }
           }
       }
+    }
+    if constexpr (kRanged) {
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float back = inverse_power(__shfl(range, 16 * i + 4 * lg + e, 64));
+          acc[i][0][e] *= back;
+          acc[i][1][e] *= back;
+        }
     }
   }
 
