@@ -14,7 +14,7 @@
 //
 // adapter_add_kernel: any types and strides, one workgroup per row: t = scale x A in 32 bits, then
 // out += t B, on an output that holds the projection already (matmul's kernels). A 16-bit output is
-// so rounded twice, by half a step each time.
+// so rounded twice, by half a step each time; a projection past the type's range is computed again, in 32 bits.
 #pragma once
 
 #include <type_traits>
@@ -30,10 +30,22 @@ struct AdapterArgs {
   void* out;
   const int* index;
   const float* scale;  // null: 1
-  long long ldx, ldw, ldo, a_l, a_k, b_l, b_r, index_stride, scale_stride;
+  long long ldx, ldw, ldo, a_l, a_k, b_l, b_r, index_stride, scale_stride, w_n, bias_stride;
   int m, n, k, rank, count;
+  bool wide_bias;  // 32 bits, not the operands' type
 };
 constexpr int kAdapterMaxRank = 512;
+
+template <typename T>
+__device__ __forceinline__ float adapter_projection(const AdapterArgs& p, const T* x, int n) {
+  const T* w = static_cast<const T*>(p.w) + n * p.w_n;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < p.k; ++k) sum = __builtin_fmaf(Elem<T>::load(x + k), Elem<T>::load(w + k * p.ldw), sum);
+  if (p.bias == nullptr) return sum;
+  return sum + (p.wide_bias ? static_cast<const float*>(p.bias)[n * p.bias_stride]
+                            : Elem<T>::load(static_cast<const T*>(p.bias) + n * p.bias_stride));
+}
 
 template <typename T>
 __global__ __launch_bounds__(256) void adapter_add_kernel(AdapterArgs p) {
@@ -76,7 +88,9 @@ __global__ __launch_bounds__(256) void adapter_add_kernel(AdapterArgs p) {
   for (int n = tid; n < p.n; n += 256) {
     float o = 0.f;
     for (int r = 0; r < p.rank; ++r) o = __builtin_fmaf(ts[r], Elem<T>::load(B + r * p.b_r + n), o);
-    Elem<T>::store(out + n, Elem<T>::load(out + n) + scale * o);
+    float base = Elem<T>::load(out + n);
+    if (sizeof(T) == 2 && !__builtin_isfinite(base)) base = adapter_projection(p, x, n);
+    Elem<T>::store(out + n, base + scale * o);
   }
 }
 

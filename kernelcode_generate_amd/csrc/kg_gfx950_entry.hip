@@ -1730,6 +1730,7 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   p.ldx = x.stride[0], p.ldw = w.stride[0], p.ldo = out.stride[0];
   p.a_l = a.stride[0], p.a_k = a.stride[1], p.b_l = b.stride[0], p.b_r = b.stride[1];
   p.index_stride = index.stride[0], p.scale_stride = scale.stride[0];
+  p.w_n = w.stride[1], p.bias_stride = bias.stride[0], p.wide_bias = bias.dtype == KG_DTYPE_F32;
   p.m = (int)M, p.n = (int)N, p.k = (int)K, p.rank = (int)rank, p.count = (int)count;
   const bool mfma = adapters && out.dtype != KG_DTYPE_F32 && K > 0 && K % 8 == 0 && N % 8 == 0 && rank % 8 == 0 &&
                     w.stride[1] == 1 && (!bias.present || bias.stride[0] == 1 || N == 1) && rows_aligned(out, 16) &&
