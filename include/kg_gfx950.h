@@ -225,7 +225,10 @@ int kg_gfx950_abi_version(void);
 enum {
   KG_OP_MATMUL = 1,
   KG_OP_CONV2D = 2,
-  KG_OP_FLASH_ATTENTION = 3
+  KG_OP_FLASH_ATTENTION = 3,
+  /* the projection's MFMAs, without the adapters', whose number depends on the indexes; fp32 sums of a split K are
+   * counted as written and read */
+  KG_OP_ADAPTER_MATMUL = 4
 };
 enum {
   KG_COST_MAC = 0,       /* multiply-accumulates of the operation (mask-kept pairs for causal attention) */

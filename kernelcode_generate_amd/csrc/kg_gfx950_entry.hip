@@ -1294,7 +1294,7 @@ bool no_elements(const Mem& m) {  // (extents of axes without a stride may have 
 }
 
 int check_view(const Mem& m, const char* name) {
-  if (!m.present || no_elements(m)) return kOk;
+  if (!m.present || no_elements(m) || g_cost != nullptr) return kOk;
   if (m.data == nullptr) return fail(kInvalid, "%s: memory slot has no data", name);
   hipPointerAttribute_t attr;
   if (hipPointerGetAttributes(&attr, m.data) != hipSuccess || attr.type != hipMemoryTypeDevice) {
@@ -1376,7 +1376,7 @@ KvSide kv_side(const KvSlots& kv, int x, const Mem& rows) {
 // Whether the rows of a view start at multiples of `unit` bytes.
 bool rows_aligned(const Mem& m, long long unit) {
   const long long es = element_bytes(m.dtype);
-  bool ok = (uintptr_t)m.data % unit == 0;
+  bool ok = g_cost != nullptr || (uintptr_t)m.data % unit == 0;  // (cost queries model aligned buffers)
   for (int i = 0; i + 1 < m.rank; ++i) ok = ok && (m.shape[i] <= 1 || m.stride[i] * es % unit == 0);
   return ok;
 }
@@ -1646,6 +1646,14 @@ AdapterPlan adapter_plan(const AdapterArgs& p) {
   return a;
 }
 
+// MFMA instructions (16x16x32) of the projection in that form, as matmul counts them.
+long long adapter_mfma(const AdapterPlan& plan, long long M, long long N, long long K) {
+  if (plan.form == AdapterPlan::kSkinny)
+    return cdiv(M, gemm_skinny_rows(M, N)) * (gemm_skinny_rows(M, N) / 16) * cdiv(N, gemms::kCols) * cdiv(K, gemms::kStep) * 2;
+  if (plan.form == AdapterPlan::kMid) return cdiv(M, gemmm::kT) * cdiv(N, gemmm::kT) * cdiv(K, gemmm::kBK) * 128;
+  return cdiv(M, plan.tile_rows) * cdiv(N, gemmp::kBN) * cdiv(K, gemmp::kBK) * plan.tile_rows;
+}
+
 template <typename Tag>
 int launch_adapter_matmul(const AdapterArgs& p, const AdapterPlan& plan, int bias_kind, char* ws) {
   float* sums = reinterpret_cast<float*>(ws + kAdapterHeader);
@@ -1722,7 +1730,7 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   if ((rc = check_view(out, "out")) || (rc = check_view(x, "x")) || (rc = check_view(w, "weight")) || (rc = check_view(bias, "bias")) ||
       (rc = check_view(a, "a")) || (rc = check_view(b, "b")) || (rc = check_view(index, "index")) || (rc = check_view(scale, "scale")))
     return rc;
-  if (M == 0 || N == 0) return finish_launch("adapter_matmul(empty)");
+  if ((M == 0 || N == 0) && !g_cost) return finish_launch("adapter_matmul(empty)");
   AdapterArgs p;
   p.x = x.data, p.w = w.data, p.bias = bias.data, p.a = a.data, p.b = b.data, p.out = out.data;
   p.index = static_cast<const int*>(index.data);
@@ -1732,7 +1740,7 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   p.index_stride = index.stride[0], p.scale_stride = scale.stride[0];
   p.w_n = w.stride[1], p.bias_stride = bias.stride[0], p.wide_bias = bias.dtype == KG_DTYPE_F32;
   p.m = (int)M, p.n = (int)N, p.k = (int)K, p.rank = (int)rank, p.count = (int)count;
-  const bool mfma = adapters && out.dtype != KG_DTYPE_F32 && K > 0 && K % 8 == 0 && N % 8 == 0 && rank % 8 == 0 &&
+  const bool mfma = adapters && M > 0 && N > 0 && out.dtype != KG_DTYPE_F32 && K > 0 && K % 8 == 0 && N % 8 == 0 && rank % 8 == 0 &&
                     w.stride[1] == 1 && (!bias.present || bias.stride[0] == 1 || N == 1) && rows_aligned(out, 16) &&
                     rows_aligned(x, 16) && rows_aligned(w, 16) && rows_aligned(b, 16) && rows_aligned(a, 16) &&
                     x.stride[0] <= kMaxPipeLd && w.stride[0] <= kMaxPipeLd;
@@ -1748,6 +1756,19 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
       part.m = (int)std::min(rows, M - m0);
       return part;
     };
+    if (g_cost) {
+      const long long es = element_bytes(out.dtype);
+      long long instructions = 0, partial = 0;
+      for (long long m0 = 0; m0 < M; m0 += rows) {
+        const AdapterArgs part = piece(m0);
+        const AdapterPlan plan = adapter_plan(part);
+        instructions += adapter_mfma(plan, part.m, N, K);
+        if (plan.splits > 1) partial += plan.splits * part.m * N * (long long)sizeof(float);
+      }
+      return record_cost(M * N * K + M * rank * (K + N), instructions, 16,
+                         (M * K + K * N + std::min(M, count) * rank * (K + N)) * es + (bias.present ? N * element_bytes(bias.dtype) : 0) + partial,
+                         M * N * es + partial);
+    }
     const size_t bytes = std::max(adapter_plan(piece(0)).bytes, adapter_plan(piece((M - 1) / rows * rows)).bytes);
     SplitLease lease;  // held until the kernels are enqueued
     if (bytes <= (size_t)kSplitMaxWorkspace) lease = split_workspace(bytes, g_stream);
@@ -1764,6 +1785,11 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
     }
   }
   if ((rc = matmul_impl(args, 4)) || !adapters) return rc;
+  if (g_cost) {
+    g_cost->v[KG_COST_MAC] += M * rank * (K + N);
+    g_cost->v[KG_COST_HBM_READ] += std::min(M, count) * rank * (K + N) * element_bytes(out.dtype);
+    return kOk;
+  }
   return with_kv_types(out.dtype, out.dtype, [&](auto t, auto) {
     hipLaunchKernelGGL((adapter_add_kernel<decltype(t)>), dim3((unsigned)M), dim3(256), 0, g_stream, p);
     return finish_launch("adapter_matmul");
@@ -1839,6 +1865,7 @@ int kg_gfx950_cost(int op, const KgArgSlot* ordered_args, unsigned long long arg
     case KG_OP_MATMUL: rc = matmul_impl(ordered_args, arg_count); break;
     case KG_OP_CONV2D: rc = conv2d_impl(ordered_args, arg_count); break;
     case KG_OP_FLASH_ATTENTION: rc = flash_attention_impl(ordered_args, arg_count); break;
+    case KG_OP_ADAPTER_MATMUL: rc = adapter_matmul_impl(ordered_args, arg_count); break;
     default: rc = fail(kInvalid, "cost: unknown op %d", op);
   }
   g_cost = nullptr;
