@@ -10,7 +10,7 @@
 // kv_store_kernel, kv_load_kernel: rows of whole 16-byte pieces (8 elements a lane), bound by their bytes where there are many:
 // 4001 tokens of 8 heads of 128 from fp16 to int8 9.0 us, 2.7 TB/s (28 with a wave per row); four ragged sequences of up to 8192
 // back from e4m3 to bf16 34.8 us, 4.1 TB/s (169). 64 tokens take 3.0 us, a launch's. kv_store_any_kernel, kv_load_any_kernel:
-// any D and alignment, one wave per row.
+// any D and alignment and any number of rows, one wave per row.
 #pragma once
 
 #include <type_traits>
@@ -104,29 +104,29 @@ __device__ __forceinline__ void split_slot(long long slot, int page_size, long l
 template <typename Src, typename C>
 __global__ __launch_bounds__(256) void kv_store_any_kernel(KvStoreArgs a) {
   const int lane = threadIdx.x & 63;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const long long rows = (long long)a.tokens * a.heads;
-  if (item >= 2 * rows) return;
-  const KvSide& s = a.side[item >= rows];
-  const long long r = item >= rows ? item - rows : item;
-  const int t = (int)(r / a.heads), h = (int)(r - (long long)t * a.heads);
-  const long long slot = a.slots[t * a.slot_stride];
-  if (slot < 0 || slot >= a.total_slots) return;  // not written
-  long long page;
-  int offset;
-  split_slot(slot, a.page_size, &page, &offset);
-  const Src* x = static_cast<const Src*>(s.rows) + t * s.r0 + h * s.r1;
-  C* c = static_cast<C*>(s.cache) + page * s.page + h * s.head + offset * s.row;
-  if constexpr (CacheElem<C>::kScaled) {
-    float top = 0.f;
-    for (int d = lane; d < a.d; d += 64) top = nan_max(top, __builtin_fabsf(Elem<Src>::load(x + d)));
+  for (long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); item < 2 * rows; item += 4ll * gridDim.x) {
+    const KvSide& s = a.side[item >= rows];
+    const long long r = item >= rows ? item - rows : item;
+    const int t = (int)(r / a.heads), h = (int)(r - (long long)t * a.heads);
+    const long long slot = a.slots[t * a.slot_stride];
+    if (slot < 0 || slot >= a.total_slots) continue;  // not written
+    long long page;
+    int offset;
+    split_slot(slot, a.page_size, &page, &offset);
+    const Src* x = static_cast<const Src*>(s.rows) + t * s.r0 + h * s.r1;
+    C* c = static_cast<C*>(s.cache) + page * s.page + h * s.head + offset * s.row;
+    if constexpr (CacheElem<C>::kScaled) {
+      float top = 0.f;
+      for (int d = lane; d < a.d; d += 64) top = nan_max(top, __builtin_fabsf(Elem<Src>::load(x + d)));
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = nan_max(top, __shfl_xor(top, o, 64));
-    const float scale = top * CacheElem<C>::kInverse;
-    for (int d = lane; d < a.d; d += 64) CacheElem<C>::store(c + d, scaled_code<C>(Elem<Src>::load(x + d), scale));
-    if (lane == 0) s.scale[page * s.s_page + h * s.s_head + offset * s.s_row] = scale;
-  } else {
-    for (int d = lane; d < a.d; d += 64) c[d] = x[d];
+      for (int o = 32; o > 0; o >>= 1) top = nan_max(top, __shfl_xor(top, o, 64));
+      const float scale = top * CacheElem<C>::kInverse;
+      for (int d = lane; d < a.d; d += 64) CacheElem<C>::store(c + d, scaled_code<C>(Elem<Src>::load(x + d), scale));
+      if (lane == 0) s.scale[page * s.s_page + h * s.s_head + offset * s.s_row] = scale;
+    } else {
+      for (int d = lane; d < a.d; d += 64) c[d] = x[d];
+    }
   }
 }
 
@@ -143,26 +143,26 @@ struct KvLoadArgs {
 template <typename C, typename Dst>
 __global__ __launch_bounds__(256) void kv_load_any_kernel(KvLoadArgs a) {
   const int lane = threadIdx.x & 63;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const long long rows = (long long)a.batch * a.heads * a.reach;
-  if (item >= 2 * rows) return;
-  const KvSide& s = a.side[item >= rows];
-  const long long r = item >= rows ? item - rows : item;
-  const int bh = (int)(r / a.reach), i = (int)(r - (long long)bh * a.reach);
-  const int b = bh / a.heads, h = bh - b * a.heads;
-  if (i >= a.lens[b * a.len_stride]) return;
-  const int p = div_page(i, a.div);
-  if (p >= a.per) return;
-  const long long page = a.table[b * a.table_stride0 + p * a.table_stride1];
-  if (page < 0 || page >= a.pages) return;  // no such page: left as it is
-  const int offset = i - p * a.page_size;
-  const C* c = static_cast<const C*>(s.cache) + page * s.page + h * s.head + offset * s.row;
-  Dst* y = static_cast<Dst*>(s.rows) + b * s.r0 + h * s.r1 + i * s.r2;
-  if constexpr (CacheElem<C>::kScaled) {
-    const float scale = s.scale[page * s.s_page + h * s.s_head + offset * s.s_row];
-    for (int d = lane; d < a.d; d += 64) Elem<Dst>::store(y + d, CacheElem<C>::load(c + d) * scale);
-  } else {
-    for (int d = lane; d < a.d; d += 64) y[d] = c[d];
+  for (long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); item < 2 * rows; item += 4ll * gridDim.x) {
+    const KvSide& s = a.side[item >= rows];
+    const long long r = item >= rows ? item - rows : item;
+    const int bh = (int)(r / a.reach), i = (int)(r - (long long)bh * a.reach);
+    const int b = bh / a.heads, h = bh - b * a.heads;
+    if (i >= a.lens[b * a.len_stride]) continue;
+    const int p = div_page(i, a.div);
+    if (p >= a.per) continue;
+    const long long page = a.table[b * a.table_stride0 + p * a.table_stride1];
+    if (page < 0 || page >= a.pages) continue;  // no such page: left as it is
+    const int offset = i - p * a.page_size;
+    const C* c = static_cast<const C*>(s.cache) + page * s.page + h * s.head + offset * s.row;
+    Dst* y = static_cast<Dst*>(s.rows) + b * s.r0 + h * s.r1 + i * s.r2;
+    if constexpr (CacheElem<C>::kScaled) {
+      const float scale = s.scale[page * s.s_page + h * s.s_head + offset * s.s_row];
+      for (int d = lane; d < a.d; d += 64) Elem<Dst>::store(y + d, CacheElem<C>::load(c + d) * scale);
+    } else {
+      for (int d = lane; d < a.d; d += 64) y[d] = c[d];
+    }
   }
 }
 

@@ -66,84 +66,86 @@ __global__ __launch_bounds__(256) void tree_attn_any_kernel(TreeArgs a) {
   __shared__ long long rows[kThreads];
   __shared__ float red[kThreads / 64];
   const int tid = threadIdx.x;
-  const int t = (int)(blockIdx.x / (unsigned)a.heads_q), hq = (int)(blockIdx.x - (unsigned)t * a.heads_q);
-  const int h = hq / a.group;
+  for (unsigned row = blockIdx.x; row < (unsigned)a.tokens * (unsigned)a.heads_q; row += gridDim.x) {
+    const int t = (int)(row / (unsigned)a.heads_q), hq = (int)(row - (unsigned)t * a.heads_q);
+    const int h = hq / a.group;
 
-  // the request: the last one that starts at or before t
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.starts[mid * a.start_stride] <= t) lo = mid;
-    else hi = mid;
-  }
-  const TreeRequest r = tree_request(a, lo);
-  const int j = t - r.first;
-  if (j < 0 || j >= r.count) return;  // a row of no request
-
-  const T* q = static_cast<const T*>(a.q) + t * a.q_token + hq * a.q_head;
-  for (int d = tid; d < a.d; d += kThreads) qs[d] = Elem<T>::load(q + d);
-  __syncthreads();
-
-  const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
-  const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
-  float acc[kMaxD / kThreads] = {0.f, 0.f};
-  float m_run = -INFINITY, l_run = 0.f;
-  for (int n0 = 0; n0 < r.keys; n0 += kThreads) {
-    const int n = n0 + tid;
-    float score = -INFINITY;
-    bool seen = n < r.keys && (n < r.context || tree_sees(a, t, j, n - r.context));
-    long long v_row = 0;
-    float v_scale = 1.f;
-    if (seen) {
-      const int p = div_page(n, a.div), offset = n - p * a.page_size;
-      const long long page = a.table[lo * a.table_0 + p * a.table_1];
-      seen = page >= 0 && page < a.pages;
-      if (seen) {
-        const C* k = kc + page * a.k_page + offset * a.k_row;
-        float dot = 0.f;
-        for (int d = 0; d < a.d; ++d) dot = __builtin_fmaf(qs[d], CacheElem<C>::load(k + d), dot);
-        if constexpr (CacheElem<C>::kScaled) {
-          dot *= a.k_scale[page * a.ks_page + h * a.ks_head + offset * a.ks_row];
-          v_scale = a.v_scale[page * a.vs_page + h * a.vs_head + offset * a.vs_row];
-        }
-        score = dot * a.scale_log2;
-        v_row = page * a.v_page + offset * a.v_row;
-      }
+    // the request: the last one that starts at or before t
+    int lo = 0, hi = a.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (a.starts[mid * a.start_stride] <= t) lo = mid;
+      else hi = mid;
     }
-    float top = score;
+    const TreeRequest r = tree_request(a, lo);
+    const int j = t - r.first;
+    if (j < 0 || j >= r.count) continue;  // a row of no request
+
+    const T* q = static_cast<const T*>(a.q) + t * a.q_token + hq * a.q_head;
+    for (int d = tid; d < a.d; d += kThreads) qs[d] = Elem<T>::load(q + d);  // (read before the last barrier of the row before)
+    __syncthreads();
+
+    const C* kc = static_cast<const C*>(a.k) + h * a.k_head;
+    const C* vc = static_cast<const C*>(a.v) + h * a.v_head;
+    float acc[kMaxD / kThreads] = {0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
+    for (int n0 = 0; n0 < r.keys; n0 += kThreads) {
+      const int n = n0 + tid;
+      float score = -INFINITY;
+      bool seen = n < r.keys && (n < r.context || tree_sees(a, t, j, n - r.context));
+      long long v_row = 0;
+      float v_scale = 1.f;
+      if (seen) {
+        const int p = div_page(n, a.div), offset = n - p * a.page_size;
+        const long long page = a.table[lo * a.table_0 + p * a.table_1];
+        seen = page >= 0 && page < a.pages;
+        if (seen) {
+          const C* k = kc + page * a.k_page + offset * a.k_row;
+          float dot = 0.f;
+          for (int d = 0; d < a.d; ++d) dot = __builtin_fmaf(qs[d], CacheElem<C>::load(k + d), dot);
+          if constexpr (CacheElem<C>::kScaled) {
+            dot *= a.k_scale[page * a.ks_page + h * a.ks_head + offset * a.ks_row];
+            v_scale = a.v_scale[page * a.vs_page + h * a.vs_head + offset * a.vs_row];
+          }
+          score = dot * a.scale_log2;
+          v_row = page * a.v_page + offset * a.v_row;
+        }
+      }
+      float top = score;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = nan_max(top, __shfl_xor(top, o, 64));
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    // a finite lowest maximum: scores of -inf, which infinite inputs give, weigh nothing beside it
-    const float m_new = nan_max(nan_max(nan_max(red[0], red[1]), nan_max(red[2], red[3])), nan_max(m_run, -3.0e38f));
-    const float p = seen ? __builtin_amdgcn_exp2f(score - m_new) : 0.f;
-    __syncthreads();
-    float sum = wave_sum(p);
-    if ((tid & 63) == 0) red[tid >> 6] = sum;
-    ps[tid] = p * v_scale;
-    rows[tid] = seen ? v_row : -1;
-    __syncthreads();
-    sum = red[0] + red[1] + red[2] + red[3];
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-    l_run = l_run * alpha + sum;
-    m_run = m_new;
-    const int keys = min(kThreads, r.keys - n0);
+      for (int o = 32; o > 0; o >>= 1) top = nan_max(top, __shfl_xor(top, o, 64));
+      if ((tid & 63) == 0) red[tid >> 6] = top;
+      __syncthreads();
+      // a finite lowest maximum: scores of -inf, which infinite inputs give, weigh nothing beside it
+      const float m_new = nan_max(nan_max(nan_max(red[0], red[1]), nan_max(red[2], red[3])), nan_max(m_run, -3.0e38f));
+      const float p = seen ? __builtin_amdgcn_exp2f(score - m_new) : 0.f;
+      __syncthreads();
+      float sum = wave_sum(p);
+      if ((tid & 63) == 0) red[tid >> 6] = sum;
+      ps[tid] = p * v_scale;
+      rows[tid] = seen ? v_row : -1;
+      __syncthreads();
+      sum = red[0] + red[1] + red[2] + red[3];
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run = l_run * alpha + sum;
+      m_run = m_new;
+      const int keys = min(kThreads, r.keys - n0);
 #pragma unroll
+      for (int e = 0; e < kMaxD / kThreads; ++e) {
+        const int d = tid + e * kThreads;
+        if (d >= a.d) continue;
+        float o = acc[e] * alpha;
+        for (int x = 0; x < keys; ++x)
+          if (rows[x] >= 0) o = __builtin_fmaf(ps[x], CacheElem<C>::load(vc + rows[x] + d), o);
+        acc[e] = o;
+      }
+      __syncthreads();
+    }
+    T* out = static_cast<T*>(a.out) + t * a.o_token + hq * a.o_head;
     for (int e = 0; e < kMaxD / kThreads; ++e) {
       const int d = tid + e * kThreads;
-      if (d >= a.d) continue;
-      float o = acc[e] * alpha;
-      for (int x = 0; x < keys; ++x)
-        if (rows[x] >= 0) o = __builtin_fmaf(ps[x], CacheElem<C>::load(vc + rows[x] + d), o);
-      acc[e] = o;
+      if (d < a.d) Elem<T>::store(out + d, l_run != 0.f ? acc[e] / l_run : 0.f);
     }
-    __syncthreads();
-  }
-  T* out = static_cast<T*>(a.out) + t * a.o_token + hq * a.o_head;
-  for (int e = 0; e < kMaxD / kThreads; ++e) {
-    const int d = tid + e * kThreads;
-    if (d < a.d) Elem<T>::store(out + d, l_run != 0.f ? acc[e] / l_run : 0.f);
   }
 }
 

@@ -40,6 +40,8 @@ struct TreePlan {
   bool join;
   size_t bytes;
 };
+// Rows in fours that a launch of the join can have, a wave each: its work-items are counted in 32 bits.
+constexpr long long kTreeMostQuads = (1ll << 26) - 4;
 // Shares of a call: as many workgroups as run at once, or as there can be units (the table's reach bounds a
 // request's keys, the batch's tokens its blocks of rows).
 inline TreePlan tree_plan(const TreeArgs& a, int cache_bytes, bool may_split, long long most_bytes) {
@@ -55,7 +57,7 @@ inline TreePlan tree_plan(const TreeArgs& a, int cache_bytes, bool may_split, lo
   const long long reach = (long long)a.per * a.page_size;
   const long long items = tree_items(a, p.split.block);
   const long long units = items * std::max(1ll, (reach + round - 1) / round);
-  may_split = may_split && reach > round && units < kTreeMostUnits && items * p.split.block / kTreeJoinRows < 0x7fffffffLL;
+  may_split = may_split && reach > round && units < kTreeMostUnits && items * p.split.block / kTreeJoinRows <= kTreeMostQuads;
   p.split.round = may_split ? (int)round : 0;
   p.split.grid = (int)std::min<long long>(may_split ? units : items, p.width == 256 ? 256 : 512);
   const long long record = 2ll * p.split.block * (p.width + kTreePad) * (long long)sizeof(float);

@@ -1246,6 +1246,11 @@ int flash_attention_impl(const KgArgSlot* args, unsigned long long n) {
 // serving: the paged cache of keys and values, attention over it, adapters
 // ---------------------------------------------------------------------------------------
 
+// A launch's work-items along an axis are counted in 32 bits: at most 2^24 - 1 workgroups of 256. The general kernels of these
+// entries walk what is left beyond that many.
+constexpr long long kMostBlocks = (1ll << 24) - 1;
+unsigned most_blocks(long long blocks) { return (unsigned)std::min(blocks, kMostBlocks); }
+
 // These entries check a call in two steps: what the slots say (kind, rank, dtype, shape, strides), for
 // all of them, and only then the memory behind them, which must lie on the current device.
 constexpr unsigned kFloatTypes = 1u << KG_DTYPE_F32 | 1u << KG_DTYPE_F16 | 1u << KG_DTYPE_BF16;
@@ -1380,6 +1385,10 @@ bool rows_aligned(const Mem& m, long long unit) {
   for (int i = 0; i + 1 < m.rank; ++i) ok = ok && (m.shape[i] <= 1 || m.stride[i] * es % unit == 0);
   return ok;
 }
+// Rows of K or V that a call may have: past that, only views of rows on one another reach.
+constexpr long long kMostRows = 1ll << 33;
+// Lanes of a row of the kernels of eight elements a lane.
+int kv_lanes(long long d) { return d <= 64 ? 8 : d <= 128 ? 16 : d <= 256 ? 32 : 64; }
 // Rows that the kernels of eight elements a lane take, of caches and of dense rows.
 bool kv_in_eights(const KvSlots& kv, const Mem* rows) {
   bool ok = kv.d % 8 == 0;
@@ -1420,6 +1429,7 @@ int kv_cache_store_impl(const KgArgSlot* args, unsigned long long n) {
       (rc = check_view(slots, "slots")))
     return rc;
   if (tokens == 0 || kv.heads == 0 || kv.pages == 0) return finish_launch("kv_cache_store(empty)");
+  if (tokens * kv.heads > kMostRows) return fail(kUnsupported, "kv_cache_store: %lld x %lld rows are too many", tokens, kv.heads);
   KvStoreArgs a;
   for (int x = 0; x < 2; ++x) a.side[x] = kv_side(kv, x, rows[x]);
   a.slots = static_cast<const long long*>(slots.data);
@@ -1431,21 +1441,22 @@ int kv_cache_store_impl(const KgArgSlot* args, unsigned long long n) {
   a.total_slots = kv.pages * kv.page_size;
   const long long items = 2 * tokens * kv.heads;
   a.by_heads = page_div((int)kv.heads);
-  if (kv_in_eights(kv, rows) && items / 2 <= 0x7fffff00LL)  // (row numbers of the last workgroup stay in 31 bits)
+  const int lanes = kv_lanes(kv.d);
+  // (row numbers of the last workgroup stay in 31 bits)
+  if (kv_in_eights(kv, rows) && items / 2 <= 0x7fffff00LL && cdiv(items / 2 * lanes, 256) <= kMostBlocks)
     return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
 #define KG_KV_STORE(LANES)                                                                                             \
   hipLaunchKernelGGL((kv_store_kernel<decltype(t), decltype(c), LANES>), dim3((unsigned)cdiv(items / 2 * LANES, 256), 2), \
                      dim3(256), 0, g_stream, a)
-      if (kv.d <= 64) KG_KV_STORE(8);
-      else if (kv.d <= 128) KG_KV_STORE(16);
-      else if (kv.d <= 256) KG_KV_STORE(32);
+      if (lanes == 8) KG_KV_STORE(8);
+      else if (lanes == 16) KG_KV_STORE(16);
+      else if (lanes == 32) KG_KV_STORE(32);
       else KG_KV_STORE(64);
 #undef KG_KV_STORE
       return finish_launch("kv_cache_store");
     });
-  if (cdiv(items, 4) > 0x7fffffffLL) return fail(kUnsupported, "kv_cache_store: %lld rows exceed the grid limit", items);
   return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
-    hipLaunchKernelGGL((kv_store_any_kernel<decltype(t), decltype(c)>), dim3((unsigned)cdiv(items, 4)), dim3(256), 0, g_stream, a);
+    hipLaunchKernelGGL((kv_store_any_kernel<decltype(t), decltype(c)>), dim3(most_blocks(cdiv(items, 4))), dim3(256), 0, g_stream, a);
     return finish_launch("kv_cache_store");
   });
 }
@@ -1475,6 +1486,8 @@ int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
       (rc = check_view(table, "page_table")) || (rc = check_view(lens, "lengths")))
     return rc;
   if (no_elements(rows[0]) || table.shape[1] == 0 || kv.pages == 0) return finish_launch("kv_cache_load(empty)");
+  if (batch * kv.heads > 0x7fffffffLL || batch * kv.heads > kMostRows / reach)
+    return fail(kUnsupported, "kv_cache_load: %lld x %lld x %lld rows are too many", batch, kv.heads, reach);
   KvLoadArgs a;
   for (int x = 0; x < 2; ++x) a.side[x] = kv_side(kv, x, rows[x]);
   a.table = static_cast<const int*>(table.data);
@@ -1490,22 +1503,21 @@ int kv_cache_load_impl(const KgArgSlot* args, unsigned long long n) {
   a.reach = (int)reach;
   a.pages = kv.pages;
   a.div = page_div((int)kv.page_size);
-  if (kv_in_eights(kv, rows) && batch * kv.heads <= 65535 && reach <= 0x7fffff00LL)
+  const int lanes = kv_lanes(kv.d);
+  if (kv_in_eights(kv, rows) && batch * kv.heads <= 65535 && reach <= 0x7fffff00LL && cdiv(reach * lanes, 1024) <= kMostBlocks)
     return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
 #define KG_KV_LOAD(LANES)                                                                                                \
   hipLaunchKernelGGL((kv_load_kernel<decltype(c), decltype(t), LANES>),                                                  \
                      dim3((unsigned)cdiv(reach * LANES, 1024), (unsigned)(batch * kv.heads), 2), dim3(256), 0, g_stream, a)
-      if (kv.d <= 64) KG_KV_LOAD(8);
-      else if (kv.d <= 128) KG_KV_LOAD(16);
-      else if (kv.d <= 256) KG_KV_LOAD(32);
+      if (lanes == 8) KG_KV_LOAD(8);
+      else if (lanes == 16) KG_KV_LOAD(16);
+      else if (lanes == 32) KG_KV_LOAD(32);
       else KG_KV_LOAD(64);
 #undef KG_KV_LOAD
       return finish_launch("kv_cache_load");
     });
-  if (batch * kv.heads > 0x7fffffffLL || cdiv(2 * batch * kv.heads, 4) > 0x7fffffffLL / reach)
-    return fail(kUnsupported, "kv_cache_load: %lld x %lld rows exceed the grid limit", batch * kv.heads, reach);
   return with_kv_types(rows[0].dtype, kv.dtype, [&](auto t, auto c) {
-    hipLaunchKernelGGL((kv_load_any_kernel<decltype(c), decltype(t)>), dim3((unsigned)cdiv(2 * batch * kv.heads * reach, 4)),
+    hipLaunchKernelGGL((kv_load_any_kernel<decltype(c), decltype(t)>), dim3(most_blocks(cdiv(2 * batch * kv.heads * reach, 4))),
                        dim3(256), 0, g_stream, a);
     return finish_launch("kv_cache_load");
   });
@@ -1550,6 +1562,7 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
       (rc = check_view(lens, "context_lens")) || (rc = check_view(starts, "starts")) || (rc = check_view(mask, "mask")))
     return rc;
   if (no_elements(out) || batch == 0) return finish_launch("tree_attention(empty)");
+  if (tokens * heads_q > 0x7fffffffLL) return fail(kUnsupported, "tree_attention: %lld x %lld rows are too many", tokens, heads_q);
   TreeArgs a;
   a.q = q.data;
   a.out = out.data;
@@ -1576,7 +1589,6 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
   a.pages = kv.pages;
   a.div = page_div((int)kv.page_size);
   a.scale_log2 = (float)(scale * 1.4426950408889634);
-  if (tokens * heads_q > 0x7fffffffLL) return fail(kUnsupported, "tree_attention: %lld rows exceed the grid limit", tokens * heads_q);
   if (q.dtype != KG_DTYPE_F32 && tree_matrix_takes(a, (int)element_bytes(kv.dtype))) {
     TreePlan plan = tree_plan(a, (int)element_bytes(kv.dtype), true, kSplitMaxWorkspace);
     SplitLease lease;  // held until both kernels are enqueued
@@ -1596,7 +1608,7 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
     return finish_launch("tree_attention(mfma)");
   }
   return with_kv_types(q.dtype, kv.dtype, [&](auto t, auto c) {
-    hipLaunchKernelGGL((tree_attn_any_kernel<decltype(t), decltype(c)>), dim3((unsigned)(tokens * heads_q)), dim3(256), 0, g_stream, a);
+    hipLaunchKernelGGL((tree_attn_any_kernel<decltype(t), decltype(c)>), dim3(most_blocks(tokens * heads_q)), dim3(256), 0, g_stream, a);
     return finish_launch("tree_attention");
   });
 }
@@ -1632,7 +1644,7 @@ AdapterPlan adapter_plan(const AdapterArgs& p) {
   // sums for every reader (1024 workgroups: 256 x 4096 x 4096 47 us, 512: 41, 256: 39; x 512 rows in runs 39, 40, 43)
   a.low_splits = (int)std::max(1ll, std::min(std::min<long long>(K / 256, kAdapterMaxSplits), 512 / (low * a.at_once)));
   a.low_bytes = (size_t)cdiv(kAdapterHeader + a.low_splits * M * adapter_low_sums(p.rank) * 4, 256) * 256;
-  if (adapter_skinny_pays(M, N, K)) {
+  if (adapter_skinny_pays(M, N, K) && cdiv(M, 16) * cdiv(N, gemms::kCols) <= kMostBlocks * 4 / gemms::kWaves) {
     a.form = AdapterPlan::kSkinny;
   } else if (gemm_mid_pays(M, N, K)) {
     a.form = AdapterPlan::kMid;
@@ -1743,7 +1755,8 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   const bool mfma = adapters && M > 0 && N > 0 && out.dtype != KG_DTYPE_F32 && K > 0 && K % 8 == 0 && N % 8 == 0 && rank % 8 == 0 &&
                     w.stride[1] == 1 && (!bias.present || bias.stride[0] == 1 || N == 1) && rows_aligned(out, 16) &&
                     rows_aligned(x, 16) && rows_aligned(w, 16) && rows_aligned(b, 16) && rows_aligned(a, 16) &&
-                    x.stride[0] <= kMaxPipeLd && w.stride[0] <= kMaxPipeLd;
+                    x.stride[0] <= kMaxPipeLd && w.stride[0] <= kMaxPipeLd &&
+                    cdiv(std::min(M, 1ll << 21), 128) * cdiv(N, gemmp::kBN) <= kMostBlocks / 2;  // (workgroups of 512, of a piece's rows)
   if (mfma) {
     // pieces of whole 256-row tiles whose sums fit the workspace (262144 rows of rank 64: two)
     const long long most = ((long long)kSplitMaxWorkspace - kAdapterHeader - 256) / (adapter_low_sums(rank) * 4) / 256 * 256;
@@ -1791,7 +1804,7 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
     return kOk;
   }
   return with_kv_types(out.dtype, out.dtype, [&](auto t, auto) {
-    hipLaunchKernelGGL((adapter_add_kernel<decltype(t)>), dim3((unsigned)M), dim3(256), 0, g_stream, p);
+    hipLaunchKernelGGL((adapter_add_kernel<decltype(t)>), dim3(most_blocks(M)), dim3(256), 0, g_stream, p);
     return finish_launch("adapter_matmul");
   });
 }
