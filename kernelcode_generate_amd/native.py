@@ -191,10 +191,11 @@ _MEMORY_KINDS: set[type] = set()  # classes whose objects are memory arguments (
 def _is_memory(value: Any) -> bool:
     if type(value) in _MEMORY_KINDS:
         return True
-    if hasattr(value, "data_ptr") and hasattr(value, "shape") and hasattr(value, "stride"):
+    names = ("data_ptr", "shape", "stride", "dtype")
+    if all(hasattr(type(value), name) for name in names):  # of the class: every object of it has them
         _MEMORY_KINDS.add(type(value))
         return True
-    return False
+    return all(hasattr(value, name) for name in names[:3])
 
 
 # A KgArgSlot is eight 64-bit words (the 32-bit fields are padded to one each), so a call's
