@@ -1541,7 +1541,8 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
   if ((rc = read_view(args, 8, 1, 1u << KG_DTYPE_I32, false, "starts", &starts))) return rc;
   if ((rc = read_view(args, 9, 2, 1u << KG_DTYPE_I64, true, "mask", &mask))) return rc;
   if ((rc = read_float(args, 10, "scale", &scale))) return rc;
-  if (!std::isfinite((float)scale)) return fail(kInvalid, "tree_attention: scale must be finite");
+  const float scale_log2 = (float)(scale * 1.4426950408889634);
+  if (!std::isfinite(scale_log2)) return fail(kInvalid, "tree_attention: scale must be finite in 32 bits, and so must scale x log2(e)");
   const long long tokens = q.shape[0], heads_q = q.shape[1], batch = lens.shape[0];
   for (int i = 0; i < 3; ++i)
     if (out.shape[i] != q.shape[i]) return fail(kInvalid, "tree_attention: q/out shape mismatch at dim %d", i);
@@ -1588,7 +1589,7 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
   a.words = mask.present ? (int)mask.shape[1] : -1;
   a.pages = kv.pages;
   a.div = page_div((int)kv.page_size);
-  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   if (q.dtype != KG_DTYPE_F32 && tree_matrix_takes(a, (int)element_bytes(kv.dtype))) {
     TreePlan plan = tree_plan(a, (int)element_bytes(kv.dtype), true, kSplitMaxWorkspace);
     SplitLease lease;  // held until both kernels are enqueued
