@@ -48,30 +48,36 @@ struct Widen;
 template <>
 struct Widen<Bf16Tag, E4m3> {
   template <bool kHigh>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHigh));
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, float ratio = 1.f) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, ratio, kHigh));
   }
 };
 template <>
 struct Widen<F16Tag, E4m3> {
   template <bool kHigh>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHigh));
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, float ratio = 1.f) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, ratio, kHigh));
   }
 };
 template <typename Tag>
 struct Widen<Tag, int8_t> {
   template <bool kHigh>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, float ratio = 1.f) {
     const int a = (int)(w << (kHigh ? 8 : 24)) >> 24, b = (int)(w << (kHigh ? 0 : 16)) >> 24;
-    return Half16<Tag>::pack2((float)a, (float)b);
+    return Half16<Tag>::pack2((float)a * ratio, (float)b * ratio);
   }
 };
-// 8 codes to 8 16-bit elements
+// 8 codes to 8 16-bit elements, times a ValueScale's ratio
 template <typename Tag, typename C>
-__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float ratio = 1.f) {
   using W = Widen<Tag, C>;
-  return u32x4{W::template pair<false>(lo), W::template pair<true>(lo), W::template pair<false>(hi), W::template pair<true>(hi)};
+  if constexpr (std::is_same<C, E4m3>::value) {  // (the conversion takes the power of two)
+    const uint32_t sign = (uint32_t)((int)__builtin_bit_cast(uint32_t, ratio) >> 31) & 0x80808080u;
+    lo ^= sign, hi ^= sign;
+    ratio = __builtin_fabsf(ratio);
+  }
+  return u32x4{W::template pair<false>(lo, ratio), W::template pair<true>(lo, ratio), W::template pair<false>(hi, ratio),
+               W::template pair<true>(hi, ratio)};
 }
 
 // a lane's columns of a V row
@@ -91,21 +97,21 @@ __device__ __forceinline__ void load_v(uint32_t (&v)[kDwords], const C* p) {
   }
 }
 
-// A value's scale, of any sign and size. What counts for the running maximum is its magnitude within 2^-80..2^80 (log_of its logarithm):
-// a sum of weights is then 2^-80..2^88 for each of up to 2^31 keys, with 46 bits or more below it that 32 bits hold. ratio_of, the scale
-// over that, multiplies the weight before it is rounded: 1 of all scales that are not odd, 0 of a scale of 0, and within 2^-69..2^48,
-// which bf16 holds. In fp16 a ratio ends at 2^7, so that weights stay finite: the result is infinite with it as without, unless
-// that key's weight is below some 2^-70.
+// A value's scale, of any sign and size. What counts for the running maximum is its magnitude with an exponent within -79..80 (`log`
+// its logarithm): a sum of weights is then 2^-80..2^88 for each of up to 2^31 keys, with 46 bits or more below it that 32 bits hold.
+// What is left goes to the value or its weight in 16 bits, without loss: `ratio`, the sign and a power of two, 1 of scales that are
+// not odd, 0 of a scale of 0, and within 2^-69..2^48, which bf16 holds. In fp16 a ratio ends at 2^7, so that what it multiplies
+// stays finite: the result is infinite with it as without, unless that key's weight is below some 2^-70.
 template <typename Tag>
 struct ValueScale {
-  static constexpr float kLeast = 0x1p-80f, kMost = 0x1p80f;
-  static __device__ __forceinline__ bool odd(float scale) { return !(scale >= kLeast && scale <= kMost); }
-  static __device__ __forceinline__ float within(float scale) { return fminf(fmaxf(__builtin_fabsf(scale), kLeast), kMost); }
-  // (NaN of a scale that is not finite: so are the rows that see the value)
-  static __device__ __forceinline__ float log_of(float scale) { return __builtin_amdgcn_logf(within(scale)) + (scale - scale); }
-  static __device__ __forceinline__ float ratio_of(float scale) {
-    const float r = scale / within(scale);
-    return std::is_same<Tag, F16Tag>::value ? fminf(fmaxf(r, -0x1p7f), 0x1p7f) : r;
+  float log, ratio;
+  static __device__ __forceinline__ bool odd(float scale) { return !(scale >= 0x1p-80f && scale <= 0x1p79f); }
+  explicit __device__ __forceinline__ ValueScale(float scale) {
+    const int exponent = scale == 0.f ? -126 : __builtin_amdgcn_frexp_expf(scale), within = max(min(exponent, 80), -79), left = exponent - within;
+    // a mantissa within 0.5..1, also of 0; an infinity or NaN passes: the rows that see the value are NaN
+    const float mantissa = nan_max(__builtin_fabsf(__builtin_amdgcn_frexp_mantf(scale)), 0.5f);
+    log = __builtin_amdgcn_logf(__builtin_ldexpf(mantissa, within));
+    ratio = __builtin_ldexpf(scale == 0.f ? 0.f : __builtin_copysignf(1.f, scale), std::is_same<Tag, F16Tag>::value ? min(left, 7) : left);
   }
 };
 
@@ -427,9 +433,13 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
       bool odd = false;  // whether there are values with a ratio
       if constexpr (kS) {
         sc_lds[wave][0][lane & (kStep - 1)] = ks * a.scale_log2;
-        sc_lds[wave][1][lane & (kStep - 1)] = ValueScale<Tag>::log_of(vs);
+        sc_lds[wave][1][lane & (kStep - 1)] = __builtin_amdgcn_logf(vs);
         odd = __builtin_amdgcn_ballot_w64(ValueScale<Tag>::odd(vs)) != 0;
-        if (odd) sc_lds[wave][2][lane & (kStep - 1)] = ValueScale<Tag>::ratio_of(vs);
+        if (odd) {
+          const ValueScale<Tag> scale(vs);
+          sc_lds[wave][1][lane & (kStep - 1)] = scale.log;
+          sc_lds[wave][2][lane & (kStep - 1)] = scale.ratio;
+        }
       }
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
@@ -502,19 +512,26 @@ __global__ __launch_bounds__(treer::kThreads, D == 256 ? 1 : 2) void tree_attn_r
           w[i] = __builtin_amdgcn_exp2f(weighed(4 * kb + i) - m_run);
           if constexpr (kS) l_run[0] += __builtin_amdgcn_exp2f((float)sc[kb][i] - m_run);
         }
-        if constexpr (kS) {
-          if (odd) {
-            const f32x4 ratio = *reinterpret_cast<const f32x4*>(&sc_lds[wave][2][16 * kb + 4 * lr]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = w[i] == 0.f ? 0.f : w[i] * ratio[i];  // (of a key that is not seen, whatever its scale)
-          }
-        }
         pp[kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
         pp[kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);
       }
       if constexpr (!kS) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) l_run = H::mfma16(ones, pp[c], l_run);
+      }
+      if constexpr (kS) {
+        if (odd) {
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) {
+            const f32x4 ratio = *reinterpret_cast<const f32x4*>(&sc_lds[wave][2][16 * kb + 4 * lr]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t p2 = pp[kb >> 1][(kb & 1) * 2 + i];
+              pp[kb >> 1][(kb & 1) * 2 + i] =
+                  H::pack2(H::to_float(p2 & 0xffffu) * ratio[2 * i], H::to_float(p2 >> 16) * ratio[2 * i + 1]);
+            }
+          }
+        }
       }
       // ---- O^T += V^T P^T ----
 #pragma unroll

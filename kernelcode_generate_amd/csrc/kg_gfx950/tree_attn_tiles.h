@@ -71,7 +71,7 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
   constexpr int kRowStep = kThreads / kPerRow;       // rows between a thread's pieces
   constexpr int kStage = kTile * D * 2;              // bytes of one tile
   __shared__ __attribute__((aligned(1024))) char lds[4 * kStage];  // K, V of stage 0, K, V of stage 1
-  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? 2 : 1][3][kTile];
+  __shared__ __attribute__((aligned(16))) float sc_lds[kS ? 2 : 1][2][kTile];
   __shared__ int found_lds[3];  // whether tile t has values that are not finite, at t % 3
 
   const int tid = threadIdx.x;
@@ -201,7 +201,6 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     u32x4 kr[kPieces], vr[kPieces];
     uint32_t row_there = 0;
     float ks = 0.f, vs = 0.f;
-    bool odd = false;  // whether the tile stored last has values with a ratio
     auto load = [&](const Place& p) __attribute__((always_inline)) {
       row_there = 0;
 #pragma unroll
@@ -223,25 +222,32 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
     };
     auto store = [&](int stage, const Place& p) __attribute__((always_inline)) {
       const uint32_t kb = lds0 + stage * 2 * kStage, vb = kb + kStage;
+      // heed: there are scales that are odd, whose ratio goes to the values. Two copies of the stores, since what the ratio takes in one
+      // costs every tile (2 x 512 rows over e4m3 behind 4096: 156 us as without it, 163 in one copy, 193 on the weights; 8 x 16 rows
+      // behind 16384: 94, 96, 94, without 90).
+      auto pieces = [&](auto heed) __attribute__((always_inline)) {
+        constexpr bool kHeed = decltype(heed)::value != 0;
+        const float ratio = kHeed ? Scale(vs).ratio : 1.f;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int n = piece_row + kRowStep * i;
-        const bool there = piece_in && (row_there >> i & 1u);
-        const u32x4 k = there ? kr[i] : u32x4{0, 0, 0, 0}, v = there ? vr[i] : u32x4{0, 0, 0, 0};
-        if constexpr (kS) {
-          put(kb + k_at<D>(n, 2 * piece), treer::widen8<Tag, C>(k[0], k[1]));
-          put(kb + k_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(k[2], k[3]));
-          put(vb + v_at<D>(n, 2 * piece), treer::widen8<Tag, C>(v[0], v[1]));
-          put(vb + v_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(v[2], v[3]));
+        for (int i = 0; i < kPieces; ++i) {
+          const int n = piece_row + kRowStep * i;
+          const bool there = piece_in && (row_there >> i & 1u);
+          const u32x4 k = there ? kr[i] : u32x4{0, 0, 0, 0}, v = there ? vr[i] : u32x4{0, 0, 0, 0};
+          if constexpr (kS) {
+            put(kb + k_at<D>(n, 2 * piece), treer::widen8<Tag, C>(k[0], k[1]));
+            put(kb + k_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(k[2], k[3]));
+            const float to = kHeed ? __shfl(ratio, n, 64) : 1.f;  // (a wave has the scales of all keys)
+            put(vb + v_at<D>(n, 2 * piece), treer::widen8<Tag, C>(v[0], v[1], to));
+            put(vb + v_at<D>(n, 2 * piece + 1), treer::widen8<Tag, C>(v[2], v[3], to));
+          }
         }
-      }
-      if (tid < kTile) {
-        sc_lds[stage][0][tid] = p.page >= 0 ? ks * a.scale_log2 : 0.f;
-        sc_lds[stage][1][tid] = p.page >= 0 ? Scale::log_of(vs) : 0.f;
-      }
-      // (every wave has the scales of all keys)
-      odd = __builtin_amdgcn_ballot_w64(p.page >= 0 && Scale::odd(vs)) != 0;
-      if (odd && tid < kTile) sc_lds[stage][2][tid] = p.page >= 0 ? Scale::ratio_of(vs) : 0.f;
+        if (tid < kTile) {
+          sc_lds[stage][0][tid] = p.page >= 0 ? ks * a.scale_log2 : 0.f;
+          sc_lds[stage][1][tid] = p.page >= 0 ? (kHeed ? Scale(vs).log : __builtin_amdgcn_logf(vs)) : 0.f;
+        }
+      };
+      if (__builtin_amdgcn_ballot_w64(p.page >= 0 && Scale::odd(vs)) == 0) pieces(Int<0>{});
+      else pieces(Int<1>{});
     };
 
     f32x4 o[kNQ][NE];
@@ -355,13 +361,6 @@ __global__ __launch_bounds__(treet::kThreads, 2) void tree_attn_tiles_kernel(Tre
             if constexpr (kS) w[i] = __builtin_amdgcn_exp2f(weighed(x, 4 * kb + i) - m_run[x]);
             else w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(weighed(x, 4 * kb + i), scale, -m_run[x]));
             if constexpr (kS) l_run[x][0] += __builtin_amdgcn_exp2f((float)sc[x][kb][i] - m_run[x]);
-          }
-          if constexpr (kS) {
-            if (odd) {
-              const f32x4 ratio = *reinterpret_cast<const f32x4*>(&sc_lds[stage][2][16 * kb + 4 * lr]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] = w[i] == 0.f ? 0.f : w[i] * ratio[i];  // (of a key that is not seen, whatever its scale)
-            }
           }
           pp[x][kb >> 1][(kb & 1) * 2] = H::pack2(w[0], w[1]);
           pp[x][kb >> 1][(kb & 1) * 2 + 1] = H::pack2(w[2], w[3]);
