@@ -9,8 +9,8 @@
 // the zeros of rows that do not use it, would be NaN in them: the products run on zeros in place of such values, and
 // where there were any each output adds those of its own row's adapter (adapter_nonfinite). For the products t is
 // rounded to the operands' type, as the output of a 16-bit layer would be; for fp16, whose range a product of x, A and a scale
-// leaves at either end, as a row's t times a power of two that brings its largest near 2^12 (adapter_range): the row's sums are
-// scaled by it before the adapter's products, and back after them, both exact.
+// leaves at either end, as a row's t times a power of two (adapter_power): the row's sums are scaled by it before the adapter's
+// products, and back after them, both exact. Rows whose t is near 1 take no part in that (with all rows scaled 4096 x 4096 x 4096 took 122 us, 118 so, 115 without any of it).
 //
 // adapter_add_kernel: any types and strides, one workgroup per row: t = scale x A in 32 bits, then
 // out += t B, on an output that holds the projection already (matmul's kernels). A 16-bit output is
@@ -105,18 +105,31 @@ struct AdapterPart {
   long long split_pitch, b_l, b_r, index_stride;  // split_pitch: M rank
   int splits, rank, count;                        // rank % 8 == 0
   PageDiv by_pieces;                              // division by rank / 8
-  const float* tops;                              // fp16: [top_count, M], the largest of a row's sums in each part of them
-  int top_count, rows;                            // rows: M
+  const float* tops;                              // fp16: [M, top_pitch], the largest of a row's sums in each part of them, or 1 (in range)
+  int top_count, top_pitch;                       // adapter_top_pitch(top_count)
 };
+constexpr int kAdapterLowCols = 64;  // columns of t per workgroup, a part
+inline __host__ __device__ int adapter_top_count(int rank, int splits) { return (rank + kAdapterLowCols - 1) / kAdapterLowCols * splits; }
+inline __host__ __device__ int adapter_top_pitch(int count) { return (count + 3) / 4 * 4; }
 template <typename H>
 constexpr bool kAdapterRanged = std::is_same<H, Half16<F16Tag>>::value;
-// The power of two for row m's t: its sums over ranges of K are below 2^12 with it, t, of up to 8 of them, below 2^15. At most 2^60,
-// which the projection's sums bear (of fp16 operands they stay below 2^50); what is smaller then is no fp16 value times any B.
-// Of infinite sums the least, so that finite ones beside them stay finite.
-__device__ __forceinline__ float adapter_range(const AdapterPart& p, int m) {
+// The power of two for row m's t, from the largest of its sums over ranges of K: 1 where that lies within 2^-3..2^12 (t, of up to 8
+// of them, is then below 2^15, and what it loses in subnormal steps less than the sums did in 32 bits), else what brings it to
+// 2^11..2^12. At most 2^60, which the projection's sums bear (of fp16 operands they stay below 2^50); what is smaller then is
+// nothing in fp16, times any B. Of infinite sums the least, so that finite ones beside them stay finite.
+constexpr float kAdapterSmall = 0x1p-3f, kAdapterLarge = 0x1p12f;
+__device__ __forceinline__ float adapter_top(const AdapterPart& p, int m) {
   float top = 0.f;
 #pragma unroll 1
-  for (int i = 0; i < p.top_count; ++i) top = fmaxf(top, p.tops[(long long)i * p.rows + m]);
+  for (int i0 = 0; i0 < p.top_count; i0 += 4) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p.tops + (long long)m * p.top_pitch + i0);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) top = i0 + y < p.top_count ? fmaxf(top, v[y]) : top;
+  }
+  return top;
+}
+__device__ __forceinline__ float adapter_power(float top) {
+  if (top == 0.f || (top >= kAdapterSmall && top < kAdapterLarge)) return 1.f;
   const int exponent = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
   return __builtin_bit_cast(float, (uint32_t)(127 + max(min(11 - exponent, 60), -116)) << 23);
 }
@@ -234,13 +247,25 @@ __device__ __forceinline__ int adapter_slots(const AdapterPart& p, int m0, int M
   return slots;
 }
 
-// fp16: range_lds[i] the power of two of row i (1 without an adapter), after adapter_slots. Every wave writes the same.
-template <int kRows>
-__device__ __forceinline__ void adapter_ranges(const AdapterPart& p, int m0, int lane, const int* row_lds, float* range_lds) {
+// The same and, in fp16, range_lds[i], the power of two of row i (1 without an adapter), and whether there are others than 1.
+template <typename H, int kRows>
+__device__ __forceinline__ int adapter_slots(const AdapterPart& p, int m0, int M, int lane, int* row_lds, int* slot_lds,
+                                             float* range_lds, bool* scaled) {
+  if constexpr (kAdapterRanged<H>) {
+    float power[kRows / 64];
 #pragma unroll
-  for (int u = 0; u < kRows / 64; ++u) {
-    const int i = 64 * u + lane;
-    range_lds[i] = row_lds[i] >= 0 ? adapter_range(p, m0 + i) : 1.f;
+    for (int u = 0; u < kRows / 64; ++u)  // (read ahead of the indexes: a row without an adapter has no value there to keep)
+      power[u] = adapter_top(p, min(m0 + 64 * u + lane, M - 1));
+    const int slots = adapter_slots<kRows>(p, m0, M, lane, row_lds, slot_lds);
+#pragma unroll
+    for (int u = 0; u < kRows / 64; ++u) {
+      power[u] = row_lds[64 * u + lane] >= 0 ? adapter_power(power[u]) : 1.f;
+      range_lds[64 * u + lane] = power[u];
+      *scaled = *scaled || __builtin_amdgcn_ballot_w64(power[u] != 1.f) != 0;
+    }
+    return slots;
+  } else {
+    return adapter_slots<kRows>(p, m0, M, lane, row_lds, slot_lds);
   }
 }
 
@@ -278,7 +303,7 @@ __device__ __forceinline__ void adapter_put(u32x4 x, uint32_t to, uint32_t& foun
 // few. Few rows also share out K over up to eight workgroups: one CU reads some 16 bytes a clock. 16 x 4096, 16 adapters of
 // rank 16: 4-5 us (one workgroup of 16 waves over all of K: 10); 200 x 2048 of rank 64, mixed: 9.6; 4096 x 4096 in runs: 12.6 us,
 // 2.7 TB/s of x.
-constexpr int kAdapterLowThreads = 256, kAdapterLowCols = 64;
+constexpr int kAdapterLowThreads = 256;
 template <typename Tag>
 __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(AdapterArgs a, uint32_t* __restrict__ zeros,
                                                                           float* __restrict__ sums, int splits,
@@ -400,12 +425,18 @@ __global__ __launch_bounds__(kAdapterLowThreads) void adapter_low_kernel(Adapter
         if (users >> (r0 + e) & 1ull) sums[((long long)split * a.m + m0 + r0 + e) * a.rank + c0 + c] = sum[e];
     }
     if constexpr (kAdapterRanged<H>) {
+      const int top_pitch = adapter_top_pitch(gridDim.z * splits);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float top = __builtin_fabsf(sum[e]);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        if (lane == 0 && (users >> (r0 + e) & 1ull)) tops[((long long)split * gridDim.z + blockIdx.z) * a.m + m0 + r0 + e] = top;
+        const bool large = __builtin_amdgcn_ballot_w64(top >= kAdapterLarge) != 0;  // (a NaN is neither)
+        if (large || __builtin_amdgcn_ballot_w64(top >= kAdapterSmall) == 0) {
+#pragma unroll 1
+          for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        } else {
+          top = 1.f;
+        }
+        if (lane == 0 && (users >> (r0 + e) & 1ull)) tops[(long long)(m0 + r0 + e) * top_pitch + split * gridDim.z + blockIdx.z] = top;
       }
     }
   }

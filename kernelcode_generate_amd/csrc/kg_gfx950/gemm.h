@@ -219,12 +219,10 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
 #pragma unroll
       for (int piece = 0; piece < kPieces; ++piece) issue_piece(st, st, piece);
   int slots = 0;
+  bool scaled = false;
   if constexpr (kAdapters) {
     if (tid == 0) found_lds = 0;
-    if (blockIdx.y == 0) {
-      slots = adapter_slots<kTM>(part, m0, M, lane, row_lds, slot_lds);
-      if constexpr (kRanged) adapter_ranges<kTM>(part, m0, lane, row_lds, range_lds);
-    }
+    if (blockIdx.y == 0) slots = adapter_slots<H, kTM>(part, m0, M, lane, row_lds, slot_lds, range_lds, &scaled);
   }
   {
     const int younger = min(kStages - 1, ktiles - 1);
@@ -319,7 +317,7 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
     const int pieces = part.rank / 8, slices = (slots * pieces + 3) / 4;
     uint32_t found = 0;
     if constexpr (kRanged) {
-      if (slots > 0) {
+      if (scaled) {
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           const float to = range_lds[wm * (kTM / 2) + 16 * i + l16];
@@ -364,7 +362,7 @@ __global__ __launch_bounds__(gemmp::kThreads, 1) void gemm_pipe_kernel(
       }
     }
     if constexpr (kRanged) {
-      if (slots > 0) {
+      if (scaled) {
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           const float to = inverse_power(range_lds[wm * (kTM / 2) + 16 * i + l16]);

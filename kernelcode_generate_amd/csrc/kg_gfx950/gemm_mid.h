@@ -144,10 +144,10 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) issue_piece(st, st, p);
   int slots = 0;
+  bool scaled = false;
   if constexpr (kAdapters) {
     if (tid == 0) found_lds = 0;
-    slots = adapter_slots<kT>(part, m0, M, lane, row_lds, slot_lds);
-    if constexpr (kRanged) adapter_ranges<kT>(part, m0, lane, row_lds, range_lds);
+    slots = adapter_slots<H, kT>(part, m0, M, lane, row_lds, slot_lds, range_lds, &scaled);
   }
   {
     const int younger = min(kStages, nk) - 1;
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
     const int pieces = part.rank / 8, slices = (slots * pieces + 7) / 8;
     uint32_t found = 0;
     if constexpr (kRanged) {
-      if (slots > 0) {
+      if (scaled) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float to = range_lds[wm * 64 + 16 * i + l16];
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(gemmm::kThreads, kStages == 2 ? 2 : 1) void gemm_mi
         }
     }
     if constexpr (kRanged) {
-      if (slots > 0) {
+      if (scaled) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float to = inverse_power(range_lds[wm * 64 + 16 * i + l16]);

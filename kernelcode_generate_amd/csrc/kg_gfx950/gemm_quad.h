@@ -190,10 +190,10 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
 #pragma unroll
       for (int piece = 0; piece < kPieces; ++piece) issue_piece(st, st, piece);
   int slots = 0;
+  bool scaled = false;
   if constexpr (kAdapters) {
     if (tid == 0) found_lds = 0;
-    slots = adapter_slots<kTM>(part, m0, M, lane, row_lds, slot_lds);
-    if constexpr (kRanged) adapter_ranges<kTM>(part, m0, lane, row_lds, range_lds);
+    slots = adapter_slots<H, kTM>(part, m0, M, lane, row_lds, slot_lds, range_lds, &scaled);
   }
   {
     const int younger = min(kStages - 1, ktiles - 1);
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
     const int pieces = part.rank / 8, slices = (slots * pieces + 3) / 4;
     uint32_t found = 0;
     if constexpr (kRanged) {
-      if (slots > 0) {
+      if (scaled) {
         mfma_drain();
 #pragma unroll
         for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
@@ -359,8 +359,10 @@ __global__ __launch_bounds__(gemmq::kThreads, 1) void gemm_quad_kernel(
         const int n = n0 + wn * 128 + j * 16 + 4 * lg;
         float v0 = acc[i][j][0], v1 = acc[i][j][1], v2 = acc[i][j][2], v3 = acc[i][j][3];
         if constexpr (kRanged) {
-          const float back = inverse_power(range_lds[wm * WM + 16 * i + l16]);
-          v0 *= back, v1 *= back, v2 *= back, v3 *= back;
+          if (scaled) {
+            const float back = inverse_power(range_lds[wm * WM + 16 * i + l16]);
+            v0 *= back, v1 *= back, v2 *= back, v3 *= back;
+          }
         }
         if constexpr (kBias == 1) {
           const float* bp = static_cast<const float*>(bias);

@@ -214,6 +214,8 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
 
   if constexpr (kAdapters) {
     // lane s: the s-th distinct adapter of the block's rows
+    float top = 0.f;  // (its reads do not wait for the index)
+    if constexpr (kAdapterRanged<Half16<Tag>>) top = adapter_top(part, m0 + min(lane, rows - 1));
     int own = lane < kRows && lane < rows ? part.index[(long long)(m0 + lane) * part.index_stride] : -1;
     if (own >= part.count) own = -1;
     int of_row[kMT], listed = -1, slots = 0;
@@ -221,21 +223,24 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
     for (int i = 0; i < kMT; ++i) of_row[i] = __shfl(own, 16 * i + l16, 64);
     constexpr bool kRanged = kAdapterRanged<Half16<Tag>>;
     float range = 1.f, range_of[kMT];  // of row `lane`, of this lane's rows of t
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) range_of[i] = 1.f;
+    bool scaled = false;
     if constexpr (kRanged) {
-      if (own >= 0) range = adapter_range(part, m0 + lane);
+      if (own >= 0) range = adapter_power(top);
+      scaled = __builtin_amdgcn_ballot_w64(range != 1.f) != 0;
+      if (scaled) {
 #pragma unroll
-      for (int i = 0; i < kMT; ++i) {
-        range_of[i] = __shfl(range, 16 * i + l16, 64);
+        for (int i = 0; i < kMT; ++i) {
+          range_of[i] = __shfl(range, 16 * i + l16, 64);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float to = __shfl(range, 16 * i + 4 * lg + e, 64);
-          acc[i][0][e] *= to;
-          acc[i][1][e] *= to;
+          for (int e = 0; e < 4; ++e) {
+            const float to = __shfl(range, 16 * i + 4 * lg + e, 64);
+            acc[i][0][e] *= to;
+            acc[i][1][e] *= to;
+          }
         }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kMT; ++i) range_of[i] = 1.f;
     }
     for (unsigned long long left = __builtin_amdgcn_ballot_w64(own >= 0); left != 0; ++slots) {
       const int l = __builtin_amdgcn_readlane(own, __builtin_ctzll(left));
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(gemms::kWaves * 64) void gemm_skinny_kernel(
           }
       }
     }
-    if constexpr (kRanged) {
+    if (scaled) {
 #pragma unroll
       for (int i = 0; i < kMT; ++i)
 #pragma unroll

@@ -1634,8 +1634,8 @@ struct AdapterPlan {
   int low_splits;  // of t's K
   size_t low_bytes, bytes;
 };
-// 32-bit values of a row and range of K: its sums, and the largest of every kAdapterLowCols.
-long long adapter_low_sums(long long rank) { return rank + cdiv(rank, kAdapterLowCols); }
+// 32-bit values of a row: its sums over ranges of K, and the largest of each part of them.
+long long adapter_low_sums(int rank, int splits) { return (long long)splits * rank + adapter_top_pitch(adapter_top_count(rank, splits)); }
 AdapterPlan adapter_plan(const AdapterArgs& p) {
   const long long M = p.m, N = p.n, K = p.k;
   AdapterPlan a{AdapterPlan::kPipe, pipe_tile_m(M, N), K, 1, 1, 1, 0, 0};
@@ -1644,7 +1644,7 @@ AdapterPlan adapter_plan(const AdapterArgs& p) {
   // 64 k for each of a workgroup's four waves at least, and some two workgroups a compute unit: more splits are more
   // sums for every reader (1024 workgroups: 256 x 4096 x 4096 47 us, 512: 41, 256: 39; x 512 rows in runs 39, 40, 43)
   a.low_splits = (int)std::max(1ll, std::min(std::min<long long>(K / 256, kAdapterMaxSplits), 512 / (low * a.at_once)));
-  a.low_bytes = (size_t)cdiv(kAdapterHeader + a.low_splits * M * adapter_low_sums(p.rank) * 4, 256) * 256;
+  a.low_bytes = (size_t)cdiv(kAdapterHeader + M * adapter_low_sums(p.rank, a.low_splits) * 4, 256) * 256;
   if (adapter_skinny_pays(M, N, K) && cdiv(M, 16) * cdiv(N, gemms::kCols) <= kMostBlocks * 4 / gemms::kWaves) {
     a.form = AdapterPlan::kSkinny;
   } else if (gemm_mid_pays(M, N, K)) {
@@ -1676,7 +1676,7 @@ int launch_adapter_matmul(const AdapterArgs& p, const AdapterPlan& plan, int bia
                      dim3(kAdapterLowThreads), 0, g_stream, p, reinterpret_cast<uint32_t*>(ws), sums, plan.low_splits, tops);
   const AdapterPart part{sums, reinterpret_cast<const uint16_t*>(ws), static_cast<const uint16_t*>(p.b), p.index, (long long)p.m * p.rank,
                          p.b_l, p.b_r, p.index_stride, plan.low_splits, p.rank, p.count, page_div(p.rank / 8), tops,
-                         plan.low_splits * (int)cdiv(p.rank, kAdapterLowCols), p.m};
+                         adapter_top_count(p.rank, plan.low_splits), adapter_top_pitch(adapter_top_count(p.rank, plan.low_splits))};
   const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.w);
   uint16_t* out = static_cast<uint16_t*>(p.out);
   hipError_t e = hipSuccess;
@@ -1760,7 +1760,7 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
                     cdiv(std::min(M, 1ll << 21), 128) * cdiv(N, gemmp::kBN) <= kMostBlocks / 2;  // (workgroups of 512, of a piece's rows)
   if (mfma) {
     // pieces of whole 256-row tiles whose sums fit the workspace (262144 rows of rank 64: two)
-    const long long most = ((long long)kSplitMaxWorkspace - kAdapterHeader - 256) / (adapter_low_sums(rank) * 4) / 256 * 256;
+    const long long most = ((long long)kSplitMaxWorkspace - kAdapterHeader - 256) / (adapter_low_sums((int)rank, 1) * 4) / 256 * 256;
     const long long rows = cdiv(cdiv(M, cdiv(M, most)), 256) * 256;
     auto piece = [&](long long m0) {
       AdapterArgs part = p;
