@@ -176,7 +176,8 @@ int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long 
  * out[m] = x[m] weight + bias + scale[l] (x[m] a[l]) b[l], l = index[m]; an index outside 0 .. L - 1 is a row without an
  * adapter; an absent scale is 1. dtypes as matmul's, a and b the operands'. R <= 512. Adapters of unequal
  * rank are padded with zeros. out must not overlap an operand. Sums are held in 32 bits; 16-bit calls round scale[l] (x[m] a[l]) to
- * their type for its product with b (f16: times a power of two for each row, so that none of it leaves the type's range at the top),
+ * their type for its product with b (f16: times a power of two where a row's largest is not near 1, so that none of it leaves the
+ * type's range at the top and what is small is off by at most 2^-22 of the largest),
  * or, where rows are not whole 16-byte pieces, the projection before the adapter's part is added.
  */
 int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);

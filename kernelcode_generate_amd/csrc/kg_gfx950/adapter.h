@@ -10,7 +10,8 @@
 // where there were any each output adds those of its own row's adapter (adapter_nonfinite). For the products t is
 // rounded to the operands' type, as the output of a 16-bit layer would be; for fp16, whose range a product of x, A and a scale
 // leaves at either end, as a row's t times a power of two (adapter_power): the row's sums are scaled by it before the adapter's
-// products, and back after them, both exact. Rows whose t is near 1 take no part in that (with all rows scaled 4096 x 4096 x 4096 took 122 us, 118 so, 115 without any of it).
+// products, and back after them, both exact. Rows whose t is near 1 take no part in that (4096 x 4096 x 4096 with all rows
+// scaled 122 us, so 118, without any of it 115).
 //
 // adapter_add_kernel: any types and strides, one workgroup per row: t = scale x A in 32 bits, then
 // out += t B, on an output that holds the projection already (matmul's kernels). A 16-bit output is
@@ -114,8 +115,8 @@ inline __host__ __device__ int adapter_top_pitch(int count) { return (count + 3)
 template <typename H>
 constexpr bool kAdapterRanged = std::is_same<H, Half16<F16Tag>>::value;
 // The power of two for row m's t, from the largest of its sums over ranges of K: 1 where that lies within 2^-3..2^12 (t, of up to 8
-// of them, is then below 2^15, and what it loses in subnormal steps less than the sums did in 32 bits), else what brings it to
-// 2^11..2^12. At most 2^60, which the projection's sums bear (of fp16 operands they stay below 2^50); what is smaller then is
+// of them, is then below 2^15, and its small values are off by half a subnormal step, 2^-22 of the largest, at most), else what
+// brings it to 2^11..2^12. At most 2^60, which the projection's sums bear (of fp16 operands they stay below 2^50); what is smaller then is
 // nothing in fp16, times any B. Of infinite sums the least, so that finite ones beside them stay finite.
 constexpr float kAdapterSmall = 0x1p-3f, kAdapterLarge = 0x1p12f;
 __device__ __forceinline__ float adapter_top(const AdapterPart& p, int m) {

@@ -62,7 +62,7 @@ template <typename T, typename C>
 __global__ __launch_bounds__(256) void tree_attn_any_kernel(TreeArgs a) {
   constexpr int kThreads = 256, kMaxD = 512;
   __shared__ float qs[kMaxD];
-  __shared__ float ps[kThreads];  // weights of a block of keys; negative: not seen
+  __shared__ float ps[kThreads];  // weights of a block of keys, times the values' scales
   __shared__ long long rows[kThreads];
   __shared__ float red[kThreads / 64];
   const int tid = threadIdx.x;

@@ -18,7 +18,9 @@
 // maximum is of s + log2(value's scale): weights of at most 2^8, whatever the scales' sizes. The sum of weights, which has no scales
 // in it, stays in 32 bits, so the scale that counts there lies within 2^-80..2^80 (ValueScale).
 //
-// Weights of 16-bit caches are rounded to 16 bits, as in the flash attention kernels, and summed as rounded.
+// Weights of 16-bit caches are rounded to 16 bits, as in the flash attention kernels, and summed as rounded. The matrix instructions
+// take them in the values' type: a second product with what rounding leaves would double that half of the work, for an error
+// of half a step a weight, which the output's own rounding has too.
 #pragma once
 
 #include <type_traits>

@@ -1615,7 +1615,12 @@ int tree_attention_impl(const KgArgSlot* args, unsigned long long n) {
 }
 
 // Few rows, whose adapters the 32-row blocks of gemm_skinny_kernel share with fewer others than 128-row tiles do, and
-// whose K no other form splits here. ns by a model of both: a round of blocks takes 3 per k, a round of tiles 450 per 64.
+// whose K no other form splits here. ns by a model of both: a round of blocks takes 3 per k, a round of tiles 450 per 64. us, blocks /
+// tiles, 16 adapters of rank 16 in mixed rows of 4096 x 4096: 64 rows 23 / 50, 128 34 / 48, 192 (from where the model takes
+// tiles) 47 / 44, 256 58 / 46, 512 110 / 53; 8192 x 2048 in runs of 4: 128 rows 32 / 41, 256 52 / 39 (the model still takes
+// blocks), 384 74 / 45. The number of adapters that meet in a tile is not known here and not in the model: 64 mixed ones of
+// rank 16, 2048 x 2048, 256 rows 27 / 63, 384 37 / 60, 512 46 / 60, of which the last two take tiles all the same; past 512 rows
+// 67 / 65.
 bool adapter_skinny_pays(long long M, long long N, long long K) {
   if (gemm_skinny_pays(M, N, K, false, true, true)) return true;
   if (M > 512 || K < 64 || N < gemms::kCols) return false;
