@@ -165,9 +165,11 @@ int kg_gfx950_kv_cache_load_entry(const KgArgSlot* ordered_args, unsigned long l
  * at positions context_lens[b] + j. Token j sees positions below context_lens[b] and those drafted tokens i whose
  * bit i % 64 of mask[starts[b] + j, i / 64] is set (bits past the request's tokens say nothing); without a mask,
  * i <= j: a decoding step (one token), a chain of drafts, a piece of a prompt. Query head h reads key head h / (Hq / heads).
- * Rows that see nothing get zeros; rows of no request are left as they are. Positions past P * page_size and
+ * Rows that see nothing, or nothing but scores of -infinity, get zeros; rows of no request are left as they are. Positions past P * page_size and
  * pages outside 0 .. pages - 1 are not seen. What is not seen has no influence, infinities and NaN included. q, out:
  * f32, f16 or bf16; of a cache that is not in 8 bits, its type. P * page_size <= 2^31 - 4096. out must not overlap q.
+ * Scores, softmax statistics and sums are held in 32 bits; with f16 or bf16 q and out the weights may be rounded to that type for their
+ * products with the values (of 8-bit caches with the value's scale in them).
  */
 int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
 

@@ -302,7 +302,7 @@ __device__ __forceinline__ void adapter_put(u32x4 x, uint32_t to, uint32_t& foun
 // as pairs straight into operands, eight loads a step, twice as long.) A workgroup takes every gridDim.y-th of its rows' distinct
 // adapters and stores the rows that use it: few rows have many adapters (gridDim.y workgroups read them at once), many rows
 // few. Few rows also share out K over up to eight workgroups: one CU reads some 16 bytes a clock. 16 x 4096, 16 adapters of
-// rank 16: 4-5 us (one workgroup of 16 waves over all of K: 10); 200 x 2048 of rank 64, mixed: 9.6; 4096 x 4096 in runs: 12.6 us,
+// rank 16: 4-5 us (one workgroup of 16 waves over all of K: 10); 200 x 2048 of rank 64, mixed: 10.6; 4096 x 4096 in runs: 12.6-13.4 us,
 // 2.7 TB/s of x.
 constexpr int kAdapterLowThreads = 256;
 template <typename Tag>

@@ -8,7 +8,7 @@
 // rounded once to the output's type.
 //
 // kv_store_kernel, kv_load_kernel: rows of whole 16-byte pieces (8 elements a lane), bound by their bytes where there are many:
-// 4001 tokens of 8 heads of 128 from fp16 to int8 9.0 us, 2.7 TB/s (28 with a wave per row); four ragged sequences of up to 8192
+// 4001 tokens of 8 heads of 128 from fp16 to int8 8.7 us, 2.7 TB/s (28 with a wave per row); four ragged sequences of up to 8192
 // back from e4m3 to bf16 34.8 us, 4.1 TB/s (169). 64 tokens take 3.0 us, a launch's. kv_store_any_kernel, kv_load_any_kernel:
 // any D and alignment and any number of rows, one wave per row.
 #pragma once

@@ -8,11 +8,11 @@
 // (16-byte chunk c of row r at c ^ (r % 16): 16 rows hit distinct banks), V^T fragments two ds_read_b64_tr_b16 per 16 d x 32
 // keys in the key order that P's lanes hold (chunk pairs at pair ^ (r % 8): the 8 rows of half a wave do).
 //
-// Measured, heads of 128 in 8 groups of 4: 2 x 512 rows behind 4096 in bf16 136 us with the join, 538 TFLOP/s (674 behind
-// 16384); with rows through registers, which spilled, and a loop over the keys of tiles with drafts, 185. Two waves a SIMD
+// Measured, heads of 128 in 8 groups of 4: 2 x 512 rows behind 4096 in bf16 127 us a call with the join, 575 TFLOP/s (740
+// behind 16384); with rows through registers, which spilled, and a loop over the keys of tiles with drafts, 185. Two waves a SIMD
 // issue vector instructions for 3000 of the 6500 cycles that two tiles of 128 rows take, MFMAs fill 2200, reads of LDS 2000: a
 // tile's scores taken under the exponentials of the one before (33 registers more, spilled) took 151. 8 x 16 rows behind
-// 16384: bf16 115 us, 4.7 TB/s of rows; e4m3 96 us, bound by each wave's chain of widening, products and softmax, not by bytes (two
+// 16384: bf16 115 us, 4.7 TB/s of rows; e4m3 94-98 us, bound by each wave's chain of widening, products and softmax, not by bytes (two
 // tiles in flight: 6 % longer; eight waves with half the keys each, in 128 registers: 56 %).
 #pragma once
 
