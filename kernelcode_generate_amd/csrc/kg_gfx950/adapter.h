@@ -116,7 +116,7 @@ template <typename H>
 constexpr bool kAdapterRanged = std::is_same<H, Half16<F16Tag>>::value;
 // The power of two for row m's t, from the largest of its sums over ranges of K: 1 where that lies within 2^-3..2^12 (t, of up to 8
 // of them, is then below 2^15, and its small values are off by half a subnormal step, 2^-22 of the largest, at most), else what
-// brings it to 2^11..2^12. At most 2^60, which the projection's sums bear (of fp16 operands they stay below 2^50); what is smaller then is
+// brings it to 2^11..2^12. At most 2^60, which the projection's sums bear (of fp16 operands they stay below 2^54); what is smaller then is
 // nothing in fp16, times any B. Of infinite sums the least, so that finite ones beside them stay finite.
 constexpr float kAdapterSmall = 0x1p-3f, kAdapterLarge = 0x1p12f;
 __device__ __forceinline__ float adapter_top(const AdapterPart& p, int m) {
