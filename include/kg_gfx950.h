@@ -52,7 +52,8 @@ enum {
 
 /* dtype codes 1-4 are the reference's (runtime_args.py:94-110, common.py:171-194);
  * 5 (float16) and 6 (bfloat16) are additive extensions for the gfx950 MFMA paths, 7 (int8) and
- * 8 (float8 e4m3fn) for the caches of the serving entries, the only ones that take them. */
+ * 8 (float8 e4m3fn) for the serving entries, the only ones that take them: caches, and (int8) the codes of
+ * quantize_rows and int8_matmul. */
 enum {
   KG_DTYPE_F32 = 1,
   KG_DTYPE_F64 = 2,
@@ -183,6 +184,57 @@ int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long 
  * or, where rows are not whole 16-byte pieces, the projection before the adapter's part is added.
  */
 int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (slots[T] i64, positions[T] i32, starts[B + 1] i32, page_table[B, P] i32, free_pages[F] i32, free_count[1] i32,
+ *  context_lens[B] i32, new_lens[B] i32, page_size INT)
+ * Pages and slots of a step's new tokens. Request b has context_lens[b] cached tokens and new_lens[b] new ones (below 0: none), the rows
+ * starts[b] .. starts[b + 1] - 1 of the batch; what passes T rows is cut off. Row starts[b] + i gets position context_lens[b] + i
+ * and the slot that kv_cache_store takes: page_table[b, position / page_size] * page_size + position % page_size. The rows behind the
+ * last request's get -1 in both. A page that begins with a new token is taken from free_pages, a stack of *free_count pages with the
+ * last one on top, in the order of requests and positions, and entered in page_table; -1 where none is left, and such
+ * tokens, as those behind P pages, get slot -1. *free_count is then what is left (values outside 0 .. F count as the nearest).
+ * B <= 8192. page_table, starts, slots and positions are what kv_cache_store, head_norm_rotate and tree_attention take.
+ * No two of the tensors may overlap. The call reads what it writes: a recorded graph takes new pages on every replay.
+ */
+int kg_gfx950_kv_cache_assign_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (page_table[B, P] i32, free_pages[F] i32, free_count[1] i32, keep_lens[B] i32, held_lens[B] i32, page_size INT)
+ * Gives back the pages of request b that its first keep_lens[b] tokens do not need, of those for held_lens[b] tokens: all of them
+ * (keep 0) where the request ends, the last ones where drafted tokens are rejected. They are put on the stack in reverse
+ * order, so that giving back what a call of kv_cache_assign took leaves the stack as it was, and are -1 in page_table. Entries below 0
+ * are passed over; pages past F on the stack are dropped. A page that stands in two entries is given back twice.
+ */
+int kg_gfx950_kv_cache_release_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (codes[M, K] i8, scale[M] f32, x[M, K])
+ * Rows in 8-bit integers: scale = max|x| * fl32(1 / 127), code = x / scale as a 32-bit quotient, rounded to nearest, ties to even,
+ * -127 .. 127; 0 where the scale is 0 or not finite (a row with an infinity or NaN has that scale). x: f32, f16, bf16. What
+ * int8_matmul takes, as its rows or as its weights.
+ */
+int kg_gfx950_quantize_rows_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (out[M, N], x[M, K], x_scale[M] f32 | absent, weight[N, K] i8, w_scale[N] f32, bias[N] | absent)
+ * out[m, n] = (sum_k x[m, k] weight[n, k]) * x_scale[m] * w_scale[n] + bias[n], one row of weight a channel. x: i8, or of out's type
+ * (f32, f16, bf16) without x_scale, and then taken as quantize_rows' codes and scales. The sums are exact (any codes, -128 included;
+ * K <= 131071), and a 32-bit float from there on, rounded once to out's type. bias: f32 or out's type. out must not overlap an operand.
+ */
+int kg_gfx950_int8_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
+
+/*
+ * (q_out[T, Hq, D], k_out[T, Hk, D], q[T, Hq, D], k[T, Hk, D], q_weight[D] | absent, k_weight[D] | absent, cos[S, R] f32, sin[S, R] f32,
+ *  positions[T] i32 or i64, eps FLOAT, neighbours INT)
+ * Norms of queries and keys for each head, with the position rotation: y = x / sqrt(mean x^2 + eps) * weight (a side without weights is
+ * rotated alone), then pair i < R of y turns by the angle of cos and sin's row positions[t]: elements i and i + R (neighbours 0), or
+ * 2 i and 2 i + 1 (neighbours 1); the elements behind 2 R <= D stay. A token with a position outside 0 .. S - 1 (-1, say) is left as it
+ * is in the outputs. q, k and the outputs: f32, f16 or bf16, weights of that type or f32; 32 bits throughout, one rounding at the end; a
+ * row whose sum of squares leaves 32 bits is 0 (NaN at infinities). D 1..512. An output may be its own input (the
+ * same view), and must not overlap anything else.
+ */
+int kg_gfx950_head_norm_rotate_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
 
 /*
  * Launch control (no counterpart in the reference, whose execute() is synchronous and

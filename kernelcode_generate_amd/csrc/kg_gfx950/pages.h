@@ -1,0 +1,186 @@
+// Pages and slots of a step's new tokens in the paged cache (kv_cache.h), found on the GPU from the requests' lengths, and the
+// pages that a request gives back. Request b has c = context[b] cached tokens and n = added[b] new ones; its new tokens are
+// the batch's rows starts[b] .. starts[b + 1] - 1, starts the running sums of n, cut where they pass the batch. Row starts[b] + i:
+//   position c + i, page p = position / page_size of the request, slot = table[b, p] page_size + position % page_size.
+// Free pages are a stack, `count` of them, the next one on top. New pages p of ceil(c / page_size) .. ceil((c + n) / page_size) - 1
+// are taken in the order of requests and pages, the i-th of all of them free[count - 1 - i], none (-1) once the stack is empty.
+// Pages that go back, of ceil(keep / page_size) .. ceil(held / page_size) - 1, are put on the stack the last one first, so that
+// giving back what a call took leaves the stack as it was.
+//
+// Each kernel is one workgroup: a call of some thousand tokens is a chain of a few dependent reads (lengths, a search for a row's
+// request in LDS, its page), which more workgroups do not shorten, and only one workgroup can take from the stack and write what is
+// left of it without a second launch.
+#pragma once
+
+#include "common.h"
+#include "kv_cache.h"
+
+namespace kg_gfx950 {
+
+constexpr int kPagesThreads = 1024;
+constexpr int kPagesMostRequests = 8192;  // their sums lie in LDS
+
+struct PagesArgs {
+  long long* slots;
+  int *positions, *starts, *table, *free, *count;
+  const int *context, *added;  // release: keep, held
+  long long slot_stride, position_stride, start_stride, table_0, table_1, free_stride, context_stride, added_stride;
+  int batch, per, tokens, page_size, stack;
+  PageDiv div;
+};
+
+// ceil(tokens / page_size), of pages that the table has
+__device__ __forceinline__ int pages_of(int tokens, const PagesArgs& a) {
+  return tokens <= 0 ? 0 : min(div_page(tokens - 1, a.div) + 1, a.per);
+}
+
+// Sums of values up to each thread's, the workgroup's total in *total; a sum is at most `most` (values are, and most < 2^31).
+template <bool kCut>
+__device__ __forceinline__ int pages_scan(int v, int most, int* lds, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto add = [&](int x, int y) __attribute__((always_inline)) {
+    return kCut ? (int)min((uint32_t)x + (uint32_t)y, (uint32_t)most) : x + y;
+  };
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(v, o, 64);
+    if (lane >= o) v = add(v, x);
+  }
+  __syncthreads();  // (the sums of the call before are read)
+  if (lane == 63) lds[wave] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPagesThreads / 64; ++w) {
+    const int x = lds[w];
+    if (w < wave) before = add(before, x);
+    all = add(all, x);
+  }
+  *total = all;
+  return add(v, before);
+}
+
+// The last of sums[0 .. batch] that is at most x: a row's request, which has rows.
+__device__ __forceinline__ int pages_owner(const int* sums, int batch, int x) {
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a) {
+  __shared__ int row_of[kPagesMostRequests + 1], fresh_of[kPagesMostRequests];  // first rows, first of all new pages
+  __shared__ int scan[kPagesThreads / 64];
+  const int tid = threadIdx.x;
+  const int count = max(min(*a.count, a.stack), 0);
+  int rows = 0, fresh = 0;  // of the requests before
+  for (int b0 = 0; b0 < a.batch; b0 += kPagesThreads) {
+    const int b = b0 + tid;
+    const bool real = b < a.batch;
+    const int c = real ? max(a.context[b * a.context_stride], 0) : 0;
+    const int n = real ? min(max(a.added[b * a.added_stride], 0), a.tokens) : 0;
+    int all;
+    const int upto = min((int)min((uint32_t)pages_scan<true>(n, a.tokens, scan, &all) + (uint32_t)rows, (uint32_t)a.tokens), a.tokens);
+    const int before = __shfl_up(upto, 1, 64);
+    // the sum before, of another wave: found by the same cut sums
+    __shared__ int last_of[kPagesThreads / 64];
+    if ((tid & 63) == 63) last_of[tid >> 6] = upto;
+    __syncthreads();
+    const int first = (tid & 63) != 0 ? before : tid == 0 ? rows : last_of[(tid >> 6) - 1];
+    const int kept = upto - first;
+    // tokens past 2^31 - 1 have no page
+    const int end = (int)min((uint32_t)c + (uint32_t)kept, 0x7fffffffu);
+    const int pages = pages_of(end, a) - pages_of(c, a);
+    int new_pages;
+    const int pages_upto = pages_scan<false>(pages, 0, scan, &new_pages);
+    if (real) {
+      row_of[b] = first;
+      fresh_of[b] = fresh + pages_upto - pages;
+      a.starts[b * a.start_stride] = first;
+    }
+    rows = (int)min((uint32_t)rows + (uint32_t)all, (uint32_t)a.tokens);
+    fresh += new_pages;
+  }
+  if (tid == 0) {
+    row_of[a.batch] = rows;
+    a.starts[a.batch * a.start_stride] = rows;
+    *a.count = count - min(fresh, count);
+  }
+  __syncthreads();
+  for (int t = tid; t < a.tokens; t += kPagesThreads) {
+    long long slot = -1;
+    int position = -1;
+    if (t < rows) {
+      const int b = pages_owner(row_of, a.batch, t);
+      const int c = max(a.context[b * a.context_stride], 0);
+      const uint32_t at = (uint32_t)c + (uint32_t)(t - row_of[b]);
+      position = (int)min(at, 0x7fffffffu);
+      if (at < 0x7fffffffu) {
+        const int p = div_page(position, a.div), offset = position - p * a.page_size;
+        if (p < a.per) {
+          const int held = pages_of(c, a);
+          int page;
+          int* entry = a.table + b * a.table_0 + p * a.table_1;
+          if (p < held) {
+            page = *entry;
+          } else {
+            const int i = fresh_of[b] + p - held;
+            page = i < count ? a.free[(count - 1 - i) * a.free_stride] : -1;
+            if (offset == 0) *entry = page;  // (each new page's first token is one of the call's)
+          }
+          if (page >= 0) slot = (long long)page * a.page_size + offset;
+        }
+      }
+    }
+    a.slots[t * a.slot_stride] = slot;
+    a.positions[t * a.position_stride] = position;
+  }
+}
+
+__global__ __launch_bounds__(kPagesThreads) void kv_release_kernel(PagesArgs a) {
+  __shared__ int entry_of[kPagesMostRequests];  // entries of the requests before
+  __shared__ int scan[kPagesThreads / 64];
+  const int tid = threadIdx.x;
+  const int count = max(min(*a.count, a.stack), 0);
+  int entries = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kPagesThreads) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < a.batch) n = max(pages_of(a.added[b * a.added_stride], a) - pages_of(a.context[b * a.context_stride], a), 0);
+    int all;
+    const int upto = pages_scan<false>(n, 0, scan, &all);
+    if (b < a.batch) entry_of[b] = entries + upto - n;
+    entries += all;
+  }
+  __syncthreads();
+  // how many of them are pages
+  auto entry = [&](int e) __attribute__((always_inline)) {
+    const int b = pages_owner(entry_of, a.batch, e);
+    const int p = pages_of(a.context[b * a.context_stride], a) + e - entry_of[b];
+    return a.table + b * a.table_0 + p * a.table_1;
+  };
+  int found = 0;
+  for (int e = tid; e < entries; e += kPagesThreads) found += *entry(e) >= 0;
+  int pages;
+  pages_scan<false>(found, 0, scan, &pages);
+  int before = 0;
+  for (int e0 = 0; e0 < entries; e0 += kPagesThreads) {
+    const int e = e0 + tid;
+    int* at = e < entries ? entry(e) : nullptr;
+    const int page = at != nullptr ? *at : -1;
+    int all;
+    const int upto = before + pages_scan<false>(page >= 0, 0, scan, &all);
+    before += all;
+    if (page >= 0) {
+      const int spot = count + pages - upto;
+      if (spot < a.stack) a.free[spot * a.free_stride] = page;
+    }
+    if (at != nullptr) *at = -1;
+  }
+  if (tid == 0) *a.count = min(count + pages, a.stack);
+}
+
+}  // namespace kg_gfx950

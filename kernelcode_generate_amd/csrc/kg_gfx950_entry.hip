@@ -22,6 +22,7 @@
 #include "kg_gfx950/flash_attn.h"
 #include "kg_gfx950/gemm.h"
 #include "kg_gfx950/gemm_f32.h"
+#include "kg_gfx950/gemm_i8.h"
 #include "kg_gfx950/gemm_mid.h"
 #include "kg_gfx950/gemm_packed.h"
 #include "kg_gfx950/gemm_skinny.h"
@@ -32,7 +33,10 @@
 #include "kg_gfx950/flash_attn_mfma.h"
 #include "kg_gfx950/flash_attn_decode.h"
 #include "kg_gfx950/flash_attn_f32.h"
+#include "kg_gfx950/head_norm.h"
 #include "kg_gfx950/kv_cache.h"
+#include "kg_gfx950/pages.h"
+#include "kg_gfx950/quantize.h"
 #include "kg_gfx950/tree_attn.h"
 #include "kg_gfx950/instances.h"  // the heavy kernel families are compiled in their own translation units
 
@@ -1815,6 +1819,260 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   });
 }
 
+// ---------------------------------------------------------------------------------------
+// serving: pages and slots of a step, rows and products in 8-bit integers, norms of heads with rotation
+// ---------------------------------------------------------------------------------------
+
+constexpr unsigned kI32 = 1u << KG_DTYPE_I32, kI64 = 1u << KG_DTYPE_I64, kF32 = 1u << KG_DTYPE_F32, kI8 = 1u << KG_DTYPE_I8;
+
+// The page table, the stack of free pages and the requests' two lengths, from slot `at` on.
+struct PagesSlots {
+  Mem table, free, count, first, second;
+  long long page_size = 0;
+};
+
+int read_pages(const KgArgSlot* args, int at, const char* op, const char* first, const char* second, PagesSlots* p) {
+  int rc;
+  if ((rc = read_view(args, at, 2, kI32, false, "page_table", &p->table))) return rc;
+  if ((rc = read_view(args, at + 1, 1, kI32, false, "free_pages", &p->free))) return rc;
+  if ((rc = read_view(args, at + 2, 1, kI32, false, "free_count", &p->count))) return rc;
+  if ((rc = read_view(args, at + 3, 1, kI32, false, first, &p->first))) return rc;
+  if ((rc = read_view(args, at + 4, 1, kI32, false, second, &p->second))) return rc;
+  if ((rc = read_int(args, at + 5, "page_size", &p->page_size))) return rc;
+  const long long batch = p->table.shape[0];
+  if (p->count.shape[0] != 1) return fail(kInvalid, "%s: free_count must have one value, got %lld", op, p->count.shape[0]);
+  if (p->first.shape[0] != batch || p->second.shape[0] != batch)
+    return fail(kInvalid, "%s: %s and %s must have a value for each of %lld requests", op, first, second, batch);
+  if (p->page_size < 1 || p->page_size > 0x7fffffffLL) return fail(kInvalid, "%s: page_size %lld not in 1..2^31-1", op, p->page_size);
+  if (batch > kPagesMostRequests) return fail(kUnsupported, "%s: %lld requests > %d", op, batch, kPagesMostRequests);
+  if (batch * p->table.shape[1] > 0x7fffffffLL) return fail(kUnsupported, "%s: page_table of more than 2^31-1 entries", op);
+  return kOk;
+}
+
+int check_pages(const PagesSlots& p, const char* first, const char* second) {
+  int rc;
+  if ((rc = check_view(p.table, "page_table")) || (rc = check_view(p.free, "free_pages")) || (rc = check_view(p.count, "free_count")) ||
+      (rc = check_view(p.first, first)))
+    return rc;
+  return check_view(p.second, second);
+}
+
+PagesArgs pages_args(const PagesSlots& p) {
+  PagesArgs a{};
+  a.table = static_cast<int*>(p.table.data);
+  a.free = static_cast<int*>(p.free.data);
+  a.count = static_cast<int*>(p.count.data);
+  a.context = static_cast<const int*>(p.first.data);
+  a.added = static_cast<const int*>(p.second.data);
+  a.table_0 = p.table.stride[0];
+  a.table_1 = p.table.stride[1];
+  a.free_stride = p.free.stride[0];
+  a.context_stride = p.first.stride[0];
+  a.added_stride = p.second.stride[0];
+  a.batch = (int)p.table.shape[0];
+  a.per = (int)p.table.shape[1];
+  a.page_size = (int)p.page_size;
+  a.stack = (int)p.free.shape[0];
+  a.div = page_div((int)p.page_size);
+  return a;
+}
+
+int kv_cache_assign_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 9) return fail(kInvalid, "kv_cache_assign expects 9 slots, got %llu", n);
+  Mem slots, positions, starts;
+  PagesSlots p;
+  int rc;
+  if ((rc = read_view(args, 0, 1, kI64, false, "slots", &slots))) return rc;
+  if ((rc = read_view(args, 1, 1, kI32, false, "positions", &positions))) return rc;
+  if ((rc = read_view(args, 2, 1, kI32, false, "starts", &starts))) return rc;
+  if ((rc = read_pages(args, 3, "kv_cache_assign", "context_lens", "new_lens", &p))) return rc;
+  const long long tokens = slots.shape[0], batch = p.table.shape[0];
+  if (positions.shape[0] != tokens)
+    return fail(kInvalid, "kv_cache_assign: %lld positions for %lld slots", positions.shape[0], tokens);
+  if (starts.shape[0] != batch + 1)
+    return fail(kInvalid, "kv_cache_assign: starts must have %lld values, got %lld", batch + 1, starts.shape[0]);
+  if ((rc = check_view(slots, "slots")) || (rc = check_view(positions, "positions")) || (rc = check_view(starts, "starts")) ||
+      (rc = check_pages(p, "context_lens", "new_lens")))
+    return rc;
+  PagesArgs a = pages_args(p);
+  a.slots = static_cast<long long*>(slots.data);
+  a.positions = static_cast<int*>(positions.data);
+  a.starts = static_cast<int*>(starts.data);
+  a.slot_stride = slots.stride[0];
+  a.position_stride = positions.stride[0];
+  a.start_stride = starts.stride[0];
+  a.tokens = (int)tokens;
+  hipLaunchKernelGGL(kv_assign_kernel, dim3(1), dim3(kPagesThreads), 0, g_stream, a);
+  return finish_launch("kv_cache_assign");
+}
+
+int kv_cache_release_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 6) return fail(kInvalid, "kv_cache_release expects 6 slots, got %llu", n);
+  PagesSlots p;
+  int rc;
+  if ((rc = read_pages(args, 0, "kv_cache_release", "keep_lens", "held_lens", &p))) return rc;
+  if ((rc = check_pages(p, "keep_lens", "held_lens"))) return rc;
+  if (no_elements(p.table)) return finish_launch("kv_cache_release(empty)");
+  hipLaunchKernelGGL(kv_release_kernel, dim3(1), dim3(kPagesThreads), 0, g_stream, pages_args(p));
+  return finish_launch("kv_cache_release");
+}
+
+template <typename F>
+int with_float_type(int dtype, F&& f) {
+  return dtype == KG_DTYPE_F32 ? f(float{}) : dtype == KG_DTYPE_BF16 ? f((__bf16)0.f) : f((_Float16)0.f);
+}
+
+int launch_quantize(const QuantizeArgs& a, int dtype) {
+  return with_float_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((quantize_rows_any_kernel<T>), dim3(most_blocks(a.rows)), dim3(256), 0, g_stream, a);
+    return finish_launch("quantize_rows");
+  });
+}
+
+int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 3) return fail(kInvalid, "quantize_rows expects 3 slots, got %llu", n);
+  Mem codes, scale, x;
+  int rc;
+  if ((rc = read_view(args, 0, 2, kI8, false, "codes", &codes))) return rc;
+  if ((rc = read_view(args, 1, 1, kF32, false, "scale", &scale))) return rc;
+  if ((rc = read_view(args, 2, 2, kFloatTypes, false, "x", &x))) return rc;
+  const long long M = x.shape[0], K = x.shape[1];
+  if (codes.shape[0] != M || codes.shape[1] != K)
+    return fail(kInvalid, "quantize_rows: codes shape [%lld,%lld] != [%lld,%lld]", codes.shape[0], codes.shape[1], M, K);
+  if (scale.shape[0] != M) return fail(kInvalid, "quantize_rows: %lld scales for %lld rows", scale.shape[0], M);
+  if (!row_contiguous(codes) || !row_contiguous(x)) return fail(kInvalid, "quantize_rows: the rows of codes and x must be contiguous");
+  if ((rc = check_view(codes, "codes")) || (rc = check_view(scale, "scale")) || (rc = check_view(x, "x"))) return rc;
+  if (K > 0x7fff0000LL) return fail(kUnsupported, "quantize_rows: rows of %lld elements", K);
+  if (M == 0) return finish_launch("quantize_rows(empty)");
+  QuantizeArgs a{x.data, static_cast<int8_t*>(codes.data), static_cast<float*>(scale.data), x.stride[0], codes.stride[0],
+                 scale.stride[0], (int)M, (int)K, (int)K};
+  return launch_quantize(a, x.dtype);
+}
+
+int int8_matmul_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 6) return fail(kInvalid, "int8_matmul expects 6 slots, got %llu", n);
+  Mem out, x, x_scale, w, w_scale, bias;
+  int rc;
+  if ((rc = read_view(args, 0, 2, kFloatTypes, false, "out", &out))) return rc;
+  if ((rc = read_view(args, 1, 2, kFloatTypes | kI8, false, "x", &x))) return rc;
+  if ((rc = read_view(args, 2, 1, kF32, true, "x_scale", &x_scale))) return rc;
+  if ((rc = read_view(args, 3, 2, kI8, false, "weight", &w))) return rc;
+  if ((rc = read_view(args, 4, 1, kF32, false, "w_scale", &w_scale))) return rc;
+  if ((rc = read_view(args, 5, 1, kFloatTypes, true, "bias", &bias))) return rc;
+  const long long M = x.shape[0], K = x.shape[1], N = w.shape[0];
+  const bool codes = x.dtype == KG_DTYPE_I8;
+  if (w.shape[1] != K) return fail(kInvalid, "int8_matmul: x K=%lld != weight K=%lld", K, w.shape[1]);
+  if (out.shape[0] != M || out.shape[1] != N)
+    return fail(kInvalid, "int8_matmul: out shape [%lld,%lld] != [%lld,%lld]", out.shape[0], out.shape[1], M, N);
+  if (!codes && x.dtype != out.dtype)
+    return fail(kInvalid, "int8_matmul: x must be int8 or of out's type (%s, %s)", dtype_name(x.dtype), dtype_name(out.dtype));
+  if (x_scale.present != codes && !(codes && M == 0))  // (no rows: a tensor without memory)
+    return fail(kInvalid, codes ? "int8_matmul: x in int8 needs x_scale" : "int8_matmul: x that the call quantises takes no x_scale");
+  if (x_scale.present && x_scale.shape[0] != M) return fail(kInvalid, "int8_matmul: %lld x_scale values for %lld rows", x_scale.shape[0], M);
+  if (w_scale.shape[0] != N) return fail(kInvalid, "int8_matmul: %lld w_scale values for %lld channels", w_scale.shape[0], N);
+  if (bias.present && bias.shape[0] != N) return fail(kInvalid, "int8_matmul: bias extent %lld != N=%lld", bias.shape[0], N);
+  if (bias.present && bias.dtype != out.dtype && bias.dtype != KG_DTYPE_F32)
+    return fail(kInvalid, "int8_matmul: bias dtype %s must be f32 or match out", dtype_name(bias.dtype));
+  if (!row_contiguous(out) || !row_contiguous(x) || !row_contiguous(w))
+    return fail(kInvalid, "int8_matmul: the rows of out, x and weight must be contiguous");
+  if (K > kInt8MostK) return fail(kUnsupported, "int8_matmul: K=%lld > %d: sums may leave 32 bits", K, kInt8MostK);
+  if ((rc = check_view(out, "out")) || (rc = check_view(x, "x")) || (rc = check_view(x_scale, "x_scale")) ||
+      (rc = check_view(w, "weight")) || (rc = check_view(w_scale, "w_scale")) || (rc = check_view(bias, "bias")))
+    return rc;
+  if (M == 0 || N == 0) return finish_launch("int8_matmul(empty)");
+  Int8Args a{x.data, static_cast<const int8_t*>(w.data), static_cast<const float*>(x_scale.data),
+             static_cast<const float*>(w_scale.data), bias.data, out.data, x.stride[0], w.stride[0], out.stride[0],
+             x_scale.stride[0], w_scale.stride[0], bias.stride[0], (int)M, (int)N, (int)K, bias.dtype == KG_DTYPE_F32};
+  return with_float_type(out.dtype, [&](auto t) {
+    using T = decltype(t);
+    const unsigned grid = most_blocks(M * cdiv(N, 64));
+    if (codes) hipLaunchKernelGGL((int8_any_kernel<T, int8_t>), dim3(grid), dim3(256), 0, g_stream, a);
+    else hipLaunchKernelGGL((int8_any_kernel<T, T>), dim3(grid), dim3(256), 0, g_stream, a);
+    return finish_launch("int8_matmul");
+  });
+}
+
+int head_norm_rotate_impl(const KgArgSlot* args, unsigned long long n) {
+  if (args == nullptr) return fail(kInvalid, "ordered_args is null");
+  if (n != 11) return fail(kInvalid, "head_norm_rotate expects 11 slots, got %llu", n);
+  static const char* const kNames[4] = {"q_out", "k_out", "q", "k"};
+  Mem rows[4], weight[2], cos, sin, positions;
+  double eps = 0.0;
+  long long neighbours = 0;
+  int rc;
+  for (int i = 0; i < 4; ++i)
+    if ((rc = read_view(args, i, 3, kFloatTypes, false, kNames[i], &rows[i]))) return rc;
+  if ((rc = read_view(args, 4, 1, kFloatTypes, true, "q_weight", &weight[0]))) return rc;
+  if ((rc = read_view(args, 5, 1, kFloatTypes, true, "k_weight", &weight[1]))) return rc;
+  if ((rc = read_view(args, 6, 2, kF32, false, "cos", &cos))) return rc;
+  if ((rc = read_view(args, 7, 2, kF32, false, "sin", &sin))) return rc;
+  if ((rc = read_view(args, 8, 1, kI32 | kI64, false, "positions", &positions))) return rc;
+  if ((rc = read_float(args, 9, "eps", &eps))) return rc;
+  if ((rc = read_int(args, 10, "neighbours", &neighbours))) return rc;
+  const long long tokens = rows[2].shape[0], d = rows[2].shape[2];
+  for (int x = 0; x < 2; ++x) {
+    const Mem &out = rows[x], &in = rows[2 + x];
+    for (int i = 0; i < 3; ++i)
+      if (out.shape[i] != in.shape[i]) return fail(kInvalid, "head_norm_rotate: %s/%s shape mismatch at dim %d", kNames[2 + x], kNames[x], i);
+    if (in.shape[0] != tokens || in.shape[2] != d)
+      return fail(kInvalid, "head_norm_rotate: q and k must have the same tokens and head dim ([%lld,heads,%lld])", tokens, d);
+    if (out.dtype != rows[2].dtype || in.dtype != rows[2].dtype)
+      return fail(kInvalid, "head_norm_rotate: q/k/q_out/k_out dtypes must match");
+    if (!row_contiguous(out) || !row_contiguous(in)) return fail(kInvalid, "head_norm_rotate: the rows of q, k and their outputs must be contiguous");
+    if (weight[x].present && weight[x].shape[0] != d)
+      return fail(kInvalid, "head_norm_rotate: weight extent %lld != head dim %lld", weight[x].shape[0], d);
+    if (weight[x].present && weight[x].dtype != rows[2].dtype && weight[x].dtype != KG_DTYPE_F32)
+      return fail(kInvalid, "head_norm_rotate: weight dtype %s must be f32 or match q", dtype_name(weight[x].dtype));
+  }
+  if (d < 1 || d > 512) return fail(kUnsupported, "head_norm_rotate: head dim %lld not in 1..512", d);
+  if (sin.shape[0] != cos.shape[0] || sin.shape[1] != cos.shape[1]) return fail(kInvalid, "head_norm_rotate: cos/sin shapes must match");
+  if (2 * cos.shape[1] > d)
+    return fail(kInvalid, "head_norm_rotate: %lld pairs are more than a head of %lld has", cos.shape[1], d);
+  if (positions.shape[0] != tokens) return fail(kInvalid, "head_norm_rotate: %lld positions for %lld tokens", positions.shape[0], tokens);
+  if (!(eps >= 0.0 && eps <= 3.0e38)) return fail(kInvalid, "head_norm_rotate: eps must be finite and not negative");
+  if (neighbours != 0 && neighbours != 1) return fail(kInvalid, "head_norm_rotate: neighbours must be 0 or 1");
+  for (int i = 0; i < 4; ++i)
+    if ((rc = check_view(rows[i], kNames[i]))) return rc;
+  if ((rc = check_view(weight[0], "q_weight")) || (rc = check_view(weight[1], "k_weight")) || (rc = check_view(cos, "cos")) ||
+      (rc = check_view(sin, "sin")) || (rc = check_view(positions, "positions")))
+    return rc;
+  const long long heads = rows[2].shape[1] + rows[3].shape[1];
+  if (tokens == 0 || heads == 0 || cos.shape[0] == 0) return finish_launch("head_norm_rotate(empty)");
+  if (heads > 0x7fffffffLL) return fail(kUnsupported, "head_norm_rotate: %lld heads", heads);
+  HeadNormArgs a{};
+  for (int x = 0; x < 2; ++x) {
+    const Mem &out = rows[x], &in = rows[2 + x], &w = weight[x];
+    a.side[x] = HeadNormSide{in.data, w.data, out.data, in.stride[0], in.stride[1], out.stride[0], out.stride[1], w.stride[0],
+                             (int)in.shape[1], w.dtype == KG_DTYPE_F32};
+  }
+  a.cos = static_cast<const float*>(cos.data);
+  a.sin = static_cast<const float*>(sin.data);
+  a.positions = positions.data;
+  a.cos_row = cos.stride[0];
+  a.sin_row = sin.stride[0];
+  a.cos_stride = cos.stride[1];
+  a.sin_stride = sin.stride[1];
+  a.position_stride = positions.stride[0];
+  a.table = cos.shape[0];
+  a.tokens = (int)tokens;
+  a.d = (int)d;
+  a.half = (int)cos.shape[1];
+  a.wide_positions = positions.dtype == KG_DTYPE_I64;
+  a.neighbours = neighbours != 0;
+  a.eps = (float)eps;
+  a.inverse_d = 1.f / (float)d;
+  return with_float_type(rows[2].dtype, [&](auto t) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((head_norm_any_kernel<T>), dim3(most_blocks(cdiv(tokens * heads, 4))), dim3(256), 0, g_stream, a);
+    return finish_launch("head_norm_rotate");
+  });
+}
+
 }  // namespace
 
 extern "C" {
@@ -1845,6 +2103,26 @@ int kg_gfx950_tree_attention_entry(const KgArgSlot* ordered_args, unsigned long 
 
 int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
   return adapter_matmul_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_kv_cache_assign_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return kv_cache_assign_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_kv_cache_release_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return kv_cache_release_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_quantize_rows_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return quantize_rows_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_int8_matmul_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return int8_matmul_impl(ordered_args, arg_count);
+}
+
+int kg_gfx950_head_norm_rotate_entry(const KgArgSlot* ordered_args, unsigned long long arg_count) {
+  return head_norm_rotate_impl(ordered_args, arg_count);
 }
 
 int kg_gfx950_fail(int code, const char* message) { return fail(code, "%s", message ? message : ""); }

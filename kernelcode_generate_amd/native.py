@@ -35,7 +35,7 @@ DTYPE_CODES = {
     "float16": 5,
     "bfloat16": 6,
 }
-# of the serving entries' caches alone
+# of the serving entries alone: caches, and int8 codes
 CACHE_DTYPE_CODES = {"int8": 7, "float8_e4m3fn": 8}
 
 ENTRY_POINTS = (
@@ -46,6 +46,11 @@ ENTRY_POINTS = (
     "kg_gfx950_kv_cache_load_entry",
     "kg_gfx950_tree_attention_entry",
     "kg_gfx950_adapter_matmul_entry",
+    "kg_gfx950_kv_cache_assign_entry",
+    "kg_gfx950_kv_cache_release_entry",
+    "kg_gfx950_quantize_rows_entry",
+    "kg_gfx950_int8_matmul_entry",
+    "kg_gfx950_head_norm_rotate_entry",
 )
 CONTROL_SYMBOLS = (
     "kg_gfx950_set_launch_mode",
@@ -394,3 +399,41 @@ def adapter_matmul(out, x, weight, bias, a, b, index, scale=None) -> None:
     (int32 [M]) is an adapter (a [L, K, R], b [L, R, N]; scale: float32 [L], 1 where None)."""
 
     call_entry("kg_gfx950_adapter_matmul_entry", (out, x, weight, bias, a, b, index, scale))
+
+
+def kv_cache_assign(slots, positions, starts, page_table, free_pages, free_count, context_lens, new_lens, page_size: int) -> None:
+    """Pages and slots of new_lens[b] new tokens behind each request's context_lens[b] cached ones (int32 [B]): starts
+    (int32 [B + 1]) of the requests' rows in the batch, and of each row its position (int32 [T]) and slot (int64 [T]), -1 behind the last.
+    New pages come off the stack free_pages (int32 [F], free_count (int32 [1]) of them) and are entered in page_table (int32 [B, P])."""
+
+    call_entry("kg_gfx950_kv_cache_assign_entry", (slots, positions, starts, page_table, free_pages, free_count, context_lens,
+                                                   new_lens, int(page_size)))
+
+
+def kv_cache_release(page_table, free_pages, free_count, keep_lens, held_lens, page_size: int) -> None:
+    """Put the pages that request b's first keep_lens[b] tokens do not need, of those for held_lens[b], back on the stack:
+    a request that ended (keep 0), drafted tokens that were rejected."""
+
+    call_entry("kg_gfx950_kv_cache_release_entry", (page_table, free_pages, free_count, keep_lens, held_lens, int(page_size)))
+
+
+def quantize_rows(codes, scale, x) -> None:
+    """Rows x [M, K] as int8 codes [M, K] and float32 scales [M]: scale = max|x| / 127, code = x / scale rounded to nearest."""
+
+    call_entry("kg_gfx950_quantize_rows_entry", (codes, scale, x))
+
+
+def int8_matmul(out, x, x_scale, weight, w_scale, bias=None) -> None:
+    """out = (x @ weight.T) * x_scale[:, None] * w_scale + bias, weight int8 [N, K], w_scale float32 [N]. x: int8 [M, K] with x_scale
+    (float32 [M]), or of out's type with None: its rows are then quantised as by quantize_rows."""
+
+    call_entry("kg_gfx950_int8_matmul_entry", (out, x, x_scale, weight, w_scale, bias))
+
+
+def head_norm_rotate(q_out, k_out, q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-6, neighbours: bool = False) -> None:
+    """Norms over the heads of q [T, Hq, D] and k [T, Hk, D] (a side whose weight [D] is None: none), then the rotation of
+    the pairs (i, i + R), or (2 i, 2 i + 1) of neighbours, by row positions[t] of cos and sin (float32 [S, R]). Tokens with positions
+    outside the table (-1) are left as they are. The outputs may be the inputs."""
+
+    call_entry("kg_gfx950_head_norm_rotate_entry", (q_out, k_out, q, k, q_weight, k_weight, cos, sin, positions, float(eps),
+                                                    int(bool(neighbours))))

@@ -1,0 +1,184 @@
+"""quantize_rows and int8_matmul against whole numbers and 64 bits: codes and scales equal, products within the roundings."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from kernelcode_generate_amd import native
+from tests.step_util import assert_close, codes_oracle, int8_oracle
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def rows(m, k, dtype, gen):
+    x = torch.randn(m, k, generator=gen) * torch.exp(torch.randn(m, 1, generator=gen))
+    return x.to(dtype)
+
+
+def check_rows(x, device, stride=None, offset=0):
+    m, k = x.shape
+    stride = k if stride is None else stride
+    wide = torch.zeros(m * stride + offset + 1, dtype=x.dtype, device=device)
+    xs = wide[offset:].as_strided((m, k), (stride, 1), offset)
+    xs.copy_(x)
+    codes = torch.full((m * stride + offset + 1,), 99, dtype=torch.int8, device=device)
+    view = codes.as_strided((m, k), (stride, 1), offset)
+    scale = torch.full((2 * m,), -1.0, device=device)
+    native.quantize_rows(view, scale[::2], xs)
+    want, want_scale = codes_oracle(x)
+    assert np.array_equal(scale[::2].cpu().numpy(), want_scale, equal_nan=True)
+    assert np.array_equal(view.cpu().numpy(), want)
+    assert (scale[1::2] == -1).all()
+    untouched = torch.ones_like(codes, dtype=torch.bool)
+    untouched.as_strided((m, k), (stride, 1), offset).fill_(False)
+    assert (codes[untouched] == 99).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, k", [(1, 1), (3, 7), (5, 8), (4, 64), (17, 100), (2, 511), (9, 512), (6, 513), (33, 1023), (8, 2048), (3, 2056),
+                                  (5, 4096), (2, 8192), (2, 9999), (3, 16384), (2, 16385), (1, 40000)])
+def test_rows(device, dtype, m, k):
+    gen = torch.Generator().manual_seed(m * k)
+    check_rows(rows(m, k, dtype, gen), device)
+    check_rows(rows(m, k, dtype, gen), device, stride=k + 5, offset=3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_special_values(device, dtype):
+    """Zeros, ties, the least and largest values, infinities and NaN, each with ordinary rows beside them."""
+
+    inf, nan, big, least = float("inf"), float("nan"), torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+    table = [[0.0] * 16, [-0.0, 0.0] * 8, [127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 63.5] * 2, [254.0, 1.0, 3.0, 5.0, -1.0, -3.0, -127.0, 125.0] * 2,
+             [big, -big, 1.0, 0.0] * 4, [least, -least, 0.0, least * 2] * 4, [inf, 1.0, -2.0, 0.0] * 4, [1.0, -inf, 3.0, 4.0] * 4,
+             [1.0, 2.0, nan, -4.0] * 4, [inf, nan, 1.0, 0.0] * 4, [1.0, -1.0, 0.25, -0.75] * 4]
+    check_rows(torch.tensor(table).to(dtype), device)
+    if dtype == torch.float32:  # scales that are no normal numbers, where the quotient may leave the codes
+        check_rows(torch.tensor([[1e-40, -3e-41, 0.0, 5e-42], [2.0**-149, 0.0, 0.0, 0.0], [2.0**-143, 2.0**-144, -(2.0**-145), 2.0**-146],
+                                 [3.3e38, -1e38, 1e30, 1e-30]]), device)
+
+
+def check_product(m, n, k, dtype, device, codes, bias, seed=0, top=False, pads=(0, 0, 0), offsets=(0, 0, 0), columns=None):
+    gen = torch.Generator().manual_seed(1000 * m + 10 * n + k + seed)
+    x = rows(m, k, dtype, gen)
+    if top:  # the largest sums
+        values, x_scale = torch.full((m, k), -128, dtype=torch.int64).numpy(), np.full(m, 0.01, np.float32)
+        weight, w_scale = torch.full((n, k), -128, dtype=torch.int8), torch.full((n,), 0.001)
+    else:
+        values, x_scale = codes_oracle(x)
+        if codes:
+            values = torch.randint(-128, 128, (m, k), generator=gen).numpy()
+        weight, w_scale = torch.randint(-128, 128, (n, k), generator=gen, dtype=torch.int8), torch.rand(n, generator=gen) * 0.01
+    b = None
+    if bias is not None:
+        b = (torch.randn(n, generator=gen) * 0.1).to(torch.float32 if bias == "f32" else dtype)
+
+    def view(t, pad, offset, fill=None):
+        width = t.shape[1] + pad
+        wide = torch.zeros(t.shape[0] * width + offset + 1, dtype=t.dtype, device=device)
+        if fill is not None:
+            wide.fill_(fill)
+        v = wide.as_strided(t.shape, (width, 1), offset)
+        v.copy_(t)
+        return wide, v
+
+    _, xs = view(torch.from_numpy(values).to(torch.int8) if codes else x, pads[0], offsets[0], 77)
+    _, ws = view(weight, pads[1], offsets[1], 77)
+    whole, out = view(torch.full((m, n), 5.0).to(dtype), pads[2], offsets[2], 5.0)
+    scales = torch.from_numpy(x_scale).to(device) if codes else None
+    native.int8_matmul(out, xs, scales, ws, w_scale.to(device), None if b is None else b.to(device))
+    assert_close(out, *int8_oracle(values, x_scale, weight, w_scale, b, dtype), f"{m}x{n}x{k}")
+    rest = torch.ones_like(whole, dtype=torch.bool)
+    rest.as_strided((m, n), (n + pads[2], 1), offsets[2]).fill_(False)
+    assert (whole[rest] == 5).all()
+
+
+SIZES = [(1, 1, 1), (1, 64, 64), (3, 5, 7), (1, 4096, 512), (2, 100, 1000), (8, 256, 4096), (15, 33, 130), (16, 1024, 2048), (16, 48, 8192),
+         (17, 512, 256), (31, 1000, 1040), (32, 128, 96), (33, 2048, 512), (64, 64, 64), (65, 272, 144), (100, 1501, 1023), (127, 130, 64),
+         (128, 128, 128), (129, 257, 1024), (200, 768, 2048), (256, 256, 256), (257, 513, 272), (300, 1024, 1000), (512, 512, 1024),
+         (700, 300, 80), (1000, 1501, 1023), (1024, 2048, 512), (515, 264, 4112), (2048, 8, 64), (40, 16384, 64), (1, 8, 131071)]
+
+
+@pytest.mark.parametrize("m, n, k", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("codes", [True, False])
+def test_products(device, m, n, k, dtype, codes):
+    check_product(m, n, k, dtype, device, codes, (None, "f32", "same")[(m + n + k) % 3])
+
+
+@pytest.mark.parametrize("m, n, k", [(5, 40, 64), (20, 100, 128), (70, 130, 272), (300, 264, 256)])
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("pads, offsets", [((16, 16, 8), (0, 0, 0)), ((3, 5, 1), (0, 0, 0)), ((0, 0, 0), (1, 3, 1)), ((16, 0, 8), (8, 16, 8)),
+                                           ((0, 7, 0), (0, 0, 0)), ((1, 0, 0), (0, 0, 0)), ((0, 0, 3), (0, 0, 0))])
+def test_strides_and_alignments(device, m, n, k, codes, pads, offsets):
+    check_product(m, n, k, torch.bfloat16, device, codes, "same", pads=pads, offsets=offsets)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 130, 300])
+def test_the_largest_sums(device, m):
+    """K = 131071 products of 2^14: 2^31 - 2^14, the largest sum, in each kernel."""
+
+    check_product(m, 70, 131071, torch.float32, device, True, None, top=True)
+    check_product(m, 64, 131056, torch.float32, device, True, None, top=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k", [(3, 40, 128), (40, 40, 128), (200, 136, 256)])
+def test_rows_that_are_not_finite(device, dtype, m, n, k):
+    """An infinity or NaN makes its own row's results NaN, and no other row's."""
+
+    gen = torch.Generator().manual_seed(m)
+    x = rows(m, k, dtype, gen)
+    x[0, 3], x[1, k - 1], x[m - 1] = float("nan"), float("inf"), 0.0
+    values, x_scale = codes_oracle(x)
+    weight, w_scale = torch.randint(-127, 128, (n, k), generator=gen, dtype=torch.int8), torch.rand(n, generator=gen) * 0.01
+    out = torch.empty(m, n, dtype=dtype, device=device)
+    native.int8_matmul(out, x.to(device), None, weight.to(device), w_scale.to(device))
+    expected, allowed = int8_oracle(values, x_scale, weight, w_scale, None, dtype)
+    assert np.isnan(expected[:2]).all() and (expected[m - 1] == 0).all()
+    assert_close(out, expected, allowed)
+
+
+def test_nothing(device):
+    empty = torch.zeros(0, 16, dtype=torch.bfloat16, device=device)
+    weight, w_scale = torch.ones(8, 16, dtype=torch.int8, device=device), torch.ones(8, device=device)
+    native.int8_matmul(torch.zeros(0, 8, dtype=torch.bfloat16, device=device), empty, None, weight, w_scale)
+    native.int8_matmul(torch.zeros(0, 8, device=device), torch.zeros(0, 16, dtype=torch.int8, device=device), torch.zeros(0, device=device), weight, w_scale)
+    native.quantize_rows(torch.zeros(0, 16, dtype=torch.int8, device=device), torch.zeros(0, device=device), empty)
+    x = torch.ones(3, 16, device=device)
+    native.int8_matmul(torch.zeros(3, 0, device=device), x, None, weight[:0], w_scale[:0])
+    out = torch.full((3, 8), 7.0, device=device)
+    native.int8_matmul(out, x[:, :0], None, weight[:, :0], w_scale, torch.arange(8.0, device=device))  # sums of nothing: the bias
+    assert torch.equal(out.cpu(), torch.arange(8.0).expand(3, 8))
+    scale = torch.full((3,), 7.0, device=device)
+    native.quantize_rows(torch.zeros(3, 0, dtype=torch.int8, device=device), scale, x[:, :0])
+    assert (scale == 0).all()
+
+
+@pytest.mark.parametrize("m, n, k", [(4, 64, 256), (150, 100, 130), (300, 512, 1024)])
+def test_recorded_products(device, m, n, k):
+    """Replays read the rows as they are then, beside other calls on the stream's workspace."""
+
+    gen = torch.Generator().manual_seed(m)
+    weight, w_scale = torch.randint(-127, 128, (n, k), generator=gen, dtype=torch.int8), torch.rand(n, generator=gen) * 0.01
+    x, out = torch.zeros(m, k, dtype=torch.bfloat16, device=device), torch.zeros(m, n, dtype=torch.bfloat16, device=device)
+    wd, sd = weight.to(device), w_scale.to(device)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            native.set_launch_mode(False, torch.cuda.current_stream().cuda_stream)
+            native.int8_matmul(out, x, None, wd, sd)
+        native.set_launch_mode(True, None)
+        for step in range(4):
+            new = rows(m, k, torch.bfloat16, gen)
+            x.copy_(new)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert_close(out, *int8_oracle(*codes_oracle(new), weight, w_scale, None, torch.bfloat16), f"replay {step}")
+            other = torch.empty_like(out)
+            native.int8_matmul(other, x, None, wd, sd)
+            assert torch.equal(other, out)
+    finally:
+        native.set_launch_mode(True, None)

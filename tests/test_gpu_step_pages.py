@@ -1,0 +1,167 @@
+"""kv_cache_assign and kv_cache_release against lists in Python: whole numbers, equal everywhere."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from kernelcode_generate_amd import native
+from tests.step_util import assign_oracle, ceil_pages, release_oracle
+
+pytestmark = pytest.mark.gpu
+I32 = torch.int32
+
+
+def make(rng, batch, per, page, context, new, spare):
+    """Lengths, a table with the pages of the cached tokens, and a stack of other pages in random order."""
+
+    context = [rng.randint(0, context) for _ in range(batch)]
+    new = [rng.choice((0, rng.randint(0, new), new)) for _ in range(batch)]
+    held = [ceil_pages(c, page, per) for c in context]
+    need = [ceil_pages(c + n, page, per) - h for c, n, h in zip(context, new, held)]
+    pages = list(range(sum(held) + int(sum(need) * spare)))
+    rng.shuffle(pages)
+    at, table = 0, []
+    for h in held:
+        table.append(pages[at : at + h] + [-1] * (per - h))
+        at += h
+    free = pages[at:]
+    return context, new, table, free
+
+
+def run_assign(table, free, count, context, new, page, tokens, device, stride=1):
+    def strided(values, dtype=I32):
+        t = torch.full((max(len(values), 1) * stride,), -77, dtype=dtype, device=device)[: len(values) * stride : stride]
+        t.copy_(torch.tensor(values, dtype=dtype))
+        return t
+
+    rows = torch.tensor(table, dtype=I32).reshape(len(table), -1)
+    t = torch.full((rows.shape[0], rows.shape[1] * stride + 3), -77, dtype=I32, device=device)[:, : rows.shape[1] * stride : stride]
+    t.copy_(rows)
+    out = [strided([-5] * tokens, torch.int64), strided([-5] * tokens), strided([-5] * (len(table) + 1))]
+    stack, left = strided(free), strided([count])
+    native.kv_cache_assign(*out, t, stack, left, strided(context), strided(new), page)
+    return [*out, t, stack, left]
+
+
+def check_assign(table, free, count, context, new, page, tokens, device, stride=1):
+    slots, positions, starts, t, stack, left = run_assign(table, free, count, context, new, page, tokens, device, stride)
+    want = assign_oracle(table, free, count, context, new, page, tokens)
+    for got, expected, what in zip((slots, positions, starts, t, left), (*want[:4], [want[4]]), ("slots", "positions", "starts", "table", "count")):
+        assert got.tolist() == expected, what
+    assert stack.tolist() == free
+    return t, stack, left, want
+
+
+@pytest.mark.parametrize("batch, per, page, context, new, slack, spare", [
+    (1, 1, 16, 15, 1, 0, 1.0), (1, 4, 16, 0, 50, 0, 1.0), (7, 20, 16, 200, 1, 0, 1.0), (64, 40, 16, 600, 1, 3, 2.0),
+    (65, 9, 64, 500, 17, 100, 1.0), (5, 300, 1, 200, 90, 11, 1.0), (33, 12, 24, 250, 30, -40, 1.0), (40, 20, 16, 200, 60, 5, 0.5),
+    (1025, 6, 16, 60, 20, 0, 1.0), (2500, 4, 16, 40, 2, 7, 0.7), (8192, 2, 16, 20, 3, -100, 1.0), (3, 5, 1000, 4000, 900, 0, 1.0),
+    (16, 70, 16, 100, 1024, 0, 1.0), (4, 1100, 16, 100, 16384, 5000, 1.0), (12, 3, 16, 100, 30, 0, 1.0), (9, 10, 16, 100, 60, 0, 0.0),
+])
+@pytest.mark.parametrize("stride", [1, 3])
+def test_assign_and_release(device, batch, per, page, context, new, slack, spare, stride):
+    rng = random.Random(batch * 1000 + per)
+    context, new, table, free = make(rng, batch, per, page, context, new, spare)
+    tokens = max(sum(new) + slack, 1)
+    t, stack, left, want = check_assign(table, free, len(free), context, new, page, tokens, device, stride)
+    # what the call took goes back: stack and table as they were
+    kept = [e - s for s, e in zip(want[2], want[2][1:])]
+    keep = torch.tensor(context, dtype=I32, device=device)
+    held = torch.tensor([c + n for c, n in zip(context, kept)], dtype=I32, device=device)
+    native.kv_cache_release(t, stack, left, keep, held, page)
+    assert t.tolist() == table and stack.tolist() == free and left.tolist() == [len(free)]
+    # every second request ends
+    keep = [0 if b % 2 else c for b, c in enumerate(context)]
+    big = torch.full((len(free) + batch * per,), -9, dtype=I32, device=device)
+    big[: len(free)] = stack
+    gone = release_oracle(table, big.tolist(), len(free), keep, context, page)
+    native.kv_cache_release(t, big, left, torch.tensor(keep, dtype=I32, device=device), torch.tensor(context, dtype=I32, device=device), page)
+    assert t.tolist() == gone[0] and big.tolist() == gone[1] and left.tolist() == [gone[2]]
+
+
+def test_odd_lengths_and_counts(device):
+    """Lengths below 0, counts outside the stack, positions past the table and past 31 bits."""
+
+    top = 2**31 - 1
+    table = [[3, 4, -1], [-1, -1, -1], [5, 6, 7], [8, 9, 10], [-1, -1, -1]]
+    free = [20, 21, 22, 23]
+    for count in (-3, 0, 2, 4, 9):
+        check_assign(table, free, count, [20, -5, 47, 48, 0], [5, 17, 3, 2, -4], 16, 30, device)
+    # a page of the context that does not exist; a page in the stack that does not exist
+    check_assign([[3, -1, -1]], [30, -1], 2, [20], [20], 16, 20, device)
+    rows = [[1, 2]] * 2
+    slots, positions, starts, *_ = run_assign(rows, [5], 1, [top - 1, top], [4, 2], 2**30, 6, device)
+    assert starts.tolist() == [0, 4, 6]
+    assert positions.tolist() == [top - 1, top, top, top, top, top]
+    assert slots.tolist() == [2 * 2**30 + 2**30 - 2, -1, -1, -1, -1, -1]
+
+
+def test_release_passes_over_what_is_not_there(device):
+    table = [[3, -1, 4, 5], [6, 7, -1, -1], [8, 9, 10, 11]]
+    for keep, held, count, size in (([0, 20, 64], [64, 99, 64], 2, 12), ([16, 0, 0], [64, 16, 200], 0, 12), ([40, 9, 0], [20, 3, -1], 1, 6),
+                                    ([0, 0, 0], [64, 64, 64], 3, 5), ([-9, 0, 0], [64, 32, 0], 7, 4)):
+        free = list(range(100, 100 + size))
+        want = release_oracle(table, free, count, keep, held, 16)
+        t, stack, left = (torch.tensor(x, dtype=I32, device=device) for x in (table, free, [count]))
+        native.kv_cache_release(t, stack, left, *(torch.tensor(x, dtype=I32, device=device) for x in (keep, held)), 16)
+        assert (t.tolist(), stack.tolist(), left.item()) == want
+
+
+def test_nothing(device):
+    """No requests, no rows, no pages, no stack."""
+
+    def ints(*shape, value=-5, dtype=I32):
+        return torch.full(shape, value, dtype=dtype, device=device)
+
+    slots, positions, starts, count = ints(4, dtype=torch.int64), ints(4), ints(1), ints(1, value=2)
+    native.kv_cache_assign(slots, positions, starts, ints(0, 3), ints(2, value=7), count, ints(0), ints(0), 16)
+    assert slots.tolist() == positions.tolist() == [-1] * 4 and starts.tolist() == [0] and count.item() == 2
+    starts = ints(3)
+    native.kv_cache_assign(ints(0, dtype=torch.int64), ints(0), starts, ints(2, 3), ints(2, value=7), count, ints(2, value=0), ints(2, value=5), 16)
+    assert starts.tolist() == [0, 0, 0] and count.item() == 2  # no rows: no tokens, no pages
+    slots, positions, starts = ints(4, dtype=torch.int64), ints(4), ints(3)
+    native.kv_cache_assign(slots, positions, starts, ints(2, 0), ints(2, value=7), count, ints(2, value=1), ints(2, value=2), 16)
+    assert slots.tolist() == [-1] * 4 and positions.tolist() == [1, 2, 1, 2] and starts.tolist() == [0, 2, 4] and count.item() == 2
+    table = ints(2, 3)
+    count = ints(1, value=0)
+    native.kv_cache_assign(slots, positions, starts, table, ints(0), count, ints(2, value=0), ints(2, value=2), 16)
+    assert slots.tolist() == [-1] * 4 and positions.tolist() == [0, 1, 0, 1] and count.item() == 0
+    native.kv_cache_release(ints(0, 3), ints(2), count, ints(0), ints(0), 16)
+    native.kv_cache_release(ints(2, 0), ints(2), count, ints(2, value=0), ints(2, value=50), 16)
+    native.kv_cache_release(ints(2, 3, value=4), ints(0), count, ints(2, value=0), ints(2, value=50), 16)
+    assert count.item() == 0
+
+
+def test_recorded_steps(device):
+    """A recorded step: every replay takes its pages from the stack as it is then."""
+
+    rng = random.Random(5)
+    context, new, table, free = make(rng, 20, 30, 16, 200, 40, 3.0)
+    tokens = 20 * 40
+    t, stack, left = (torch.tensor(x, dtype=I32, device=device) for x in (table, free, [len(free)]))
+    c, n = (torch.tensor(x, dtype=I32, device=device) for x in (context, new))
+    slots, positions, starts = (torch.zeros(x, dtype=d, device=device) for x, d in ((tokens, torch.int64), (tokens, I32), (21, I32)))
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            native.set_launch_mode(False, torch.cuda.current_stream().cuda_stream)
+            native.kv_cache_assign(slots, positions, starts, t, stack, left, c, n, 16)
+            c += starts[1:] - starts[:-1]
+        count = len(free)
+        for step in range(4):
+            graph.replay()
+            torch.cuda.synchronize()
+            want = assign_oracle(table, free, count, context, new, 16, tokens)
+            assert slots.tolist() == want[0] and positions.tolist() == want[1] and starts.tolist() == want[2] and t.tolist() == want[3]
+            assert left.item() == want[4]
+            table, count = want[3], want[4]
+            context = [x + e - s for x, s, e in zip(context, want[2], want[2][1:])]
+            assert c.tolist() == context
+            new = [rng.randint(0, 20) for _ in new]
+            n.copy_(torch.tensor(new, dtype=I32))
+    finally:
+        native.set_launch_mode(True, None)
