@@ -1,0 +1,306 @@
+// gemm_i8_kernel: products in 8-bit integers (gemm_i8.h) in tiles, four waves of 2 x 2, each a (16 NA) x (16 NB) quarter in blocks of
+// v_mfma_i32_16x16x64_i8. Both operands lie along k, so both are copied to LDS and read back the same way: rows of kBK
+// bytes, fragments of 16 bytes (16 k) a lane, which is the form that the instruction takes from both sides. A 64-deep step of codes
+// has the bytes of a 32-deep step of bf16 at twice its operations, so the K loop is that of the 16-bit kernels: a ring of kStages
+// slices of kBK k filled by copies straight from memory to LDS, one barrier a slice, and a step's MFMAs from registers while the
+// next step's fragments are read and later slices' copies are issued between them.
+//
+// The barrier before a slice's last step finds all its fragments read: it publishes the next slice's copies and
+// frees this slice's stage for its refill.
+//
+// kRagged: extents that are no multiples of the tile: copies through buffer loads that land zeros outside the matrices, stores
+// inside alone. K is a multiple of 16 (rows of others are copied into padded ones first).
+#pragma once
+
+#include "gemm.h"
+#include "gemm_i8.h"
+#include "lds_dma.h"
+
+namespace kg_gfx950 {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+namespace gemmi {
+constexpr int kThreads = 256;
+// acc += a b on one 16 x 16 block. The tied form keeps the accumulator in one register tuple of the accumulation file, for tiles
+// whose accumulators fill it (as gemm_quad_kernel's); its results are read behind mfma_drain and mfma_order.
+template <bool kTied>
+__device__ __forceinline__ void mfma(i32x4& acc, u32x4 a, u32x4 b) {
+  if constexpr (kTied) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  else acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), acc, 0, 0, 0);
+}
+// more than the instruction's result latency (8 passes) before its result is read
+__device__ __forceinline__ void mfma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void mfma_order(i32x4 (&a)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+a"(a[i]));
+}
+// 16-byte chunk c of a row lies at c ^ swizzle(row): the fragments' reads hit distinct banks
+template <int kBK>
+__device__ __forceinline__ int swizzle(int row) {
+  if constexpr (kBK == 64) return (row >> 2) & 3;
+  else return (row >> 1) & 7;
+}
+}  // namespace gemmi
+
+struct Int8Tiles {
+  const int8_t *x, *w;
+  const float *x_scale, *w_scale;
+  const void* bias;
+  void* out;
+  long long ldx, ldw, ldo, x_scale_stride, w_scale_stride, bias_stride;
+  int m, n, k;
+  bool wide_bias, vectors;  // vectors: rows of out are whole 16-byte pieces
+};
+
+template <typename T, int NA, int NB, int kBK, int kStages, bool kRagged>
+__global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8_kernel(Int8Tiles g) {
+  using namespace gemmi;
+  constexpr int TM = 32 * NA, TN = 32 * NB;
+  constexpr int kSteps = kBK / 64;
+  constexpr bool kTied = NA * NB == 64;
+  constexpr int kRowsPiece = 1024 / kBK;  // rows of a wave's copy
+  constexpr int AP = TM / kRowsPiece / 4, BP = TN / kRowsPiece / 4, kPieces = AP + BP;  // copies per wave and slice
+  constexpr int kStageA = TM * kBK, kStageB = TN * kBK, kStage = kStageA + kStageB;
+  constexpr int kMfmas = NA * NB, kReads = NA + NB;
+  static_assert(kSteps == 1 || kSteps == 2, "steps");
+  static_assert(AP >= 1 && BP >= 1 && kPieces % kSteps == 0, "pieces");
+  static_assert(kStages >= 2 && (kSteps == 2 || kStages % 2 == 0), "a step's registers are constants of the unrolled ring");
+  static_assert(sizeof(T) == 4 || kStages * kStage >= TM * TN * 2, "the tile's 16-bit results fit the ring");
+  __shared__ __attribute__((aligned(1024))) char lds[kStages * kStage];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int l16 = lane & 15, lg = lane >> 4;
+  const int tiles_n = (g.n + TN - 1) / TN, tiles_m = (g.m + TM - 1) / TM;
+  // each XCD takes a contiguous range of tiles in groups of 4 tile rows (few panels per L2)
+  const int total = gridDim.x, xcd = blockIdx.x % 8;
+  const int logical = xcd * (total / 8) + min(xcd, total % 8) + blockIdx.x / 8;
+  constexpr int kGroupM = 4;
+  const int group = logical / (kGroupM * tiles_n), first_m = group * kGroupM;
+  const int gm = min(tiles_m - first_m, kGroupM), in_group = logical - group * kGroupM * tiles_n;
+  const int m0 = (first_m + in_group % gm) * TM, n0 = (in_group / gm) * TN;
+
+  // ---- memory -> LDS: piece p of a wave is rows (wave AP + p) kRowsPiece + lane / (kBK / 16) ----
+  constexpr int kChunks = kBK / 16;
+  uint32_t a_off[AP], b_off[BP];
+  int chunk_k[2];  // the k of a lane's chunk within the slice, by the parity of the piece's first row / 8
+#pragma unroll
+  for (int p = 0; p < AP; ++p) {
+    const int row = (wave * AP + p) * kRowsPiece + lane / kChunks;
+    a_off[p] = (uint32_t)(row * g.ldx + 16 * ((lane % kChunks) ^ swizzle<kBK>(row)));
+    if (kRagged && m0 + row >= g.m) a_off[p] = kBufOOB;
+  }
+#pragma unroll
+  for (int p = 0; p < BP; ++p) {
+    const int row = (wave * BP + p) * kRowsPiece + lane / kChunks;
+    b_off[p] = (uint32_t)(row * g.ldw + 16 * ((lane % kChunks) ^ swizzle<kBK>(row)));
+    if (kRagged && n0 + row >= g.n) b_off[p] = kBufOOB;
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) chunk_k[x] = 16 * ((lane % kChunks) ^ swizzle<kBK>(x * kRowsPiece + lane / kChunks));
+  const char* a_tile = reinterpret_cast<const char*>(g.x) + (long long)m0 * g.ldx;
+  const char* b_tile = reinterpret_cast<const char*>(g.w) + (long long)n0 * g.ldw;
+  const uint32_t lds0 = lds_addr(lds);
+  auto issue_piece = [&](int kt, int stage, int piece) __attribute__((always_inline)) {
+    const bool a = piece < AP;
+    const int p = a ? piece : piece - AP;
+    const char* src = (a ? a_tile : b_tile) + (long long)kt * kBK;
+    const uint32_t dst = lds0 + stage * kStage + (a ? (wave * AP + p) * 1024 : kStageA + (wave * BP + p) * 1024);
+    const uint32_t off = a ? a_off[a ? p : 0] : b_off[a ? 0 : p];
+    if constexpr (kRagged) {
+      const int k = chunk_k[kBK == 64 ? 0 : ((a ? wave * AP : wave * BP) + p) & 1];
+      buf2lds16_s(kt * kBK + k < g.k ? off : kBufOOB, src, dst);
+    } else {
+      g2lds16_s(off, src, dst);
+    }
+  };
+
+  // ---- fragments of step ks: rows 16 i + lane % 16 of the wave's half, chunk 4 ks + lane / 16 ----
+  uint32_t a_rd[kSteps], b_rd[kSteps];
+#pragma unroll
+  for (int ks = 0; ks < kSteps; ++ks) {
+    const int at = 16 * ((4 * ks + lg) ^ swizzle<kBK>(l16));
+    a_rd[ks] = lds0 + (wm * 16 * NA + l16) * kBK + at;
+    b_rd[ks] = lds0 + kStageA + (wn * 16 * NB + l16) * kBK + at;
+  }
+  struct Frags {
+    u32x4 a[NA], b[NB];
+  };
+  auto read_step = [&](int stage, int ks, Frags& f, int r) __attribute__((always_inline)) {  // w first
+    const uint32_t at = (r < NB ? b_rd[ks] + r * 16 * kBK : a_rd[ks] + (r - NB) * 16 * kBK) + stage * kStage;
+    const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
+    if (r < NB) f.b[r < NB ? r : 0] = v;
+    else f.a[r < NB ? 0 : r - NB] = v;
+  };
+
+  i32x4 acc[NA][NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  if constexpr (kTied) {
+    // (opaque from here on: zeros made again right before the first MFMAs would lack the wait that these need)
+#pragma unroll
+    for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
+  }
+
+  const int nk = (g.k + kBK - 1) / kBK;
+#pragma unroll
+  for (int st = 0; st < kStages; ++st)
+    if (st < nk)
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) issue_piece(st, st, p);
+  auto wait_younger = [&](int younger) __attribute__((always_inline)) {
+    if (kStages > 4 && younger >= 4) wait_and_barrier<(kStages > 4 ? 4 : 0) * kPieces>();
+    else if (kStages > 3 && younger >= 3) wait_and_barrier<(kStages > 3 ? 3 : 0) * kPieces>();
+    else if (kStages > 2 && younger >= 2) wait_and_barrier<(kStages > 2 ? 2 : 0) * kPieces>();
+    else if (younger >= 1) wait_and_barrier<kPieces>();
+    else wait_and_barrier<0>();
+  };
+  wait_younger(min(kStages, nk) - 1);
+  Frags fr[2];
+#pragma unroll
+  for (int r = 0; r < kReads; ++r) read_step(0, 0, fr[0], r);
+
+  // Slice kt in stage S. kSteady: slices up to kt + kStages exist. The refill of stage S (slice kt + kStages) goes into the last
+  // step, behind its barrier, and where there are two steps half of it into the next slice's first.
+  auto slice = [&](int kt, auto stage_tag, auto steady_tag) __attribute__((always_inline)) {
+    constexpr int S = decltype(stage_tag)::value;
+    constexpr bool kSteady = decltype(steady_tag)::value != 0;
+    constexpr int kPrev = (S + kStages - 1) % kStages, kNext = (S + 1) % kStages, kCopies = kPieces / kSteps;
+    const bool more = kSteady || kt + 1 < nk;
+    const bool refill_before = kSteady || (kt >= 1 && kt - 1 + kStages < nk);  // (the first slice: the prologue filled all stages)
+    const bool refill = kSteady || kt + kStages < nk;
+    static_for<kSteps>([&](auto step_tag) __attribute__((always_inline)) {
+      constexpr int ks = decltype(step_tag)::value;
+      constexpr bool kLast = ks == kSteps - 1;
+      constexpr int P = kSteps == 2 ? ks : S & 1;
+      if constexpr (kLast) {
+        if constexpr (kSteady) wait_and_barrier<(kStages - 2) * kPieces>();
+        else if (more) wait_younger(min(kStages - 2, nk - 2 - kt));
+      }
+      static_for<kMfmas>([&](auto idx_tag) __attribute__((always_inline)) {
+        constexpr int idx = decltype(idx_tag)::value;
+        constexpr int i = idx / NB, j = idx % NB;
+        mfma<kTied>(acc[i][j], fr[P].b[j], fr[P].a[i]);  // blocks of the transpose: a lane's columns lie side by side
+        constexpr int r0 = (idx * 2 * kReads + kMfmas - 1) / kMfmas, r1 = ((idx + 1) * 2 * kReads + kMfmas - 1) / kMfmas;
+        static_for<(r1 < kReads ? r1 : kReads) - (r0 < kReads ? r0 : kReads)>([&](auto r_tag) __attribute__((always_inline)) {
+          constexpr int r = r0 + decltype(r_tag)::value;
+          if constexpr (!kLast) read_step(S, 1, fr[P ^ 1], r);
+          else if (more) read_step(kNext, 0, fr[P ^ 1], r);
+        });
+        static_for<kCopies>([&](auto c_tag) __attribute__((always_inline)) {
+          constexpr int c = decltype(c_tag)::value;
+          if constexpr (idx == (2 * c + 1) * kMfmas / (2 * kCopies)) {
+            if constexpr (kLast) {
+              if (refill) issue_piece(kt + kStages, S, c);
+            } else {
+              if (refill_before) issue_piece(kt - 1 + kStages, kPrev, kCopies + c);
+            }
+          }
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
+  };
+  auto turn = [&](int kt0, auto steady_tag) __attribute__((always_inline)) {
+    static_for<kStages>([&](auto u_tag) __attribute__((always_inline)) {
+      constexpr int u = decltype(u_tag)::value;
+      if (decltype(steady_tag)::value == 1 || kt0 + u < nk) slice(kt0 + u, gemmp::StageIdx<u>{}, steady_tag);
+    });
+  };
+  int kt = 0;
+  if (kSteps == 2 && nk > 0) {  // (the first turn's first step has no refill)
+    turn(0, Int<0>{});
+    kt = kStages;
+  }
+  for (; kt + 2 * kStages <= nk; kt += kStages) turn(kt, Int<1>{});
+  for (; kt < nk; kt += kStages) turn(kt, Int<0>{});
+
+  // ---- a lane holds out[16 i + lane % 16][16 j + 4 (lane / 16) .. + 3] of each block (i, j) ----
+  if constexpr (kTied) {
+    mfma_drain();
+#pragma unroll
+    for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
+  }
+  wait_and_barrier<0>();  // the ring is read
+  const int mw = m0 + wm * 16 * NA, nw = n0 + wn * 16 * NB;
+  float xs[NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) xs[i] = g.x_scale[(long long)min(mw + 16 * i + l16, g.m - 1) * g.x_scale_stride];
+  constexpr int kRow = 32 * NB, kRowChunks = kRow / 16;  // bytes and chunks of a row of 16-bit results
+  const uint32_t region = lds0 + wave * 16 * NA * kRow;
+  auto row_swizzle = [](int r) { return kRowChunks == 4 ? (r >> 1) & 3 : r & (kRowChunks - 1); };
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int n = nw + 16 * j + 4 * lg;
+    float ws[4], bv[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long long at = kRagged ? min(n + e, g.n - 1) : n + e;
+      ws[e] = g.w_scale[at * g.w_scale_stride];
+      if (g.bias != nullptr)
+        bv[e] = g.wide_bias ? static_cast<const float*>(g.bias)[at * g.bias_stride] : Elem<T>::load(static_cast<const T*>(g.bias) + at * g.bias_stride);
+    }
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)acc[i][j][e] * xs[i], ws[e], bv[e]);
+      if constexpr (sizeof(T) == 4) {
+        const int m = mw + 16 * i + l16;
+        float* to = static_cast<float*>(g.out) + m * g.ldo + n;
+        if (!kRagged || (m < g.m && n + 4 <= g.n)) {
+          if (g.vectors) {
+            *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+            continue;
+          }
+        }
+        if (!kRagged || m < g.m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!kRagged || n + e < g.n) to[e] = v[e];
+      } else {
+        using H = Half16<typename Eight<T>::Tag>;
+        const u32x2 packed = {H::pack2(v[0], v[1]), H::pack2(v[2], v[3])};
+        const int r = 16 * i + l16;
+        const uint32_t at = region + r * kRow + (((2 * j + (lg >> 1)) ^ row_swizzle(r)) * 16) + (lg & 1) * 8;
+        *(__attribute__((address_space(3))) u32x2*)(uintptr_t)at = packed;
+      }
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    // whole row segments, 16 bytes a lane, of what the wave itself packed
+    constexpr int kRowsStore = 64 / kRowChunks;
+#pragma unroll
+    for (int q = 0; q < 16 * NA / kRowsStore; ++q) {
+      const int r = kRowsStore * q + lane / kRowChunks, c = lane % kRowChunks;
+      const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(region + r * kRow + ((c ^ row_swizzle(r)) * 16));
+      const int m = mw + r, n = nw + 8 * c;
+      if (kRagged && (m >= g.m || n >= g.n)) continue;
+      uint16_t* to = static_cast<uint16_t*>(g.out) + (long long)m * g.ldo + n;
+      if (g.vectors && (!kRagged || n + 8 <= g.n)) {
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < g.n) to[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+}
+
+template <typename T, int NA, int NB, int kBK, int kStages>
+hipError_t launch_gemm_i8(const Int8Tiles& g, hipStream_t stream) {
+  constexpr int TM = 32 * NA, TN = 32 * NB;
+  const unsigned grid = (unsigned)(((long long)g.m + TM - 1) / TM * (((long long)g.n + TN - 1) / TN));
+  const bool ragged = g.m % TM != 0 || g.n % TN != 0 || g.k % kBK != 0;
+  if (ragged) hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages, true>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
+  else hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages, false>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
+  return hipGetLastError();
+}
+
+}  // namespace kg_gfx950

@@ -39,6 +39,7 @@
 #include "kg_gfx950/quantize.h"
 #include "kg_gfx950/tree_attn.h"
 #include "kg_gfx950/instances.h"  // the heavy kernel families are compiled in their own translation units
+#include "kg_gfx950/instances_int8.h"
 
 namespace {
 
@@ -1924,12 +1925,10 @@ int with_float_type(int dtype, F&& f) {
   return dtype == KG_DTYPE_F32 ? f(float{}) : dtype == KG_DTYPE_BF16 ? f((__bf16)0.f) : f((_Float16)0.f);
 }
 
-int launch_quantize(const QuantizeArgs& a, int dtype) {
-  return with_float_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    hipLaunchKernelGGL((quantize_rows_any_kernel<T>), dim3(most_blocks(a.rows)), dim3(256), 0, g_stream, a);
-    return finish_launch("quantize_rows");
-  });
+hipError_t launch_quantize_rows(const QuantizeArgs& a, int dtype) {
+  return dtype == KG_DTYPE_F32 ? launch_quantize<float>(a, g_stream)
+         : dtype == KG_DTYPE_BF16 ? launch_quantize<__bf16>(a, g_stream)
+                                  : launch_quantize<_Float16>(a, g_stream);
 }
 
 int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
@@ -1950,7 +1949,86 @@ int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
   if (M == 0) return finish_launch("quantize_rows(empty)");
   QuantizeArgs a{x.data, static_cast<int8_t*>(codes.data), static_cast<float*>(scale.data), x.stride[0], codes.stride[0],
                  scale.stride[0], (int)M, (int)K, (int)K};
-  return launch_quantize(a, x.dtype);
+  (void)launch_quantize_rows(a, x.dtype);
+  return finish_launch("quantize_rows");
+}
+
+// Rows that the few-row kernels take.
+constexpr long long kInt8FewRows = 64;
+
+// Rows of the square tiles that a product takes.
+int int8_tile(long long M, long long N) {
+  if (cdiv(M, 256) * cdiv(N, 256) >= 192) return 256;
+  if (cdiv(M, 128) * cdiv(N, 128) >= 160) return 128;
+  return 64;
+}
+
+// The matrix-core forms of int8_matmul. kUnsupported: none of them, since there is no workspace to be had, or not enough.
+template <typename T>
+int launch_int8(const Int8Args& a, bool codes, bool out_aligned, bool x_aligned, bool w_aligned) {
+  const bool few = a.m <= kInt8FewRows;
+  Int8Tiles g{static_cast<const int8_t*>(a.x), a.w, a.x_scale, a.w_scale, a.bias, a.out, a.x_row, a.w_row, a.out_row,
+              a.x_scale_stride, a.w_scale_stride, a.bias_stride, a.m, a.n, a.k, a.wide_bias, out_aligned};
+  if constexpr (sizeof(T) == 2) {
+    if (!codes && a.m <= 16 && a.k <= kInt8FewQuantizeMostK) {
+      (void)launch_int8_few_quantize<T>(g, a.x, a.x_row, 16, g_stream);
+      return finish_launch("int8_matmul");
+    }
+  }
+  // rows and weights in the workspace: codes of rows that are quantised here; for the tiles, copies of rows that are not whole 16-byte pieces
+  const long long pitch = cdiv(a.k, 64) * 64;
+  const bool whole = a.k % 16 == 0;
+  const bool take_x = !codes || (!few && !(whole && x_aligned && a.x_row <= kMaxPipeLd));
+  const bool take_w = !few && !(whole && w_aligned && a.w_row <= kMaxPipeLd);
+  const long long w_bytes = take_w ? a.n * pitch : 0, row_bytes = take_x ? pitch + (codes ? 0 : (long long)sizeof(float)) : 0;
+  const long long room = kSplitMaxWorkspace - w_bytes - 512;
+  long long rows = a.m;  // of a piece that the workspace holds: whole tiles
+  if (row_bytes > 0 && a.m * row_bytes > room) rows = room / row_bytes / 256 * 256;
+  if (rows <= 0) return kUnsupported;
+  SplitLease lease;  // held until the kernels are enqueued
+  char* ws = nullptr;
+  if (take_x || take_w) {
+    lease = split_workspace((size_t)(w_bytes + rows * row_bytes + 512), g_stream);
+    if ((ws = static_cast<char*>(lease.ptr)) == nullptr) return kUnsupported;
+  }
+  auto pack = [&](const int8_t* from, long long ld, char* to, int count) {
+    hipLaunchKernelGGL((int8_pack_kernel<>), dim3((unsigned)std::min(cdiv(count * (pitch / 16), 256), 4096ll)), dim3(256), 0, g_stream, from, ld,
+                       reinterpret_cast<int8_t*>(to), (int)pitch, count, a.k);
+  };
+  if (take_w) {
+    pack(a.w, a.w_row, ws, a.n);
+    g.w = reinterpret_cast<const int8_t*>(ws);
+    g.ldw = pitch;
+  }
+  char* x_ws = ws + w_bytes;
+  for (long long m0 = 0; m0 < a.m; m0 += rows) {
+    g.m = (int)std::min(rows, a.m - m0);
+    g.out = static_cast<T*>(a.out) + m0 * a.out_row;
+    if (codes) {
+      g.x_scale = a.x_scale + m0 * a.x_scale_stride;
+      g.x = static_cast<const int8_t*>(a.x) + m0 * a.x_row;
+      if (take_x) pack(g.x, a.x_row, x_ws, g.m);
+    } else {
+      float* scales = reinterpret_cast<float*>(x_ws + cdiv(rows * pitch, 256) * 256);
+      const QuantizeArgs q{static_cast<const T*>(a.x) + m0 * a.x_row, reinterpret_cast<int8_t*>(x_ws), scales, a.x_row, pitch, 1,
+                           g.m, a.k, (int)pitch};
+      (void)launch_quantize<T>(q, g_stream);
+      g.x_scale = scales;
+      g.x_scale_stride = 1;
+    }
+    if (take_x) {
+      g.x = reinterpret_cast<const int8_t*>(x_ws);
+      g.ldx = pitch;
+    }
+    if (few) {
+      (void)launch_int8_few<T>(g, g.m <= 16 ? 16 : g.m <= 32 ? 32 : 64, 16, g_stream);
+    } else {
+      if (take_x && take_w) g.k = (int)pitch;  // (zeros behind the rows' ends)
+      else g.k = (int)(cdiv(a.k, 16) * 16);
+      (void)launch_int8_tiles<T>(g, int8_tile(g.m, g.n), g_stream);
+    }
+  }
+  return finish_launch("int8_matmul");
 }
 
 int int8_matmul_impl(const KgArgSlot* args, unsigned long long n) {
@@ -1985,11 +2063,15 @@ int int8_matmul_impl(const KgArgSlot* args, unsigned long long n) {
       (rc = check_view(w, "weight")) || (rc = check_view(w_scale, "w_scale")) || (rc = check_view(bias, "bias")))
     return rc;
   if (M == 0 || N == 0) return finish_launch("int8_matmul(empty)");
-  Int8Args a{x.data, static_cast<const int8_t*>(w.data), static_cast<const float*>(x_scale.data),
-             static_cast<const float*>(w_scale.data), bias.data, out.data, x.stride[0], w.stride[0], out.stride[0],
-             x_scale.stride[0], w_scale.stride[0], bias.stride[0], (int)M, (int)N, (int)K, bias.dtype == KG_DTYPE_F32};
+  const Int8Args a{x.data, static_cast<const int8_t*>(w.data), static_cast<const float*>(x_scale.data),
+                   static_cast<const float*>(w_scale.data), bias.data, out.data, x.stride[0], w.stride[0], out.stride[0],
+                   x_scale.stride[0], w_scale.stride[0], bias.stride[0], (int)M, (int)N, (int)K, bias.dtype == KG_DTYPE_F32};
   return with_float_type(out.dtype, [&](auto t) {
     using T = decltype(t);
+    if (K >= 16) {
+      const int done = launch_int8<T>(a, codes, rows_aligned(out, 16), rows_aligned(x, 16), rows_aligned(w, 16));
+      if (done != kUnsupported) return done;
+    }
     const unsigned grid = most_blocks(M * cdiv(N, 64));
     if (codes) hipLaunchKernelGGL((int8_any_kernel<T, int8_t>), dim3(grid), dim3(256), 0, g_stream, a);
     else hipLaunchKernelGGL((int8_any_kernel<T, T>), dim3(grid), dim3(256), 0, g_stream, a);
