@@ -39,7 +39,7 @@ __device__ __forceinline__ void mfma_order(i32x4 (&a)[N]) {
 // 16-byte chunk c of a row lies at c ^ swizzle(row): the fragments' reads hit distinct banks
 template <int kBK>
 __device__ __forceinline__ int swizzle(int row) {
-  if constexpr (kBK == 64) return (row >> 2) & 3;
+  if constexpr (kBK == 64) return (row >> 1) & 3;
   else return (row >> 1) & 7;
 }
 }  // namespace gemmi
@@ -69,6 +69,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   static_assert(kStages >= 2 && (kSteps == 2 || kStages % 2 == 0), "a step's registers are constants of the unrolled ring");
   static_assert(sizeof(T) == 4 || kStages * kStage >= TM * TN * 2, "the tile's 16-bit results fit the ring");
   __shared__ __attribute__((aligned(1024))) char lds[kStages * kStage];
+  __shared__ __attribute__((aligned(16))) float xs_lds[TM], ws_lds[TN], bias_lds[TN];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -82,6 +83,10 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   const int group = logical / (kGroupM * tiles_n), first_m = group * kGroupM;
   const int gm = min(tiles_m - first_m, kGroupM), in_group = logical - group * kGroupM * tiles_n;
   const int m0 = (first_m + in_group % gm) * TM, n0 = (in_group / gm) * TN;
+
+  // slices of K; in the one-step form a multiple of two (registers go by a slice's parity), and at least a ring of them: kRagged, zeros
+  const int slices = (g.k + kBK - 1) / kBK;
+  const int count = max(kSteps == 1 ? (slices + 1) / 2 * 2 : slices, kStages);
 
   // ---- memory -> LDS: piece p of a wave is rows (wave AP + p) kRowsPiece + lane / (kBK / 16) ----
   constexpr int kChunks = kBK / 16;
@@ -129,12 +134,29 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   struct Frags {
     u32x4 a[NA], b[NB];
   };
-  auto read_step = [&](int stage, int ks, Frags& f, int r) __attribute__((always_inline)) {  // w first
-    const uint32_t at = (r < NB ? b_rd[ks] + r * 16 * kBK : a_rd[ks] + (r - NB) * 16 * kBK) + stage * kStage;
+  // (a step's two addresses by themselves: the blocks' distances are then the instructions' own offsets)
+  uint32_t b_at = 0, a_at = 0;
+  auto read_from = [&](int stage, int ks) __attribute__((always_inline)) {
+    b_at = b_rd[ks] + stage * kStage;
+    a_at = a_rd[ks] + stage * kStage;
+    asm volatile("" : "+v"(b_at), "+v"(a_at));
+  };
+  auto read_step = [&](Frags& f, int r) __attribute__((always_inline)) {  // w first
+    const uint32_t at = r < NB ? b_at + r * 16 * kBK : a_at + (r - NB) * 16 * kBK;
     const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
     if (r < NB) f.b[r < NB ? r : 0] = v;
     else f.a[r < NB ? 0 : r - NB] = v;
   };
+
+  // scales and bias of the tile: read ahead of the K loop, into LDS behind it
+  float xs_own = 0.f, ws_own = 0.f, bias_own = 0.f;
+  if (tid < TM) xs_own = g.x_scale[(long long)min(m0 + tid, g.m - 1) * g.x_scale_stride];
+  if (tid < TN) {
+    const long long at = min(n0 + tid, g.n - 1);
+    ws_own = g.w_scale[at * g.w_scale_stride];
+    if (g.bias != nullptr)
+      bias_own = g.wide_bias ? static_cast<const float*>(g.bias)[at * g.bias_stride] : Elem<T>::load(static_cast<const T*>(g.bias) + at * g.bias_stride);
+  }
 
   i32x4 acc[NA][NB];
 #pragma unroll
@@ -147,41 +169,33 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
     for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
   }
 
-  const int nk = (g.k + kBK - 1) / kBK;
+  constexpr int kCopies = kPieces / kSteps;  // a step's
 #pragma unroll
-  for (int st = 0; st < kStages; ++st)
-    if (st < nk)
+  for (int i = 0; i < kStages; ++i)
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p) issue_piece(st, st, p);
-  auto wait_younger = [&](int younger) __attribute__((always_inline)) {
-    if (kStages > 4 && younger >= 4) wait_and_barrier<(kStages > 4 ? 4 : 0) * kPieces>();
-    else if (kStages > 3 && younger >= 3) wait_and_barrier<(kStages > 3 ? 3 : 0) * kPieces>();
-    else if (kStages > 2 && younger >= 2) wait_and_barrier<(kStages > 2 ? 2 : 0) * kPieces>();
-    else if (younger >= 1) wait_and_barrier<kPieces>();
-    else wait_and_barrier<0>();
-  };
-  wait_younger(min(kStages, nk) - 1);
+    for (int p = 0; p < kPieces; ++p)
+      if (kSteps == 1 || i < kStages - 1 || p < kCopies) issue_piece(i, i, p);  // (two steps: the first slice brings the last one's second half)
+  wait_and_barrier<(kStages - 2) * kPieces + kCopies>();
   Frags fr[2];
+  read_from(0, 0);
 #pragma unroll
-  for (int r = 0; r < kReads; ++r) read_step(0, 0, fr[0], r);
+  for (int r = 0; r < kReads; ++r) read_step(fr[0], r);
 
-  // Slice kt in stage S. kSteady: slices up to kt + kStages exist. The refill of stage S (slice kt + kStages) goes into the last
-  // step, behind its barrier, and where there are two steps half of it into the next slice's first.
-  auto slice = [&](int kt, auto stage_tag, auto steady_tag) __attribute__((always_inline)) {
-    constexpr int S = decltype(stage_tag)::value;
-    constexpr bool kSteady = decltype(steady_tag)::value != 0;
-    constexpr int kPrev = (S + kStages - 1) % kStages, kNext = (S + 1) % kStages, kCopies = kPieces / kSteps;
-    const bool more = kSteady || kt + 1 < nk;
-    const bool refill_before = kSteady || (kt >= 1 && kt - 1 + kStages < nk);  // (the first slice: the prologue filled all stages)
-    const bool refill = kSteady || kt + kStages < nk;
+  // Slice kt, in stage `stage`, its registers by kParity. kBehind: slices behind it, kStages where there are so many. The refill of its
+  // stage (slice kt + kStages) goes into the last step, behind its barrier, and where there are two steps half of it into the next
+  // slice's first. The last kStages slices are a compile-time group whose waits, reads and copies carry no conditions (with
+  // conditions they took about twice a steady one's cycles).
+  auto slice = [&](int kt, int stage, auto parity_tag, auto behind_tag) __attribute__((always_inline)) {
+    constexpr int kParity = decltype(parity_tag)::value, kBehind = decltype(behind_tag)::value;
+    constexpr int kYounger = (kBehind < kStages - 1 ? kBehind : kStages - 1) - 1;  // slices behind the next one that are on their way
+    const int next = stage + 1 == kStages ? 0 : stage + 1, before = stage == 0 ? kStages - 1 : stage - 1;
     static_for<kSteps>([&](auto step_tag) __attribute__((always_inline)) {
       constexpr int ks = decltype(step_tag)::value;
       constexpr bool kLast = ks == kSteps - 1;
-      constexpr int P = kSteps == 2 ? ks : S & 1;
-      if constexpr (kLast) {
-        if constexpr (kSteady) wait_and_barrier<(kStages - 2) * kPieces>();
-        else if (more) wait_younger(min(kStages - 2, nk - 2 - kt));
-      }
+      constexpr int P = kSteps == 2 ? ks : kParity;
+      if constexpr (kLast && kBehind > 0) wait_and_barrier<(kYounger > 0 ? kYounger : 0) * kPieces>();
+      if constexpr (!kLast) read_from(stage, 1);
+      else if constexpr (kBehind > 0) read_from(next, 0);
       static_for<kMfmas>([&](auto idx_tag) __attribute__((always_inline)) {
         constexpr int idx = decltype(idx_tag)::value;
         constexpr int i = idx / NB, j = idx % NB;
@@ -189,36 +203,35 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
         constexpr int r0 = (idx * 2 * kReads + kMfmas - 1) / kMfmas, r1 = ((idx + 1) * 2 * kReads + kMfmas - 1) / kMfmas;
         static_for<(r1 < kReads ? r1 : kReads) - (r0 < kReads ? r0 : kReads)>([&](auto r_tag) __attribute__((always_inline)) {
           constexpr int r = r0 + decltype(r_tag)::value;
-          if constexpr (!kLast) read_step(S, 1, fr[P ^ 1], r);
-          else if (more) read_step(kNext, 0, fr[P ^ 1], r);
+          if constexpr (!kLast || kBehind > 0) read_step(fr[P ^ 1], r);
         });
         static_for<kCopies>([&](auto c_tag) __attribute__((always_inline)) {
           constexpr int c = decltype(c_tag)::value;
           if constexpr (idx == (2 * c + 1) * kMfmas / (2 * kCopies)) {
-            if constexpr (kLast) {
-              if (refill) issue_piece(kt + kStages, S, c);
-            } else {
-              if (refill_before) issue_piece(kt - 1 + kStages, kPrev, kCopies + c);
-            }
+            if constexpr (kLast && kBehind == kStages) issue_piece(kt + kStages, stage, c);
+            if constexpr (!kLast && kBehind >= kStages - 1) issue_piece(kt - 1 + kStages, before, kCopies + c);
           }
         });
         __builtin_amdgcn_sched_barrier(0);
       });
     });
   };
-  auto turn = [&](int kt0, auto steady_tag) __attribute__((always_inline)) {
-    static_for<kStages>([&](auto u_tag) __attribute__((always_inline)) {
-      constexpr int u = decltype(u_tag)::value;
-      if (decltype(steady_tag)::value == 1 || kt0 + u < nk) slice(kt0 + u, gemmp::StageIdx<u>{}, steady_tag);
-    });
-  };
-  int kt = 0;
-  if (kSteps == 2 && nk > 0) {  // (the first turn's first step has no refill)
-    turn(0, Int<0>{});
-    kt = kStages;
+  int kt = 0, stage = 0;
+  auto step = [&]() __attribute__((always_inline)) { stage = stage + 1 == kStages ? 0 : stage + 1; };
+#pragma unroll 1
+  for (; kt + kStages < count; kt += 3 - kSteps) {
+    slice(kt, stage, Int<0>{}, Int<kStages>{});
+    step();
+    if constexpr (kSteps == 1) {
+      slice(kt + 1, stage, Int<1>{}, Int<kStages>{});
+      step();
+    }
   }
-  for (; kt + 2 * kStages <= nk; kt += kStages) turn(kt, Int<1>{});
-  for (; kt < nk; kt += kStages) turn(kt, Int<0>{});
+  static_for<kStages>([&](auto u_tag) __attribute__((always_inline)) {
+    constexpr int u = decltype(u_tag)::value;
+    slice(kt + u, stage, Int<(kSteps == 1 ? u & 1 : 0)>{}, Int<kStages - 1 - u>{});
+    step();
+  });
 
   // ---- a lane holds out[16 i + lane % 16][16 j + 4 (lane / 16) .. + 3] of each block (i, j) ----
   if constexpr (kTied) {
@@ -226,25 +239,21 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
 #pragma unroll
     for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
   }
+  if (tid < TM) xs_lds[tid] = xs_own;
+  if (tid < TN) ws_lds[tid] = ws_own, bias_lds[tid] = bias_own;
   wait_and_barrier<0>();  // the ring is read
   const int mw = m0 + wm * 16 * NA, nw = n0 + wn * 16 * NB;
   float xs[NA];
 #pragma unroll
-  for (int i = 0; i < NA; ++i) xs[i] = g.x_scale[(long long)min(mw + 16 * i + l16, g.m - 1) * g.x_scale_stride];
+  for (int i = 0; i < NA; ++i) xs[i] = xs_lds[wm * 16 * NA + 16 * i + l16];
   constexpr int kRow = 32 * NB, kRowChunks = kRow / 16;  // bytes and chunks of a row of 16-bit results
   const uint32_t region = lds0 + wave * 16 * NA * kRow;
   auto row_swizzle = [](int r) { return kRowChunks == 4 ? (r >> 1) & 3 : r & (kRowChunks - 1); };
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int n = nw + 16 * j + 4 * lg;
-    float ws[4], bv[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const long long at = kRagged ? min(n + e, g.n - 1) : n + e;
-      ws[e] = g.w_scale[at * g.w_scale_stride];
-      if (g.bias != nullptr)
-        bv[e] = g.wide_bias ? static_cast<const float*>(g.bias)[at * g.bias_stride] : Elem<T>::load(static_cast<const T*>(g.bias) + at * g.bias_stride);
-    }
+    const f32x4 ws = *reinterpret_cast<const f32x4*>(&ws_lds[wn * 16 * NB + 16 * j + 4 * lg]);
+    const f32x4 bv = *reinterpret_cast<const f32x4*>(&bias_lds[wn * 16 * NB + 16 * j + 4 * lg]);
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       float v[4];
@@ -271,6 +280,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
         *(__attribute__((address_space(3))) u32x2*)(uintptr_t)at = packed;
       }
     }
+    __builtin_amdgcn_sched_barrier(0);  // (a column of blocks at a time: all of them at once are more than the registers hold)
   }
   if constexpr (sizeof(T) == 2) {
     // whole row segments, 16 bytes a lane, of what the wave itself packed
@@ -297,7 +307,8 @@ template <typename T, int NA, int NB, int kBK, int kStages>
 hipError_t launch_gemm_i8(const Int8Tiles& g, hipStream_t stream) {
   constexpr int TM = 32 * NA, TN = 32 * NB;
   const unsigned grid = (unsigned)(((long long)g.m + TM - 1) / TM * (((long long)g.n + TN - 1) / TN));
-  const bool ragged = g.m % TM != 0 || g.n % TN != 0 || g.k % kBK != 0;
+  // (pairs of slices of 64, or slices of 128, a ring of them at least)
+  const bool ragged = g.m % TM != 0 || g.n % TN != 0 || g.k % 128 != 0 || g.k < kStages * kBK;
   if (ragged) hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages, true>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
   else hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages, false>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
   return hipGetLastError();

@@ -4,6 +4,9 @@
 // of neighbours; elements behind 2 half stay as they are. All of it in 32 bits, rounded once to the output's type. A sum of
 // squares past 3.4e38 is infinite there, and the row 0.
 //
+// head_norm_kernel: L lanes per head, each with the W elements on both sides of its pairs (2 W side by side of neighbours), so that a
+// pair never leaves its lane, and G heads of a token at a time, whose reads are in flight together and whose angles and weights are read
+// once; half a multiple of W, D of 2 W, rows that start anywhere. Bound by its bytes where there are many.
 // head_norm_any_kernel: any D up to 512, half, strides and alignment: a wave per token and head, each lane some pairs of elements.
 #pragma once
 
@@ -86,6 +89,171 @@ __global__ __launch_bounds__(256) void head_norm_any_kernel(HeadNormArgs a) {
       if (second(u) < a.d) Elem<T>::store(y + second(u), e[i][1]);
     }
   }
+}
+
+// W elements from any address, in 32 bits, and back.
+template <typename T, int W>
+struct Elements {
+  static constexpr int kDwords = W * sizeof(T) / 4;
+  struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+    uint32_t w[kDwords];
+  };
+  static __device__ __forceinline__ void load(const T* p, float (&x)[W]) {
+    const Piece q = *reinterpret_cast<const Piece*>(p);
+#pragma unroll
+    for (int i = 0; i < kDwords; ++i) {
+      const uint32_t u = q.w[i];
+      if constexpr (sizeof(T) == 4) {
+        x[i] = __builtin_bit_cast(float, u);
+      } else {
+        using H = Half16<typename Eight<T>::Tag>;
+        x[2 * i] = H::to_float(u & 0xffffu);
+        x[2 * i + 1] = H::to_float(u >> 16);
+      }
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&x)[W]) {
+    Piece q;
+#pragma unroll
+    for (int i = 0; i < kDwords; ++i) {
+      if constexpr (sizeof(T) == 4) q.w[i] = __builtin_bit_cast(uint32_t, x[i]);
+      else q.w[i] = Half16<typename Eight<T>::Tag>::pack2(x[2 * i], x[2 * i + 1]);
+    }
+    *reinterpret_cast<Piece*>(p) = q;
+  }
+};
+
+struct HeadNormItems {
+  int items, chunks, chunks_q;  // of G heads: of a token, of its queries
+  PageDiv by_chunks;
+};
+
+// (weights, cos and sin contiguous)
+template <typename T, int W, int L, int G>
+__global__ __launch_bounds__(256) void head_norm_kernel(HeadNormArgs a, HeadNormItems n) {
+  using E = Elements<T, W>;
+  const int part = threadIdx.x % L;
+  const int item = blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (item >= n.items) return;
+  const int t = div_page(item, n.by_chunks), c = item - t * n.chunks;
+  const long long position = head_norm_position(a, t);
+  if (position < 0 || position >= a.table) return;
+  const bool keys = c >= n.chunks_q;
+  const HeadNormSide& s = a.side[keys];
+  const int h0 = (keys ? c - n.chunks_q : c) * G;
+  const bool in = 2 * W * part < a.d, turned = in && W * part < a.half;
+  // the lane's elements: first .. + W - 1 and second .. + W - 1
+  const int first = !in ? 0 : turned && !a.neighbours ? W * part : 2 * W * part;
+  const int second = !in ? 0 : turned && !a.neighbours ? a.half + W * part : 2 * W * part + W;
+  const T* x = static_cast<const T*>(s.x) + t * s.x_token;
+  float p[G][W], q[G][W];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const T* row = x + min(h0 + g, s.heads - 1) * s.x_head;
+    E::load(row + first, p[g]);
+    E::load(row + second, q[g]);
+  }
+  float cs[W], sn[W];
+  if (turned) {
+    Elements<float, W>::load(a.cos + position * a.cos_row + W * part, cs);
+    Elements<float, W>::load(a.sin + position * a.sin_row + W * part, sn);
+  }
+  if (s.w != nullptr) {
+    float u[W], v[W];
+    if (s.wide) {
+      Elements<float, W>::load(static_cast<const float*>(s.w) + first, u);
+      Elements<float, W>::load(static_cast<const float*>(s.w) + second, v);
+    } else {
+      E::load(static_cast<const T*>(s.w) + first, u);
+      E::load(static_cast<const T*>(s.w) + second, v);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) sum = __builtin_fmaf(p[g][i], p[g][i], __builtin_fmaf(q[g][i], q[g][i], sum));
+      if (!in) sum = 0.f;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      const float by = __builtin_amdgcn_rsqf(sum * a.inverse_d + a.eps);
+#pragma unroll
+      for (int i = 0; i < W; ++i) p[g][i] *= by * u[i], q[g][i] *= by * v[i];
+    }
+  }
+  if (turned) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (a.neighbours) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {  // pair i: elements 2 i and 2 i + 1 of both pieces in a row
+          float& e = 2 * i < W ? p[g][2 * i % W] : q[g][2 * i % W];
+          float& f = 2 * i < W ? p[g][(2 * i + 1) % W] : q[g][(2 * i + 1) % W];
+          const float r = e * cs[i] - f * sn[i];
+          f = f * cs[i] + e * sn[i];
+          e = r;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float r = p[g][i] * cs[i] - q[g][i] * sn[i];
+          q[g][i] = q[g][i] * cs[i] + p[g][i] * sn[i];
+          p[g][i] = r;
+        }
+      }
+    }
+  }
+  if (!in) return;
+  T* y = static_cast<T*>(s.y) + t * s.y_token;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    if (h0 + g >= s.heads) continue;
+    T* row = y + (h0 + g) * s.y_head;
+    E::store(row + first, p[g]);
+    E::store(row + second, q[g]);
+  }
+}
+
+// Whether the kernel above takes the call with pieces of `w` elements; 0 lanes: it does not.
+inline int head_norm_lanes(const HeadNormArgs& a, int w) {
+  if (a.half % w != 0 || a.d % (2 * w) != 0 || a.d / (2 * w) > 64) return 0;
+  for (const HeadNormSide& s : a.side)
+    if (s.w != nullptr && s.w_stride != 1) return 0;
+  if (a.half > 1 && (a.cos_stride != 1 || a.sin_stride != 1)) return 0;
+  int lanes = 4;
+  while (lanes * 2 * w < a.d) lanes *= 2;
+  return lanes;
+}
+
+template <typename T, int W, int G>
+bool launch_head_norm(const HeadNormArgs& a, int lanes, hipStream_t stream) {
+  HeadNormItems n;
+  n.chunks_q = (a.side[0].heads + G - 1) / G;
+  n.chunks = n.chunks_q + (a.side[1].heads + G - 1) / G;
+  const long long items = (long long)a.tokens * n.chunks, blocks = (items + 256 / lanes - 1) / (256 / lanes);
+  if (items > 0x7fffff00LL || blocks > (1 << 24) - 1) return false;
+  n.items = (int)items;
+  n.by_chunks = page_div(n.chunks);
+#define KG_HEAD_NORM(L) hipLaunchKernelGGL((head_norm_kernel<T, W, L, G>), dim3((unsigned)blocks), dim3(256), 0, stream, a, n)
+  if (lanes == 4) KG_HEAD_NORM(4);
+  else if (lanes == 8) KG_HEAD_NORM(8);
+  else if (lanes == 16) KG_HEAD_NORM(16);
+  else if (lanes == 32) KG_HEAD_NORM(32);
+  else KG_HEAD_NORM(64);
+#undef KG_HEAD_NORM
+  return true;
+}
+
+// False: no form of the kernel takes the call.
+template <typename T>
+bool launch_head_norm(const HeadNormArgs& a, hipStream_t stream) {
+  const bool many = (long long)a.tokens * (a.side[0].heads + a.side[1].heads) * a.d >= 1 << 21;
+  if (const int lanes = head_norm_lanes(a, 8))
+    return many ? launch_head_norm<T, 8, 4>(a, lanes, stream) : launch_head_norm<T, 8, 1>(a, lanes, stream);
+  if (const int lanes = head_norm_lanes(a, 4))
+    return many ? launch_head_norm<T, 4, 4>(a, lanes, stream) : launch_head_norm<T, 4, 1>(a, lanes, stream);
+  if (const int lanes = head_norm_lanes(a, 2))
+    return many ? launch_head_norm<T, 2, 4>(a, lanes, stream) : launch_head_norm<T, 2, 1>(a, lanes, stream);
+  return false;
 }
 
 }  // namespace kg_gfx950

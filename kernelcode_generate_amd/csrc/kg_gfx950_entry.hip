@@ -2150,6 +2150,7 @@ int head_norm_rotate_impl(const KgArgSlot* args, unsigned long long n) {
   a.inverse_d = 1.f / (float)d;
   return with_float_type(rows[2].dtype, [&](auto t) {
     using T = decltype(t);
+    if (launch_head_norm<T>(a, g_stream)) return finish_launch("head_norm_rotate");
     hipLaunchKernelGGL((head_norm_any_kernel<T>), dim3(most_blocks(cdiv(tokens * heads, 4))), dim3(256), 0, g_stream, a);
     return finish_launch("head_norm_rotate");
   });
