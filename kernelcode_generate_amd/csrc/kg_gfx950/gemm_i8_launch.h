@@ -28,54 +28,51 @@ hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// rows: 16, 32 or 64, at least m; channels: 16 or 32 a workgroup
+// m <= 32
 template <typename T>
-hipError_t launch_int8_few(const Int8Tiles& g, int rows, int channels, hipStream_t stream) {
-  const dim3 grid((unsigned)((g.n + channels - 1) / channels));
-#define KG_INT8_FEW(MB, NB) hipLaunchKernelGGL((int8_few_kernel<T, MB, NB>), grid, dim3(fewi::kThreads), 0, stream, g)
-  if (channels == 16) {
-    if (rows == 16) KG_INT8_FEW(1, 1);
-    else if (rows == 32) KG_INT8_FEW(2, 1);
-    else KG_INT8_FEW(4, 1);
-  } else {
-    if (rows == 16) KG_INT8_FEW(1, 2);
-    else if (rows == 32) KG_INT8_FEW(2, 2);
-    else KG_INT8_FEW(4, 2);
-  }
-#undef KG_INT8_FEW
+hipError_t launch_int8_few(const Int8Tiles& g, hipStream_t stream) {
+  const int blocks = (g.n + 15) / 16;
+  const dim3 grid((unsigned)(blocks < 512 ? blocks : 512));
+  if (g.m <= 16) hipLaunchKernelGGL((int8_few_kernel<T, 1, 1>), grid, dim3(fewi::kThreads), 0, stream, g);
+  else hipLaunchKernelGGL((int8_few_kernel<T, 2, 1>), grid, dim3(fewi::kThreads), 0, stream, g);
   return hipGetLastError();
 }
 
-constexpr int kInt8FewQuantizeMostK = 8 * 64 * fewi::kWaves;
-template <typename T>
-hipError_t launch_int8_few_quantize(const Int8Tiles& g, const void* x, long long x_row, int channels, hipStream_t stream) {
-  const dim3 grid((unsigned)((g.n + channels - 1) / channels));
-#define KG_INT8_FEW(STEPS, NB)                                                                                              \
-  do {                                                                                                                      \
-    if (g.k % 64 == 0)                                                                                                      \
-      hipLaunchKernelGGL((int8_few_quantize_kernel<T, STEPS, NB, true>), grid, dim3(fewi::kThreads), 0, stream, g,          \
-                         static_cast<const T*>(x), x_row);                                                                  \
-    else                                                                                                                    \
-      hipLaunchKernelGGL((int8_few_quantize_kernel<T, STEPS, NB, false>), grid, dim3(fewi::kThreads), 0, stream, g,         \
-                         static_cast<const T*>(x), x_row);                                                                  \
-  } while (0)
-  if (g.k <= kInt8FewQuantizeMostK / 2) {
-    if (channels == 16) KG_INT8_FEW(4, 1);
-    else KG_INT8_FEW(4, 2);
-  } else {
-    if (channels == 16) KG_INT8_FEW(8, 1);
-    else KG_INT8_FEW(8, 2);
+// The tiles of a product by a model of each form's time (ns): a launch, a further round of 256 tiles, a slice of 128 k, and percent more of
+// a slice where all CUs have a tile (their clocks go down). Fitted to 350 products of 1..4096 rows, 1024..16384 channels and K of
+// 512..11008, of which the one that it picks is 2.9 % above the fastest on average, the measurements' own spread with it. us of the forms in
+// their order: 4096^3 58 / 66 / 82 / 98 / 113 / - / -; 1000 x 4096 x 4096 44 / 29 / 19.3 / 23 / 31 / - / -; 300 x 4096 x 4096 43 / 26 / 17 / 13.1 /
+// 13.5 / 15 / 17.3; 64 x 4096 x 4096 - / - / - / 12.7 / 9.5 / 8.4 / 6.1; 16 x 11008 x 11008 - / - / - / 43.7 / 33.3 / 32.7 / 30.7. A deeper ring than
+// these changes nothing: what a slice of a small tile costs is its own chain of barrier, LDS reads and products.
+struct Int8Form {
+  int rows, channels, stages, fixed, round, slice, load;
+};
+constexpr Int8Form kInt8Forms[7] = {{256, 256, 2, 7800, 7600, 1140, 46}, {256, 128, 3, 5500, 4000, 610, 37}, {128, 128, 4, 3900, 1800, 420, 46},
+                                    {128, 64, 3, 3350, 220, 290, 15},    {64, 64, 4, 3200, 200, 220, 7},      {32, 64, 4, 3300, 80, 158, 4},
+                                    {32, 32, 8, 2800, 140, 98, 6}};
+inline int int8_form(long long m, long long n, long long k) {
+  int best = 0;
+  long long least = 0;
+  for (int i = 0; i < 7; ++i) {
+    const Int8Form& f = kInt8Forms[i];
+    const long long tiles = ((m + f.rows - 1) / f.rows) * ((n + f.channels - 1) / f.channels), rounds = (tiles + 255) / 256;
+    const long long slices = (k + 127) / 128 < f.stages ? f.stages : (k + 127) / 128;
+    const long long ns = f.fixed + (rounds - 1) * f.round + rounds * slices * f.slice * (25600 + f.load * (tiles < 256 ? tiles : 256)) / 25600;
+    if (i == 0 || ns < least) best = i, least = ns;
   }
-#undef KG_INT8_FEW
-  return hipGetLastError();
+  return best;
 }
-
-// tile: rows of a square tile
 template <typename T>
-hipError_t launch_int8_tiles(const Int8Tiles& g, int tile, hipStream_t stream) {
-  if (tile == 256) return launch_gemm_i8<T, 8, 8, 64, 4>(g, stream);
-  if (tile == 128) return launch_gemm_i8<T, 4, 4, 128, 4>(g, stream);
-  return launch_gemm_i8<T, 2, 2, 128, 4>(g, stream);
+hipError_t launch_int8_tiles(const Int8Tiles& g, int form, hipStream_t stream) {
+  switch (form) {
+    case 0: return launch_gemm_i8<T, 8, 8, 128, 2>(g, stream);
+    case 1: return launch_gemm_i8<T, 8, 4, 128, 3>(g, stream);
+    case 2: return launch_gemm_i8<T, 4, 4, 128, 4>(g, stream);
+    case 3: return launch_gemm_i8<T, 4, 2, 128, 3>(g, stream);
+    case 4: return launch_gemm_i8<T, 2, 2, 128, 4>(g, stream);
+    case 5: return launch_gemm_i8<T, 1, 2, 128, 4>(g, stream);
+    default: return launch_gemm_i8<T, 1, 1, 128, 8>(g, stream);
+  }
 }
 
 }  // namespace kg_gfx950

@@ -8,8 +8,8 @@
 // The barrier before a slice's last step finds all its fragments read: it publishes the next slice's copies and
 // frees this slice's stage for its refill.
 //
-// kRagged: extents that are no multiples of the tile: copies through buffer loads that land zeros outside the matrices, stores
-// inside alone. K is a multiple of 16 (rows of others are copied into padded ones first).
+// Copies are buffer loads that land zeros outside the matrices (as fast as plain ones), stores are made inside alone: any M and N. K is a
+// multiple of 16 (rows of others are copied into padded ones first).
 #pragma once
 
 #include "gemm.h"
@@ -22,12 +22,11 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 namespace gemmi {
 constexpr int kThreads = 256;
-// acc += a b on one 16 x 16 block. The tied form keeps the accumulator in one register tuple of the accumulation file, for tiles
-// whose accumulators fill it (as gemm_quad_kernel's); its results are read behind mfma_drain and mfma_order.
-template <bool kTied>
+// acc += a b on one 16 x 16 block, the accumulator tied to one register tuple of the accumulation file for the whole kernel (the compiler
+// rotates the accumulators of its own form through that file at the loop's edge: 128 x 128 tiles of K = 4096 21.2 us, tied 16.6);
+// results are read behind mfma_drain and mfma_order.
 __device__ __forceinline__ void mfma(i32x4& acc, u32x4 a, u32x4 b) {
-  if constexpr (kTied) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-  else acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), acc, 0, 0, 0);
+  asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 // more than the instruction's result latency (8 passes) before its result is read
 __device__ __forceinline__ void mfma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
@@ -54,19 +53,19 @@ struct Int8Tiles {
   bool wide_bias, vectors;  // vectors: rows of out are whole 16-byte pieces
 };
 
-template <typename T, int NA, int NB, int kBK, int kStages, bool kRagged>
+template <typename T, int NA, int NB, int kBK, int kStages>
 __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8_kernel(Int8Tiles g) {
   using namespace gemmi;
   constexpr int TM = 32 * NA, TN = 32 * NB;
   constexpr int kSteps = kBK / 64;
-  constexpr bool kTied = NA * NB == 64;
   constexpr int kRowsPiece = 1024 / kBK;  // rows of a wave's copy
   constexpr int AP = TM / kRowsPiece / 4, BP = TN / kRowsPiece / 4, kPieces = AP + BP;  // copies per wave and slice
   constexpr int kStageA = TM * kBK, kStageB = TN * kBK, kStage = kStageA + kStageB;
   constexpr int kMfmas = NA * NB, kReads = NA + NB;
   static_assert(kSteps == 1 || kSteps == 2, "steps");
-  static_assert(AP >= 1 && BP >= 1 && kPieces % kSteps == 0, "pieces");
+  static_assert(AP >= 1 && BP >= 1, "pieces");
   static_assert(kStages >= 2 && (kSteps == 2 || kStages % 2 == 0), "a step's registers are constants of the unrolled ring");
+  static_assert(16 * NA % (64 / (2 * NB)) == 0 || NA * NB == 1, "a wave's results are whole stores, or half of one");
   static_assert(sizeof(T) == 4 || kStages * kStage >= TM * TN * 2, "the tile's 16-bit results fit the ring");
   __shared__ __attribute__((aligned(1024))) char lds[kStages * kStage];
   __shared__ __attribute__((aligned(16))) float xs_lds[TM], ws_lds[TN], bias_lds[TN];
@@ -84,7 +83,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   const int gm = min(tiles_m - first_m, kGroupM), in_group = logical - group * kGroupM * tiles_n;
   const int m0 = (first_m + in_group % gm) * TM, n0 = (in_group / gm) * TN;
 
-  // slices of K; in the one-step form a multiple of two (registers go by a slice's parity), and at least a ring of them: kRagged, zeros
+  // slices of K; in the one-step form a multiple of two (registers go by a slice's parity), and at least a ring of them: zeros behind K
   const int slices = (g.k + kBK - 1) / kBK;
   const int count = max(kSteps == 1 ? (slices + 1) / 2 * 2 : slices, kStages);
 
@@ -96,13 +95,13 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   for (int p = 0; p < AP; ++p) {
     const int row = (wave * AP + p) * kRowsPiece + lane / kChunks;
     a_off[p] = (uint32_t)(row * g.ldx + 16 * ((lane % kChunks) ^ swizzle<kBK>(row)));
-    if (kRagged && m0 + row >= g.m) a_off[p] = kBufOOB;
+    if (m0 + row >= g.m) a_off[p] = kBufOOB;
   }
 #pragma unroll
   for (int p = 0; p < BP; ++p) {
     const int row = (wave * BP + p) * kRowsPiece + lane / kChunks;
     b_off[p] = (uint32_t)(row * g.ldw + 16 * ((lane % kChunks) ^ swizzle<kBK>(row)));
-    if (kRagged && n0 + row >= g.n) b_off[p] = kBufOOB;
+    if (n0 + row >= g.n) b_off[p] = kBufOOB;
   }
 #pragma unroll
   for (int x = 0; x < 2; ++x) chunk_k[x] = 16 * ((lane % kChunks) ^ swizzle<kBK>(x * kRowsPiece + lane / kChunks));
@@ -115,12 +114,8 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
     const char* src = (a ? a_tile : b_tile) + (long long)kt * kBK;
     const uint32_t dst = lds0 + stage * kStage + (a ? (wave * AP + p) * 1024 : kStageA + (wave * BP + p) * 1024);
     const uint32_t off = a ? a_off[a ? p : 0] : b_off[a ? 0 : p];
-    if constexpr (kRagged) {
-      const int k = chunk_k[kBK == 64 ? 0 : ((a ? wave * AP : wave * BP) + p) & 1];
-      buf2lds16_s(kt * kBK + k < g.k ? off : kBufOOB, src, dst);
-    } else {
-      g2lds16_s(off, src, dst);
-    }
+    const int k = chunk_k[kBK == 64 ? 0 : ((a ? wave * AP : wave * BP) + p) & 1];
+    buf2lds16_s(kt * kBK + k < g.k ? off : kBufOOB, src, dst);
   };
 
   // ---- fragments of step ks: rows 16 i + lane % 16 of the wave's half, chunk 4 ks + lane / 16 ----
@@ -163,26 +158,26 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   for (int i = 0; i < NA; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-  if constexpr (kTied) {
-    // (opaque from here on: zeros made again right before the first MFMAs would lack the wait that these need)
+  // (opaque from here on: zeros made again right before the first MFMAs would lack the wait that these need)
 #pragma unroll
-    for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
-  }
+  for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
 
-  constexpr int kCopies = kPieces / kSteps;  // a step's
+  // copies of a slice in its last step, and (kHalves) the others in the next slice's first one
+  constexpr bool kHalves = kSteps == 2 && kStages > 2;
+  constexpr int kCopies = kHalves ? (kPieces + 1) / 2 : kPieces, kRest = kPieces - kCopies;
 #pragma unroll
   for (int i = 0; i < kStages; ++i)
 #pragma unroll
     for (int p = 0; p < kPieces; ++p)
-      if (kSteps == 1 || i < kStages - 1 || p < kCopies) issue_piece(i, i, p);  // (two steps: the first slice brings the last one's second half)
-  wait_and_barrier<(kStages - 2) * kPieces + kCopies>();
+      if (i < kStages - 1 || p < kCopies) issue_piece(i, i, p);  // (kHalves: the first slice brings the last one's second half)
+  wait_and_barrier<(kStages - 2) * kPieces + kCopies>();  // slice 0 has landed
   Frags fr[2];
   read_from(0, 0);
 #pragma unroll
   for (int r = 0; r < kReads; ++r) read_step(fr[0], r);
 
   // Slice kt, in stage `stage`, its registers by kParity. kBehind: slices behind it, kStages where there are so many. The refill of its
-  // stage (slice kt + kStages) goes into the last step, behind its barrier, and where there are two steps half of it into the next
+  // stage (slice kt + kStages) goes into the last step, behind its barrier, with more than two stages half of it into the next
   // slice's first. The last kStages slices are a compile-time group whose waits, reads and copies carry no conditions (with
   // conditions they took about twice a steady one's cycles).
   auto slice = [&](int kt, int stage, auto parity_tag, auto behind_tag) __attribute__((always_inline)) {
@@ -199,15 +194,16 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
       static_for<kMfmas>([&](auto idx_tag) __attribute__((always_inline)) {
         constexpr int idx = decltype(idx_tag)::value;
         constexpr int i = idx / NB, j = idx % NB;
-        mfma<kTied>(acc[i][j], fr[P].b[j], fr[P].a[i]);  // blocks of the transpose: a lane's columns lie side by side
+        mfma(acc[i][j], fr[P].b[j], fr[P].a[i]);  // blocks of the transpose: a lane's columns lie side by side
         constexpr int r0 = (idx * 2 * kReads + kMfmas - 1) / kMfmas, r1 = ((idx + 1) * 2 * kReads + kMfmas - 1) / kMfmas;
         static_for<(r1 < kReads ? r1 : kReads) - (r0 < kReads ? r0 : kReads)>([&](auto r_tag) __attribute__((always_inline)) {
           constexpr int r = r0 + decltype(r_tag)::value;
           if constexpr (!kLast || kBehind > 0) read_step(fr[P ^ 1], r);
         });
-        static_for<kCopies>([&](auto c_tag) __attribute__((always_inline)) {
+        constexpr int kOwn = kLast ? kCopies : kRest;
+        static_for<kOwn>([&](auto c_tag) __attribute__((always_inline)) {
           constexpr int c = decltype(c_tag)::value;
-          if constexpr (idx == (2 * c + 1) * kMfmas / (2 * kCopies)) {
+          if constexpr (idx == (2 * c + 1) * kMfmas / (2 * kOwn)) {
             if constexpr (kLast && kBehind == kStages) issue_piece(kt + kStages, stage, c);
             if constexpr (!kLast && kBehind >= kStages - 1) issue_piece(kt - 1 + kStages, before, kCopies + c);
           }
@@ -234,11 +230,9 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   });
 
   // ---- a lane holds out[16 i + lane % 16][16 j + 4 (lane / 16) .. + 3] of each block (i, j) ----
-  if constexpr (kTied) {
-    mfma_drain();
+  mfma_drain();
 #pragma unroll
-    for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
-  }
+  for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
   if (tid < TM) xs_lds[tid] = xs_own;
   if (tid < TN) ws_lds[tid] = ws_own, bias_lds[tid] = bias_own;
   wait_and_barrier<0>();  // the ring is read
@@ -262,16 +256,16 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
       if constexpr (sizeof(T) == 4) {
         const int m = mw + 16 * i + l16;
         float* to = static_cast<float*>(g.out) + m * g.ldo + n;
-        if (!kRagged || (m < g.m && n + 4 <= g.n)) {
+        if (m < g.m && n + 4 <= g.n) {
           if (g.vectors) {
             *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
             continue;
           }
         }
-        if (!kRagged || m < g.m)
+        if (m < g.m)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!kRagged || n + e < g.n) to[e] = v[e];
+            if (n + e < g.n) to[e] = v[e];
       } else {
         using H = Half16<typename Eight<T>::Tag>;
         const u32x2 packed = {H::pack2(v[0], v[1]), H::pack2(v[2], v[3])};
@@ -286,13 +280,14 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
     // whole row segments, 16 bytes a lane, of what the wave itself packed
     constexpr int kRowsStore = 64 / kRowChunks;
 #pragma unroll
-    for (int q = 0; q < 16 * NA / kRowsStore; ++q) {
+    for (int q = 0; q < (16 * NA + kRowsStore - 1) / kRowsStore; ++q) {
       const int r = kRowsStore * q + lane / kRowChunks, c = lane % kRowChunks;
+      if (16 * NA < kRowsStore && r >= 16 * NA) continue;  // (16 x 16 results have 32 pieces)
       const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(region + r * kRow + ((c ^ row_swizzle(r)) * 16));
       const int m = mw + r, n = nw + 8 * c;
-      if (kRagged && (m >= g.m || n >= g.n)) continue;
+      if (m >= g.m || n >= g.n) continue;
       uint16_t* to = static_cast<uint16_t*>(g.out) + (long long)m * g.ldo + n;
-      if (g.vectors && (!kRagged || n + 8 <= g.n)) {
+      if (g.vectors && n + 8 <= g.n) {
         __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to));
       } else {
 #pragma unroll
@@ -307,10 +302,7 @@ template <typename T, int NA, int NB, int kBK, int kStages>
 hipError_t launch_gemm_i8(const Int8Tiles& g, hipStream_t stream) {
   constexpr int TM = 32 * NA, TN = 32 * NB;
   const unsigned grid = (unsigned)(((long long)g.m + TM - 1) / TM * (((long long)g.n + TN - 1) / TN));
-  // (pairs of slices of 64, or slices of 128, a ring of them at least)
-  const bool ragged = g.m % TM != 0 || g.n % TN != 0 || g.k % 128 != 0 || g.k < kStages * kBK;
-  if (ragged) hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages, true>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
-  else hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages, false>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
+  hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
   return hipGetLastError();
 }
 

@@ -25,13 +25,11 @@ KG_INT8_INSTANCE(_Float16)
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_INT8_FEW)
 #define KG_INT8_INSTANCE(T)                                                                                     \
   KG_INSTANCE hipError_t launch_quantize<T>(const QuantizeArgs&, hipStream_t);                                  \
-  KG_INSTANCE hipError_t launch_int8_few<T>(const Int8Tiles&, int, int, hipStream_t);
+  KG_INSTANCE hipError_t launch_int8_few<T>(const Int8Tiles&, hipStream_t);
 KG_INT8_INSTANCE(float)
 KG_INT8_INSTANCE(__bf16)
 KG_INT8_INSTANCE(_Float16)
 #undef KG_INT8_INSTANCE
-KG_INSTANCE hipError_t launch_int8_few_quantize<__bf16>(const Int8Tiles&, const void*, long long, int, hipStream_t);
-KG_INSTANCE hipError_t launch_int8_few_quantize<_Float16>(const Int8Tiles&, const void*, long long, int, hipStream_t);
 #endif
 
 }  // namespace kg_gfx950

@@ -1953,33 +1953,20 @@ int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
   return finish_launch("quantize_rows");
 }
 
-// Rows that the few-row kernels take.
-constexpr long long kInt8FewRows = 64;
-
-// Rows of the square tiles that a product takes.
-int int8_tile(long long M, long long N) {
-  if (cdiv(M, 256) * cdiv(N, 256) >= 192) return 256;
-  if (cdiv(M, 128) * cdiv(N, 128) >= 160) return 128;
-  return 64;
-}
+// Rows that the kernel for weights of any alignment takes.
+constexpr long long kInt8FewRows = 32;
 
 // The matrix-core forms of int8_matmul. kUnsupported: none of them, since there is no workspace to be had, or not enough.
 template <typename T>
 int launch_int8(const Int8Args& a, bool codes, bool out_aligned, bool x_aligned, bool w_aligned) {
-  const bool few = a.m <= kInt8FewRows;
+  const bool whole = a.k % 16 == 0, whole_w = whole && w_aligned && a.w_row <= kMaxPipeLd;
+  const bool few = a.m <= kInt8FewRows && !whole_w;
   Int8Tiles g{static_cast<const int8_t*>(a.x), a.w, a.x_scale, a.w_scale, a.bias, a.out, a.x_row, a.w_row, a.out_row,
               a.x_scale_stride, a.w_scale_stride, a.bias_stride, a.m, a.n, a.k, a.wide_bias, out_aligned};
-  if constexpr (sizeof(T) == 2) {
-    if (!codes && a.m <= 16 && a.k <= kInt8FewQuantizeMostK) {
-      (void)launch_int8_few_quantize<T>(g, a.x, a.x_row, 16, g_stream);
-      return finish_launch("int8_matmul");
-    }
-  }
   // rows and weights in the workspace: codes of rows that are quantised here; for the tiles, copies of rows that are not whole 16-byte pieces
   const long long pitch = cdiv(a.k, 64) * 64;
-  const bool whole = a.k % 16 == 0;
   const bool take_x = !codes || (!few && !(whole && x_aligned && a.x_row <= kMaxPipeLd));
-  const bool take_w = !few && !(whole && w_aligned && a.w_row <= kMaxPipeLd);
+  const bool take_w = !few && !whole_w;
   const long long w_bytes = take_w ? a.n * pitch : 0, row_bytes = take_x ? pitch + (codes ? 0 : (long long)sizeof(float)) : 0;
   const long long room = kSplitMaxWorkspace - w_bytes - 512;
   long long rows = a.m;  // of a piece that the workspace holds: whole tiles
@@ -2021,11 +2008,11 @@ int launch_int8(const Int8Args& a, bool codes, bool out_aligned, bool x_aligned,
       g.ldx = pitch;
     }
     if (few) {
-      (void)launch_int8_few<T>(g, g.m <= 16 ? 16 : g.m <= 32 ? 32 : 64, 16, g_stream);
+      (void)launch_int8_few<T>(g, g_stream);
     } else {
       if (take_x && take_w) g.k = (int)pitch;  // (zeros behind the rows' ends)
       else g.k = (int)(cdiv(a.k, 16) * 16);
-      (void)launch_int8_tiles<T>(g, int8_tile(g.m, g.n), g_stream);
+      (void)launch_int8_tiles<T>(g, int8_form(g.m, g.n, g.k), g_stream);
     }
   }
   return finish_launch("int8_matmul");

@@ -98,7 +98,9 @@ def check_product(m, n, k, dtype, device, codes, bias, seed=0, top=False, pads=(
 SIZES = [(1, 1, 1), (1, 64, 64), (3, 5, 7), (1, 4096, 512), (2, 100, 1000), (8, 256, 4096), (15, 33, 130), (16, 1024, 2048), (16, 48, 8192),
          (17, 512, 256), (31, 1000, 1040), (32, 128, 96), (33, 2048, 512), (64, 64, 64), (65, 272, 144), (100, 1501, 1023), (127, 130, 64),
          (128, 128, 128), (129, 257, 1024), (200, 768, 2048), (256, 256, 256), (257, 513, 272), (300, 1024, 1000), (512, 512, 1024),
-         (700, 300, 80), (1000, 1501, 1023), (1024, 2048, 512), (515, 264, 4112), (2048, 8, 64), (40, 16384, 64), (1, 8, 131071)]
+         (700, 300, 80), (1000, 1501, 1023), (1024, 2048, 512), (515, 264, 4112), (2048, 8, 64), (40, 16384, 64), (1, 8, 131071),
+         (4096, 4096, 256), (3900, 4000, 400), (2048, 4096, 512), (1900, 4100, 272), (1024, 4096, 1024), (130, 4096, 2048), (16, 4096, 4096),
+         (33, 1030, 4096), (16, 512, 4095), (32, 300, 2047)]
 
 
 @pytest.mark.parametrize("m, n, k", SIZES)
