@@ -12,28 +12,11 @@ namespace kg_gfx950 {
 namespace fewi {
 constexpr int kWaves = 16, kThreads = 64 * kWaves;
 
-// 16 codes of a row of `count` >= 16 from column k, zeros behind its end, without a branch.
-__device__ __forceinline__ u32x4 load_codes(const int8_t* row, int k, int count) {
-  const int at = min(k, count - 16);
-  return shift_bytes(load_bytes(row + at), min(k - at, 16));
-}
-
 __device__ __forceinline__ i32x4 mfma(u32x4 a, u32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
 }  // namespace fewi
-
-// Rows of k >= 16 codes copied into rows of `pitch` bytes, a multiple of 16, zeros behind k: for copies to LDS, which take whole
-// 16-byte pieces.
-template <int kUnused = 0>
-__global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* src, long long ld, int8_t* dst, int pitch, int rows, int k) {
-  const int pieces = pitch / 16;
-  for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < (long long)rows * pieces; at += 256ll * gridDim.x) {
-    const int r = (int)(at / pieces), c = 16 * (int)(at - (long long)r * pieces);
-    st16(dst + (long long)r * pitch + c, fewi::load_codes(src + r * ld, c, k));
-  }
-}
 
 // m <= 16 MB. A workgroup's blocks of channels are blockIdx.x, + gridDim.x, ...; kAhead steps of a wave are a group, and the next
 // group's reads, of the next block's first where a block ends, are on their way while this one's products and sums are made.

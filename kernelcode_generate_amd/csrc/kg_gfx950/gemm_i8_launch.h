@@ -7,19 +7,36 @@
 
 namespace kg_gfx950 {
 
-// Rows of 8 to 16384 elements in one pass, others in two.
+__global__ __launch_bounds__(256) static void int8_pack_kernel(PackArgs x, PackArgs w) {
+  pack_rows(blockIdx.y == 0 ? x : w, (long long)blockIdx.x * 256 + threadIdx.x, 256ll * gridDim.x);
+}
+inline unsigned pack_blocks(const PackArgs& p) {
+  const long long blocks = ((long long)p.rows * (p.pitch / 16) + 255) / 256;
+  return (unsigned)(blocks < 4096 ? blocks : 4096);
+}
+// (either may have no rows)
+inline hipError_t launch_int8_pack(const PackArgs& x, const PackArgs& w, hipStream_t stream) {
+  const unsigned blocks = pack_blocks(x) > pack_blocks(w) ? pack_blocks(x) : pack_blocks(w);
+  if (blocks > 0) hipLaunchKernelGGL(int8_pack_kernel, dim3(blocks, 2), dim3(256), 0, stream, x, w);
+  return hipGetLastError();
+}
+
+// Rows of 8 to 16384 elements in one pass, others in two; and codes packed beside them.
 template <typename T>
-hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
+hipError_t launch_quantize(const QuantizeArgs& a, const PackArgs& pack, hipStream_t stream) {
+  constexpr int kMostBlocks = (1 << 24) - 1;
   const int pieces = (a.width + 2047) / 2048;
 #define KG_QUANTIZE(PIECES, WAVES)                                                                                                \
   do {                                                                                                                            \
-    const dim3 grid((unsigned)((a.rows + 4 / WAVES - 1) / (4 / WAVES)));                                                          \
-    if (a.k % 8 == 0) hipLaunchKernelGGL((quantize_rows_kernel<T, PIECES, WAVES, true>), grid, dim3(256), 0, stream, a);          \
-    else hipLaunchKernelGGL((quantize_rows_kernel<T, PIECES, WAVES, false>), grid, dim3(256), 0, stream, a);                      \
+    const dim3 grid((unsigned)((a.rows + 4 / WAVES - 1) / (4 / WAVES)) + pack_blocks(pack));                                      \
+    if (a.k % 8 == 0) hipLaunchKernelGGL((quantize_rows_kernel<T, PIECES, WAVES, true>), grid, dim3(256), 0, stream, a, pack);    \
+    else hipLaunchKernelGGL((quantize_rows_kernel<T, PIECES, WAVES, false>), grid, dim3(256), 0, stream, a, pack);                \
   } while (0)
-  if (a.k < 8 || pieces > 8 || a.rows > (1 << 24) - 1)
-    hipLaunchKernelGGL((quantize_rows_any_kernel<T>), dim3((unsigned)(a.rows < (1 << 24) - 1 ? a.rows : (1 << 24) - 1)), dim3(256), 0, stream, a);
-  else if (a.width <= 512) KG_QUANTIZE(1, 1);
+  if (a.k < 8 || pieces > 8 || a.rows > kMostBlocks - 4096) {
+    hipLaunchKernelGGL((quantize_rows_any_kernel<T>), dim3((unsigned)(a.rows < kMostBlocks ? a.rows : kMostBlocks)), dim3(256), 0, stream, a);
+    return launch_int8_pack(pack, PackArgs{}, stream);
+  }
+  if (a.width <= 512) KG_QUANTIZE(1, 1);
   else if (pieces == 1) KG_QUANTIZE(1, 4);
   else if (pieces == 2) KG_QUANTIZE(2, 4);
   else if (pieces <= 4) KG_QUANTIZE(4, 4);

@@ -43,6 +43,14 @@ __device__ __forceinline__ int swizzle(int row) {
 }
 }  // namespace gemmi
 
+// 16 bytes to any address, past the L2
+__device__ __forceinline__ void store_bytes(void* p, u32x4 v) {
+  struct __attribute__((packed, aligned(2))) Piece {
+    u32x4 w;
+  };
+  __builtin_nontemporal_store(v, &reinterpret_cast<Piece*>(p)->w);
+}
+
 struct Int8Tiles {
   const int8_t *x, *w;
   const float *x_scale, *w_scale;
@@ -50,7 +58,7 @@ struct Int8Tiles {
   void* out;
   long long ldx, ldw, ldo, x_scale_stride, w_scale_stride, bias_stride;
   int m, n, k;
-  bool wide_bias, vectors;  // vectors: rows of out are whole 16-byte pieces
+  bool wide_bias;
 };
 
 template <typename T, int NA, int NB, int kBK, int kStages>
@@ -257,15 +265,12 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
         const int m = mw + 16 * i + l16;
         float* to = static_cast<float*>(g.out) + m * g.ldo + n;
         if (m < g.m && n + 4 <= g.n) {
-          if (g.vectors) {
-            *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-            continue;
-          }
-        }
-        if (m < g.m)
+          store_bytes(to, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
+        } else if (m < g.m) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (n + e < g.n) to[e] = v[e];
+        }
       } else {
         using H = Half16<typename Eight<T>::Tag>;
         const u32x2 packed = {H::pack2(v[0], v[1]), H::pack2(v[2], v[3])};
@@ -287,8 +292,8 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
       const int m = mw + r, n = nw + 8 * c;
       if (m >= g.m || n >= g.n) continue;
       uint16_t* to = static_cast<uint16_t*>(g.out) + (long long)m * g.ldo + n;
-      if (g.vectors && n + 8 <= g.n) {
-        __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to));
+      if (n + 8 <= g.n) {
+        store_bytes(to, v);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)

@@ -7,9 +7,9 @@
 // Pages that go back, of ceil(keep / page_size) .. ceil(held / page_size) - 1, are put on the stack the last one first, so that
 // giving back what a call took leaves the stack as it was.
 //
-// Each kernel is one workgroup: a call of some thousand tokens is a chain of a few dependent reads (lengths, a search for a row's
-// request in LDS, its page), which more workgroups do not shorten, and only one workgroup can take from the stack and write what is
-// left of it without a second launch.
+// A call of some thousand tokens is a chain of a few dependent reads (lengths, a search for a row's request in LDS, its page), which more
+// workgroups do not shorten, and only one workgroup can take from the stack and write what is left of it without a second launch: up to
+// 2048 rows one workgroup does all. More rows are written by a second launch.
 #pragma once
 
 #include "common.h"
@@ -71,9 +71,44 @@ __device__ __forceinline__ int pages_owner(const int* sums, int batch, int x) {
   return lo;
 }
 
-__global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a) {
-  __shared__ int row_of[kPagesMostRequests + 1], fresh_of[kPagesMostRequests];  // first rows, first of all new pages
-  __shared__ int scan[kPagesThreads / 64];
+// Slot and position of row t, behind the sums of all requests. row_of, fresh_of: a request's first row and first of all new pages.
+__device__ __forceinline__ void assign_row(const PagesArgs& a, int t, int rows, int count, const int* row_of, const int* fresh_of) {
+  long long slot = -1;
+  int position = -1;
+  if (t < rows) {
+    const int b = pages_owner(row_of, a.batch, t);
+    const int c = max(a.context[b * a.context_stride], 0);
+    const uint32_t at = (uint32_t)c + (uint32_t)(t - row_of[b]);
+    position = (int)min(at, 0x7fffffffu);
+    if (at < 0x7fffffffu) {
+      const int p = div_page(position, a.div), offset = position - p * a.page_size;
+      if (p < a.per) {
+        const int held = pages_of(c, a);
+        int page;
+        int* entry = a.table + b * a.table_0 + p * a.table_1;
+        if (p < held) {
+          page = *entry;
+        } else {
+          const int i = fresh_of[b] + p - held;
+          page = i < count ? a.free[(count - 1 - i) * a.free_stride] : -1;
+          if (offset == 0) *entry = page;  // (each new page's first token is one of the call's)
+        }
+        if (page >= 0) slot = (long long)page * a.page_size + offset;
+      }
+    }
+  }
+  a.slots[t * a.slot_stride] = slot;
+  a.positions[t * a.position_stride] = position;
+}
+
+// The requests' sums, and (kSums false) the rows. kSums: the sums go to memory for kv_assign_rows_kernel: the count of free pages as it
+// was, first rows (batch + 1 of them), first new pages.
+template <bool kSums>
+__global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a, int* sums) {
+  __shared__ int row_lds[kSums ? 1 : kPagesMostRequests + 1], fresh_lds[kSums ? 1 : kPagesMostRequests];
+  __shared__ int scan[kPagesThreads / 64], last_of[kPagesThreads / 64];
+  int* row_of = kSums ? sums + 1 : row_lds;
+  int* fresh_of = kSums ? sums + 2 + a.batch : fresh_lds;
   const int tid = threadIdx.x;
   const int count = max(min(*a.count, a.stack), 0);
   int rows = 0, fresh = 0;  // of the requests before
@@ -83,13 +118,11 @@ __global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a) {
     const int c = real ? max(a.context[b * a.context_stride], 0) : 0;
     const int n = real ? min(max(a.added[b * a.added_stride], 0), a.tokens) : 0;
     int all;
-    const int upto = min((int)min((uint32_t)pages_scan<true>(n, a.tokens, scan, &all) + (uint32_t)rows, (uint32_t)a.tokens), a.tokens);
+    const int upto = (int)min((uint32_t)pages_scan<true>(n, a.tokens, scan, &all) + (uint32_t)rows, (uint32_t)a.tokens);
     const int before = __shfl_up(upto, 1, 64);
-    // the sum before, of another wave: found by the same cut sums
-    __shared__ int last_of[kPagesThreads / 64];
     if ((tid & 63) == 63) last_of[tid >> 6] = upto;
     __syncthreads();
-    const int first = (tid & 63) != 0 ? before : tid == 0 ? rows : last_of[(tid >> 6) - 1];
+    const int first = (tid & 63) != 0 ? before : tid == 0 ? rows : last_of[(tid >> 6) - 1];  // (cut as the sums are)
     const int kept = upto - first;
     // tokens past 2^31 - 1 have no page
     const int end = (int)min((uint32_t)c + (uint32_t)kept, 0x7fffffffu);
@@ -107,37 +140,23 @@ __global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a) {
   if (tid == 0) {
     row_of[a.batch] = rows;
     a.starts[a.batch * a.start_stride] = rows;
+    if (kSums) sums[0] = count;
     *a.count = count - min(fresh, count);
   }
-  __syncthreads();
-  for (int t = tid; t < a.tokens; t += kPagesThreads) {
-    long long slot = -1;
-    int position = -1;
-    if (t < rows) {
-      const int b = pages_owner(row_of, a.batch, t);
-      const int c = max(a.context[b * a.context_stride], 0);
-      const uint32_t at = (uint32_t)c + (uint32_t)(t - row_of[b]);
-      position = (int)min(at, 0x7fffffffu);
-      if (at < 0x7fffffffu) {
-        const int p = div_page(position, a.div), offset = position - p * a.page_size;
-        if (p < a.per) {
-          const int held = pages_of(c, a);
-          int page;
-          int* entry = a.table + b * a.table_0 + p * a.table_1;
-          if (p < held) {
-            page = *entry;
-          } else {
-            const int i = fresh_of[b] + p - held;
-            page = i < count ? a.free[(count - 1 - i) * a.free_stride] : -1;
-            if (offset == 0) *entry = page;  // (each new page's first token is one of the call's)
-          }
-          if (page >= 0) slot = (long long)page * a.page_size + offset;
-        }
-      }
-    }
-    a.slots[t * a.slot_stride] = slot;
-    a.positions[t * a.position_stride] = position;
+  if constexpr (!kSums) {
+    __syncthreads();
+    for (int t = tid; t < a.tokens; t += kPagesThreads) assign_row(a, t, rows, count, row_of, fresh_of);
   }
+}
+
+__global__ __launch_bounds__(256) void kv_assign_rows_kernel(PagesArgs a, const int* sums) {
+  __shared__ int row_of[kPagesMostRequests + 1];
+  for (int b = threadIdx.x; b <= a.batch; b += 256) row_of[b] = sums[1 + b];
+  const int count = sums[0];
+  __syncthreads();
+  const int rows = row_of[a.batch];
+  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < a.tokens; t += 256ll * gridDim.x)
+    assign_row(a, (int)t, rows, count, row_of, sums + 2 + a.batch);
 }
 
 __global__ __launch_bounds__(kPagesThreads) void kv_release_kernel(PagesArgs a) {

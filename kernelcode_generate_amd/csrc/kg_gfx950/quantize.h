@@ -174,9 +174,37 @@ __device__ __forceinline__ void quantize_row(const QuantizeArgs& a, long long ro
   }
 }
 
+// 16 codes of a row of `count` >= 16 from column k, zeros behind its end, without a branch.
+__device__ __forceinline__ u32x4 load_codes(const int8_t* row, int k, int count) {
+  const int at = min(k, count - 16);
+  return shift_bytes(load_bytes(row + at), min(k - at, 16));
+}
+
+// Rows of k >= 16 codes copied into rows of `pitch` bytes, a multiple of 16, zeros behind k: for copies to LDS, which take whole
+// 16-byte pieces.
+struct PackArgs {
+  const int8_t* src;
+  int8_t* dst;
+  long long ld;
+  int pitch, rows, k;
+};
+__device__ __forceinline__ void pack_rows(const PackArgs& p, long long thread, long long threads) {
+  const int pieces = p.pitch / 16;
+  for (long long at = thread; at < (long long)p.rows * pieces; at += threads) {
+    const int r = (int)(at / pieces), c = 16 * (int)(at - (long long)r * pieces);
+    st16(p.dst + (long long)r * p.pitch + c, load_codes(p.src + r * p.ld, c, p.k));
+  }
+}
+
+// The workgroups behind those of the rows pack: weights beside the rows of one call.
 template <typename T, int kPieces, int kWaves, bool kWhole>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
+__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a, PackArgs pack) {
   __shared__ float lds[4];
+  const int own = (a.rows + 4 / kWaves - 1) / (4 / kWaves);
+  if ((int)blockIdx.x >= own) {
+    pack_rows(pack, ((long long)blockIdx.x - own) * 256 + threadIdx.x, 256ll * ((int)gridDim.x - own));
+    return;
+  }
   quantize_row<T, kPieces, kWaves, kWhole>(a, (long long)blockIdx.x * (4 / kWaves) + threadIdx.x / (64 * kWaves), lds);
 }
 

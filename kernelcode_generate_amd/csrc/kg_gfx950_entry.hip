@@ -1878,6 +1878,9 @@ PagesArgs pages_args(const PagesSlots& p) {
   return a;
 }
 
+// Rows that the workgroup of the sums writes too; more go to workgroups of a second launch (pages.h has both measured).
+constexpr long long kAssignFewTokens = 2048;
+
 int kv_cache_assign_impl(const KgArgSlot* args, unsigned long long n) {
   if (args == nullptr) return fail(kInvalid, "ordered_args is null");
   if (n != 9) return fail(kInvalid, "kv_cache_assign expects 9 slots, got %llu", n);
@@ -1904,7 +1907,16 @@ int kv_cache_assign_impl(const KgArgSlot* args, unsigned long long n) {
   a.position_stride = positions.stride[0];
   a.start_stride = starts.stride[0];
   a.tokens = (int)tokens;
-  hipLaunchKernelGGL(kv_assign_kernel, dim3(1), dim3(kPagesThreads), 0, g_stream, a);
+  if (tokens > kAssignFewTokens) {
+    SplitLease lease = split_workspace((2 * (size_t)batch + 2) * sizeof(int), g_stream);  // held until both kernels are enqueued
+    if (int* sums = static_cast<int*>(lease.ptr)) {
+      hipLaunchKernelGGL((kv_assign_kernel<true>), dim3(1), dim3(kPagesThreads), 0, g_stream, a, sums);
+      const unsigned grid = (unsigned)std::min(cdiv(tokens, 256), 1024ll);
+      hipLaunchKernelGGL(kv_assign_rows_kernel, dim3(grid), dim3(256), 0, g_stream, a, sums);
+      return finish_launch("kv_cache_assign");
+    }
+  }
+  hipLaunchKernelGGL((kv_assign_kernel<false>), dim3(1), dim3(kPagesThreads), 0, g_stream, a, nullptr);
   return finish_launch("kv_cache_assign");
 }
 
@@ -1921,14 +1933,12 @@ int kv_cache_release_impl(const KgArgSlot* args, unsigned long long n) {
 }
 
 template <typename F>
-int with_float_type(int dtype, F&& f) {
+auto with_float_type(int dtype, F&& f) {
   return dtype == KG_DTYPE_F32 ? f(float{}) : dtype == KG_DTYPE_BF16 ? f((__bf16)0.f) : f((_Float16)0.f);
 }
 
 hipError_t launch_quantize_rows(const QuantizeArgs& a, int dtype) {
-  return dtype == KG_DTYPE_F32 ? launch_quantize<float>(a, g_stream)
-         : dtype == KG_DTYPE_BF16 ? launch_quantize<__bf16>(a, g_stream)
-                                  : launch_quantize<_Float16>(a, g_stream);
+  return with_float_type(dtype, [&](auto t) { return launch_quantize<decltype(t)>(a, PackArgs{}, g_stream); });
 }
 
 int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
@@ -1956,63 +1966,60 @@ int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
 // Rows that the kernel for weights of any alignment takes.
 constexpr long long kInt8FewRows = 32;
 
-// The matrix-core forms of int8_matmul. kUnsupported: none of them, since there is no workspace to be had, or not enough.
+// The matrix-core forms of int8_matmul. kUnsupported: none of them, since there is no workspace to be had.
 template <typename T>
-int launch_int8(const Int8Args& a, bool codes, bool out_aligned, bool x_aligned, bool w_aligned) {
+int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
   const bool whole = a.k % 16 == 0, whole_w = whole && w_aligned && a.w_row <= kMaxPipeLd;
   const bool few = a.m <= kInt8FewRows && !whole_w;
-  Int8Tiles g{static_cast<const int8_t*>(a.x), a.w, a.x_scale, a.w_scale, a.bias, a.out, a.x_row, a.w_row, a.out_row,
-              a.x_scale_stride, a.w_scale_stride, a.bias_stride, a.m, a.n, a.k, a.wide_bias, out_aligned};
   // rows and weights in the workspace: codes of rows that are quantised here; for the tiles, copies of rows that are not whole 16-byte pieces
   const long long pitch = cdiv(a.k, 64) * 64;
   const bool take_x = !codes || (!few && !(whole && x_aligned && a.x_row <= kMaxPipeLd));
   const bool take_w = !few && !whole_w;
-  const long long w_bytes = take_w ? a.n * pitch : 0, row_bytes = take_x ? pitch + (codes ? 0 : (long long)sizeof(float)) : 0;
-  const long long room = kSplitMaxWorkspace - w_bytes - 512;
-  long long rows = a.m;  // of a piece that the workspace holds: whole tiles
-  if (row_bytes > 0 && a.m * row_bytes > room) rows = room / row_bytes / 256 * 256;
-  if (rows <= 0) return kUnsupported;
+  // pieces of channels and rows that the workspace holds (a row: at most 128 KiB), of fewer tiles than a launch has workgroups
+  long long channels = std::min<long long>(a.n, 1 << 22);
+  if (take_w) channels = std::min(channels, std::max(256ll, (kSplitMaxWorkspace >> 1) / pitch / 256 * 256));
+  const long long w_bytes = take_w ? channels * pitch : 0, row_bytes = take_x ? pitch + (codes ? 0 : (long long)sizeof(float)) : 0;
+  long long rows = std::min<long long>(a.m, (kMostBlocks * 32 / cdiv(channels, 32)) / 256 * 256);
+  if (row_bytes > 0) rows = std::min(rows, std::max(256ll, (kSplitMaxWorkspace - w_bytes - 512) / row_bytes / 256 * 256));
   SplitLease lease;  // held until the kernels are enqueued
   char* ws = nullptr;
   if (take_x || take_w) {
     lease = split_workspace((size_t)(w_bytes + rows * row_bytes + 512), g_stream);
     if ((ws = static_cast<char*>(lease.ptr)) == nullptr) return kUnsupported;
   }
-  auto pack = [&](const int8_t* from, long long ld, char* to, int count) {
-    hipLaunchKernelGGL((int8_pack_kernel<>), dim3((unsigned)std::min(cdiv(count * (pitch / 16), 256), 4096ll)), dim3(256), 0, g_stream, from, ld,
-                       reinterpret_cast<int8_t*>(to), (int)pitch, count, a.k);
-  };
-  if (take_w) {
-    pack(a.w, a.w_row, ws, a.n);
-    g.w = reinterpret_cast<const int8_t*>(ws);
-    g.ldw = pitch;
-  }
-  char* x_ws = ws + w_bytes;
-  for (long long m0 = 0; m0 < a.m; m0 += rows) {
-    g.m = (int)std::min(rows, a.m - m0);
-    g.out = static_cast<T*>(a.out) + m0 * a.out_row;
-    if (codes) {
-      g.x_scale = a.x_scale + m0 * a.x_scale_stride;
-      g.x = static_cast<const int8_t*>(a.x) + m0 * a.x_row;
-      if (take_x) pack(g.x, a.x_row, x_ws, g.m);
-    } else {
-      float* scales = reinterpret_cast<float*>(x_ws + cdiv(rows * pitch, 256) * 256);
-      const QuantizeArgs q{static_cast<const T*>(a.x) + m0 * a.x_row, reinterpret_cast<int8_t*>(x_ws), scales, a.x_row, pitch, 1,
-                           g.m, a.k, (int)pitch};
-      (void)launch_quantize<T>(q, g_stream);
-      g.x_scale = scales;
-      g.x_scale_stride = 1;
-    }
-    if (take_x) {
-      g.x = reinterpret_cast<const int8_t*>(x_ws);
-      g.ldx = pitch;
-    }
-    if (few) {
-      (void)launch_int8_few<T>(g, g_stream);
-    } else {
-      if (take_x && take_w) g.k = (int)pitch;  // (zeros behind the rows' ends)
-      else g.k = (int)(cdiv(a.k, 16) * 16);
-      (void)launch_int8_tiles<T>(g, int8_form(g.m, g.n, g.k), g_stream);
+  const long long bias_bytes = (a.wide_bias ? 4 : (long long)sizeof(T)) * a.bias_stride;
+  for (long long n0 = 0; n0 < a.n; n0 += channels) {
+    PackArgs pack_w{};
+    const int count = (int)std::min(channels, a.n - n0);
+    const int8_t* w = a.w + n0 * a.w_row;
+    if (take_w) pack_w = PackArgs{w, reinterpret_cast<int8_t*>(ws), a.w_row, (int)pitch, count, a.k};
+    for (long long m0 = 0; m0 < a.m; m0 += rows) {
+      Int8Tiles g{static_cast<const int8_t*>(a.x), take_w ? pack_w.dst : w, a.x_scale, a.w_scale + n0 * a.w_scale_stride,
+                  a.bias == nullptr ? nullptr : static_cast<const char*>(a.bias) + n0 * bias_bytes, static_cast<T*>(a.out) + m0 * a.out_row + n0,
+                  a.x_row, take_w ? pitch : a.w_row, a.out_row, a.x_scale_stride, a.w_scale_stride, a.bias_stride,
+                  (int)std::min(rows, a.m - m0), count, a.k, a.wide_bias};
+      int8_t* x_ws = reinterpret_cast<int8_t*>(ws + w_bytes);
+      if (codes) {
+        g.x += m0 * a.x_row;
+        g.x_scale += m0 * a.x_scale_stride;
+        PackArgs pack_x{};
+        if (take_x) pack_x = PackArgs{g.x, x_ws, a.x_row, (int)pitch, g.m, a.k};
+        (void)launch_int8_pack(pack_x, pack_w, g_stream);
+      } else {
+        float* scales = reinterpret_cast<float*>(x_ws + cdiv(rows * pitch, 256) * 256);
+        const QuantizeArgs q{static_cast<const T*>(a.x) + m0 * a.x_row, x_ws, scales, a.x_row, pitch, 1, g.m, a.k, (int)pitch};
+        (void)launch_quantize<T>(q, pack_w, g_stream);
+        g.x_scale = scales;
+        g.x_scale_stride = 1;
+      }
+      pack_w.rows = 0;  // (packed with the first piece of rows)
+      if (take_x) g.x = x_ws, g.ldx = pitch;
+      if (few) {
+        (void)launch_int8_few<T>(g, g_stream);
+      } else {
+        if (!whole) g.k = (int)pitch;  // (both are copies, zeros behind the rows' ends)
+        (void)launch_int8_tiles<T>(g, int8_form(g.m, g.n, g.k), g_stream);
+      }
     }
   }
   return finish_launch("int8_matmul");
@@ -2056,7 +2063,7 @@ int int8_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   return with_float_type(out.dtype, [&](auto t) {
     using T = decltype(t);
     if (K >= 16) {
-      const int done = launch_int8<T>(a, codes, rows_aligned(out, 16), rows_aligned(x, 16), rows_aligned(w, 16));
+      const int done = launch_int8<T>(a, codes, rows_aligned(x, 16), rows_aligned(w, 16));
       if (done != kUnsupported) return done;
     }
     const unsigned grid = most_blocks(M * cdiv(N, 64));
