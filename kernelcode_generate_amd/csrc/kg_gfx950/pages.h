@@ -71,13 +71,15 @@ __device__ __forceinline__ int pages_owner(const int* sums, int batch, int x) {
   return lo;
 }
 
-// Slot and position of row t, behind the sums of all requests. row_of, fresh_of: a request's first row and first of all new pages.
-__device__ __forceinline__ void assign_row(const PagesArgs& a, int t, int rows, int count, const int* row_of, const int* fresh_of) {
+// Slot and position of row t, behind the sums of all requests. row_of, fresh_of: a request's first row and first of all new pages;
+// context(b): its cached tokens.
+template <typename F>
+__device__ __forceinline__ void assign_row(const PagesArgs& a, int t, int rows, int count, const int* row_of, const int* fresh_of, F context) {
   long long slot = -1;
   int position = -1;
   if (t < rows) {
     const int b = pages_owner(row_of, a.batch, t);
-    const int c = max(a.context[b * a.context_stride], 0);
+    const int c = context(b);
     const uint32_t at = (uint32_t)c + (uint32_t)(t - row_of[b]);
     position = (int)min(at, 0x7fffffffu);
     if (at < 0x7fffffffu) {
@@ -105,7 +107,8 @@ __device__ __forceinline__ void assign_row(const PagesArgs& a, int t, int rows, 
 // was, first rows (batch + 1 of them), first new pages.
 template <bool kSums>
 __global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a, int* sums) {
-  __shared__ int row_lds[kSums ? 1 : kPagesMostRequests + 1], fresh_lds[kSums ? 1 : kPagesMostRequests];
+  __shared__ int row_lds[kSums ? 1 : kPagesMostRequests + 1], fresh_lds[kSums ? 1 : kPagesMostRequests],
+      context_lds[kSums ? 1 : kPagesMostRequests];
   __shared__ int scan[kPagesThreads / 64], last_of[kPagesThreads / 64];
   int* row_of = kSums ? sums + 1 : row_lds;
   int* fresh_of = kSums ? sums + 2 + a.batch : fresh_lds;
@@ -132,6 +135,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a, i
     if (real) {
       row_of[b] = first;
       fresh_of[b] = fresh + pages_upto - pages;
+      if (!kSums) context_lds[b] = c;
       a.starts[b * a.start_stride] = first;
     }
     rows = (int)min((uint32_t)rows + (uint32_t)all, (uint32_t)a.tokens);
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_assign_kernel(PagesArgs a, i
   }
   if constexpr (!kSums) {
     __syncthreads();
-    for (int t = tid; t < a.tokens; t += kPagesThreads) assign_row(a, t, rows, count, row_of, fresh_of);
+    for (int t = tid; t < a.tokens; t += kPagesThreads) assign_row(a, t, rows, count, row_of, fresh_of, [&](int b) { return context_lds[b]; });
   }
 }
 
@@ -156,35 +160,43 @@ __global__ __launch_bounds__(256) void kv_assign_rows_kernel(PagesArgs a, const 
   __syncthreads();
   const int rows = row_of[a.batch];
   for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < a.tokens; t += 256ll * gridDim.x)
-    assign_row(a, (int)t, rows, count, row_of, sums + 2 + a.batch);
+    assign_row(a, (int)t, rows, count, row_of, sums + 2 + a.batch, [&](int b) { return max(a.context[b * a.context_stride], 0); });
 }
 
 __global__ __launch_bounds__(kPagesThreads) void kv_release_kernel(PagesArgs a) {
-  __shared__ int entry_of[kPagesMostRequests];  // entries of the requests before
+  __shared__ int entry_of[kPagesMostRequests], page_of[kPagesMostRequests];  // entries of the requests before, a request's first page
   __shared__ int scan[kPagesThreads / 64];
   const int tid = threadIdx.x;
   const int count = max(min(*a.count, a.stack), 0);
   int entries = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kPagesThreads) {
     const int b = b0 + tid;
-    int n = 0;
-    if (b < a.batch) n = max(pages_of(a.added[b * a.added_stride], a) - pages_of(a.context[b * a.context_stride], a), 0);
+    int n = 0, first = 0;
+    if (b < a.batch) {
+      first = pages_of(a.context[b * a.context_stride], a);
+      n = max(pages_of(a.added[b * a.added_stride], a) - first, 0);
+    }
     int all;
     const int upto = pages_scan<false>(n, 0, scan, &all);
-    if (b < a.batch) entry_of[b] = entries + upto - n;
+    if (b < a.batch) {
+      entry_of[b] = entries + upto - n;
+      page_of[b] = first;
+    }
     entries += all;
   }
   __syncthreads();
-  // how many of them are pages
   auto entry = [&](int e) __attribute__((always_inline)) {
     const int b = pages_owner(entry_of, a.batch, e);
-    const int p = pages_of(a.context[b * a.context_stride], a) + e - entry_of[b];
-    return a.table + b * a.table_0 + p * a.table_1;
+    return a.table + b * a.table_0 + (page_of[b] + e - entry_of[b]) * a.table_1;
   };
-  int found = 0;
-  for (int e = tid; e < entries; e += kPagesThreads) found += *entry(e) >= 0;
-  int pages;
-  pages_scan<false>(found, 0, scan, &pages);
+  // how many of the entries are pages: of more than a thread has one of, by a walk of its own
+  const bool one = entries <= kPagesThreads;
+  int pages = 0;
+  if (!one) {
+    int found = 0;
+    for (int e = tid; e < entries; e += kPagesThreads) found += *entry(e) >= 0;
+    pages_scan<false>(found, 0, scan, &pages);
+  }
   int before = 0;
   for (int e0 = 0; e0 < entries; e0 += kPagesThreads) {
     const int e = e0 + tid;
@@ -192,6 +204,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_release_kernel(PagesArgs a) 
     const int page = at != nullptr ? *at : -1;
     int all;
     const int upto = before + pages_scan<false>(page >= 0, 0, scan, &all);
+    if (one) pages = all;
     before += all;
     if (page >= 0) {
       const int spot = count + pages - upto;
