@@ -283,7 +283,9 @@ enum {
   KG_OP_FLASH_ATTENTION = 3,
   /* the projection's MFMAs, without the adapters', whose number depends on the indexes; fp32 sums of a split K are
    * counted as written and read */
-  KG_OP_ADAPTER_MATMUL = 4
+  KG_OP_ADAPTER_MATMUL = 4,
+  /* codes that the call makes, and weights that it copies, are counted as written and read */
+  KG_OP_INT8_MATMUL = 5
 };
 enum {
   KG_COST_MAC = 0,       /* multiply-accumulates of the operation (mask-kept pairs for causal attention) */

@@ -79,6 +79,16 @@ inline int int8_form(long long m, long long n, long long k) {
   }
   return best;
 }
+// MFMA instructions of the two forms (cost queries).
+inline long long int8_tiles_mfma(long long m, long long n, long long k) {
+  const Int8Form& f = kInt8Forms[int8_form(m, n, k)];
+  const long long tiles = ((m + f.rows - 1) / f.rows) * ((n + f.channels - 1) / f.channels), slices = (k + 127) / 128;
+  return tiles * (f.rows / 16) * (f.channels / 16) * 2 * (slices < f.stages ? f.stages : slices);
+}
+inline long long int8_few_mfma(long long m, long long n, long long k) {
+  const long long each = ((k + 63) / 64 + fewi::kWaves - 1) / fewi::kWaves;  // steps of a wave, four at a time
+  return (n + 15) / 16 * fewi::kWaves * ((each + 3) / 4 * 4) * (m <= 16 ? 1 : 2);
+}
 template <typename T>
 hipError_t launch_int8_tiles(const Int8Tiles& g, int form, hipStream_t stream) {
   switch (form) {

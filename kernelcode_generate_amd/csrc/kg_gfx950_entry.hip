@@ -1981,6 +1981,17 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
   const long long w_bytes = take_w ? channels * pitch : 0, row_bytes = take_x ? pitch + (codes ? 0 : (long long)sizeof(float)) : 0;
   long long rows = std::min<long long>(a.m, (kMostBlocks * 32 / cdiv(channels, 32)) / 256 * 256);
   if (row_bytes > 0) rows = std::min(rows, std::max(256ll, (kSplitMaxWorkspace - w_bytes - 512) / row_bytes / 256 * 256));
+  if (g_cost != nullptr) {
+    const long long k = whole ? a.k : pitch;
+    long long mfma = 0;
+    for (long long n0 = 0; n0 < a.n; n0 += channels)
+      for (long long m0 = 0; m0 < a.m; m0 += rows) {
+        const long long m = std::min(rows, a.m - m0), n = std::min(channels, a.n - n0);
+        mfma += few ? int8_few_mfma(m, n, a.k) : int8_tiles_mfma(m, n, k);
+      }
+    const long long copies = (take_x ? (long long)a.m * pitch : 0) + (take_w ? (long long)a.n * pitch : 0);
+    return record_cost((long long)a.m * a.n * a.k, mfma, 16, copies, copies);
+  }
   SplitLease lease;  // held until the kernels are enqueued
   char* ws = nullptr;
   if (take_x || take_w) {
@@ -2056,16 +2067,21 @@ int int8_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   if ((rc = check_view(out, "out")) || (rc = check_view(x, "x")) || (rc = check_view(x_scale, "x_scale")) ||
       (rc = check_view(w, "weight")) || (rc = check_view(w_scale, "w_scale")) || (rc = check_view(bias, "bias")))
     return rc;
-  if (M == 0 || N == 0) return finish_launch("int8_matmul(empty)");
+  if ((M == 0 || N == 0) && !g_cost) return finish_launch("int8_matmul(empty)");
   const Int8Args a{x.data, static_cast<const int8_t*>(w.data), static_cast<const float*>(x_scale.data),
                    static_cast<const float*>(w_scale.data), bias.data, out.data, x.stride[0], w.stride[0], out.stride[0],
                    x_scale.stride[0], w_scale.stride[0], bias.stride[0], (int)M, (int)N, (int)K, bias.dtype == KG_DTYPE_F32};
   return with_float_type(out.dtype, [&](auto t) {
     using T = decltype(t);
-    if (K >= 16) {
-      const int done = launch_int8<T>(a, codes, rows_aligned(x, 16), rows_aligned(w, 16));
-      if (done != kUnsupported) return done;
+    if (g_cost) record_cost(M * N * K, 0, 16, 0, 0);
+    int done = kUnsupported;
+    if (K >= 16 && M > 0 && N > 0) done = launch_int8<T>(a, codes, rows_aligned(x, 16), rows_aligned(w, 16));
+    if (g_cost) {
+      g_cost->v[KG_COST_HBM_READ] += M * K * element_bytes(x.dtype) + N * K + 4 * N + (codes ? 4 * M : 0) + (bias.present ? N * element_bytes(bias.dtype) : 0);
+      g_cost->v[KG_COST_HBM_WRITE] += M * N * (long long)sizeof(T);
+      return kOk;
     }
+    if (done != kUnsupported) return done;
     const unsigned grid = most_blocks(M * cdiv(N, 64));
     if (codes) hipLaunchKernelGGL((int8_any_kernel<T, int8_t>), dim3(grid), dim3(256), 0, g_stream, a);
     else hipLaunchKernelGGL((int8_any_kernel<T, T>), dim3(grid), dim3(256), 0, g_stream, a);
@@ -2240,6 +2256,7 @@ int kg_gfx950_cost(int op, const KgArgSlot* ordered_args, unsigned long long arg
     case KG_OP_CONV2D: rc = conv2d_impl(ordered_args, arg_count); break;
     case KG_OP_FLASH_ATTENTION: rc = flash_attention_impl(ordered_args, arg_count); break;
     case KG_OP_ADAPTER_MATMUL: rc = adapter_matmul_impl(ordered_args, arg_count); break;
+    case KG_OP_INT8_MATMUL: rc = int8_matmul_impl(ordered_args, arg_count); break;
     default: rc = fail(kInvalid, "cost: unknown op %d", op);
   }
   g_cost = nullptr;

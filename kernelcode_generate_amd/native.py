@@ -65,7 +65,7 @@ CONTROL_SYMBOLS = (
 )
 
 # kg_gfx950_cost: op codes (KG_OP_*) and the order of its output array (KG_COST_*).
-COST_OPS = {"matmul": 1, "conv2d": 2, "flash_attention": 3, "adapter_matmul": 4}
+COST_OPS = {"matmul": 1, "conv2d": 2, "flash_attention": 3, "adapter_matmul": 4, "int8_matmul": 5}
 COST_KINDS = ("MAC", "MFMA", "HBM_READ", "HBM_WRITE", "MFMA_CYCLES")
 
 
