@@ -194,7 +194,7 @@ int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long 
  * last request's get -1 in both. A page that begins with a new token is taken from free_pages, a stack of *free_count pages with the
  * last one on top, in the order of requests and positions, and entered in page_table; -1 where none is left, and such
  * tokens, as those behind P pages, get slot -1. *free_count is then what is left (values outside 0 .. F count as the nearest).
- * B <= 8192. page_table, starts, slots and positions are what kv_cache_store, head_norm_rotate and tree_attention take.
+ * B <= 8192, B * P and T at most 2^31 - 4096. page_table, starts, slots and positions are what kv_cache_store, head_norm_rotate and tree_attention take.
  * No two of the tensors may overlap. The call reads what it writes: a recorded graph takes new pages on every replay.
  */
 int kg_gfx950_kv_cache_assign_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
@@ -212,7 +212,7 @@ int kg_gfx950_kv_cache_release_entry(const KgArgSlot* ordered_args, unsigned lon
  * (codes[M, K] i8, scale[M] f32, x[M, K])
  * Rows in 8-bit integers: scale = max|x| * fl32(1 / 127), code = x / scale as a 32-bit quotient, rounded to nearest, ties to even,
  * -127 .. 127; 0 where the scale is 0 or not finite (a row with an infinity or NaN has that scale). x: f32, f16, bf16. What
- * int8_matmul takes, as its rows or as its weights.
+ * int8_matmul takes, as its rows or as its weights. No two of the tensors may overlap.
  */
 int kg_gfx950_quantize_rows_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
 

@@ -48,7 +48,7 @@ SOURCES = ("kg_gfx950_entry.hip", "kg_gfx950_gemm.hip", "kg_gfx950_gemm_quad.hip
            "kg_gfx950_fa_persist.hip", "kg_gfx950_fa_decode.hip", "kg_gfx950_conv_rowvec.hip", "kg_gfx950_conv_igemm.hip",
            "kg_gfx950_conv_nhwc.hip", "kg_gfx950_gemm_skinny.hip", "kg_gfx950_tree_bf16.hip", "kg_gfx950_tree_f16.hip",
            "kg_gfx950_adapter_mid.hip", "kg_gfx950_adapter_quad.hip", "kg_gfx950_adapter_pipe.hip", "kg_gfx950_int8_f32.hip",
-           "kg_gfx950_int8_bf16.hip", "kg_gfx950_int8_f16.hip", "kg_gfx950_int8_few.hip")
+           "kg_gfx950_int8_bf16.hip", "kg_gfx950_int8_f16.hip", "kg_gfx950_quantize.hip")
 
 
 def build_library(output: Path = OUTPUT, extra_flags: tuple[str, ...] = (), verbose: bool = False) -> Path:

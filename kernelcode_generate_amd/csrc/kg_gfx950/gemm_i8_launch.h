@@ -1,7 +1,6 @@
 // Host side of the matrix-core kernels of int8_matmul and of quantize_rows: their forms and launches.
 #pragma once
 
-#include "gemm_i8_few.h"
 #include "gemm_i8_tiles.h"
 #include "quantize.h"
 
@@ -45,16 +44,6 @@ hipError_t launch_quantize(const QuantizeArgs& a, const PackArgs& pack, hipStrea
   return hipGetLastError();
 }
 
-// m <= 32
-template <typename T>
-hipError_t launch_int8_few(const Int8Tiles& g, hipStream_t stream) {
-  const int blocks = (g.n + 15) / 16;
-  const dim3 grid((unsigned)(blocks < 512 ? blocks : 512));
-  if (g.m <= 16) hipLaunchKernelGGL((int8_few_kernel<T, 1, 1>), grid, dim3(fewi::kThreads), 0, stream, g);
-  else hipLaunchKernelGGL((int8_few_kernel<T, 2, 1>), grid, dim3(fewi::kThreads), 0, stream, g);
-  return hipGetLastError();
-}
-
 // The tiles of a product by a model of each form's time (ns): a launch, a further round of 256 tiles, a slice of 128 k, and percent more of
 // a slice where all CUs have a tile (their clocks go down). Fitted to 350 products of 1..4096 rows, 1024..16384 channels and K of
 // 512..11008, of which the one that it picks is 2.9 % above the fastest on average, the measurements' own spread with it. us of the forms in
@@ -79,15 +68,11 @@ inline int int8_form(long long m, long long n, long long k) {
   }
   return best;
 }
-// MFMA instructions of the two forms (cost queries).
+// MFMA instructions of a product (cost queries).
 inline long long int8_tiles_mfma(long long m, long long n, long long k) {
   const Int8Form& f = kInt8Forms[int8_form(m, n, k)];
   const long long tiles = ((m + f.rows - 1) / f.rows) * ((n + f.channels - 1) / f.channels), slices = (k + 127) / 128;
   return tiles * (f.rows / 16) * (f.channels / 16) * 2 * (slices < f.stages ? f.stages : slices);
-}
-inline long long int8_few_mfma(long long m, long long n, long long k) {
-  const long long each = ((k + 63) / 64 + fewi::kWaves - 1) / fewi::kWaves;  // steps of a wave, four at a time
-  return (n + 15) / 16 * fewi::kWaves * ((each + 3) / 4 * 4) * (m <= 16 ? 1 : 2);
 }
 template <typename T>
 hipError_t launch_int8_tiles(const Int8Tiles& g, int form, hipStream_t stream) {

@@ -22,14 +22,12 @@ KG_INT8_INSTANCE(__bf16)
 KG_INT8_INSTANCE(_Float16)
 #endif
 #undef KG_INT8_INSTANCE
-#if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_INT8_FEW)
-#define KG_INT8_INSTANCE(T)                                                                                     \
-  KG_INSTANCE hipError_t launch_quantize<T>(const QuantizeArgs&, const PackArgs&, hipStream_t);                  \
-  KG_INSTANCE hipError_t launch_int8_few<T>(const Int8Tiles&, hipStream_t);
-KG_INT8_INSTANCE(float)
-KG_INT8_INSTANCE(__bf16)
-KG_INT8_INSTANCE(_Float16)
-#undef KG_INT8_INSTANCE
+#if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_QUANTIZE)
+#define KG_QUANTIZE_INSTANCE(T) KG_INSTANCE hipError_t launch_quantize<T>(const QuantizeArgs&, const PackArgs&, hipStream_t);
+KG_QUANTIZE_INSTANCE(float)
+KG_QUANTIZE_INSTANCE(__bf16)
+KG_QUANTIZE_INSTANCE(_Float16)
+#undef KG_QUANTIZE_INSTANCE
 #endif
 
 }  // namespace kg_gfx950

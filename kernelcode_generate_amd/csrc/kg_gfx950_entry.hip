@@ -1826,6 +1826,8 @@ int adapter_matmul_impl(const KgArgSlot* args, unsigned long long n) {
 
 constexpr unsigned kI32 = 1u << KG_DTYPE_I32, kI64 = 1u << KG_DTYPE_I64, kF32 = 1u << KG_DTYPE_F32, kI8 = 1u << KG_DTYPE_I8;
 
+constexpr long long kPagesMostWalk = (1ll << 31) - 4096;
+
 // The page table, the stack of free pages and the requests' two lengths, from slot `at` on.
 struct PagesSlots {
   Mem table, free, count, first, second;
@@ -1846,7 +1848,8 @@ int read_pages(const KgArgSlot* args, int at, const char* op, const char* first,
     return fail(kInvalid, "%s: %s and %s must have a value for each of %lld requests", op, first, second, batch);
   if (p->page_size < 1 || p->page_size > 0x7fffffffLL) return fail(kInvalid, "%s: page_size %lld not in 1..2^31-1", op, p->page_size);
   if (batch > kPagesMostRequests) return fail(kUnsupported, "%s: %lld requests > %d", op, batch, kPagesMostRequests);
-  if (batch * p->table.shape[1] > 0x7fffffffLL) return fail(kUnsupported, "%s: page_table of more than 2^31-1 entries", op);
+  // (a workgroup's walks over entries and rows stay in 31 bits)
+  if (batch * p->table.shape[1] > kPagesMostWalk) return fail(kUnsupported, "%s: page_table of more than %lld entries", op, kPagesMostWalk);
   return kOk;
 }
 
@@ -1896,6 +1899,7 @@ int kv_cache_assign_impl(const KgArgSlot* args, unsigned long long n) {
     return fail(kInvalid, "kv_cache_assign: %lld positions for %lld slots", positions.shape[0], tokens);
   if (starts.shape[0] != batch + 1)
     return fail(kInvalid, "kv_cache_assign: starts must have %lld values, got %lld", batch + 1, starts.shape[0]);
+  if (tokens > kPagesMostWalk) return fail(kUnsupported, "kv_cache_assign: more than %lld rows", kPagesMostWalk);
   if ((rc = check_view(slots, "slots")) || (rc = check_view(positions, "positions")) || (rc = check_view(starts, "starts")) ||
       (rc = check_pages(p, "context_lens", "new_lens")))
     return rc;
@@ -1932,6 +1936,11 @@ int kv_cache_release_impl(const KgArgSlot* args, unsigned long long n) {
   return finish_launch("kv_cache_release");
 }
 
+// What a launcher returned, which took the error; the last launch of a call is finish_launch's.
+int launched(hipError_t err, const char* what) {
+  return err == hipSuccess ? kOk : fail(kHipFailure, "%s: launch failed: %s", what, hipGetErrorString(err));
+}
+
 template <typename F>
 auto with_float_type(int dtype, F&& f) {
   return dtype == KG_DTYPE_F32 ? f(float{}) : dtype == KG_DTYPE_BF16 ? f((__bf16)0.f) : f((_Float16)0.f);
@@ -1959,22 +1968,19 @@ int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
   if (M == 0) return finish_launch("quantize_rows(empty)");
   QuantizeArgs a{x.data, static_cast<int8_t*>(codes.data), static_cast<float*>(scale.data), x.stride[0], codes.stride[0],
                  scale.stride[0], (int)M, (int)K, (int)K};
-  (void)launch_quantize_rows(a, x.dtype);
+  if ((rc = launched(launch_quantize_rows(a, x.dtype), "quantize_rows"))) return rc;
   return finish_launch("quantize_rows");
 }
-
-// Rows that the kernel for weights of any alignment takes.
-constexpr long long kInt8FewRows = 32;
 
 // The matrix-core forms of int8_matmul. kUnsupported: none of them, since there is no workspace to be had.
 template <typename T>
 int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
-  const bool whole = a.k % 16 == 0, whole_w = whole && w_aligned && a.w_row <= kMaxPipeLd;
-  const bool few = a.m <= kInt8FewRows && !whole_w;
-  // rows and weights in the workspace: codes of rows that are quantised here; for the tiles, copies of rows that are not whole 16-byte pieces
+  // rows and weights in the workspace: codes of rows that are quantised here, and copies of rows that are not whole 16-byte pieces
+  // (33 x 4096 x 4095: 18.5 us, x 4096 7.2; a kernel of few rows that reads such weights as they are took 17.1 for 16 rows, 24 for 32)
   const long long pitch = cdiv(a.k, 64) * 64;
-  const bool take_x = !codes || (!few && !(whole && x_aligned && a.x_row <= kMaxPipeLd));
-  const bool take_w = !few && !whole_w;
+  const bool whole = a.k % 16 == 0;
+  const bool take_x = !codes || !(whole && x_aligned && a.x_row <= kMaxPipeLd);
+  const bool take_w = !(whole && w_aligned && a.w_row <= kMaxPipeLd);
   // pieces of channels and rows that the workspace holds (a row: at most 128 KiB), of fewer tiles than a launch has workgroups
   long long channels = std::min<long long>(a.n, 1 << 22);
   if (take_w) channels = std::min(channels, std::max(256ll, (kSplitMaxWorkspace >> 1) / pitch / 256 * 256));
@@ -1987,7 +1993,7 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
     for (long long n0 = 0; n0 < a.n; n0 += channels)
       for (long long m0 = 0; m0 < a.m; m0 += rows) {
         const long long m = std::min(rows, a.m - m0), n = std::min(channels, a.n - n0);
-        mfma += few ? int8_few_mfma(m, n, a.k) : int8_tiles_mfma(m, n, k);
+        mfma += int8_tiles_mfma(m, n, k);
       }
     const long long copies = (take_x ? (long long)a.m * pitch : 0) + (take_w ? (long long)a.n * pitch : 0);
     return record_cost((long long)a.m * a.n * a.k, mfma, 16, copies, copies);
@@ -2010,27 +2016,25 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
                   a.x_row, take_w ? pitch : a.w_row, a.out_row, a.x_scale_stride, a.w_scale_stride, a.bias_stride,
                   (int)std::min(rows, a.m - m0), count, a.k, a.wide_bias};
       int8_t* x_ws = reinterpret_cast<int8_t*>(ws + w_bytes);
+      hipError_t err = hipSuccess;
       if (codes) {
         g.x += m0 * a.x_row;
         g.x_scale += m0 * a.x_scale_stride;
         PackArgs pack_x{};
         if (take_x) pack_x = PackArgs{g.x, x_ws, a.x_row, (int)pitch, g.m, a.k};
-        (void)launch_int8_pack(pack_x, pack_w, g_stream);
+        err = launch_int8_pack(pack_x, pack_w, g_stream);
       } else {
         float* scales = reinterpret_cast<float*>(x_ws + cdiv(rows * pitch, 256) * 256);
         const QuantizeArgs q{static_cast<const T*>(a.x) + m0 * a.x_row, x_ws, scales, a.x_row, pitch, 1, g.m, a.k, (int)pitch};
-        (void)launch_quantize<T>(q, pack_w, g_stream);
+        err = launch_quantize<T>(q, pack_w, g_stream);
         g.x_scale = scales;
         g.x_scale_stride = 1;
       }
       pack_w.rows = 0;  // (packed with the first piece of rows)
       if (take_x) g.x = x_ws, g.ldx = pitch;
-      if (few) {
-        (void)launch_int8_few<T>(g, g_stream);
-      } else {
-        if (!whole) g.k = (int)pitch;  // (both are copies, zeros behind the rows' ends)
-        (void)launch_int8_tiles<T>(g, int8_form(g.m, g.n, g.k), g_stream);
-      }
+      if (!whole) g.k = (int)pitch;  // (both are copies, zeros behind the rows' ends)
+      if (err == hipSuccess) err = launch_int8_tiles<T>(g, int8_form(g.m, g.n, g.k), g_stream);
+      if (const int rc = launched(err, "int8_matmul")) return rc;
     }
   }
   return finish_launch("int8_matmul");

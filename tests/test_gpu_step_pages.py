@@ -135,12 +135,12 @@ def test_nothing(device):
     assert count.item() == 0
 
 
-def test_recorded_steps(device):
-    """A recorded step: every replay takes its pages from the stack as it is then."""
+@pytest.mark.parametrize("tokens", [20 * 40, 5000])
+def test_recorded_steps(device, tokens):
+    """A recorded step, of one launch and of two: every replay takes its pages from the stack as it is then."""
 
     rng = random.Random(5)
     context, new, table, free = make(rng, 20, 30, 16, 200, 40, 3.0)
-    tokens = 20 * 40
     t, stack, left = (torch.tensor(x, dtype=I32, device=device) for x in (table, free, [len(free)]))
     c, n = (torch.tensor(x, dtype=I32, device=device) for x in (context, new))
     slots, positions, starts = (torch.zeros(x, dtype=d, device=device) for x, d in ((tokens, torch.int64), (tokens, I32), (21, I32)))

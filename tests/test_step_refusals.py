@@ -102,13 +102,15 @@ def test_pages(op, first, second):
     many = torch.zeros(8193, dtype=I32)
     extra = {"starts": torch.zeros(8194, dtype=I32)} if op == "assign" else {}
     refused(op, -3, "8193 requests > 8192", page_table=torch.zeros(8193, 1, dtype=I32), **{first: many, second: many}, **extra)
-    refused(op, -3, "2.31-1 entries", page_table=torch.zeros(3, 1, dtype=I32).expand(3, 2**30))
+    refused(op, -3, "more than 2147479552 entries", page_table=torch.zeros(3, 1, dtype=I32).expand(3, 2**30))
 
 
 def test_assign():
     refused("assign", -1, "9 positions for 10 slots", positions=torch.zeros(9, dtype=I32))
     refused("assign", -1, "starts must have 4 values", starts=torch.zeros(3, dtype=I32))
     refused("assign", -1, "unsupported dtype_code 3", slots=torch.zeros(10, dtype=I32))
+    long = native.TensorSpec((2**31 - 4095,), "int64", (0,)), native.TensorSpec((2**31 - 4095,), "int32", (0,))
+    refused("assign", -3, "more than 2147479552 rows", slots=long[0], positions=long[1])
 
 
 def test_rows():
