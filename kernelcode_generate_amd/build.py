@@ -18,6 +18,7 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PACKAGE_DIR.parent
 CSRC = PACKAGE_DIR / "csrc"
 OUTPUT = PACKAGE_DIR / "libkg_gfx950.so"
+CALL_OUTPUT = PACKAGE_DIR / "_kg_call.so"  # the entries called with torch tensors, without Python's packing of slots
 PROBE_OUTPUT = PACKAGE_DIR / "libkg_gfx950_probe.so"  # bench.py's measurement library
 OFFLOAD_ARCH = "gfx950"
 
@@ -96,10 +97,34 @@ def build_probe_library(output: Path = PROBE_OUTPUT, verbose: bool = False) -> P
     return output
 
 
+def build_call_module(output: Path = CALL_OUTPUT, verbose: bool = False) -> Path:
+    """Compile csrc/python/kg_call.cpp, a host module of the running Python against the torch that is installed."""
+
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    tmp = output.with_suffix(".so.tmp")
+    libraries = library_paths()
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *include_flags()[:1],
+           f"-I{sysconfig.get_paths()['include']}", *(f"-I{p}" for p in include_paths()), str(CSRC / "python" / "kg_call.cpp"),
+           "-o", str(tmp), *(f"-L{p}" for p in libraries), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    proc = subprocess.run(cmd, capture_output=True, text=True, env=dict(os.environ))
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stderr[-4000:]}")
+    os.replace(tmp, output)
+    return output
+
+
 def main() -> int:
     path = build_library(verbose=True)
     print(f"built {path}")
     print(f"built {build_probe_library(verbose=True)}")
+    print(f"built {build_call_module(verbose=True)}")
     return 0
 
 

@@ -95,6 +95,9 @@ class NativeLibraryError(RuntimeError):
 _LIBRARY: ctypes.CDLL | None = None
 # the entries taking the slots' address as an integer (call_entry packs them itself)
 _ADDRESS_CALLS: dict[str, Any] = {}
+# the entries' own addresses, and the host module that packs torch tensors into slots (None: not built, or no torch)
+_ENTRY_ADDRESSES: dict[str, int] = {}
+_FAST_CALL: Any = None
 
 
 def library_path() -> Path:
@@ -105,7 +108,7 @@ def library_path() -> Path:
 def load_library() -> ctypes.CDLL:
     """Load (once) and return the gfx950 library; raise if it has not been built."""
 
-    global _LIBRARY
+    global _LIBRARY, _FAST_CALL
     if _LIBRARY is not None:
         return _LIBRARY
     path = library_path()
@@ -129,6 +132,7 @@ def load_library() -> ctypes.CDLL:
         by_address.argtypes = [ctypes.c_void_p, ctypes.c_ulonglong]
         by_address.restype = ctypes.c_int
         _ADDRESS_CALLS[name] = by_address
+        _ENTRY_ADDRESSES[name] = ctypes.cast(fn, ctypes.c_void_p).value
     lib.kg_gfx950_set_launch_mode.argtypes = [ctypes.c_int, ctypes.c_void_p]
     lib.kg_gfx950_set_launch_mode.restype = ctypes.c_int
     lib.kg_gfx950_last_error.argtypes = []
@@ -138,6 +142,12 @@ def load_library() -> ctypes.CDLL:
     lib.kg_gfx950_cost.argtypes = [ctypes.c_int, ctypes.POINTER(KgArgSlot), ctypes.c_ulonglong,
                                    ctypes.POINTER(ctypes.c_longlong)]
     lib.kg_gfx950_cost.restype = ctypes.c_int
+    try:
+        from kernelcode_generate_amd import _kg_call
+
+        _FAST_CALL = _kg_call.call
+    except ImportError:  # (built against another torch, or without one: the slots are packed here)
+        _FAST_CALL = None
     _LIBRARY = lib
     return lib
 
@@ -297,24 +307,34 @@ def marshal_slots(args: Sequence[Any]) -> tuple[ctypes.Array, list[Any]]:
 def call_entry(entry_point: str, args: Sequence[Any], *, check: bool = True) -> int:
     """Invoke one gfx950 entry point with reference-ordered args; raise on non-zero if check."""
 
-    lib = load_library()
+    lib = _LIBRARY or load_library()
+    status = None
+    if _FAST_CALL is not None and type(args) is tuple:
+        address = _ENTRY_ADDRESSES.get(entry_point)
+        if address is not None:
+            status = _FAST_CALL(address, args)
+    if status is None:
+        status = _packed_call(lib, entry_point, args)
+    if check and status != 0:
+        detail = lib.kg_gfx950_last_error().decode("utf-8", "replace")
+        raise NativeLibraryError(f"{entry_point} returned {status}: {detail}", status)
+    return status
+
+
+def _packed_call(lib: ctypes.CDLL, entry_point: str, args: Sequence[Any]) -> int:
     fn = _ADDRESS_CALLS.get(entry_point)
     own = _take_words()
     try:
         words = _slot_words(args, own[1])
         if fn is not None and len(words) <= _CALL_WORDS:
             _put_words(words, own[0])
-            status = fn(own[1], len(args))
-        else:
-            slots, keepalive = marshal_slots(args)
-            status = int(getattr(lib, entry_point)(slots, ctypes.c_ulonglong(len(args))))
-            del keepalive
+            return fn(own[1], len(args))
+        slots, keepalive = marshal_slots(args)
+        status = int(getattr(lib, entry_point)(slots, ctypes.c_ulonglong(len(args))))
+        del keepalive
+        return status
     finally:
         _FREE_WORDS.append(own)
-    if check and status != 0:
-        detail = lib.kg_gfx950_last_error().decode("utf-8", "replace")
-        raise NativeLibraryError(f"{entry_point} returned {status}: {detail}", status)
-    return status
 
 
 def cost(family: str, args: Sequence[Any]) -> dict[str, int]:
