@@ -85,16 +85,13 @@ __device__ __forceinline__ void assign_row(const PagesArgs& a, int t, int rows, 
     if (at < 0x7fffffffu) {
       const int p = div_page(position, a.div), offset = position - p * a.page_size;
       if (p < a.per) {
-        const int held = pages_of(c, a);
-        int page;
+        const int held = pages_of(c, a), i = fresh_of[b] + p - held;
         int* entry = a.table + b * a.table_0 + p * a.table_1;
-        if (p < held) {
-          page = *entry;
-        } else {
-          const int i = fresh_of[b] + p - held;
-          page = i < count ? a.free[(count - 1 - i) * a.free_stride] : -1;
-          if (offset == 0) *entry = page;  // (each new page's first token is one of the call's)
-        }
+        int old_page = -1, new_page = -1;  // (both reads on their way before either is used)
+        if (p < held) old_page = *entry;
+        if (p >= held && i < count) new_page = a.free[(count - 1 - i) * a.free_stride];
+        const int page = p < held ? old_page : new_page;
+        if (p >= held && offset == 0) *entry = page;  // (each new page's first token is one of the call's)
         if (page >= 0) slot = (long long)page * a.page_size + offset;
       }
     }
