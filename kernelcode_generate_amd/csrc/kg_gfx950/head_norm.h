@@ -6,7 +6,8 @@
 //
 // head_norm_kernel: L lanes per head, each with the W elements on both sides of its pairs (2 W side by side of neighbours), so that a
 // pair never leaves its lane, and G heads of a token at a time, whose reads are in flight together and whose angles and weights are read
-// once; half a multiple of W, D of 2 W, rows that start anywhere. Bound by its bytes where there are many.
+// once; half a multiple of W, an even D of 2 W, rows that start anywhere. Bound by its bytes where there are many: 8192 tokens of 32 and 8
+// heads of 128 in bf16 34.2 us, 4.7 TB/s, in fp32 62, 5.1 TB/s; 64 tokens take 3.3, a launch's 2.3 and one chain of reads.
 // head_norm_any_kernel: any D up to 512, half, strides and alignment: a wave per token and head, each lane some pairs of elements.
 #pragma once
 
@@ -94,32 +95,41 @@ __global__ __launch_bounds__(256) void head_norm_any_kernel(HeadNormArgs a) {
 // W elements from any address, in 32 bits, and back.
 template <typename T, int W>
 struct Elements {
-  static constexpr int kDwords = W * sizeof(T) / 4;
+  static constexpr bool kOne = W * sizeof(T) < 4;  // one element of 16 bits
+  static constexpr int kDwords = kOne ? 1 : W * sizeof(T) / 4;
   struct __attribute__((packed, aligned(sizeof(T)))) Piece {
     uint32_t w[kDwords];
   };
   static __device__ __forceinline__ void load(const T* p, float (&x)[W]) {
-    const Piece q = *reinterpret_cast<const Piece*>(p);
+    if constexpr (kOne) {
+      x[0] = Elem<T>::load(p);
+    } else {
+      const Piece q = *reinterpret_cast<const Piece*>(p);
 #pragma unroll
-    for (int i = 0; i < kDwords; ++i) {
-      const uint32_t u = q.w[i];
-      if constexpr (sizeof(T) == 4) {
-        x[i] = __builtin_bit_cast(float, u);
-      } else {
-        using H = Half16<typename Eight<T>::Tag>;
-        x[2 * i] = H::to_float(u & 0xffffu);
-        x[2 * i + 1] = H::to_float(u >> 16);
+      for (int i = 0; i < kDwords; ++i) {
+        const uint32_t u = q.w[i];
+        if constexpr (sizeof(T) == 4) {
+          x[i] = __builtin_bit_cast(float, u);
+        } else {
+          using H = Half16<typename Eight<T>::Tag>;
+          x[2 * i] = H::to_float(u & 0xffffu);
+          x[2 * i + 1] = H::to_float(u >> 16);
+        }
       }
     }
   }
   static __device__ __forceinline__ void store(T* p, const float (&x)[W]) {
-    Piece q;
+    if constexpr (kOne) {
+      Elem<T>::store(p, x[0]);
+    } else {
+      Piece q;
 #pragma unroll
-    for (int i = 0; i < kDwords; ++i) {
-      if constexpr (sizeof(T) == 4) q.w[i] = __builtin_bit_cast(uint32_t, x[i]);
-      else q.w[i] = Half16<typename Eight<T>::Tag>::pack2(x[2 * i], x[2 * i + 1]);
+      for (int i = 0; i < kDwords; ++i) {
+        if constexpr (sizeof(T) == 4) q.w[i] = __builtin_bit_cast(uint32_t, x[i]);
+        else q.w[i] = Half16<typename Eight<T>::Tag>::pack2(x[2 * i], x[2 * i + 1]);
+      }
+      *reinterpret_cast<Piece*>(p) = q;
     }
-    *reinterpret_cast<Piece*>(p) = q;
   }
 };
 
@@ -187,7 +197,7 @@ __global__ __launch_bounds__(256) void head_norm_kernel(HeadNormArgs a, HeadNorm
 #pragma unroll
         for (int i = 0; i < W; ++i) {  // pair i: elements 2 i and 2 i + 1 of both pieces in a row
           float& e = 2 * i < W ? p[g][2 * i % W] : q[g][2 * i % W];
-          float& f = 2 * i < W ? p[g][(2 * i + 1) % W] : q[g][(2 * i + 1) % W];
+          float& f = 2 * i + 1 < W ? p[g][(2 * i + 1) % W] : q[g][(2 * i + 1) % W];
           const float r = e * cs[i] - f * sn[i];
           f = f * cs[i] + e * sn[i];
           e = r;
@@ -243,16 +253,21 @@ bool launch_head_norm(const HeadNormArgs& a, int lanes, hipStream_t stream) {
   return true;
 }
 
-// False: no form of the kernel takes the call.
+// False: no form of the kernel takes the call. The widest pieces that the halves allow, and heads at a time that the measurements say, us
+// with 1 / 2 / 4: 8 elements, 1600 x 40 x 128 bf16 8.7 / 8.9 / 9.2, 8192 x 40 x 128 35.7 / 34.2 / 36.3; 4 elements, 4000 x 24 x 72 f16 18.9 / 14.1 / 12.5; 2,
+// 4000 x 24 x 80 of which 20 turn 16.2 / 12.5 / 11.2; 1, 4000 x 36 x 72 of which 18 turn 30.3 / 20.7 / 16.9 (the kernel of any head 68); few rows 3.3 with any.
 template <typename T>
 bool launch_head_norm(const HeadNormArgs& a, hipStream_t stream) {
-  const bool many = (long long)a.tokens * (a.side[0].heads + a.side[1].heads) * a.d >= 1 << 21;
+  const long long elements = (long long)a.tokens * (a.side[0].heads + a.side[1].heads) * a.d;
+  const bool many = elements >= 1 << 21;
   if (const int lanes = head_norm_lanes(a, 8))
-    return many ? launch_head_norm<T, 8, 4>(a, lanes, stream) : launch_head_norm<T, 8, 1>(a, lanes, stream);
+    return elements >= 1 << 24 ? launch_head_norm<T, 8, 2>(a, lanes, stream) : launch_head_norm<T, 8, 1>(a, lanes, stream);
   if (const int lanes = head_norm_lanes(a, 4))
     return many ? launch_head_norm<T, 4, 4>(a, lanes, stream) : launch_head_norm<T, 4, 1>(a, lanes, stream);
   if (const int lanes = head_norm_lanes(a, 2))
     return many ? launch_head_norm<T, 2, 4>(a, lanes, stream) : launch_head_norm<T, 2, 1>(a, lanes, stream);
+  if (const int lanes = head_norm_lanes(a, 1))
+    return many ? launch_head_norm<T, 1, 4>(a, lanes, stream) : launch_head_norm<T, 1, 1>(a, lanes, stream);
   return false;
 }
 

@@ -7,9 +7,11 @@
 // Pages that go back, of ceil(keep / page_size) .. ceil(held / page_size) - 1, are put on the stack the last one first, so that
 // giving back what a call took leaves the stack as it was.
 //
-// A call of some thousand tokens is a chain of a few dependent reads (lengths, a search for a row's request in LDS, its page), which more
-// workgroups do not shorten, and only one workgroup can take from the stack and write what is left of it without a second launch: up to
-// 2048 rows one workgroup does all. More rows are written by a second launch.
+// A call is a chain of a few dependent reads (lengths, a search for a row's request in LDS, its page), which more workgroups do not shorten,
+// and only one workgroup can take from the stack and write what is left of it without a second launch: up to 4096 rows one
+// workgroup does all, more are written by a second launch. us with one launch / two, 256 requests of a token each 4.6 / 5.9, 6 of 512
+// tokens 5.6 / 6.2, 8 of 512 6.3 / 6.3, 24 prompts in 16384 rows 18.7 / 6.7; a launch by itself takes 2.3. Pages of 256 requests given
+// back: 4.0.
 #pragma once
 
 #include "common.h"

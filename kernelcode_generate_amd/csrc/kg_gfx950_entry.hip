@@ -1882,7 +1882,7 @@ PagesArgs pages_args(const PagesSlots& p) {
 }
 
 // Rows that the workgroup of the sums writes too; more go to workgroups of a second launch (pages.h has both measured).
-constexpr long long kAssignFewTokens = 2048;
+constexpr long long kAssignFewTokens = 4096;
 
 int kv_cache_assign_impl(const KgArgSlot* args, unsigned long long n) {
   if (args == nullptr) return fail(kInvalid, "ordered_args is null");

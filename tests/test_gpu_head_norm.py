@@ -52,6 +52,15 @@ def test_heads(device, t, heads_q, heads, d, half, dtype, neighbours):
     check(device, t, heads_q, heads, d, half, dtype, neighbours, ("none", "same", "f32", "mixed", "keys")[(t + d + half) % 5])
 
 
+@pytest.mark.parametrize("t, heads_q, heads, d, half", [(1300, 12, 12, 72, 36), (1300, 11, 13, 72, 9), (1500, 10, 9, 80, 10), (1250, 7, 7, 128, 64),
+                                                        (3400, 33, 7, 128, 64), (900, 65, 9, 256, 128)])
+@pytest.mark.parametrize("neighbours", [False, True])
+def test_many_heads(device, t, heads_q, heads, d, half, neighbours):
+    """Several heads at a time, their number no multiple of that, and in place."""
+
+    check(device, t, heads_q, heads, d, half, torch.bfloat16, neighbours, "mixed", inside=bool(t % 500))
+
+
 @pytest.mark.parametrize("d, half", [(64, 32), (128, 64), (128, 32), (72, 18), (80, 40), (256, 128), (33, 7)])
 @pytest.mark.parametrize("neighbours", [False, True])
 @pytest.mark.parametrize("how", ["inside", "pad 8", "pad 1", "offset 1", "offset 4", "positions", "keys", "large", "small"])
