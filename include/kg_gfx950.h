@@ -21,7 +21,8 @@
  * and element strides. Kernels allocate nothing per call, with one exception: calls that need
  * memory between their launches (fp32 partial sums of a K split over workgroups, packed operands
  * of matmuls with unaligned rows, a conv's channel-last copy, partial outputs of split attention
- * keys, the low-rank sums of projections with adapters) take it from a workspace held per
+ * keys, the low-rank sums of projections with adapters, the codes of rows that int8_matmul quantises, the sums of
+ * kv_cache_assign past 4096 rows) take it from a workspace held per
  * (device, stream) for the life of the process (at most
  * 64 MiB, for 8 streams per device), allocated on the first such call on that stream and
  * reallocated when a later one needs more. While a stream records a HIP graph such calls take a
@@ -127,10 +128,11 @@ int kg_gfx950_flash_attention_entry(const KgArgSlot* ordered_args, unsigned long
 
 /*
  * Serving entries (no counterpart in the reference): a paged cache of keys and values written and read
- * back, attention of drafted tokens over it, and a projection with low-rank adapters beside it. Same slot
+ * back, attention of drafted tokens over it, a projection with low-rank adapters beside it; pages and slots of a step's
+ * tokens, rows and products in 8-bit integers, norms of queries and keys with the position rotation. Same slot
  * structure, return codes, launch modes and workspaces as the entries above. Memory must lie on the
  * current device; all but the last axis of a tensor may have any non-negative strides, and the last is contiguous
- * (page_table, lens, starts, slots, mask, index and scales: any). Values that lie in device memory (slots,
+ * (page_table, lens, starts, slots, positions, free_pages, mask, index, scales, biases, cos, sin and weights of norms: any). Values that lie in device memory (slots,
  * page tables, lengths, masks, adapter indexes) are not checked by the host: each entry says below what it makes of
  * values that are out of range. None of them reads or writes outside the tensors.
  *

@@ -1,12 +1,17 @@
 // gemm_i8_kernel: products in 8-bit integers (gemm_i8.h) in tiles, four waves of 2 x 2, each a (16 NA) x (16 NB) quarter in blocks of
 // v_mfma_i32_16x16x64_i8. Both operands lie along k, so both are copied to LDS and read back the same way: rows of kBK
-// bytes, fragments of 16 bytes (16 k) a lane, which is the form that the instruction takes from both sides. A 64-deep step of codes
-// has the bytes of a 32-deep step of bf16 at twice its operations, so the K loop is that of the 16-bit kernels: a ring of kStages
-// slices of kBK k filled by copies straight from memory to LDS, one barrier a slice, and a step's MFMAs from registers while the
-// next step's fragments are read and later slices' copies are issued between them.
+// bytes, fragments of 16 bytes (16 k) a lane, which is the form that the instruction takes from both sides. The K loop: a ring of kStages
+// slices of kBK k filled by copies straight from memory to LDS, one barrier a slice, and a step's MFMAs (64 k) from registers while the
+// next step's fragments are read and a later slice's copies are issued between them. The barrier before a slice's last step finds all its
+// fragments read: it publishes the next slice's copies and frees this slice's stage for its refill.
 //
-// The barrier before a slice's last step finds all its fragments read: it publishes the next slice's copies and
-// frees this slice's stage for its refill.
+// Slices of 128 k: a copy then takes whole 128-byte lines. With 64, each line passes from the L2 twice, and 256 x 256 tiles were bound by
+// that (8192^3 410 us with four slices of 64 in the ring, 378 with two of 128). What bounds them now, 8192^3 with codes of a normal
+// distribution: power. The products alone would take 262 us at the 4.2 POPS that the instruction reaches on registers, where the clock has
+// fallen to 2.0 GHz; here it is 1.9, with the matrix units busy in 69 % of all cycles (the form with slices of 64 took 419 us, 322 with the
+// copies left out, 374 with the reads of LDS left out, in as many cycles as with them). 2.74 to 2.9 POPS; the library's product 2.44. 4096^3 58 us, of which 11 are a launch, a ring to fill and the
+// results' way to memory. Small tiles are bound by a slice's chain of barrier, LDS reads and products (0.1 us for 32 x 32, 0.2 for 64 x 64), middle
+// ones by the L2 (20 TB/s).
 //
 // Copies are buffer loads that land zeros outside the matrices (as fast as plain ones), stores are made inside alone: any M and N. K is a
 // multiple of 16 (rows of others are copied into padded ones first).
@@ -35,7 +40,8 @@ __device__ __forceinline__ void mfma_order(i32x4 (&a)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+a"(a[i]));
 }
-// 16-byte chunk c of a row lies at c ^ swizzle(row): the fragments' reads hit distinct banks
+// 16-byte chunk c of a row lies at c ^ swizzle(row): the 16 rows of a fragment's read hit distinct banks (256 bytes a cycle; with the rows
+// of 64 bytes at c ^ row / 4 % 4 half of the LDS cycles were conflicts)
 template <int kBK>
 __device__ __forceinline__ int swizzle(int row) {
   if constexpr (kBK == 64) return (row >> 1) & 3;

@@ -3,7 +3,8 @@
 // of the row infinite or NaN).
 //
 // quantize_rows_kernel: a row's lanes hold it in registers, 8 elements a piece, from the one read that there is to the codes; rows of 8
-// up to 16384 elements, starting anywhere. quantize_rows_any_kernel reads its rows twice, element by element.
+// up to 16384 elements, starting anywhere. A wave a row up to 512 elements, four beyond: 4001 rows of 4096 in fp16 9.2 us, 5.3 TB/s, bound by
+// their bytes; 16 rows 2.4, a launch's. quantize_rows_any_kernel reads its rows twice, element by element.
 #pragma once
 
 #include <type_traits>
