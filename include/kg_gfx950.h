@@ -197,7 +197,9 @@ int kg_gfx950_adapter_matmul_entry(const KgArgSlot* ordered_args, unsigned long 
  * last one on top, in the order of requests and positions, and entered in page_table; -1 where none is left, and such
  * tokens, as those behind P pages, get slot -1. *free_count is then what is left (values outside 0 .. F count as the nearest).
  * B <= 8192, B * P and T at most 2^31 - 4096. page_table, starts, slots and positions are what kv_cache_store, head_norm_rotate and tree_attention take.
- * No two of the tensors may overlap. The call reads what it writes: a recorded graph takes new pages on every replay.
+ * No two of the tensors may overlap. The call reads what it writes: a recorded graph takes new pages on every replay, and a call
+ * that is repeated for the same tokens, after a shortage say, takes other pages: give the first ones back before (kv_cache_release
+ * with keep_lens = context_lens).
  */
 int kg_gfx950_kv_cache_assign_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);
 

@@ -9,8 +9,8 @@
 //
 // A call is a chain of a few dependent reads (lengths, a search for a row's request in LDS, its page), which more workgroups do not shorten,
 // and only one workgroup can take from the stack and write what is left of it without a second launch: up to 4096 rows one
-// workgroup does all, more are written by a second launch. us with one launch / two, 256 requests of a token each 4.6 / 5.9, 6 of 512
-// tokens 5.6 / 6.2, 8 of 512 6.3 / 6.3, 24 prompts in 16384 rows 18.7 / 6.7; a launch by itself takes 2.3. Pages of 256 requests given
+// workgroup does all, more are written by a second launch. us with one launch / two, 256 requests of a token each 4.6 / 5.9, 6 requests
+// in 3000 rows 5.6 / 6.2, 8 in 4096 6.3 / 6.3, 24 prompts in 16384 rows 18.7 / 6.7; a launch by itself takes 2.3. Pages of 256 requests given
 // back: 4.0.
 #pragma once
 

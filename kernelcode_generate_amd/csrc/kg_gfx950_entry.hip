@@ -1983,10 +1983,10 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
   const bool take_w = !(whole && w_aligned && a.w_row <= kMaxPipeLd);
   // pieces of channels and rows that the workspace holds (a row: at most 128 KiB), of fewer tiles than a launch has workgroups
   long long channels = std::min<long long>(a.n, 1 << 22);
-  if (take_w) channels = std::min(channels, std::max(256ll, (kSplitMaxWorkspace >> 1) / pitch / 256 * 256));
+  if (take_w) channels = std::min(channels, std::max(128ll, ((kSplitMaxWorkspace >> 1) - 1024) / pitch / 128 * 128));
   const long long w_bytes = take_w ? channels * pitch : 0, row_bytes = take_x ? pitch + (codes ? 0 : (long long)sizeof(float)) : 0;
   long long rows = std::min<long long>(a.m, (kMostBlocks * 32 / cdiv(channels, 32)) / 256 * 256);
-  if (row_bytes > 0) rows = std::min(rows, std::max(256ll, (kSplitMaxWorkspace - w_bytes - 512) / row_bytes / 256 * 256));
+  if (row_bytes > 0) rows = std::min(rows, std::max(128ll, (kSplitMaxWorkspace - w_bytes - 512) / row_bytes / 128 * 128));
   if (g_cost != nullptr) {
     const long long k = whole ? a.k : pitch;
     long long mfma = 0;

@@ -184,3 +184,59 @@ def test_recorded_products(device, m, n, k):
             assert torch.equal(other, out)
     finally:
         native.set_launch_mode(True, None)
+
+
+def test_two_recorded_products_at_once(device):
+    """Graphs that each hold a workspace of their own, replayed on two streams beside eager calls on a third."""
+
+    gen = torch.Generator().manual_seed(5)
+    calls = []
+    for m, n, k in ((700, 1100, 1023), (300, 2048, 4096), (40, 520, 2000)):
+        weight, w_scale = torch.randint(-127, 128, (n, k), generator=gen, dtype=torch.int8).to(device), (torch.rand(n, generator=gen) * 0.01).to(device)
+        x = rows(m, k, torch.bfloat16, gen).to(device)
+        out, want = (torch.zeros(m, n, dtype=torch.bfloat16, device=device) for _ in range(2))
+        native.int8_matmul(want, x, None, weight, w_scale)
+        calls.append((out, x, weight, w_scale, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    graphs = []
+    try:
+        for out, x, weight, w_scale, _, stream in calls[:2]:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                native.set_launch_mode(False, stream.cuda_stream)
+                for _ in range(3):
+                    native.int8_matmul(out, x, None, weight, w_scale)
+            graphs.append(graph)
+        out, x, weight, w_scale, _, stream = calls[2]
+        native.set_launch_mode(False, stream.cuda_stream)
+        for _ in range(4):
+            for c in calls:
+                c[0].zero_()
+            torch.cuda.synchronize()
+            for graph, c in zip(graphs, calls):
+                with torch.cuda.stream(c[5]):
+                    graph.replay()
+            for _ in range(5):
+                native.int8_matmul(out, x, None, weight, w_scale)
+            torch.cuda.synchronize()
+            for c in calls:
+                assert torch.equal(c[0], c[4])
+    finally:
+        native.set_launch_mode(True, None)
+
+
+@pytest.mark.parametrize("m, n, k", [(5, 40, 64), (300, 264, 1024)])
+def test_shared_scales_and_biases(device, m, n, k):
+    """One scale for all rows or channels, as views without strides, and scales of any sign and size."""
+
+    gen = torch.Generator().manual_seed(m)
+    values = torch.randint(-127, 128, (m, k), generator=gen)
+    weight = torch.randint(-127, 128, (n, k), generator=gen, dtype=torch.int8)
+    one = torch.tensor([-0.003], device=device)
+    for x_scale, w_scale in ((one.expand(m), one.expand(n)), (torch.linspace(-1e20, 1e20, m, device=device), torch.full((n,), 1e-22, device=device)),
+                             (torch.full((m,), 1e-30, device=device), torch.linspace(-1e28, 1e28, n, device=device))):
+        out = torch.empty(m, n, device=device)
+        bias = torch.tensor([0.5], device=device).expand(n)
+        native.int8_matmul(out, values.to(torch.int8).to(device), x_scale, weight.to(device), w_scale, bias)
+        expected, allowed = int8_oracle(values.numpy(), x_scale.cpu().numpy(), weight, w_scale, bias, torch.float32)
+        assert_close(out, expected, allowed)
