@@ -301,3 +301,60 @@ def test_heads_past_32_bits(device):
     rows = torch.tensor([0, 1, 63549, 63550, 65536, t - 1], device=device)
     want = head_norm_oracle(q[rows].cpu(), weight, cos, sin, positions[rows], 1e-6, False, torch.zeros(len(rows), heads, d))
     assert_close(out[rows], *want)
+
+
+def test_recorded_without_a_workspace(device):
+    """Graphs that hold all the workspace that recordings may have: a call recorded then takes a form that needs none, with the same results."""
+
+    gen = torch.Generator(device=device).manual_seed(7)
+    big = torch.randn(16000, 4096, generator=gen, device=device).to(BF16)
+    w = torch.randint(-127, 128, (16, 4096), generator=gen, device=device, dtype=torch.int8)
+    stream, graphs = torch.cuda.Stream(), []
+    stream.wait_stream(torch.cuda.current_stream())
+
+    def recorded(call):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            native.set_launch_mode(False, stream.cuda_stream)
+            call()
+        native.set_launch_mode(True, None)
+        return graph
+
+    out = torch.empty(16000, 16, dtype=BF16, device=device)
+    try:
+        w_scale = torch.ones(16, device=device)
+        for m in (16000, 4000, 1000, 250, 60, 10, 2):  # until no piece of any size is left
+            for _ in range(17 if m == 16000 else 5):
+                graphs.append(recorded(lambda: native.int8_matmul(out[:m], big[:m], None, w, w_scale)))
+        # rows that the call quantises, codes whose rows are no whole pieces, pages of many rows
+        cases = []
+        for m, n, k, codes in ((130, 200, 272, False), (9, 70, 9000, False), (40, 100, 1023, True)):
+            x = torch.randn(m, k, generator=gen, device=device).to(BF16)
+            weight = torch.randint(-127, 128, (n, k), generator=gen, device=device, dtype=torch.int8)
+            w_scale = torch.rand(n, generator=gen, device=device) * 0.01
+            scale = None
+            values, row_scale = codes_oracle(x)
+            if codes:
+                x, scale = torch.from_numpy(values).to(torch.int8).to(device), torch.from_numpy(row_scale).to(device)
+            got = torch.zeros(m, n, dtype=BF16, device=device)
+            graph = recorded(lambda: native.int8_matmul(got, x, scale, weight, w_scale))
+            cases.append((graph, got, int8_oracle(values, row_scale, weight, w_scale, None, BF16), (x, scale, weight, w_scale)))  # (held for the replays)
+        slots, positions, starts = (torch.zeros(n, dtype=t, device=device) for n, t in ((5000, torch.int64), (5000, I32), (4, I32)))
+        table, free = torch.full((3, 200), -1, dtype=I32, device=device), torch.arange(400, dtype=I32, device=device)
+        count, context, new = (torch.tensor(x, dtype=I32, device=device) for x in ([400], [0, 0, 0], [1500, 2000, 700]))
+        pages = recorded(lambda: native.kv_cache_assign(slots, positions, starts, table, free, count, context, new, PAGE))
+        for _ in range(2):
+            for graph, got, want, _ in cases:
+                got.zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert_close(got, *want)
+            table.fill_(-1)
+            count.fill_(400)
+            pages.replay()
+            torch.cuda.synchronize()
+            want = assign_oracle([[-1] * 200] * 3, list(range(400)), 400, [0] * 3, [1500, 2000, 700], PAGE, 5000)
+            assert [t.tolist() for t in (slots, positions, starts, table)] == list(want[:4]) and count.item() == want[4]
+    finally:
+        native.set_launch_mode(True, None)
+    del graphs, cases, pages
