@@ -21,8 +21,8 @@
  * and element strides. Kernels allocate nothing per call, with one exception: calls that need
  * memory between their launches (fp32 partial sums of a K split over workgroups, packed operands
  * of matmuls with unaligned rows, a conv's channel-last copy, partial outputs of split attention
- * keys, the low-rank sums of projections with adapters, the codes of rows that int8_matmul quantises, the sums of
- * kv_cache_assign past 4096 rows) take it from a workspace held per
+ * keys, the low-rank sums of projections with adapters, the codes of rows that int8_matmul quantises and its sums of
+ * a split K, the sums of kv_cache_assign past 4096 rows) take it from a workspace held per
  * (device, stream) for the life of the process (at most
  * 64 MiB, for 8 streams per device), allocated on the first such call on that stream and
  * reallocated when a later one needs more. While a stream records a HIP graph such calls take a

@@ -27,9 +27,9 @@ struct Int8Args {
 };
 
 template <typename T>
-__device__ __forceinline__ float int8_bias(const Int8Args& a, int n) {
-  if (a.bias == nullptr) return 0.f;
-  return a.wide_bias ? static_cast<const float*>(a.bias)[n * a.bias_stride] : Elem<T>::load(static_cast<const T*>(a.bias) + n * a.bias_stride);
+__device__ __forceinline__ float int8_bias(const void* bias, long long stride, bool wide, long long n) {
+  if (bias == nullptr) return 0.f;
+  return wide ? static_cast<const float*>(bias)[n * stride] : Elem<T>::load(static_cast<const T*>(bias) + n * stride);
 }
 
 // X: int8_t (codes) or T
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
       for (int o = 32; o > 0; o >>= 1) acc[i] += __shfl_xor(acc[i], o, 64);
       const int n = n0 + i;
       if (lane == 0 && n < a.n)
-        Elem<T>::store(static_cast<T*>(a.out) + m * a.out_row + n, (float)acc[i] * scale * a.w_scale[n * a.w_scale_stride] + int8_bias<T>(a, n));
+        Elem<T>::store(static_cast<T*>(a.out) + m * a.out_row + n, (float)acc[i] * scale * a.w_scale[n * a.w_scale_stride] + int8_bias<T>(a.bias, a.bias_stride, a.wide_bias, n));
     }
   }
 }

@@ -56,27 +56,65 @@ struct Int8Form {
 constexpr Int8Form kInt8Forms[7] = {{256, 256, 2, 7800, 7600, 1140, 46}, {256, 128, 3, 5500, 4000, 610, 37}, {128, 128, 4, 3900, 1800, 420, 46},
                                     {128, 64, 3, 3350, 220, 290, 15},    {64, 64, 4, 3200, 200, 220, 7},      {32, 64, 4, 3300, 80, 158, 4},
                                     {32, 32, 8, 2800, 140, 98, 6}};
-inline int int8_form(long long m, long long n, long long k) {
-  int best = 0;
+// A product's form and the chunk of k that a workgroup takes. Chunks (two, four or eight, of the three smallest tiles) are for few tiles of
+// a long K: a CU takes some 80 GB/s into its LDS, whatever its tile, and has a slice no sooner. Their sums go through the
+// workspace, and a second launch joins them: 2700 ns and the sums' way there and back. us without / with: 16 x 500 x 16384 17.6 / 8.8, 16 x 1024 x
+// 11008 12.7 / 8.9, 200 x 500 x 16384 18.3 / 12.3; 16 x 4096 x 11008, which the memory bounds, is not split.
+struct Int8Plan {
+  int form, chunk, chunks;
+  long long ld, bytes;  // of the sums: a row's (in elements), all
+};
+constexpr long long kInt8MostSums = 16ll << 20;
+inline Int8Plan int8_plan(long long m, long long n, long long k, bool may_split) {
+  Int8Plan best{};
   long long least = 0;
-  for (int i = 0; i < 7; ++i) {
-    const Int8Form& f = kInt8Forms[i];
-    const long long tiles = ((m + f.rows - 1) / f.rows) * ((n + f.channels - 1) / f.channels), rounds = (tiles + 255) / 256;
-    const long long slices = (k + 127) / 128 < f.stages ? f.stages : (k + 127) / 128;
-    const long long ns = f.fixed + (rounds - 1) * f.round + rounds * slices * f.slice * (25600 + f.load * (tiles < 256 ? tiles : 256)) / 25600;
-    if (i == 0 || ns < least) best = i, least = ns;
+  const long long floor = 2000 + (m + n) * k / 4400;  // operands from memory
+  for (int split = 1; split <= (may_split ? 8 : 1); split *= 2) {
+    const long long chunk = split == 1 ? k : (k / split + 127) / 128 * 128, chunks = (k + chunk - 1) / chunk, ld = (n + 3) / 4 * 4;
+    const long long bytes = split == 1 ? 0 : chunks * m * ld * 4;
+    if (split > 1 && (chunks < 2 || bytes > kInt8MostSums || chunk < 1024)) break;
+    for (int i = split == 1 ? 0 : 4; i < 7; ++i) {
+      const Int8Form& f = kInt8Forms[i];
+      const long long tiles = ((m + f.rows - 1) / f.rows) * ((n + f.channels - 1) / f.channels) * chunks, rounds = (tiles + 255) / 256;
+      const long long slices = (chunk + 127) / 128 < f.stages ? f.stages : (chunk + 127) / 128;
+      long long ns = f.fixed + (rounds - 1) * f.round + rounds * slices * f.slice * (25600 + f.load * (tiles < 256 ? tiles : 256)) / 25600;
+      ns = ns > floor ? ns : floor;
+      if (split > 1) ns += 2700 + bytes / 2000;
+      if (least == 0 || ns < least) {
+        least = ns;
+        best = Int8Plan{i, (int)chunk, (int)chunks, ld, bytes};
+      }
+    }
   }
   return best;
 }
 // MFMA instructions of a product (cost queries).
-inline long long int8_tiles_mfma(long long m, long long n, long long k) {
-  const Int8Form& f = kInt8Forms[int8_form(m, n, k)];
-  const long long tiles = ((m + f.rows - 1) / f.rows) * ((n + f.channels - 1) / f.channels), slices = (k + 127) / 128;
-  return tiles * (f.rows / 16) * (f.channels / 16) * 2 * (slices < f.stages ? f.stages : slices);
+inline long long int8_tiles_mfma(long long m, long long n, long long k, const Int8Plan& p) {
+  const Int8Form& f = kInt8Forms[p.form];
+  const long long tiles = ((m + f.rows - 1) / f.rows) * ((n + f.channels - 1) / f.channels);
+  long long slices = 0;
+  for (int c = 0; c < p.chunks; ++c) {
+    const long long own = (k - (long long)c * p.chunk < p.chunk ? k - (long long)c * p.chunk : p.chunk);
+    slices += (own + 127) / 128 < f.stages ? f.stages : (own + 127) / 128;
+  }
+  return tiles * (f.rows / 16) * (f.channels / 16) * 2 * slices;
 }
+hipError_t launch_int8_chunks(const Int8Tiles& g, int form, hipStream_t stream);
+// partial: the workspace of a plan of several chunks
 template <typename T>
-hipError_t launch_int8_tiles(const Int8Tiles& g, int form, hipStream_t stream) {
-  switch (form) {
+hipError_t launch_int8_tiles(const Int8Tiles& g, const Int8Plan& p, int* partial, hipStream_t stream) {
+  if (p.chunks > 1) {
+    Int8Tiles sums = g;
+    sums.out = partial;
+    sums.ldo = p.ld;
+    sums.chunk = p.chunk;
+    const hipError_t err = launch_int8_chunks(sums, p.form, stream);
+    if (err != hipSuccess) return err;
+    const unsigned grid = (unsigned)((g.m * (p.ld / 4) + 255) / 256);
+    hipLaunchKernelGGL((int8_join_kernel<T>), dim3(grid), dim3(256), 0, stream, g, partial, p.chunks, (int)p.ld);
+    return hipGetLastError();
+  }
+  switch (p.form) {
     case 0: return launch_gemm_i8<T, 8, 8, 128, 2>(g, stream);
     case 1: return launch_gemm_i8<T, 8, 4, 128, 3>(g, stream);
     case 2: return launch_gemm_i8<T, 4, 4, 128, 4>(g, stream);

@@ -65,8 +65,10 @@ struct Int8Tiles {
   long long ldx, ldw, ldo, x_scale_stride, w_scale_stride, bias_stride;
   int m, n, k;
   bool wide_bias;
+  int chunk;  // of k, a workgroup's (blockIdx.y)
 };
 
+// T int: the sums as they are, of one chunk of k: out is [chunks][m][ldo].
 template <typename T, int NA, int NB, int kBK, int kStages>
 __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8_kernel(Int8Tiles g) {
   using namespace gemmi;
@@ -95,8 +97,10 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   const int gm = min(tiles_m - first_m, kGroupM), in_group = logical - group * kGroupM * tiles_n;
   const int m0 = (first_m + in_group % gm) * TM, n0 = (in_group / gm) * TN;
 
+  constexpr bool kPartial = std::is_same<T, int>::value;
+  const int k0 = kPartial ? blockIdx.y * g.chunk : 0, k_own = kPartial ? min(g.k - k0, g.chunk) : g.k;
   // slices of K; in the one-step form a multiple of two (registers go by a slice's parity), and at least a ring of them: zeros behind K
-  const int slices = (g.k + kBK - 1) / kBK;
+  const int slices = (k_own + kBK - 1) / kBK;
   const int count = max(kSteps == 1 ? (slices + 1) / 2 * 2 : slices, kStages);
 
   // ---- memory -> LDS: piece p of a wave is rows (wave AP + p) kRowsPiece + lane / (kBK / 16) ----
@@ -117,8 +121,8 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   }
 #pragma unroll
   for (int x = 0; x < 2; ++x) chunk_k[x] = 16 * ((lane % kChunks) ^ swizzle<kBK>(x * kRowsPiece + lane / kChunks));
-  const char* a_tile = reinterpret_cast<const char*>(g.x) + (long long)m0 * g.ldx;
-  const char* b_tile = reinterpret_cast<const char*>(g.w) + (long long)n0 * g.ldw;
+  const char* a_tile = reinterpret_cast<const char*>(g.x) + (long long)m0 * g.ldx + k0;
+  const char* b_tile = reinterpret_cast<const char*>(g.w) + (long long)n0 * g.ldw + k0;
   const uint32_t lds0 = lds_addr(lds);
   auto issue_piece = [&](int kt, int stage, int piece) __attribute__((always_inline)) {
     const bool a = piece < AP;
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
     const uint32_t dst = lds0 + stage * kStage + (a ? (wave * AP + p) * 1024 : kStageA + (wave * BP + p) * 1024);
     const uint32_t off = a ? a_off[a ? p : 0] : b_off[a ? 0 : p];
     const int k = chunk_k[kBK == 64 ? 0 : ((a ? wave * AP : wave * BP) + p) & 1];
-    buf2lds16_s(kt * kBK + k < g.k ? off : kBufOOB, src, dst);
+    buf2lds16_s(kt * kBK + k < k_own ? off : kBufOOB, src, dst);
   };
 
   // ---- fragments of step ks: rows 16 i + lane % 16 of the wave's half, chunk 4 ks + lane / 16 ----
@@ -157,12 +161,13 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
 
   // scales and bias of the tile: read ahead of the K loop, into LDS behind it
   float xs_own = 0.f, ws_own = 0.f, bias_own = 0.f;
-  if (tid < TM) xs_own = g.x_scale[(long long)min(m0 + tid, g.m - 1) * g.x_scale_stride];
-  if (tid < TN) {
-    const long long at = min(n0 + tid, g.n - 1);
-    ws_own = g.w_scale[at * g.w_scale_stride];
-    if (g.bias != nullptr)
-      bias_own = g.wide_bias ? static_cast<const float*>(g.bias)[at * g.bias_stride] : Elem<T>::load(static_cast<const T*>(g.bias) + at * g.bias_stride);
+  if constexpr (!kPartial) {
+    if (tid < TM) xs_own = g.x_scale[(long long)min(m0 + tid, g.m - 1) * g.x_scale_stride];
+    if (tid < TN) {
+      const long long at = min(n0 + tid, g.n - 1);
+      ws_own = g.w_scale[at * g.w_scale_stride];
+      bias_own = int8_bias<T>(g.bias, g.bias_stride, g.wide_bias, at);
+    }
   }
 
   i32x4 acc[NA][NB];
@@ -269,7 +274,10 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
       for (int i = i0; i < i0 + P; ++i) {
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)acc[i][j][e] * xs[i], ws[e], bv[e]);
+        for (int e = 0; e < 4; ++e) {
+          const int sum = acc[i][j][e];
+          v[e] = kPartial ? __builtin_bit_cast(float, sum) : __builtin_fmaf((float)sum * xs[i], ws[e], bv[e]);
+        }
         const int r = 16 * (i - i0) + l16;
         if constexpr (sizeof(T) == 4) {
           const uint32_t at = region + r * kRow + (((4 * j + lg) ^ row_swizzle(r)) * 16);
@@ -290,7 +298,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
       const u32x4 v = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(region + r * kRow + ((c ^ row_swizzle(r)) * 16));
       const int m = mw + 16 * i0 + r, n = nw + kEach * c;
       if (m >= g.m || n >= g.n) continue;
-      T* to = static_cast<T*>(g.out) + (long long)m * g.ldo + n;
+      T* to = static_cast<T*>(g.out) + ((kPartial ? (long long)blockIdx.y * g.m : 0ll) + m) * g.ldo + n;
       if (n + kEach <= g.n) {
         store_bytes(to, v);
       } else {
@@ -309,8 +317,29 @@ template <typename T, int NA, int NB, int kBK, int kStages>
 hipError_t launch_gemm_i8(const Int8Tiles& g, hipStream_t stream) {
   constexpr int TM = 32 * NA, TN = 32 * NB;
   const unsigned grid = (unsigned)(((long long)g.m + TM - 1) / TM * (((long long)g.n + TN - 1) / TN));
-  hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages>), dim3(grid), dim3(gemmi::kThreads), 0, stream, g);
+  const unsigned chunks = std::is_same<T, int>::value ? (unsigned)((g.k + g.chunk - 1) / g.chunk) : 1u;
+  hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages>), dim3(grid, chunks), dim3(gemmi::kThreads), 0, stream, g);
   return hipGetLastError();
+}
+
+// The chunks' sums joined: whole numbers, so the bits are those of one chunk. partial: [chunks][m][ld], ld a multiple of 4; four
+// channels a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void int8_join_kernel(Int8Tiles g, const int* partial, int chunks, int ld) {
+  const int at = blockIdx.x * 256 + threadIdx.x, quads = ld / 4;
+  const int m = at / quads, n = 4 * (at - m * quads);
+  if (m >= g.m) return;
+  i32x4 sum = {0, 0, 0, 0};
+  const int* from = partial + (long long)m * ld + n;
+#pragma unroll 4
+  for (int c = 0; c < chunks; ++c) sum += *reinterpret_cast<const i32x4*>(from + (long long)c * g.m * ld);
+  const float xs = g.x_scale[m * g.x_scale_stride];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= g.n) continue;
+    const float bias = int8_bias<T>(g.bias, g.bias_stride, g.wide_bias, n + e);
+    Elem<T>::store(static_cast<T*>(g.out) + m * g.ldo + n + e, __builtin_fmaf((float)sum[e] * xs, g.w_scale[(n + e) * g.w_scale_stride], bias));
+  }
 }
 
 }  // namespace kg_gfx950

@@ -11,7 +11,7 @@
 
 namespace kg_gfx950 {
 
-#define KG_INT8_INSTANCE(T) KG_INSTANCE hipError_t launch_int8_tiles<T>(const Int8Tiles&, int, hipStream_t);
+#define KG_INT8_INSTANCE(T) KG_INSTANCE hipError_t launch_int8_tiles<T>(const Int8Tiles&, const Int8Plan&, int*, hipStream_t);
 #if !defined(KG_INSTANTIATE) || defined(KG_INSTANTIATE_INT8_F32)
 KG_INT8_INSTANCE(float)
 #endif

@@ -1986,23 +1986,29 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
   if (take_w) channels = std::min(channels, std::max(128ll, ((kSplitMaxWorkspace >> 1) - 1024) / pitch / 128 * 128));
   const long long w_bytes = take_w ? channels * pitch : 0, row_bytes = take_x ? pitch + (codes ? 0 : (long long)sizeof(float)) : 0;
   long long rows = std::min<long long>(a.m, (kMostBlocks * 32 / cdiv(channels, 32)) / 256 * 256);
-  if (row_bytes > 0) rows = std::min(rows, std::max(128ll, (kSplitMaxWorkspace - w_bytes - 512) / row_bytes / 128 * 128));
+  if (row_bytes > 0) rows = std::min(rows, std::max(128ll, (kSplitMaxWorkspace - w_bytes - 1024) / row_bytes / 128 * 128));
+  // K split over workgroups, where a product of one piece has few tiles
+  const long long k = whole ? a.k : pitch;
+  const bool one = rows == a.m && channels == a.n;
+  Int8Plan plan = int8_plan(rows, channels, k, one && w_bytes + rows * row_bytes + kInt8MostSums + 1024 <= kSplitMaxWorkspace);
   if (g_cost != nullptr) {
-    const long long k = whole ? a.k : pitch;
     long long mfma = 0;
     for (long long n0 = 0; n0 < a.n; n0 += channels)
       for (long long m0 = 0; m0 < a.m; m0 += rows) {
         const long long m = std::min(rows, a.m - m0), n = std::min(channels, a.n - n0);
-        mfma += int8_tiles_mfma(m, n, k);
+        mfma += int8_tiles_mfma(m, n, k, one ? plan : int8_plan(m, n, k, false));
       }
-    const long long copies = (take_x ? (long long)a.m * pitch : 0) + (take_w ? (long long)a.n * pitch : 0);
+    const long long copies = (take_x ? (long long)a.m * pitch : 0) + (take_w ? (long long)a.n * pitch : 0) + plan.bytes;
     return record_cost((long long)a.m * a.n * a.k, mfma, 16, copies, copies);
   }
   SplitLease lease;  // held until the kernels are enqueued
   char* ws = nullptr;
-  if (take_x || take_w) {
-    lease = split_workspace((size_t)(w_bytes + rows * row_bytes + 512), g_stream);
-    if ((ws = static_cast<char*>(lease.ptr)) == nullptr) return kUnsupported;
+  const long long copy_bytes = cdiv(w_bytes + rows * row_bytes + 256, 256) * 256;
+  if (take_x || take_w || plan.chunks > 1) {
+    lease = split_workspace((size_t)(copy_bytes + plan.bytes), g_stream);
+    ws = static_cast<char*>(lease.ptr);
+    if (ws == nullptr && (take_x || take_w)) return kUnsupported;
+    if (ws == nullptr) plan = int8_plan(rows, channels, k, false);
   }
   const long long bias_bytes = (a.wide_bias ? 4 : (long long)sizeof(T)) * a.bias_stride;
   for (long long n0 = 0; n0 < a.n; n0 += channels) {
@@ -2014,7 +2020,7 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
       Int8Tiles g{static_cast<const int8_t*>(a.x), take_w ? pack_w.dst : w, a.x_scale, a.w_scale + n0 * a.w_scale_stride,
                   a.bias == nullptr ? nullptr : static_cast<const char*>(a.bias) + n0 * bias_bytes, static_cast<T*>(a.out) + m0 * a.out_row + n0,
                   a.x_row, take_w ? pitch : a.w_row, a.out_row, a.x_scale_stride, a.w_scale_stride, a.bias_stride,
-                  (int)std::min(rows, a.m - m0), count, a.k, a.wide_bias};
+                  (int)std::min(rows, a.m - m0), count, (int)k, a.wide_bias, 0};  // (k: zeros behind the ends of copied rows)
       int8_t* x_ws = reinterpret_cast<int8_t*>(ws + w_bytes);
       hipError_t err = hipSuccess;
       if (codes) {
@@ -2032,8 +2038,8 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
       }
       pack_w.rows = 0;  // (packed with the first piece of rows)
       if (take_x) g.x = x_ws, g.ldx = pitch;
-      if (!whole) g.k = (int)pitch;  // (both are copies, zeros behind the rows' ends)
-      if (err == hipSuccess) err = launch_int8_tiles<T>(g, int8_form(g.m, g.n, g.k), g_stream);
+      if (err == hipSuccess)
+        err = launch_int8_tiles<T>(g, one ? plan : int8_plan(g.m, g.n, k, false), reinterpret_cast<int*>(ws + copy_bytes), g_stream);
       if (const int rc = launched(err, "int8_matmul")) return rc;
     }
   }

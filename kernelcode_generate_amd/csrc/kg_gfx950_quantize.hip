@@ -3,3 +3,13 @@
 #define KG_INSTANTIATE
 #define KG_INSTANTIATE_QUANTIZE
 #include "kg_gfx950/instances_int8.h"
+
+namespace kg_gfx950 {
+
+hipError_t launch_int8_chunks(const Int8Tiles& g, int form, hipStream_t stream) {
+  if (form == 4) return launch_gemm_i8<int, 2, 2, 128, 4>(g, stream);
+  if (form == 5) return launch_gemm_i8<int, 1, 2, 128, 4>(g, stream);
+  return launch_gemm_i8<int, 1, 1, 128, 8>(g, stream);
+}
+
+}  // namespace kg_gfx950

@@ -100,7 +100,8 @@ SIZES = [(1, 1, 1), (1, 64, 64), (3, 5, 7), (1, 4096, 512), (2, 100, 1000), (8, 
          (128, 128, 128), (129, 257, 1024), (200, 768, 2048), (256, 256, 256), (257, 513, 272), (300, 1024, 1000), (512, 512, 1024),
          (700, 300, 80), (1000, 1501, 1023), (1024, 2048, 512), (515, 264, 4112), (2048, 8, 64), (40, 16384, 64), (1, 8, 131071),
          (4096, 4096, 256), (3900, 4000, 400), (2048, 4096, 512), (1900, 4100, 272), (1024, 4096, 1024), (130, 4096, 2048), (16, 4096, 4096),
-         (33, 1030, 4096), (16, 512, 4095), (32, 300, 2047)]
+         (33, 1030, 4096), (16, 512, 4095), (32, 300, 2047),
+         (16, 1000, 11008), (1, 4096, 11008), (100, 301, 8191), (60, 130, 16384), (33, 1030, 6000)]
 
 
 @pytest.mark.parametrize("m, n, k", SIZES)
@@ -159,7 +160,7 @@ def test_nothing(device):
     assert (scale == 0).all()
 
 
-@pytest.mark.parametrize("m, n, k", [(4, 64, 256), (150, 100, 130), (300, 512, 1024)])
+@pytest.mark.parametrize("m, n, k", [(4, 64, 256), (150, 100, 130), (300, 512, 1024), (20, 300, 8192)])
 def test_recorded_products(device, m, n, k):
     """Replays read the rows as they are then, beside other calls on the stream's workspace."""
 
