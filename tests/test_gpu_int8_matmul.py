@@ -127,8 +127,14 @@ def test_the_largest_sums(device, m):
     check_product(m, 64, 131056, torch.float32, device, True, None, top=True)
 
 
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("pads, offsets", [((16, 32, 8), (16, 48, 8)), ((3, 5, 1), (0, 0, 0)), ((0, 0, 3), (0, 0, 1)), ((0, 7, 0), (1, 3, 1))])
+def test_strides_of_a_long_k(device, codes, pads, offsets):
+    check_product(20, 101, 8192, torch.bfloat16, device, codes, "f32", pads=pads, offsets=offsets)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m, n, k", [(3, 40, 128), (40, 40, 128), (200, 136, 256)])
+@pytest.mark.parametrize("m, n, k", [(3, 40, 128), (40, 40, 128), (200, 136, 256), (20, 130, 8192)])
 def test_rows_that_are_not_finite(device, dtype, m, n, k):
     """An infinity or NaN makes its own row's results NaN, and no other row's."""
 
@@ -187,12 +193,13 @@ def test_recorded_products(device, m, n, k):
         native.set_launch_mode(True, None)
 
 
-def test_two_recorded_products_at_once(device):
+@pytest.mark.parametrize("sizes", [((700, 1100, 1023), (300, 2048, 4096), (40, 520, 2000)), ((16, 500, 16384), (200, 500, 8192), (33, 512, 12000))])
+def test_two_recorded_products_at_once(device, sizes):
     """Graphs that each hold a workspace of their own, replayed on two streams beside eager calls on a third."""
 
     gen = torch.Generator().manual_seed(5)
     calls = []
-    for m, n, k in ((700, 1100, 1023), (300, 2048, 4096), (40, 520, 2000)):
+    for m, n, k in sizes:
         weight, w_scale = torch.randint(-127, 128, (n, k), generator=gen, dtype=torch.int8).to(device), (torch.rand(n, generator=gen) * 0.01).to(device)
         x = rows(m, k, torch.bfloat16, gen).to(device)
         out, want = (torch.zeros(m, n, dtype=torch.bfloat16, device=device) for _ in range(2))
@@ -226,7 +233,7 @@ def test_two_recorded_products_at_once(device):
         native.set_launch_mode(True, None)
 
 
-@pytest.mark.parametrize("m, n, k", [(5, 40, 64), (300, 264, 1024)])
+@pytest.mark.parametrize("m, n, k", [(5, 40, 64), (300, 264, 1024), (20, 100, 8192)])
 def test_shared_scales_and_biases(device, m, n, k):
     """One scale for all rows or channels, as views without strides, and scales of any sign and size."""
 

@@ -326,9 +326,9 @@ def test_recorded_without_a_workspace(device):
         for m in (16000, 4000, 1000, 250, 60, 10, 2):  # until no piece of any size is left
             for _ in range(17 if m == 16000 else 5):
                 graphs.append(recorded(lambda: native.int8_matmul(out[:m], big[:m], None, w, w_scale)))
-        # rows that the call quantises, codes whose rows are no whole pieces, pages of many rows
+        # rows that the call quantises, codes whose rows are no whole pieces, few tiles of a long K, pages of many rows
         cases = []
-        for m, n, k, codes in ((130, 200, 272, False), (9, 70, 9000, False), (40, 100, 1023, True)):
+        for m, n, k, codes in ((130, 200, 272, False), (9, 70, 9000, False), (40, 100, 1023, True), (16, 300, 8192, True)):
             x = torch.randn(m, k, generator=gen, device=device).to(BF16)
             weight = torch.randint(-127, 128, (n, k), generator=gen, device=device, dtype=torch.int8)
             w_scale = torch.rand(n, generator=gen, device=device) * 0.01

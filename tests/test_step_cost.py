@@ -37,6 +37,18 @@ def test_weights_of_no_whole_pieces():
     assert cost(16, 512, 8)["MFMA"] == 0  # the general kernel
 
 
+def test_few_tiles_of_a_long_k():
+    """The sums of the chunks of K, four bytes each, are written and read; the products are those of one chunk."""
+
+    c = cost(16, 500, 16384)
+    base = 16 * 500 * 2
+    chunks = (c["HBM_WRITE"] - base) / (16 * 500 * 4)
+    assert chunks in (2, 4, 8)
+    assert c["HBM_READ"] == (16 + 500) * 16384 + 4 * 500 + 4 * 16 + c["HBM_WRITE"] - base
+    assert c["MFMA"] % (16384 // 64) == 0 and c["MFMA"] * 16 * 16 * 64 >= c["MAC"]
+    assert cost(4096, 4096, 16384)["HBM_WRITE"] == 2 * 4096**2  # many tiles: none
+
+
 def test_refusals_are_the_entry_s():
     with pytest.raises(native.NativeLibraryError, match="sums may leave 32 bits"):
         cost(4, 4, 131072)
