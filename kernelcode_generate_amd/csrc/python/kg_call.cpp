@@ -54,7 +54,7 @@ bool fill(KgArgSlot* slot, PyObject* arg) {
     slot->rank = (unsigned long long)t.dim();
     slot->shape = t.dim() == 0 ? kScalar : reinterpret_cast<const long long*>(t.sizes().data());
     slot->stride = t.dim() == 0 ? kScalar : reinterpret_cast<const long long*>(t.strides().data());
-    slot->data = const_cast<void*>(t.const_data_ptr());
+    slot->data = t.mutable_data_ptr();  // (an entry may write it: a lazy copy is made here, as by data_ptr())
     return slot->dtype_code != 0;
   } else {
     return false;

@@ -48,6 +48,13 @@ def test_slots_are_marshal_slots_own():
     del keep
 
 
+def test_a_lazy_copy_is_made_before_an_entry_writes_it():
+    x = torch.ones(40)
+    y = torch._lazy_clone(x)  # shares x's memory until either is written
+    _, got = seen_by_an_entry((y,))
+    assert got[0][1] == y.data_ptr() != x.data_ptr()
+
+
 class Odd(torch.Tensor):
     pass
 
