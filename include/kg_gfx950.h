@@ -235,7 +235,8 @@ int kg_gfx950_int8_matmul_entry(const KgArgSlot* ordered_args, unsigned long lon
  * rotated alone), then pair i < R of y turns by the angle of cos and sin's row positions[t]: elements i and i + R (neighbours 0), or
  * 2 i and 2 i + 1 (neighbours 1); the elements behind 2 R <= D stay. A token with a position outside 0 .. S - 1 (-1, say) is left as it
  * is in the outputs. q, k and the outputs: f32, f16 or bf16, weights of that type or f32; 32 bits throughout, one rounding at the end; a
- * row whose sum of squares leaves 32 bits is 0 (NaN at infinities). D 1..512. An output may be its own input (the
+ * row whose sum of squares leaves 32 bits is 0 (NaN at infinities), and a row of zeros without an eps NaN; eps may be 0 or as small as it
+ * likes, and elements of any size. D 1..512. An output may be its own input (the
  * same view), and must not overlap anything else.
  */
 int kg_gfx950_head_norm_rotate_entry(const KgArgSlot* ordered_args, unsigned long long arg_count);

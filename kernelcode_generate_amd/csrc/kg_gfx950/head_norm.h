@@ -2,7 +2,8 @@
 //   y = x / sqrt(sum_d x_d^2 / D + eps) w   (where the side has weights w; y = x otherwise),
 //   (a, b) -> (a cos - b sin, b cos + a sin) for pair i of the token's position, i < half: elements (i, i + half), or (2 i, 2 i + 1)
 // of neighbours; elements behind 2 half stay as they are. All of it in 32 bits, rounded once to the output's type. A sum of
-// squares past 3.4e38 is infinite there, and the row 0.
+// squares past 3.4e38 is infinite there, and the row 0. A mean square with eps below 2^-100 is taken of 2^100 times the elements, which
+// is exact: squares, mean and the inverse root's input (v_rsq_f32 takes subnormal ones for 0) are then normal numbers for elements of any size.
 //
 // head_norm_kernel: L lanes per head, each with the W elements on both sides of its pairs (2 W side by side of neighbours), so that a
 // pair never leaves its lane, and G heads of a token at a time, whose reads are in flight together and whose angles and weights are read
@@ -38,6 +39,17 @@ __device__ __forceinline__ long long head_norm_position(const HeadNormArgs& a, i
                           : (long long)static_cast<const int*>(a.positions)[t * a.position_stride];
 }
 
+// 1 / sqrt(sum of squares / D + eps). squares(): the sum over the head, the same in all of its lanes; enlarge(by): multiplies the elements.
+template <typename F, typename G>
+__device__ __forceinline__ float head_norm_inverse(const HeadNormArgs& a, F squares, G enlarge) {
+  float mean = squares() * a.inverse_d + a.eps;
+  if (mean < 0x1p-100f) {
+    enlarge(0x1p100f);
+    mean = squares() * a.inverse_d + a.eps * 0x1p100f * 0x1p100f;  // (eps is below 2^-100)
+  }
+  return __builtin_amdgcn_rsqf(mean);
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void head_norm_any_kernel(HeadNormArgs a) {
   constexpr int kMost = 4;  // pairs of a lane: 512 elements
@@ -54,7 +66,6 @@ __global__ __launch_bounds__(256) void head_norm_any_kernel(HeadNormArgs a) {
     T* y = static_cast<T*>(s.y) + t * s.y_token + h * s.y_head;
     // unit u: pair u, or for u >= half the elements 2 u and 2 u + 1
     float e[kMost][2];
-    float sum = 0.f;
     auto first = [&](int u) { return u < a.half && !a.neighbours ? u : 2 * u; };
     auto second = [&](int u) { return u < a.half && !a.neighbours ? u + a.half : 2 * u + 1; };
 #pragma unroll
@@ -62,10 +73,18 @@ __global__ __launch_bounds__(256) void head_norm_any_kernel(HeadNormArgs a) {
       const int u = lane + 64 * i;
       e[i][0] = first(u) < a.d ? Elem<T>::load(x + first(u)) : 0.f;
       e[i][1] = second(u) < a.d ? Elem<T>::load(x + second(u)) : 0.f;
-      sum += e[i][0] * e[i][0] + e[i][1] * e[i][1];
     }
     if (s.w != nullptr) {
-      const float by = __builtin_amdgcn_rsqf(wave_sum(sum) * a.inverse_d + a.eps);
+      auto squares = [&]() {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) sum += e[i][0] * e[i][0] + e[i][1] * e[i][1];
+        return wave_sum(sum);
+      };
+      const float by = head_norm_inverse(a, squares, [&](float f) {
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) e[i][0] *= f, e[i][1] *= f;
+      });
       auto weight = [&](int d) {
         if (d >= a.d) return 0.f;
         return s.wide ? static_cast<const float*>(s.w)[d * s.w_stride] : Elem<T>::load(static_cast<const T*>(s.w) + d * s.w_stride);
@@ -179,13 +198,19 @@ __global__ __launch_bounds__(256) void head_norm_kernel(HeadNormArgs a, HeadNorm
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float sum = 0.f;
+      auto squares = [&]() {
+        float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) sum = __builtin_fmaf(p[g][i], p[g][i], __builtin_fmaf(q[g][i], q[g][i], sum));
-      if (!in) sum = 0.f;
+        for (int i = 0; i < W; ++i) sum = __builtin_fmaf(p[g][i], p[g][i], __builtin_fmaf(q[g][i], q[g][i], sum));
+        if (!in) sum = 0.f;
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-      const float by = __builtin_amdgcn_rsqf(sum * a.inverse_d + a.eps);
+        for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        return sum;
+      };
+      const float by = head_norm_inverse(a, squares, [&](float f) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) p[g][i] *= f, q[g][i] *= f;
+      });
 #pragma unroll
       for (int i = 0; i < W; ++i) p[g][i] *= by * u[i], q[g][i] *= by * v[i];
     }
