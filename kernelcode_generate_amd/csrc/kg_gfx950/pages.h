@@ -206,12 +206,12 @@ __global__ __launch_bounds__(kPagesThreads) void kv_release_kernel(PagesArgs a) 
     if (one) pages = all;
     before += all;
     if (page >= 0) {
-      const int spot = count + pages - upto;
-      if (spot < a.stack) a.free[spot * a.free_stride] = page;
+      const uint32_t spot = (uint32_t)count + (uint32_t)(pages - upto);  // (a stack of nearly 2^31 places and what goes back pass 31 bits)
+      if (spot < (uint32_t)a.stack) a.free[spot * a.free_stride] = page;
     }
     if (at != nullptr) *at = -1;
   }
-  if (tid == 0) *a.count = min(count + pages, a.stack);
+  if (tid == 0) *a.count = (int)min((uint32_t)count + (uint32_t)pages, (uint32_t)a.stack);
 }
 
 }  // namespace kg_gfx950
