@@ -262,8 +262,9 @@ inline int head_norm_lanes(const HeadNormArgs& a, int w) {
 template <typename T, int W, int G>
 bool launch_head_norm(const HeadNormArgs& a, int lanes, hipStream_t stream) {
   HeadNormItems n;
-  n.chunks_q = (a.side[0].heads + G - 1) / G;
-  n.chunks = n.chunks_q + (a.side[1].heads + G - 1) / G;
+  auto chunks = [](int heads) { return heads / G + (heads % G != 0); };  // (up to 2^31 - 1 heads)
+  n.chunks_q = chunks(a.side[0].heads);
+  n.chunks = n.chunks_q + chunks(a.side[1].heads);
   const long long items = (long long)a.tokens * n.chunks, blocks = (items + 256 / lanes - 1) / (256 / lanes);
   if (items > 0x7fffff00LL || blocks > (1 << 24) - 1) return false;
   n.items = (int)items;
