@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void int8_any_kernel(Int8Args a) {
   __shared__ int8_t codes[kChunk];
   __shared__ float lds[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int blocks = (a.n + 4 * kChannels - 1) / (4 * kChannels);
+  const int blocks = (int)((a.n + 4ll * kChannels - 1) / (4 * kChannels));  // (up to 2^31 - 1 channels)
   for (long long item = blockIdx.x; item < (long long)a.m * blocks; item += gridDim.x) {
     const int m = (int)(item / blocks), n0 = (int)(item - (long long)m * blocks) * 4 * kChannels + wave * kChannels;
     const X* x = static_cast<const X*>(a.x) + m * a.x_row;
