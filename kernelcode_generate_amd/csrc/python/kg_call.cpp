@@ -11,6 +11,7 @@
 namespace {
 
 constexpr Py_ssize_t kMostArgs = 32;
+constexpr int64_t kMostAxes = 8;  // of a tensor; no entry takes as many
 using Entry = int (*)(const KgArgSlot*, unsigned long long);
 
 int dtype_code(at::ScalarType type) {
@@ -30,8 +31,13 @@ int dtype_code(at::ScalarType type) {
 const long long kAbsent[2] = {0, 1};  // extent and stride of an absent memory slot
 const long long kScalar[1] = {0};     // of a tensor of rank 0
 
+// A tensor's extents and strides, copied: the entry runs without the interpreter's lock, and another thread may change the tensor's view.
+struct Axes {
+  long long shape[kMostAxes], stride[kMostAxes];
+};
+
 // False: an argument that native.py takes its own way (a subclass, another number type, an integer past 64 bits).
-bool fill(KgArgSlot* slot, PyObject* arg) {
+bool fill(KgArgSlot* slot, Axes* axes, PyObject* arg) {
   *slot = KgArgSlot{};
   if (arg == Py_None) {
     slot->kind = KG_ARG_MEMORY;
@@ -48,12 +54,17 @@ bool fill(KgArgSlot* slot, PyObject* arg) {
     slot->float_value = PyFloat_AS_DOUBLE(arg);
   } else if (THPVariable_CheckExact(arg)) {
     const at::Tensor& t = THPVariable_Unpack(arg);
-    static_assert(sizeof(int64_t) == sizeof(long long), "extents are taken as they are");
+    const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+    if (t.dim() > kMostAxes) return false;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      axes->shape[i] = sizes[i];
+      axes->stride[i] = strides[i];
+    }
     slot->kind = KG_ARG_MEMORY;
     slot->dtype_code = dtype_code(t.scalar_type());
     slot->rank = (unsigned long long)t.dim();
-    slot->shape = t.dim() == 0 ? kScalar : reinterpret_cast<const long long*>(t.sizes().data());
-    slot->stride = t.dim() == 0 ? kScalar : reinterpret_cast<const long long*>(t.strides().data());
+    slot->shape = t.dim() == 0 ? kScalar : axes->shape;
+    slot->stride = t.dim() == 0 ? kScalar : axes->stride;
     slot->data = t.mutable_data_ptr();  // (an entry may write it: a lazy copy is made here, as by data_ptr())
     return slot->dtype_code != 0;
   } else {
@@ -72,9 +83,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t count) {
   const Py_ssize_t slots = PyTuple_GET_SIZE(args[1]);
   if (entry == nullptr || slots > kMostArgs) Py_RETURN_NONE;
   KgArgSlot slot[kMostArgs];
+  Axes axes[kMostArgs];
   try {
     for (Py_ssize_t i = 0; i < slots; ++i)
-      if (!fill(&slot[i], PyTuple_GET_ITEM(args[1], i))) Py_RETURN_NONE;
+      if (!fill(&slot[i], &axes[i], PyTuple_GET_ITEM(args[1], i))) Py_RETURN_NONE;
   } catch (...) {  // (a tensor without extents or memory of its own)
     Py_RETURN_NONE;
   }
