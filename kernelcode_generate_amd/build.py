@@ -98,7 +98,8 @@ def build_probe_library(output: Path = PROBE_OUTPUT, verbose: bool = False) -> P
 
 
 def build_call_module(output: Path = CALL_OUTPUT, verbose: bool = False) -> Path:
-    """Compile csrc/python/kg_call.cpp, a host module of the running Python against the torch that is installed."""
+    """Compile csrc/python/kg_call.cpp, a host module of the running Python against the torch that is installed. It holds both
+    versions and refuses to load under others."""
 
     import sysconfig
 
@@ -107,7 +108,10 @@ def build_call_module(output: Path = CALL_OUTPUT, verbose: bool = False) -> Path
 
     tmp = output.with_suffix(".so.tmp")
     libraries = library_paths()
-    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
+    running = " ".join(str(v) for v in (torch.__version__, getattr(torch.version, "git_version", None)) if v is not None)
+    versions = [f"-DKG_PYTHON=\"{sys.version_info.major}.{sys.version_info.minor}.\"",
+                f"-DKG_TORCH=\"{running}\""]
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", *versions,
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *include_flags()[:1],
            f"-I{sysconfig.get_paths()['include']}", *(f"-I{p}" for p in include_paths()), str(CSRC / "python" / "kg_call.cpp"),
            "-o", str(tmp), *(f"-L{p}" for p in libraries), "-ltorch_python", "-ltorch_cpu", "-lc10"]

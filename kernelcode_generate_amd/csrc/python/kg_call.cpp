@@ -6,6 +6,8 @@
 
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstring>
+
 #include "kg_gfx950.h"
 
 namespace {
@@ -102,6 +104,38 @@ PyMethodDef kMethods[] = {{"call", reinterpret_cast<PyCFunction>(reinterpret_cas
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_kg_call", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
+// "version commit" of the torch that runs, as build.py writes KG_TORCH from the one that it compiles against.
+PyObject* running_torch() {
+  PyObject *torch = PyImport_ImportModule("torch"), *text = nullptr;
+  PyObject* version = torch != nullptr ? PyObject_GetAttrString(torch, "__version__") : nullptr;
+  PyObject* versions = version != nullptr ? PyObject_GetAttrString(torch, "version") : nullptr;
+  PyObject* commit = versions != nullptr ? PyObject_GetAttrString(versions, "git_version") : nullptr;
+  if (versions != nullptr) {
+    PyErr_Clear();  // (a torch may name no commit)
+    text = commit == nullptr || commit == Py_None ? PyUnicode_FromFormat("%S", version) : PyUnicode_FromFormat("%S %S", version, commit);
+  }
+  Py_XDECREF(commit);
+  Py_XDECREF(versions);
+  Py_XDECREF(version);
+  Py_XDECREF(torch);
+  return text;
+}
+
 }  // namespace
 
-PyMODINIT_FUNC PyInit__kg_call() { return PyModule_Create(&kModule); }
+// Tensors are read by torch's inlined layouts and Python's objects by its macros, which no missing symbol tells apart: another version
+// of either is refused.
+PyMODINIT_FUNC PyInit__kg_call() {
+  const char* const python = Py_GetVersion();
+  const size_t own = sizeof(KG_PYTHON) - 1;  // "3.10."
+  if (strncmp(python, KG_PYTHON, own) != 0) {
+    PyErr_Format(PyExc_ImportError, "built against Python %sx, this is %s", KG_PYTHON, python);
+    return nullptr;
+  }
+  PyObject* const torch = running_torch();
+  if (torch == nullptr) return nullptr;
+  const bool same = PyUnicode_CompareWithASCIIString(torch, KG_TORCH) == 0;
+  if (!same) PyErr_Format(PyExc_ImportError, "built against torch %s, this is %S", KG_TORCH, torch);
+  Py_DECREF(torch);
+  return same ? PyModule_Create(&kModule) : nullptr;
+}

@@ -146,7 +146,7 @@ def load_library() -> ctypes.CDLL:
         from kernelcode_generate_amd import _kg_call
 
         _FAST_CALL = _kg_call.call
-    except ImportError:  # (built against another torch, or without one: the slots are packed here)
+    except ImportError:  # (not built, built against another torch or Python, or no torch: the slots are packed here)
         _FAST_CALL = None
     _LIBRARY = lib
     return lib
