@@ -289,7 +289,8 @@ enum {
   /* the projection's MFMAs, without the adapters', whose number depends on the indexes; fp32 sums of a split K are
    * counted as written and read */
   KG_OP_ADAPTER_MATMUL = 4,
-  /* codes that the call makes, and weights that it copies, are counted as written and read */
+  /* codes that the call makes, and weights that it copies, are counted as written and read; rows whose channels go in
+   * pieces, since their copies pass the workspace, are counted for each piece */
   KG_OP_INT8_MATMUL = 5
 };
 enum {

@@ -1998,8 +1998,10 @@ int launch_int8(const Int8Args& a, bool codes, bool x_aligned, bool w_aligned) {
         const long long m = std::min(rows, a.m - m0), n = std::min(channels, a.n - n0);
         mfma += int8_tiles_mfma(m, n, k, one ? plan : int8_plan(m, n, k, false));
       }
-    const long long copies = (take_x ? (long long)a.m * pitch : 0) + (take_w ? (long long)a.n * pitch : 0) + plan.bytes;
-    return record_cost((long long)a.m * a.n * a.k, mfma, 16, copies, copies);
+    // (each piece of channels makes its rows ready anew: the entry counts their first read)
+    const long long turns = cdiv(a.n, channels), again = take_x ? (turns - 1) * a.m * a.k * (codes ? 1 : (long long)sizeof(T)) : 0;
+    const long long copies = (take_x ? turns * a.m * pitch : 0) + (take_w ? (long long)a.n * pitch : 0) + plan.bytes;
+    return record_cost((long long)a.m * a.n * a.k, mfma, 16, copies + again, copies);
   }
   SplitLease lease;  // held until the kernels are enqueued
   char* ws = nullptr;
