@@ -115,13 +115,13 @@ hipError_t launch_int8_tiles(const Int8Tiles& g, const Int8Plan& p, int* partial
     return hipGetLastError();
   }
   switch (p.form) {
-    case 0: return launch_gemm_i8<T, 8, 8, 128, 2>(g, stream);
-    case 1: return launch_gemm_i8<T, 8, 4, 128, 3>(g, stream);
-    case 2: return launch_gemm_i8<T, 4, 4, 128, 4>(g, stream);
-    case 3: return launch_gemm_i8<T, 4, 2, 128, 3>(g, stream);
-    case 4: return launch_gemm_i8<T, 2, 2, 128, 4>(g, stream);
-    case 5: return launch_gemm_i8<T, 1, 2, 128, 4>(g, stream);
-    default: return launch_gemm_i8<T, 1, 1, 128, 8>(g, stream);
+    case 0: return launch_gemm_i8<T, 8, 8, 2>(g, stream);
+    case 1: return launch_gemm_i8<T, 8, 4, 3>(g, stream);
+    case 2: return launch_gemm_i8<T, 4, 4, 4>(g, stream);
+    case 3: return launch_gemm_i8<T, 4, 2, 3>(g, stream);
+    case 4: return launch_gemm_i8<T, 2, 2, 4>(g, stream);
+    case 5: return launch_gemm_i8<T, 1, 2, 4>(g, stream);
+    default: return launch_gemm_i8<T, 1, 1, 8>(g, stream);
   }
 }
 

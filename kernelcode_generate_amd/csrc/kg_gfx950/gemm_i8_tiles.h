@@ -1,7 +1,7 @@
 // gemm_i8_kernel: products in 8-bit integers (gemm_i8.h) in tiles, four waves of 2 x 2, each a (16 NA) x (16 NB) quarter in blocks of
-// v_mfma_i32_16x16x64_i8. Both operands lie along k, so both are copied to LDS and read back the same way: rows of kBK
+// v_mfma_i32_16x16x64_i8. Both operands lie along k, so both are copied to LDS and read back the same way: rows of 128
 // bytes, fragments of 16 bytes (16 k) a lane, which is the form that the instruction takes from both sides. The K loop: a ring of kStages
-// slices of kBK k filled by copies straight from memory to LDS, one barrier a slice, and a step's MFMAs (64 k) from registers while the
+// slices of 128 k filled by copies straight from memory to LDS, one barrier a slice, and a step's MFMAs (64 k) from registers while the
 // next step's fragments are read and a later slice's copies are issued between them. The barrier before a slice's last step finds all its
 // fragments read: it publishes the next slice's copies and frees this slice's stage for its refill.
 //
@@ -27,6 +27,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 namespace gemmi {
 constexpr int kThreads = 256;
+constexpr int kBK = 128, kSteps = kBK / 64;  // k of a slice, its steps
 // acc += a b on one 16 x 16 block, the accumulator tied to one register tuple of the accumulation file for the whole kernel (the compiler
 // rotates the accumulators of its own form through that file at the loop's edge: 128 x 128 tiles of K = 4096 21.2 us, tied 16.6);
 // results are read behind mfma_drain and mfma_order.
@@ -40,13 +41,8 @@ __device__ __forceinline__ void mfma_order(i32x4 (&a)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+a"(a[i]));
 }
-// 16-byte chunk c of a row lies at c ^ swizzle(row): the 16 rows of a fragment's read hit distinct banks (256 bytes a cycle; with the rows
-// of 64 bytes at c ^ row / 4 % 4 half of the LDS cycles were conflicts)
-template <int kBK>
-__device__ __forceinline__ int swizzle(int row) {
-  if constexpr (kBK == 64) return (row >> 1) & 3;
-  else return (row >> 1) & 7;
-}
+// 16-byte chunk c of a row lies at c ^ swizzle(row): the 16 rows of a fragment's read hit distinct banks (256 bytes a cycle)
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 }  // namespace gemmi
 
 // 16 bytes to any address, past the L2
@@ -69,18 +65,16 @@ struct Int8Tiles {
 };
 
 // T int: the sums as they are, of one chunk of k: out is [chunks][m][ldo].
-template <typename T, int NA, int NB, int kBK, int kStages>
+template <typename T, int NA, int NB, int kStages>
 __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8_kernel(Int8Tiles g) {
   using namespace gemmi;
   constexpr int TM = 32 * NA, TN = 32 * NB;
-  constexpr int kSteps = kBK / 64;
   constexpr int kRowsPiece = 1024 / kBK;  // rows of a wave's copy
   constexpr int AP = TM / kRowsPiece / 4, BP = TN / kRowsPiece / 4, kPieces = AP + BP;  // copies per wave and slice
   constexpr int kStageA = TM * kBK, kStageB = TN * kBK, kStage = kStageA + kStageB;
   constexpr int kMfmas = NA * NB, kReads = NA + NB;
-  static_assert(kSteps == 1 || kSteps == 2, "steps");
   static_assert(AP >= 1 && BP >= 1, "pieces");
-  static_assert(kStages >= 2 && (kSteps == 2 || kStages % 2 == 0), "a step's registers are constants of the unrolled ring");
+  static_assert(kStages >= 2, "a ring");
   __shared__ __attribute__((aligned(1024))) char lds[kStages * kStage];
   __shared__ __attribute__((aligned(16))) float xs_lds[TM], ws_lds[TN], bias_lds[TN];
 
@@ -99,9 +93,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
 
   constexpr bool kPartial = std::is_same<T, int>::value;
   const int k0 = kPartial ? blockIdx.y * g.chunk : 0, k_own = kPartial ? min(g.k - k0, g.chunk) : g.k;
-  // slices of K; in the one-step form a multiple of two (registers go by a slice's parity), and at least a ring of them: zeros behind K
-  const int slices = (k_own + kBK - 1) / kBK;
-  const int count = max(kSteps == 1 ? (slices + 1) / 2 * 2 : slices, kStages);
+  const int count = max((k_own + kBK - 1) / kBK, kStages);  // slices of K, at least a ring of them: zeros behind K
 
   // ---- memory -> LDS: piece p of a wave is rows (wave AP + p) kRowsPiece + lane / (kBK / 16) ----
   constexpr int kChunks = kBK / 16;
@@ -110,17 +102,17 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
 #pragma unroll
   for (int p = 0; p < AP; ++p) {
     const int row = (wave * AP + p) * kRowsPiece + lane / kChunks;
-    a_off[p] = (uint32_t)(row * g.ldx + 16 * ((lane % kChunks) ^ swizzle<kBK>(row)));
+    a_off[p] = (uint32_t)(row * g.ldx + 16 * ((lane % kChunks) ^ swizzle(row)));
     if (m0 + row >= g.m) a_off[p] = kBufOOB;
   }
 #pragma unroll
   for (int p = 0; p < BP; ++p) {
     const int row = (wave * BP + p) * kRowsPiece + lane / kChunks;
-    b_off[p] = (uint32_t)(row * g.ldw + 16 * ((lane % kChunks) ^ swizzle<kBK>(row)));
+    b_off[p] = (uint32_t)(row * g.ldw + 16 * ((lane % kChunks) ^ swizzle(row)));
     if (n0 + row >= g.n) b_off[p] = kBufOOB;
   }
 #pragma unroll
-  for (int x = 0; x < 2; ++x) chunk_k[x] = 16 * ((lane % kChunks) ^ swizzle<kBK>(x * kRowsPiece + lane / kChunks));
+  for (int x = 0; x < 2; ++x) chunk_k[x] = 16 * ((lane % kChunks) ^ swizzle(x * kRowsPiece + lane / kChunks));
   const char* a_tile = reinterpret_cast<const char*>(g.x) + (long long)m0 * g.ldx + k0;
   const char* b_tile = reinterpret_cast<const char*>(g.w) + (long long)n0 * g.ldw + k0;
   const uint32_t lds0 = lds_addr(lds);
@@ -130,7 +122,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
     const char* src = (a ? a_tile : b_tile) + (long long)kt * kBK;
     const uint32_t dst = lds0 + stage * kStage + (a ? (wave * AP + p) * 1024 : kStageA + (wave * BP + p) * 1024);
     const uint32_t off = a ? a_off[a ? p : 0] : b_off[a ? 0 : p];
-    const int k = chunk_k[kBK == 64 ? 0 : ((a ? wave * AP : wave * BP) + p) & 1];
+    const int k = chunk_k[((a ? wave * AP : wave * BP) + p) & 1];
     buf2lds16_s(kt * kBK + k < k_own ? off : kBufOOB, src, dst);
   };
 
@@ -138,7 +130,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   uint32_t a_rd[kSteps], b_rd[kSteps];
 #pragma unroll
   for (int ks = 0; ks < kSteps; ++ks) {
-    const int at = 16 * ((4 * ks + lg) ^ swizzle<kBK>(l16));
+    const int at = 16 * ((4 * ks + lg) ^ swizzle(l16));
     a_rd[ks] = lds0 + (wm * 16 * NA + l16) * kBK + at;
     b_rd[ks] = lds0 + kStageA + (wn * 16 * NB + l16) * kBK + at;
   }
@@ -180,7 +172,7 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   for (int i = 0; i < NA; ++i) mfma_order(acc[i]);
 
   // copies of a slice in its last step, and (kHalves) the others in the next slice's first one
-  constexpr bool kHalves = kSteps == 2 && kStages > 2;
+  constexpr bool kHalves = kStages > 2;
   constexpr int kCopies = kHalves ? (kPieces + 1) / 2 : kPieces, kRest = kPieces - kCopies;
 #pragma unroll
   for (int i = 0; i < kStages; ++i)
@@ -193,29 +185,28 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
 #pragma unroll
   for (int r = 0; r < kReads; ++r) read_step(fr[0], r);
 
-  // Slice kt, in stage `stage`, its registers by kParity. kBehind: slices behind it, kStages where there are so many. The refill of its
+  // Slice kt, in stage `stage`. kBehind: slices behind it, kStages where there are so many. The refill of its
   // stage (slice kt + kStages) goes into the last step, behind its barrier, with more than two stages half of it into the next
   // slice's first. The last kStages slices are a compile-time group whose waits, reads and copies carry no conditions (with
   // conditions they took about twice a steady one's cycles).
-  auto slice = [&](int kt, int stage, auto parity_tag, auto behind_tag) __attribute__((always_inline)) {
-    constexpr int kParity = decltype(parity_tag)::value, kBehind = decltype(behind_tag)::value;
+  auto slice = [&](int kt, int stage, auto behind_tag) __attribute__((always_inline)) {
+    constexpr int kBehind = decltype(behind_tag)::value;
     constexpr int kYounger = (kBehind < kStages - 1 ? kBehind : kStages - 1) - 1;  // slices behind the next one that are on their way
     const int next = stage + 1 == kStages ? 0 : stage + 1, before = stage == 0 ? kStages - 1 : stage - 1;
     static_for<kSteps>([&](auto step_tag) __attribute__((always_inline)) {
       constexpr int ks = decltype(step_tag)::value;
       constexpr bool kLast = ks == kSteps - 1;
-      constexpr int P = kSteps == 2 ? ks : kParity;
       if constexpr (kLast && kBehind > 0) wait_and_barrier<(kYounger > 0 ? kYounger : 0) * kPieces>();
       if constexpr (!kLast) read_from(stage, 1);
       else if constexpr (kBehind > 0) read_from(next, 0);
       static_for<kMfmas>([&](auto idx_tag) __attribute__((always_inline)) {
         constexpr int idx = decltype(idx_tag)::value;
         constexpr int i = idx / NB, j = idx % NB;
-        mfma(acc[i][j], fr[P].b[j], fr[P].a[i]);  // blocks of the transpose: a lane's columns lie side by side
+        mfma(acc[i][j], fr[ks].b[j], fr[ks].a[i]);  // blocks of the transpose: a lane's columns lie side by side
         constexpr int r0 = (idx * 2 * kReads + kMfmas - 1) / kMfmas, r1 = ((idx + 1) * 2 * kReads + kMfmas - 1) / kMfmas;
         static_for<(r1 < kReads ? r1 : kReads) - (r0 < kReads ? r0 : kReads)>([&](auto r_tag) __attribute__((always_inline)) {
           constexpr int r = r0 + decltype(r_tag)::value;
-          if constexpr (!kLast || kBehind > 0) read_step(fr[P ^ 1], r);
+          if constexpr (!kLast || kBehind > 0) read_step(fr[ks ^ 1], r);
         });
         constexpr int kOwn = kLast ? kCopies : kRest;
         static_for<kOwn>([&](auto c_tag) __attribute__((always_inline)) {
@@ -232,17 +223,13 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   int kt = 0, stage = 0;
   auto step = [&]() __attribute__((always_inline)) { stage = stage + 1 == kStages ? 0 : stage + 1; };
 #pragma unroll 1
-  for (; kt + kStages < count; kt += 3 - kSteps) {
-    slice(kt, stage, Int<0>{}, Int<kStages>{});
+  for (; kt + kStages < count; ++kt) {
+    slice(kt, stage, Int<kStages>{});
     step();
-    if constexpr (kSteps == 1) {
-      slice(kt + 1, stage, Int<1>{}, Int<kStages>{});
-      step();
-    }
   }
   static_for<kStages>([&](auto u_tag) __attribute__((always_inline)) {
     constexpr int u = decltype(u_tag)::value;
-    slice(kt + u, stage, Int<(kSteps == 1 ? u & 1 : 0)>{}, Int<kStages - 1 - u>{});
+    slice(kt + u, stage, Int<kStages - 1 - u>{});
     step();
   });
 
@@ -313,12 +300,12 @@ __global__ __launch_bounds__(gemmi::kThreads, NA * NB > 16 ? 1 : 2) void gemm_i8
   }
 }
 
-template <typename T, int NA, int NB, int kBK, int kStages>
+template <typename T, int NA, int NB, int kStages>
 hipError_t launch_gemm_i8(const Int8Tiles& g, hipStream_t stream) {
   constexpr int TM = 32 * NA, TN = 32 * NB;
   const unsigned grid = (unsigned)(((long long)g.m + TM - 1) / TM * (((long long)g.n + TN - 1) / TN));
   const unsigned chunks = std::is_same<T, int>::value ? (unsigned)((g.k + g.chunk - 1) / g.chunk) : 1u;
-  hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kBK, kStages>), dim3(grid, chunks), dim3(gemmi::kThreads), 0, stream, g);
+  hipLaunchKernelGGL((gemm_i8_kernel<T, NA, NB, kStages>), dim3(grid, chunks), dim3(gemmi::kThreads), 0, stream, g);
   return hipGetLastError();
 }
 

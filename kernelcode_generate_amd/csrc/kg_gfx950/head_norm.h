@@ -274,7 +274,7 @@ bool launch_head_norm(const HeadNormArgs& a, int lanes, hipStream_t stream) {
   else if (lanes == 8) KG_HEAD_NORM(8);
   else if (lanes == 16) KG_HEAD_NORM(16);
   else if (lanes == 32) KG_HEAD_NORM(32);
-  else KG_HEAD_NORM(64);
+  else if constexpr (W < 8) KG_HEAD_NORM(64);  // (pieces of 8: 512 elements in 32 lanes)
 #undef KG_HEAD_NORM
   return true;
 }

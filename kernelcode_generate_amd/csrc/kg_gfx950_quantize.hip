@@ -7,9 +7,9 @@
 namespace kg_gfx950 {
 
 hipError_t launch_int8_chunks(const Int8Tiles& g, int form, hipStream_t stream) {
-  if (form == 4) return launch_gemm_i8<int, 2, 2, 128, 4>(g, stream);
-  if (form == 5) return launch_gemm_i8<int, 1, 2, 128, 4>(g, stream);
-  return launch_gemm_i8<int, 1, 1, 128, 8>(g, stream);
+  if (form == 4) return launch_gemm_i8<int, 2, 2, 4>(g, stream);
+  if (form == 5) return launch_gemm_i8<int, 1, 2, 4>(g, stream);
+  return launch_gemm_i8<int, 1, 1, 8>(g, stream);
 }
 
 }  // namespace kg_gfx950
