@@ -39,13 +39,17 @@ __device__ __forceinline__ long long head_norm_position(const HeadNormArgs& a, i
                           : (long long)static_cast<const int*>(a.positions)[t * a.position_stride];
 }
 
+// Of a mean square with eps below kTinyMean, elements are taken kEnlarge times; both products with eps, which is below 2^-100 too, stay in range.
+constexpr float kTinyMean = 0x1p-100f, kEnlarge = 0x1p100f;
+__device__ __forceinline__ float enlarged_mean(const HeadNormArgs& a, float sum) { return sum * a.inverse_d + a.eps * kEnlarge * kEnlarge; }
+
 // 1 / sqrt(sum of squares / D + eps). squares(): the sum over the head, the same in all of its lanes; enlarge(by): multiplies the elements.
 template <typename F, typename G>
 __device__ __forceinline__ float head_norm_inverse(const HeadNormArgs& a, F squares, G enlarge) {
   float mean = squares() * a.inverse_d + a.eps;
-  if (mean < 0x1p-100f) {
-    enlarge(0x1p100f);
-    mean = squares() * a.inverse_d + a.eps * 0x1p100f * 0x1p100f;  // (eps is below 2^-100)
+  if (mean < kTinyMean) {
+    enlarge(kEnlarge);
+    mean = enlarged_mean(a, squares());
   }
   return __builtin_amdgcn_rsqf(mean);
 }
@@ -66,6 +70,7 @@ __global__ __launch_bounds__(256) void head_norm_any_kernel(HeadNormArgs a) {
     T* y = static_cast<T*>(s.y) + t * s.y_token + h * s.y_head;
     // unit u: pair u, or for u >= half the elements 2 u and 2 u + 1
     float e[kMost][2];
+    float sum = 0.f;
     auto first = [&](int u) { return u < a.half && !a.neighbours ? u : 2 * u; };
     auto second = [&](int u) { return u < a.half && !a.neighbours ? u + a.half : 2 * u + 1; };
 #pragma unroll
@@ -73,18 +78,20 @@ __global__ __launch_bounds__(256) void head_norm_any_kernel(HeadNormArgs a) {
       const int u = lane + 64 * i;
       e[i][0] = first(u) < a.d ? Elem<T>::load(x + first(u)) : 0.f;
       e[i][1] = second(u) < a.d ? Elem<T>::load(x + second(u)) : 0.f;
+      sum += e[i][0] * e[i][0] + e[i][1] * e[i][1];
     }
     if (s.w != nullptr) {
-      auto squares = [&]() {
-        float sum = 0.f;
+      float mean = wave_sum(sum) * a.inverse_d + a.eps;
+      if (mean < kTinyMean) {
+        sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < kMost; ++i) sum += e[i][0] * e[i][0] + e[i][1] * e[i][1];
-        return wave_sum(sum);
-      };
-      const float by = head_norm_inverse(a, squares, [&](float f) {
-#pragma unroll
-        for (int i = 0; i < kMost; ++i) e[i][0] *= f, e[i][1] *= f;
-      });
+        for (int i = 0; i < kMost; ++i) {
+          e[i][0] *= kEnlarge, e[i][1] *= kEnlarge;
+          sum += e[i][0] * e[i][0] + e[i][1] * e[i][1];
+        }
+        mean = enlarged_mean(a, wave_sum(sum));
+      }
+      const float by = __builtin_amdgcn_rsqf(mean);
       auto weight = [&](int d) {
         if (d >= a.d) return 0.f;
         return s.wide ? static_cast<const float*>(s.w)[d * s.w_stride] : Elem<T>::load(static_cast<const T*>(s.w) + d * s.w_stride);
