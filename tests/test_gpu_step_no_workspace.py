@@ -4,6 +4,7 @@ number of the graph's nodes."""
 from __future__ import annotations
 
 import ctypes
+import gc
 import random
 
 import pytest
@@ -82,6 +83,9 @@ def test_pages_and_long_sums_without_a_workspace(device):
     big, w = torch.zeros(16000, 4096, dtype=BF16, device=device), torch.ones(16, 4096, dtype=torch.int8, device=device)
     out, one = torch.empty(16000, 16, dtype=BF16, device=device), torch.ones(16, device=device)
     pages = {requests: Pages(device, requests) for requests in (8192, 1000, 100, 20, 3)}
+    gc.collect()
+    torch.cuda.synchronize()
+    pages[3].run()  # an eager call that takes a workspace frees those of graphs that are gone
     recorded = {requests: [record(p.run)] for requests, p in pages.items()}
     assert all(r[0][1] == 2 for r in recorded.values())  # with a workspace: the sums, then the rows
     for m in (16000, 4000, 1000, 250, 60, 10, 2):  # 65 MB and less a recording; then a call of each size of pages until it gets none
