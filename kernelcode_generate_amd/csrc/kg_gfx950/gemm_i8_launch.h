@@ -46,9 +46,12 @@ hipError_t launch_quantize(const QuantizeArgs& a, const PackArgs& pack, hipStrea
 
 // The tiles of a product by a model of each form's time (ns): a launch, a further round of 256 tiles, a slice of 128 k, and percent more of
 // a slice where all CUs have a tile (their clocks go down). Fitted to 350 products of 1..4096 rows, 1024..16384 channels and K of
-// 512..11008, of which the one that it picks is 2.9 % above the fastest on average, the measurements' own spread with it. us of the forms in
-// their order: 4096^3 58 / 66 / 82 / 98 / 113 / - / -; 1000 x 4096 x 4096 44 / 29 / 19.3 / 23 / 31 / - / -; 300 x 4096 x 4096 43 / 26 / 17 / 13.1 /
-// 13.5 / 15 / 17.3; 64 x 4096 x 4096 - / - / - / 12.7 / 9.5 / 8.4 / 6.1; 16 x 11008 x 11008 - / - / - / 43.7 / 33.3 / 32.7 / 30.7. A deeper ring than
+// 512..11008, of which the one that it picks is 2.9 % above the fastest on average, the measurements' own spread with it. On 165 others of
+// 65..640 rows, 4096..14336 channels and K of 4096..14336 it picks what is as fast as the fastest on average, 8 % slower at most (65 rows of K = 8192: 32 x 64
+// 19.6, 32 x 32 17.9). us of the forms in
+// their order: 4096^3 58 / 66 / 82 / 98 / 113 / - / -; 1000 x 4096 x 4096 44 / 29 / 19.3 / 23 / 31 / - / -; 300 x 4096 x 4096 43 / 27 / 17.5 / 14.0 /
+// 14.2 / 16 / 20; 130 x 4096 x 4096 43 / 26 / 17.1 / 13.6 / 10.5 / 11.8 / 13.6; 300 x 11008 x 4096 50 / 31.2 / 33.7 / 35 / 34 / 42 / 54;
+// 64 x 4096 x 4096 - / - / - / 12.7 / 9.5 / 8.4 / 6.1; 16 x 11008 x 11008 - / - / - / 43.7 / 33.3 / 32.7 / 30.7. A deeper ring than
 // these changes nothing: what a slice of a small tile costs is its own chain of barrier, LDS reads and products.
 struct Int8Form {
   int rows, channels, stages, fixed, round, slice, load;

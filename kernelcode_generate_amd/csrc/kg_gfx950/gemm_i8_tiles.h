@@ -6,12 +6,12 @@
 // fragments read: it publishes the next slice's copies and frees this slice's stage for its refill.
 //
 // Slices of 128 k: a copy then takes whole 128-byte lines. With 64, each line passes from the L2 twice, and 256 x 256 tiles were bound by
-// that (8192^3 410 us with four slices of 64 in the ring, 378 with two of 128). What bounds them now, 8192^3 with codes of a normal
-// distribution: power. The products alone would take 262 us at the 4.2 POPS that the instruction reaches on registers, where the clock has
-// fallen to 2.0 GHz; here it is 1.9, with the matrix units busy in 69 % of all cycles (the form with slices of 64 took 419 us, 322 with the
-// copies left out, 374 with the reads of LDS left out, in as many cycles as with them). 2.74 to 2.9 POPS; the library's product 2.44. 4096^3 58 us, of which 11 are a launch, a ring to fill and the
-// results' way to memory. Small tiles are bound by a slice's chain of barrier, LDS reads and products (0.1 us for 32 x 32, 0.2 for 64 x 64), middle
-// ones by the L2 (20 TB/s).
+// that (8192^3, 8 % longer with four slices of 64 in the ring than with two of 128). What bounds them now, 8192^3 with codes of a normal
+// distribution, 401 to 413 us: power. The products are 524288 cycles of a SIMD, 268 us at the 1.95 GHz to which the clock falls here (on
+// registers alone it is 2.0, 4.2 POPS), and 65 % of the cycles that pass (the form with slices of 64 took 419 us, 322 with the
+// copies left out, 374 with the reads of LDS left out, in as many cycles as with them). 2.66 to 2.74 POPS; the library's product 2.44. 4096^3 54 us,
+// of which 11 are a launch, a ring to fill and the results' way to memory. Small tiles are bound by a slice's chain of barrier, LDS reads and
+// products (0.1 us for 32 x 32, 0.2 for 64 x 64), middle ones by what a CU takes into its LDS, some 80 GB/s (20 TB/s where all 256 have a tile).
 //
 // Copies are buffer loads that land zeros outside the matrices (as fast as plain ones), stores are made inside alone: any M and N. K is a
 // multiple of 16 (rows of others are copied into padded ones first).

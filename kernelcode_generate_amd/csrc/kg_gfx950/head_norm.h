@@ -8,7 +8,7 @@
 // head_norm_kernel: L lanes per head, each with the W elements on both sides of its pairs (2 W side by side of neighbours), so that a
 // pair never leaves its lane, and G heads of a token at a time, whose reads are in flight together and whose angles and weights are read
 // once; half a multiple of W, an even D of 2 W, rows that start anywhere. Bound by its bytes where there are many: 8192 tokens of 32 and 8
-// heads of 128 in bf16 34.2 us, 4.7 TB/s, in fp32 62, 5.1 TB/s; 64 tokens take 3.3, a launch's 2.3 and one chain of reads.
+// heads of 128 in bf16 33 us, 4.9 TB/s, in fp32 62, 5.1 TB/s; 64 tokens take 3.3, a launch's 2.3 and one chain of reads.
 // head_norm_any_kernel: any D up to 512, half, strides and alignment: a wave per token and head, each lane some pairs of elements.
 #pragma once
 

@@ -9,9 +9,10 @@
 //
 // A call is a chain of a few dependent reads (lengths, a search for a row's request in LDS, its page), which more workgroups do not shorten,
 // and only one workgroup can take from the stack and write what is left of it without a second launch: up to 4096 rows one
-// workgroup does all, more are written by a second launch. us with one launch / two, 256 requests of a token each 4.6 / 5.9, 6 requests
-// in 3000 rows 5.6 / 6.2, 8 in 4096 6.3 / 6.3, 24 prompts in 16384 rows 18.7 / 6.7; a launch by itself takes 2.3. Pages of 256 requests given
-// back: 4.0.
+// workgroup does all, more are written by a second launch. us with one launch / two, 256 requests of a token each 5.0 / 6.3, 1024 5.8 / 8.0, 4000
+// 16.5 / 17.3; 6 requests in 3000 rows 6.4 / 6.5, 8 in 4096 7.3 / 6.3, 100 in 4000 8.4 / 6.8, 12 in 4800 7.9 / 6.4, 24 prompts in 16384 rows
+// 19.2 / 6.6: few requests of 3000 to 4096 rows would be a microsecond or so faster with two. A launch by itself takes 2.3. Pages given back: 4.1
+// for 256 entries, 4.6 for 1024; further ones go 1024 at a time, in two walks of the one workgroup: 16384 entries 36 to 41, 131072 230 to 300.
 #pragma once
 
 #include "common.h"

@@ -4,7 +4,8 @@
 //
 // quantize_rows_kernel: a row's lanes hold it in registers, 8 elements a piece, from the one read that there is to the codes; rows of 8
 // up to 16384 elements, starting anywhere. A wave a row up to 512 elements, four beyond: 4001 rows of 4096 in fp16 9.2 us, 5.3 TB/s, bound by
-// their bytes; 16 rows 2.4, a launch's. quantize_rows_any_kernel reads its rows twice, element by element.
+// their bytes; 4096 rows of 16384 in bf16 36 us, in fp32 68; 16 rows 2.4, a launch's. quantize_rows_any_kernel reads its rows twice, element by
+// element: 4096 rows of 28672 in bf16 224 us, 1.6 TB/s, in fp32 281; 16 rows 39.
 #pragma once
 
 #include <type_traits>
