@@ -134,7 +134,8 @@ int kg_gfx950_flash_attention_entry(const KgArgSlot* ordered_args, unsigned long
  * current device; all but the last axis of a tensor may have any non-negative strides, and the last is contiguous
  * (page_table, lens, starts, slots, positions, free_pages, mask, index, scales, biases, cos, sin and weights of norms: any). Values that lie in device memory (slots,
  * page tables, lengths, masks, adapter indexes) are not checked by the host: each entry says below what it makes of
- * values that are out of range. None of them reads or writes outside the tensors.
+ * values that are out of range. None of them reads or writes outside the tensors. Results of rows on one another (axes without
+ * strides) of more bytes than a card has, 2^39 for the entries from quantize_rows on, are refused.
  *
  * Caches: k_cache, v_cache [pages, heads, page_size, D] (D 1..512, any page_size), f32, f16, bf16, or 8-bit
  * (i8, e4m3) with k_scale, v_scale f32 [pages, heads, page_size] (absent otherwise). An 8-bit element stands

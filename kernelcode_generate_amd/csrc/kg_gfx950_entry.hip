@@ -1936,6 +1936,9 @@ int kv_cache_release_impl(const KgArgSlot* args, unsigned long long n) {
   return finish_launch("kv_cache_release");
 }
 
+// Bytes that no memory of a card reaches: only rows on one another (axes without strides) have results of more, whose work would not end.
+constexpr long long kMostBytes = 1ll << 39;
+
 // What a launcher returned, which took the error; the last launch of a call is finish_launch's.
 int launched(hipError_t err, const char* what) {
   return err == hipSuccess ? kOk : fail(kHipFailure, "%s: launch failed: %s", what, hipGetErrorString(err));
@@ -1963,8 +1966,8 @@ int quantize_rows_impl(const KgArgSlot* args, unsigned long long n) {
     return fail(kInvalid, "quantize_rows: codes shape [%lld,%lld] != [%lld,%lld]", codes.shape[0], codes.shape[1], M, K);
   if (scale.shape[0] != M) return fail(kInvalid, "quantize_rows: %lld scales for %lld rows", scale.shape[0], M);
   if (!row_contiguous(codes) || !row_contiguous(x)) return fail(kInvalid, "quantize_rows: the rows of codes and x must be contiguous");
+  if (K > 0x7fff0000LL || M * K > kMostBytes) return fail(kUnsupported, "quantize_rows: %lld rows of %lld elements are too many", M, K);
   if ((rc = check_view(codes, "codes")) || (rc = check_view(scale, "scale")) || (rc = check_view(x, "x"))) return rc;
-  if (K > 0x7fff0000LL) return fail(kUnsupported, "quantize_rows: rows of %lld elements", K);
   if (M == 0) return finish_launch("quantize_rows(empty)");
   QuantizeArgs a{x.data, static_cast<int8_t*>(codes.data), static_cast<float*>(scale.data), x.stride[0], codes.stride[0],
                  scale.stride[0], (int)M, (int)K, (int)K};
@@ -2076,6 +2079,7 @@ int int8_matmul_impl(const KgArgSlot* args, unsigned long long n) {
   if (!row_contiguous(out) || !row_contiguous(x) || !row_contiguous(w))
     return fail(kInvalid, "int8_matmul: the rows of out, x and weight must be contiguous");
   if (K > kInt8MostK) return fail(kUnsupported, "int8_matmul: K=%lld > %d: sums may leave 32 bits", K, kInt8MostK);
+  if (M * N > kMostBytes / 2) return fail(kUnsupported, "int8_matmul: %lld x %lld results are too many", M, N);
   if ((rc = check_view(out, "out")) || (rc = check_view(x, "x")) || (rc = check_view(x_scale, "x_scale")) ||
       (rc = check_view(w, "weight")) || (rc = check_view(w_scale, "w_scale")) || (rc = check_view(bias, "bias")))
     return rc;
@@ -2140,14 +2144,15 @@ int head_norm_rotate_impl(const KgArgSlot* args, unsigned long long n) {
   if (positions.shape[0] != tokens) return fail(kInvalid, "head_norm_rotate: %lld positions for %lld tokens", positions.shape[0], tokens);
   if (!(eps >= 0.0 && eps <= 3.0e38)) return fail(kInvalid, "head_norm_rotate: eps must be finite and not negative");
   if (neighbours != 0 && neighbours != 1) return fail(kInvalid, "head_norm_rotate: neighbours must be 0 or 1");
+  const long long heads = rows[2].shape[1] + rows[3].shape[1];
+  if (heads > 0x7fffffffLL || tokens * heads > kMostBytes / 2 / d)
+    return fail(kUnsupported, "head_norm_rotate: %lld x %lld heads of %lld elements are too many", tokens, heads, d);
   for (int i = 0; i < 4; ++i)
     if ((rc = check_view(rows[i], kNames[i]))) return rc;
   if ((rc = check_view(weight[0], "q_weight")) || (rc = check_view(weight[1], "k_weight")) || (rc = check_view(cos, "cos")) ||
       (rc = check_view(sin, "sin")) || (rc = check_view(positions, "positions")))
     return rc;
-  const long long heads = rows[2].shape[1] + rows[3].shape[1];
   if (tokens == 0 || heads == 0 || cos.shape[0] == 0) return finish_launch("head_norm_rotate(empty)");
-  if (heads > 0x7fffffffLL) return fail(kUnsupported, "head_norm_rotate: %lld heads", heads);
   HeadNormArgs a{};
   for (int x = 0; x < 2; ++x) {
     const Mem &out = rows[x], &in = rows[2 + x], &w = weight[x];
